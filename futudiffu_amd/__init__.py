@@ -21,6 +21,11 @@ from .attention_srcii import (  # noqa: F401
     sage_bwd_masked_op,
     sage_bwd_op,
 )
+from .block_ops import (  # noqa: F401  (registers the ops around the attention)
+    rms_norm_gate_residual,
+    rms_norm_gate_residual_modulate,
+    rms_norm_modulate,
+)
 from .block_mask import build_block_mask, build_doc_ids  # noqa: F401
 from .sage_attention import (  # noqa: F401
     configure_sage,

@@ -57,6 +57,24 @@ SIGNATURES = {
     "sage_attn_bwd": (_c.c_int, [
         _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _c.c_int, _c.c_int, _c.c_float, _c.c_float,
         _P, _I64, _I64, _I64, _P, _P, _c.c_size_t, _P, _P, _P, _P]),
+    "sage_rms_norm_modulate": (_c.c_int, [
+        _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _c.c_int, _c.c_int, _c.c_float, _P, _P]),
+    "sage_rms_norm_gate_residual": (_c.c_int, [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _c.c_int, _c.c_int,
+        _c.c_float, _P, _P]),
+    "sage_rms_norm_gate_residual_modulate": (_c.c_int, [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
+        _c.c_int, _c.c_int, _c.c_float, _P, _P, _P]),
+    "sage_rms_norm_bwd_workspace_bytes": (_c.c_size_t, [_I64, _I64, _I64, _I64, _c.c_int, _c.c_int]),
+    "sage_rms_norm_modulate_bwd": (_c.c_int, [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _c.c_int, _c.c_int,
+        _c.c_float, _P, _c.c_size_t, _P, _P, _P, _P]),
+    "sage_rms_norm_gate_residual_bwd": (_c.c_int, [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _c.c_int, _c.c_int,
+        _c.c_float, _P, _c.c_size_t, _P, _P, _P, _P]),
+    "sage_rms_norm_gate_residual_modulate_bwd": (_c.c_int, [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _I64,
+        _I64, _P, _I64, _I64, _I64, _c.c_int, _c.c_int, _c.c_float, _P, _c.c_size_t, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 _lock = threading.Lock()

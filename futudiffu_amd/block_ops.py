@@ -1,0 +1,389 @@
+"""What surrounds the attention in a transformer block, on MI355X.
+
+* :func:`rms_norm_modulate`      the norm before a block: ``xhat * weight * (1 + scale)``
+* :func:`rms_norm_gate_residual` the norm after it: ``residual + gate * xhat * weight``
+* :func:`rms_norm_gate_residual_modulate` the norm after one half of a block and the
+  norm before the next, in one pass
+
+``xhat = x / sqrt(mean(x^2) + eps)`` over the channels; arithmetic in fp32, one rounding
+per output.  ``x`` is ``[B, N, C]`` (or ``[N, C]``), bfloat16 or float16, with any strides
+(channels that are not contiguous are copied).  ``weight`` is ``[C]`` or None; ``scale``
+and ``gate`` have a row per batch item, ``[B, C]``, or with ``doc_ids`` (int32 ``[B, N]``,
+as :func:`futudiffu_amd.build_doc_ids` makes them) a row per document of a packed
+sequence, ``[B, G, C]``: a token whose id is not in ``0 .. G-1`` (padding) has scale 0 and
+gate 0.  Parameters are of ``x``'s type or float32; chunks of one projection's output are
+read in place.
+
+The functions differentiate: where a gradient is wanted, or under ``torch.compile``,
+they go through the custom ops ``futudiffu_ii::rms_norm_modulate``,
+``::rms_norm_gate_residual`` and ``::rms_norm_gate_residual_modulate``, whose gradients
+are ops of their own; channel sums are added in a fixed order, so gradients repeat bit
+for bit.  An empty batch gives empty outputs and zero parameter gradients.
+"""
+
+from __future__ import annotations
+
+import contextlib
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .sage_attention import _ptr, _stream_handle
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_ops = torch.library.Library("futudiffu_ii", "FRAGMENT")
+
+
+def _on(device: torch.device):
+    """The library launches on the current device: make it ``device``."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _tokens(name: str, t: Tensor, like: Tensor | None = None) -> Tensor:
+    """A token tensor the kernels read in place: channels contiguous."""
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name} must be a {like.dtype} {list(like.shape)} tensor on {like.device}, got "
+                         f"{t.dtype} {list(t.shape)} on {t.device}")
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _dims(t: Tensor) -> tuple[int, int]:
+    """Element strides per batch item and token."""
+    s = t.stride()
+    return (s[0], s[1]) if len(s) == 3 else (0, s[0])
+
+
+def _check_x(x: Tensor, eps: float) -> tuple[int, int, int]:
+    if x.ndim not in (2, 3):
+        raise ValueError(f"x must be [B, N, C] or [N, C], got {list(x.shape)}")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
+    if not x.is_cuda:
+        raise ValueError(f"x must be a GPU tensor (device {x.device})")
+    if not eps >= 0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
+    B, N, C = x.shape if x.ndim == 3 else (1, *x.shape)
+    if C < 1:
+        raise ValueError(f"x needs at least one channel, got {list(x.shape)}")
+    return B, N, C
+
+
+def _check_weight(name: str, w: Tensor | None, x: Tensor, C: int) -> Tensor | None:
+    if w is None:
+        return None
+    if w.shape != (C,) or w.device != x.device or (w.dtype != x.dtype and w.dtype != torch.float32):
+        raise ValueError(f"{name} must be a [{C}] tensor of {x.dtype} or float32 on {x.device}, got {w.dtype} "
+                         f"{list(w.shape)} on {w.device}")
+    return w.contiguous()
+
+
+def _check_cond(name: str, k: Tensor | None, x: Tensor, B: int, C: int, docs: bool):
+    """A conditioning tensor and its (batch, row) strides and rows."""
+    if k is None:
+        return None, 0, 0, 0
+    want = f"[{B}, G, {C}] (with doc_ids)" if docs else f"[{B}, {C}]"
+    ok = (k.ndim == 3 and k.shape[0] == B and k.shape[1] >= 1 and k.shape[2] == C) if docs else k.shape == (B, C)
+    if not ok or k.device != x.device or (k.dtype != x.dtype and k.dtype != torch.float32):
+        raise ValueError(f"{name} must be a {want} tensor of {x.dtype} or float32 on {x.device}, got {k.dtype} "
+                         f"{list(k.shape)} on {k.device}")
+    if k.stride(-1) != 1 and C != 1:
+        k = k.contiguous()
+    return (k, k.stride(0), k.stride(1), k.shape[1]) if docs else (k, k.stride(0), 0, 1)
+
+
+def _check_docs(doc_ids: Tensor | None, x: Tensor, B: int, N: int) -> Tensor | None:
+    if doc_ids is None:
+        return None
+    if doc_ids.shape != ((B, N) if x.ndim == 3 else (N,)) and doc_ids.shape != (B, N):
+        raise ValueError(f"doc_ids must be [B, N] = [{B}, {N}], got {list(doc_ids.shape)}")
+    if doc_ids.dtype.is_floating_point or doc_ids.dtype == torch.bool:
+        raise ValueError(f"doc_ids must hold integers, got {doc_ids.dtype}")
+    return doc_ids.to(device=x.device, dtype=torch.int32).contiguous()
+
+
+def _f32(*params: Tensor | None) -> int:
+    """Bit i: parameter i is fp32."""
+    return sum(1 << i for i, p in enumerate(params) if p is not None and p.dtype == torch.float32)
+
+
+def _through_op(*tensors: Tensor | None) -> bool:
+    if torch.compiler.is_compiling():
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _Norm:
+    """The checked arguments of a norm call, as the library takes them."""
+
+    def __init__(self, x: Tensor, weight, cond_name: str, cond, doc_ids, eps: float, next_weight=None,
+                 next_scale=None):
+        self.B, self.N, self.C = B, N, C = _check_x(x, eps)
+        self.x = x = _tokens("x", x)
+        if cond is None and next_scale is None:
+            if doc_ids is not None:
+                _check_docs(doc_ids, x, B, N)
+            doc_ids = None  # nothing differs between documents
+        self.doc = _check_docs(doc_ids, x, B, N)
+        self.weight = _check_weight("weight", weight, x, C)
+        docs = self.doc is not None
+        self.cond, self.cbs, self.cgs, g1 = _check_cond(cond_name, cond, x, B, C, docs)
+        self.next_weight = _check_weight("next_weight", next_weight, x, C)
+        self.next_scale, self.sbs, self.sgs, g2 = _check_cond("next_scale", next_scale, x, B, C, docs)
+        if g1 and g2 and g1 != g2:
+            raise ValueError(f"{cond_name} and next_scale must have a row for the same documents, got {g1} and {g2}")
+        self.groups = g1 or g2 or 1
+        self.f32 = _f32(self.weight, self.cond, self.next_weight, self.next_scale)
+        self.empty = B == 0 or N == 0
+        self.eps = eps
+
+    def tail(self):
+        return (self.groups, _ptr(self.doc), self.B, self.N, self.C, _DTYPES[self.x.dtype], self.f32, self.eps)
+
+    def workspace(self, wanted: bool, fused: bool):
+        if not wanted:
+            return None, 0
+        size = _lib.load().sage_rms_norm_bwd_workspace_bytes(self.B, self.N, self.C, self.groups,
+                                                             self.doc is not None, fused)
+        return torch.empty(size, dtype=torch.uint8, device=self.x.device), size
+
+    def zeros(self, *grads: Tensor | None):
+        """The gradients of an empty batch."""
+        for g in grads:
+            if g is not None:
+                g.zero_()
+
+
+def _grad(t: Tensor | None, wanted: bool) -> Tensor | None:
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted and t is not None else None
+
+
+def _modulate_forward(x: Tensor, weight: Tensor | None, scale: Tensor | None, doc_ids: Tensor | None,
+                      eps: float) -> Tensor:
+    a = _Norm(x, weight, "scale", scale, doc_ids, eps)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if a.empty:
+        return out
+    with _on(x.device):
+        _lib.check(_lib.load().sage_rms_norm_modulate(
+            a.x.data_ptr(), *_dims(a.x), _ptr(a.weight), _ptr(a.cond), a.cbs, a.cgs, *a.tail(), out.data_ptr(),
+            _stream_handle(x.device)))
+    return out
+
+
+def _gate_forward(residual: Tensor, x: Tensor, weight: Tensor | None, gate: Tensor | None,
+                  doc_ids: Tensor | None, eps: float) -> Tensor:
+    a = _Norm(x, weight, "gate", gate, doc_ids, eps)
+    r = _tokens("residual", residual, x)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if a.empty:
+        return out
+    with _on(x.device):
+        _lib.check(_lib.load().sage_rms_norm_gate_residual(
+            r.data_ptr(), *_dims(r), a.x.data_ptr(), *_dims(a.x), _ptr(a.weight), _ptr(a.cond), a.cbs, a.cgs,
+            *a.tail(), out.data_ptr(), _stream_handle(x.device)))
+    return out
+
+
+def _gate_modulate_forward(residual: Tensor, x: Tensor, weight: Tensor | None, gate: Tensor | None,
+                           next_weight: Tensor | None, next_scale: Tensor | None, doc_ids: Tensor | None,
+                           eps: float) -> tuple[Tensor, Tensor]:
+    a = _Norm(x, weight, "gate", gate, doc_ids, eps, next_weight, next_scale)
+    r = _tokens("residual", residual, x)
+    hidden = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if a.empty:
+        return hidden, out
+    with _on(x.device):
+        _lib.check(_lib.load().sage_rms_norm_gate_residual_modulate(
+            r.data_ptr(), *_dims(r), a.x.data_ptr(), *_dims(a.x), _ptr(a.weight), _ptr(a.cond), a.cbs, a.cgs,
+            _ptr(a.next_weight), _ptr(a.next_scale), a.sbs, a.sgs, *a.tail(), hidden.data_ptr(), out.data_ptr(),
+            _stream_handle(x.device)))
+    return hidden, out
+
+
+def _norm_backward(name: str, cond_name: str, dout: Tensor, x: Tensor, weight: Tensor | None, cond: Tensor | None,
+                   doc_ids: Tensor | None, eps: float, wanted: list[bool]) -> tuple[Tensor | None, ...]:
+    """dx, dweight and the conditioning's gradient (None where not wanted)."""
+    a = _Norm(x, weight, cond_name, cond, doc_ids, eps)
+    d = _tokens("dout", dout, x)
+    dx, dw, dc = _grad(x, wanted[0]), _grad(weight, wanted[1]), _grad(cond, wanted[2])
+    if a.empty:
+        a.zeros(dw, dc)
+        return dx, dw, dc
+    if dx is None and dw is None and dc is None:
+        return dx, dw, dc
+    with _on(x.device):
+        ws, wsb = a.workspace(dw is not None or dc is not None, False)
+        _lib.check(getattr(_lib.load(), name)(
+            d.data_ptr(), *_dims(d), a.x.data_ptr(), *_dims(a.x), _ptr(a.weight), _ptr(a.cond), a.cbs, a.cgs,
+            *a.tail(), _ptr(ws), wsb, _ptr(dx), _ptr(dw), _ptr(dc), _stream_handle(x.device)))
+    return dx, dw, dc
+
+
+def _gate_modulate_backward(dhidden: Tensor, dout: Tensor, residual: Tensor, x: Tensor, weight: Tensor | None,
+                            gate: Tensor | None, next_weight: Tensor | None, next_scale: Tensor | None,
+                            doc_ids: Tensor | None, eps: float, wanted: list[bool]) -> tuple[Tensor | None, ...]:
+    """Gradients of residual, x, weight, gate, next_weight, next_scale (None where not
+    wanted; the residual's, which the others come from, is always formed)."""
+    a = _Norm(x, weight, "gate", gate, doc_ids, eps, next_weight, next_scale)
+    r, d, dh = _tokens("residual", residual, x), _tokens("dout", dout, x), _tokens("dhidden", dhidden, x)
+    dr, dx = _grad(x, True), _grad(x, wanted[1])
+    params = [_grad(p, w) for p, w in zip((weight, gate, next_weight, next_scale), wanted[2:])]
+    if a.empty:
+        a.zeros(*params)
+        return dr, dx, *params
+    with _on(x.device):
+        ws, wsb = a.workspace(any(p is not None for p in params), True)
+        _lib.check(_lib.load().sage_rms_norm_gate_residual_modulate_bwd(
+            dh.data_ptr(), *_dims(dh), d.data_ptr(), *_dims(d), r.data_ptr(), *_dims(r), a.x.data_ptr(),
+            *_dims(a.x), _ptr(a.weight), _ptr(a.cond), a.cbs, a.cgs, _ptr(a.next_weight), _ptr(a.next_scale),
+            a.sbs, a.sgs, *a.tail(), _ptr(ws), wsb, dr.data_ptr(), _ptr(dx), *map(_ptr, params),
+            _stream_handle(x.device)))
+    return dr, dx, *params
+
+
+# ---- ops and their autograd formulas ---------------------------------------------------
+#
+# A gradient op returns an empty tensor in the place of a gradient that is not wanted
+# (an op's outputs cannot be None).
+
+def _define(schema: str, impl, fake) -> None:
+    name = schema.split("(")[0]
+    _ops.define(schema)
+    _ops.impl(name, impl, "CompositeExplicitAutograd")
+    torch.library.register_fake(f"futudiffu_ii::{name}", fake, lib=_ops)
+
+
+def _present(grads, like: Tensor) -> tuple[Tensor, ...]:
+    return tuple(like.new_empty(0) if g is None else g for g in grads)
+
+
+def _fake_grads(like: Tensor, *pairs) -> tuple[Tensor, ...]:
+    return tuple(like.new_empty(0) if t is None or not w else t.new_empty(t.shape) for t, w in pairs)
+
+
+def _wanted(ctx, places, tensors) -> list[bool]:
+    return [t is not None and ctx.needs_input_grad[i] for i, t in zip(places, tensors)]
+
+
+def _only(grads, wanted):
+    return [g if w else None for g, w in zip(grads, wanted)]
+
+
+_define("rms_norm_modulate(Tensor x, Tensor? weight, Tensor? scale, Tensor? doc_ids, float eps) -> Tensor",
+        _modulate_forward, lambda x, weight, scale, doc_ids, eps: x.new_empty(x.shape))
+_define("rms_norm_modulate_backward(Tensor dout, Tensor x, Tensor? weight, Tensor? scale, Tensor? doc_ids, "
+        "float eps, bool[] wanted) -> (Tensor, Tensor, Tensor)",
+        lambda dout, x, weight, scale, doc_ids, eps, wanted: _present(
+            _norm_backward("sage_rms_norm_modulate_bwd", "scale", dout, x, weight, scale, doc_ids, eps, wanted), x),
+        lambda dout, x, weight, scale, doc_ids, eps, wanted: _fake_grads(
+            x, *zip((x, weight, scale), wanted)))
+_define("rms_norm_gate_residual(Tensor residual, Tensor x, Tensor? weight, Tensor? gate, Tensor? doc_ids, "
+        "float eps) -> Tensor",
+        _gate_forward, lambda residual, x, weight, gate, doc_ids, eps: x.new_empty(x.shape))
+_define("rms_norm_gate_residual_backward(Tensor dout, Tensor x, Tensor? weight, Tensor? gate, Tensor? doc_ids, "
+        "float eps, bool[] wanted) -> (Tensor, Tensor, Tensor)",
+        lambda dout, x, weight, gate, doc_ids, eps, wanted: _present(
+            _norm_backward("sage_rms_norm_gate_residual_bwd", "gate", dout, x, weight, gate, doc_ids, eps, wanted),
+            x),
+        lambda dout, x, weight, gate, doc_ids, eps, wanted: _fake_grads(x, *zip((x, weight, gate), wanted)))
+_define("rms_norm_gate_residual_modulate(Tensor residual, Tensor x, Tensor? weight, Tensor? gate, "
+        "Tensor? next_weight, Tensor? next_scale, Tensor? doc_ids, float eps) -> (Tensor, Tensor)",
+        _gate_modulate_forward,
+        lambda residual, x, weight, gate, next_weight, next_scale, doc_ids, eps: (x.new_empty(x.shape),
+                                                                                 x.new_empty(x.shape)))
+_define("rms_norm_gate_residual_modulate_backward(Tensor dhidden, Tensor dout, Tensor residual, Tensor x, "
+        "Tensor? weight, Tensor? gate, Tensor? next_weight, Tensor? next_scale, Tensor? doc_ids, float eps, "
+        "bool[] wanted) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)",
+        lambda dhidden, dout, residual, x, *rest: _present(
+            _gate_modulate_backward(dhidden, dout, residual, x, *rest), x),
+        lambda dhidden, dout, residual, x, weight, gate, next_weight, next_scale, doc_ids, eps, wanted: _fake_grads(
+            x, (x, True), (x, wanted[1]), *zip((weight, gate, next_weight, next_scale), wanted[2:])))
+
+
+def _modulate_setup(ctx, inputs, output):
+    x, weight, scale, doc_ids, eps = inputs
+    ctx.save_for_backward(x, weight, scale, doc_ids)
+    ctx.eps = eps
+
+
+def _modulate_autograd(ctx, dout):
+    x, weight, scale, doc_ids = ctx.saved_tensors
+    wanted = _wanted(ctx, (0, 1, 2), (x, weight, scale))
+    grads = torch.ops.futudiffu_ii.rms_norm_modulate_backward(dout, x, weight, scale, doc_ids, ctx.eps, wanted)
+    return *_only(grads, wanted), None, None
+
+
+def _gate_setup(ctx, inputs, output):
+    residual, x, weight, gate, doc_ids, eps = inputs
+    ctx.save_for_backward(x, weight, gate, doc_ids)
+    ctx.eps = eps
+
+
+def _gate_autograd(ctx, dout):
+    x, weight, gate, doc_ids = ctx.saved_tensors
+    wanted = _wanted(ctx, (1, 2, 3), (x, weight, gate))
+    grads = (None, None, None)
+    if any(wanted):
+        grads = torch.ops.futudiffu_ii.rms_norm_gate_residual_backward(dout, x, weight, gate, doc_ids, ctx.eps,
+                                                                       wanted)
+    return dout if ctx.needs_input_grad[0] else None, *_only(grads, wanted), None, None
+
+
+def _gate_modulate_setup(ctx, inputs, output):
+    residual, x, weight, gate, next_weight, next_scale, doc_ids, eps = inputs
+    ctx.save_for_backward(residual, x, weight, gate, next_weight, next_scale, doc_ids)
+    ctx.eps = eps
+
+
+def _gate_modulate_autograd(ctx, dhidden, dout):
+    residual, x, weight, gate, next_weight, next_scale, doc_ids = ctx.saved_tensors
+    wanted = _wanted(ctx, range(6), (residual, x, weight, gate, next_weight, next_scale))
+    grads = torch.ops.futudiffu_ii.rms_norm_gate_residual_modulate_backward(
+        dhidden, dout, residual, x, weight, gate, next_weight, next_scale, doc_ids, ctx.eps, wanted)
+    return *_only(grads, wanted), None, None
+
+
+torch.library.register_autograd("futudiffu_ii::rms_norm_modulate", _modulate_autograd,
+                                setup_context=_modulate_setup, lib=_ops)
+torch.library.register_autograd("futudiffu_ii::rms_norm_gate_residual", _gate_autograd, setup_context=_gate_setup,
+                                lib=_ops)
+torch.library.register_autograd("futudiffu_ii::rms_norm_gate_residual_modulate", _gate_modulate_autograd,
+                                setup_context=_gate_modulate_setup, lib=_ops)
+
+
+# ---- the functions ---------------------------------------------------------------------
+
+def rms_norm_modulate(x: Tensor, weight: Tensor | None = None, scale: Tensor | None = None, *,
+                      doc_ids: Tensor | None = None, eps: float = 1e-5) -> Tensor:
+    """``xhat * weight * (1 + scale)``: the norm before a block with its modulation."""
+    if _through_op(x, weight, scale):
+        return torch.ops.futudiffu_ii.rms_norm_modulate(x, weight, scale, doc_ids, eps)
+    return _modulate_forward(x, weight, scale, doc_ids, eps)
+
+
+def rms_norm_gate_residual(residual: Tensor, x: Tensor, weight: Tensor | None = None, gate: Tensor | None = None, *,
+                           doc_ids: Tensor | None = None, eps: float = 1e-5) -> Tensor:
+    """``residual + gate * xhat * weight``: the norm after a block, gated, onto the residual."""
+    if _through_op(residual, x, weight, gate):
+        return torch.ops.futudiffu_ii.rms_norm_gate_residual(residual, x, weight, gate, doc_ids, eps)
+    return _gate_forward(residual, x, weight, gate, doc_ids, eps)
+
+
+def rms_norm_gate_residual_modulate(residual: Tensor, x: Tensor, weight: Tensor | None = None,
+                                    gate: Tensor | None = None, next_weight: Tensor | None = None,
+                                    next_scale: Tensor | None = None, *, doc_ids: Tensor | None = None,
+                                    eps: float = 1e-5) -> tuple[Tensor, Tensor]:
+    """``hidden = residual + gate * xhat * weight`` and the norm of ``hidden`` before the
+    next block, ``(hidden, out)``.
+
+    The second norm takes ``hidden`` unrounded: ``out`` is nearer the exact value than the
+    two calls' one after the other, which normalize the rounded ``hidden``.
+    """
+    if _through_op(residual, x, weight, gate, next_weight, next_scale):
+        return torch.ops.futudiffu_ii.rms_norm_gate_residual_modulate(residual, x, weight, gate, next_weight,
+                                                                      next_scale, doc_ids, eps)
+    return _gate_modulate_forward(residual, x, weight, gate, next_weight, next_scale, doc_ids, eps)

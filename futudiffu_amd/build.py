@@ -23,7 +23,8 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 # the attention kernel's pipelined loop (sage_phase_read), for bench.py
 # --phase-timing; never loaded by the product path
 PHASE_LIB_PATH = os.path.join(HERE, "libsage_mi355x_phase.so")
-SOURCES = ["sage_quant.hip", "sage_attn.hip", "sage_mask.hip", "sage_bwd.hip", "sage_capi.hip"]
+SOURCES = ["sage_quant.hip", "sage_attn.hip", "sage_mask.hip", "sage_bwd.hip", "sage_capi.hip",
+           "sage_norm.hip"]
 ARCH = "gfx950"
 
 

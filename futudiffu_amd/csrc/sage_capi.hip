@@ -681,3 +681,201 @@ int sage_doc_ids_from_cu_seqlens(const int32_t* cu_seqlens, int64_t b, int64_t n
 }
 
 }  // extern "C"
+
+namespace {
+
+int check_norm(const sage::NormArgs& a, int64_t b, int64_t n, int64_t c, int64_t groups, int dtype, int fp32_params) {
+  if (b <= 0 || n <= 0 || c <= 0)
+    return fail(SAGE_ERR_ARG, "b=%lld, n=%lld and c=%lld must be positive", (long long)b, (long long)n, (long long)c);
+  if (c > sage::kNormMaxC) return fail(SAGE_ERR_ARG, "c=%lld exceeds %lld", (long long)c, (long long)sage::kNormMaxC);
+  if (b > 65535 || n >= (int64_t)1 << 23 || b * n >= (int64_t)1 << 23)
+    return fail(SAGE_ERR_ARG, "b=%lld x n=%lld exceeds the grid limit 2^23", (long long)b, (long long)n);
+  if (groups <= 0 || groups > 32767 || b * groups > 32767)
+    return fail(SAGE_ERR_ARG, "b=%lld x groups=%lld must be between 1 and 32767", (long long)b, (long long)groups);
+  if (!a.doc && groups != 1) return fail(SAGE_ERR_ARG, "groups=%lld needs doc_ids", (long long)groups);
+  if (dtype != SAGE_DTYPE_BF16 && dtype != SAGE_DTYPE_FP16) return fail(SAGE_ERR_ARG, "unknown dtype %d", dtype);
+  if (fp32_params < 0 || fp32_params > 15) return fail(SAGE_ERR_ARG, "unknown fp32_params %d", fp32_params);
+  if (!(a.eps >= 0.0f)) return fail(SAGE_ERR_ARG, "eps must be >= 0");
+  return SAGE_OK;
+}
+
+sage::NormArgs norm_args(const void* x, int64_t x_bs, int64_t x_rs, const void* w, const void* cond, int64_t cond_bs,
+                         int64_t cond_gs, int64_t groups, const int32_t* doc, int64_t b, int64_t n, int64_t c,
+                         int fp32_params, float eps) {
+  sage::NormArgs a{};
+  a.x = {x, x_bs, x_rs};
+  a.w = {w, fp32_params & SAGE_FP32_WEIGHT ? 1 : 0};
+  a.cond = {cond, fp32_params & SAGE_FP32_COND ? 1 : 0, (int)groups, cond_bs, cond_gs};
+  a.doc = doc;
+  a.groups = (int)groups;
+  a.b = (int)b;
+  a.n = n;
+  a.c = (int)c;
+  a.eps = eps;
+  return a;
+}
+
+// Element alignment of a call's pointers: 2 bytes, fp32 parameters 4.
+int check_norm_align(const sage::NormArgs& a) {
+  const void* two[] = {a.x.p, a.res.p, a.dout.p, a.dhidden.p, a.out, a.hidden, a.dx, a.dres};
+  for (const void* p : two)
+    if (reinterpret_cast<uintptr_t>(p) & 1u) return fail(SAGE_ERR_ALIGN, "tensor pointers must be aligned to their elements");
+  const struct { const void* p; int f32; } params[] = {
+      {a.w.p, a.w.f32},   {a.w2.p, a.w2.f32}, {a.cond.p, a.cond.f32},   {a.cond2.p, a.cond2.f32},
+      {a.dw, a.w.f32},    {a.dw2, a.w2.f32},  {a.dcond, a.cond.f32},    {a.dcond2, a.cond2.f32}};
+  for (const auto& q : params)
+    if (reinterpret_cast<uintptr_t>(q.p) & (q.f32 ? 3u : 1u))
+      return fail(SAGE_ERR_ALIGN, "parameter pointers must be aligned to their elements");
+  return SAGE_OK;
+}
+
+size_t norm_workspace(int64_t b, const sage::NormChunks& k, int sets, size_t* id_off) {
+  const size_t part = (size_t)(b * k.chunks * k.slots * sets * k.cp) * sizeof(float);
+  *id_off = part;
+  return part + (size_t)(b * k.chunks * k.slots) * sizeof(int32_t);
+}
+
+// The backward's chunks and workspace, and its launch.
+int run_norm_bwd(int op, sage::NormArgs& a, int dtype, void* workspace, size_t workspace_bytes, hipStream_t stream,
+                 const char* what) {
+  const sage::NormChunks k = sage::norm_chunks(a.b, a.n, a.c, a.groups, a.doc != nullptr);
+  a.chunks = (int)k.chunks;
+  a.chunk = k.chunk;
+  a.slots = (int)k.slots;
+  a.cp = k.cp;
+  if (a.dw || a.dw2 || a.dcond || a.dcond2) {
+    size_t id_off;
+    const size_t need = norm_workspace(a.b, k, op == sage::kNormGateModulate ? 2 : 1, &id_off);
+    if (!workspace || workspace_bytes < need)
+      return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace_bytes);
+    if (!aligned16(workspace)) return fail(SAGE_ERR_ALIGN, "workspace must be 16-byte aligned");
+    a.part = static_cast<float*>(workspace);
+    a.part_id = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + id_off);
+  }
+  return launch_status(sage::launch_norm_bwd(op, dtype, a, stream), what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sage_rms_norm_modulate(const void* x, int64_t x_bs, int64_t x_rs, const void* weight, const void* scale,
+                           int64_t scale_bs, int64_t scale_gs, int64_t groups, const int32_t* doc_ids, int64_t b,
+                           int64_t n, int64_t c, int dtype, int fp32_params, float eps, void* out,
+                           hipStream_t stream) {
+  sage::NormArgs a = norm_args(x, x_bs, x_rs, weight, scale, scale_bs, scale_gs, groups, doc_ids, b, n, c,
+                               fp32_params, eps);
+  if (const int e = check_norm(a, b, n, c, groups, dtype, fp32_params)) return e;
+  if (!x || !out) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  a.out = out;
+  if (const int e = check_norm_align(a)) return e;
+  return launch_status(sage::launch_norm_fwd(sage::kNormModulate, dtype, a, stream), "sage_rms_norm_modulate");
+}
+
+int sage_rms_norm_gate_residual(const void* residual, int64_t r_bs, int64_t r_rs, const void* x, int64_t x_bs,
+                                int64_t x_rs, const void* weight, const void* gate, int64_t gate_bs, int64_t gate_gs,
+                                int64_t groups, const int32_t* doc_ids, int64_t b, int64_t n, int64_t c, int dtype,
+                                int fp32_params, float eps, void* out, hipStream_t stream) {
+  sage::NormArgs a = norm_args(x, x_bs, x_rs, weight, gate, gate_bs, gate_gs, groups, doc_ids, b, n, c, fp32_params,
+                               eps);
+  if (const int e = check_norm(a, b, n, c, groups, dtype, fp32_params)) return e;
+  if (!residual || !x || !out) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  a.res = {residual, r_bs, r_rs};
+  a.out = out;
+  if (const int e = check_norm_align(a)) return e;
+  return launch_status(sage::launch_norm_fwd(sage::kNormGate, dtype, a, stream), "sage_rms_norm_gate_residual");
+}
+
+int sage_rms_norm_gate_residual_modulate(const void* residual, int64_t r_bs, int64_t r_rs, const void* x,
+                                         int64_t x_bs, int64_t x_rs, const void* weight, const void* gate,
+                                         int64_t gate_bs, int64_t gate_gs, const void* next_weight,
+                                         const void* next_scale, int64_t scale_bs, int64_t scale_gs, int64_t groups,
+                                         const int32_t* doc_ids, int64_t b, int64_t n, int64_t c, int dtype,
+                                         int fp32_params, float eps, void* hidden, void* out, hipStream_t stream) {
+  sage::NormArgs a = norm_args(x, x_bs, x_rs, weight, gate, gate_bs, gate_gs, groups, doc_ids, b, n, c, fp32_params,
+                               eps);
+  if (const int e = check_norm(a, b, n, c, groups, dtype, fp32_params)) return e;
+  if (!residual || !x || !hidden || !out) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  a.res = {residual, r_bs, r_rs};
+  a.w2 = {next_weight, fp32_params & SAGE_FP32_NEXT_WEIGHT ? 1 : 0};
+  a.cond2 = {next_scale, fp32_params & SAGE_FP32_NEXT_SCALE ? 1 : 0, (int)groups, scale_bs, scale_gs};
+  a.hidden = hidden;
+  a.out = out;
+  if (const int e = check_norm_align(a)) return e;
+  return launch_status(sage::launch_norm_fwd(sage::kNormGateModulate, dtype, a, stream),
+                       "sage_rms_norm_gate_residual_modulate");
+}
+
+size_t sage_rms_norm_bwd_workspace_bytes(int64_t b, int64_t n, int64_t c, int64_t groups, int with_doc_ids,
+                                         int fused) {
+  if (b <= 0 || n <= 0 || c <= 0 || groups <= 0 || b > 65535 || groups > 32767 || b * groups > 32767 ||
+      c > sage::kNormMaxC || n >= (int64_t)1 << 23 || b * n >= (int64_t)1 << 23)
+    return 0;
+  size_t id_off;
+  return norm_workspace(b, sage::norm_chunks(b, n, c, groups, with_doc_ids != 0), fused ? 2 : 1, &id_off);
+}
+
+int sage_rms_norm_modulate_bwd(const void* dout, int64_t d_bs, int64_t d_rs, const void* x, int64_t x_bs,
+                               int64_t x_rs, const void* weight, const void* scale, int64_t scale_bs,
+                               int64_t scale_gs, int64_t groups, const int32_t* doc_ids, int64_t b, int64_t n,
+                               int64_t c, int dtype, int fp32_params, float eps, void* workspace,
+                               size_t workspace_bytes, void* dx, void* dweight, void* dscale, hipStream_t stream) {
+  sage::NormArgs a = norm_args(x, x_bs, x_rs, weight, scale, scale_bs, scale_gs, groups, doc_ids, b, n, c,
+                               fp32_params, eps);
+  if (const int e = check_norm(a, b, n, c, groups, dtype, fp32_params)) return e;
+  if (!dout || !x) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  a.dout = {dout, d_bs, d_rs};
+  a.dx = dx;
+  a.dw = dweight;
+  a.dcond = dscale;
+  if (const int e = check_norm_align(a)) return e;
+  return run_norm_bwd(sage::kNormModulate, a, dtype, workspace, workspace_bytes, stream, "sage_rms_norm_modulate_bwd");
+}
+
+int sage_rms_norm_gate_residual_bwd(const void* dout, int64_t d_bs, int64_t d_rs, const void* x, int64_t x_bs,
+                                    int64_t x_rs, const void* weight, const void* gate, int64_t gate_bs,
+                                    int64_t gate_gs, int64_t groups, const int32_t* doc_ids, int64_t b, int64_t n,
+                                    int64_t c, int dtype, int fp32_params, float eps, void* workspace,
+                                    size_t workspace_bytes, void* dx, void* dweight, void* dgate,
+                                    hipStream_t stream) {
+  sage::NormArgs a = norm_args(x, x_bs, x_rs, weight, gate, gate_bs, gate_gs, groups, doc_ids, b, n, c, fp32_params,
+                               eps);
+  if (const int e = check_norm(a, b, n, c, groups, dtype, fp32_params)) return e;
+  if (!dout || !x) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  a.dout = {dout, d_bs, d_rs};
+  a.dx = dx;
+  a.dw = dweight;
+  a.dcond = dgate;
+  if (const int e = check_norm_align(a)) return e;
+  return run_norm_bwd(sage::kNormGate, a, dtype, workspace, workspace_bytes, stream,
+                      "sage_rms_norm_gate_residual_bwd");
+}
+
+int sage_rms_norm_gate_residual_modulate_bwd(
+    const void* dhidden, int64_t dh_bs, int64_t dh_rs, const void* dout, int64_t d_bs, int64_t d_rs,
+    const void* residual, int64_t r_bs, int64_t r_rs, const void* x, int64_t x_bs, int64_t x_rs, const void* weight,
+    const void* gate, int64_t gate_bs, int64_t gate_gs, const void* next_weight, const void* next_scale,
+    int64_t scale_bs, int64_t scale_gs, int64_t groups, const int32_t* doc_ids, int64_t b, int64_t n, int64_t c,
+    int dtype, int fp32_params, float eps, void* workspace, size_t workspace_bytes, void* dresidual, void* dx,
+    void* dweight, void* dgate, void* dnext_weight, void* dnext_scale, hipStream_t stream) {
+  sage::NormArgs a = norm_args(x, x_bs, x_rs, weight, gate, gate_bs, gate_gs, groups, doc_ids, b, n, c, fp32_params,
+                               eps);
+  if (const int e = check_norm(a, b, n, c, groups, dtype, fp32_params)) return e;
+  if (!dhidden || !dout || !residual || !x || !dresidual) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  a.dhidden = {dhidden, dh_bs, dh_rs};
+  a.dout = {dout, d_bs, d_rs};
+  a.res = {residual, r_bs, r_rs};
+  a.w2 = {next_weight, fp32_params & SAGE_FP32_NEXT_WEIGHT ? 1 : 0};
+  a.cond2 = {next_scale, fp32_params & SAGE_FP32_NEXT_SCALE ? 1 : 0, (int)groups, scale_bs, scale_gs};
+  a.dres = dresidual;
+  a.dx = dx;
+  a.dw = dweight;
+  a.dcond = dgate;
+  a.dw2 = dnext_weight;
+  a.dcond2 = dnext_scale;
+  if (const int e = check_norm_align(a)) return e;
+  return run_norm_bwd(sage::kNormGateModulate, a, dtype, workspace, workspace_bytes, stream,
+                      "sage_rms_norm_gate_residual_modulate_bwd");
+}
+
+}  // extern "C"

@@ -319,4 +319,49 @@ hipError_t launch_bwd(int qk, int mask, const BwdParams& p, int64_t d, int64_t b
 hipError_t launch_doc_from_cu(const int32_t* cu, int64_t nb, int64_t nseg, int64_t n, int32_t* doc,
                               hipStream_t st);
 
+// RMS norms around a block (sage_norm.hip).
+constexpr int kNormModulate = 0, kNormGate = 1, kNormGateModulate = 2;
+constexpr int64_t kNormMaxC = 8192;  // the widest token a thread group holds in registers
+
+struct NormRows {  // [B, N, C] rows of 16-bit elements, channels contiguous; strides in elements
+  const void* p;
+  int64_t bs, rs;
+};
+struct NormParam {  // [C], 16-bit or fp32; null: ones
+  const void* p;
+  int f32;
+};
+struct NormCond {  // scale or gate rows [B, groups, C]; null: scale 0, gate 1
+  const void* p;
+  int f32;
+  int groups;
+  int64_t bs, gs;
+};
+struct NormArgs {
+  NormRows x, res, dout, dhidden;
+  NormParam w, w2;
+  NormCond cond, cond2;
+  const int32_t* doc;  // [B, N], or null: row 0 of each batch item
+  int groups;          // conditioning rows a batch item (1 without doc)
+  int b, c;
+  int64_t n;
+  float eps;
+  // contiguous outputs [B, N, C]; dx may be null in the backward
+  void *out, *hidden, *dx, *dres;
+  // parameter gradients (each may be null), in the parameters' types
+  void *dw, *dw2, *dcond, *dcond2;
+  // partial channel sums [B * chunks][slots][sets][cp] and, with doc, their ids
+  // [B * chunks][slots] (-1: none, and none after it); null: no parameter gradient
+  float* part;
+  int32_t* part_id;
+  int chunks, slots;
+  int64_t chunk, cp;
+};
+struct NormChunks {
+  int64_t chunks, chunk, slots, cp;
+};
+NormChunks norm_chunks(int64_t b, int64_t n, int64_t c, int64_t groups, bool doc);
+hipError_t launch_norm_fwd(int op, int f16, const NormArgs& a, hipStream_t st);
+hipError_t launch_norm_bwd(int op, int f16, const NormArgs& a, hipStream_t st);
+
 }  // namespace sage

@@ -1,0 +1,579 @@
+// The RMS norms around the attention of a transformer block, for gfx950: before
+// it with the modulation's scale, after it with the gate and the residual, and
+// the norm after one half of a block together with the one before the next.
+//
+//   xhat = x * rrms, rrms = 1 / sqrt(mean(x^2) + eps)   over the C channels of a token
+//   modulate:       y = xhat * w * (1 + s)
+//   gate:           y = r + g * xhat * w
+//   gate, modulate: h = r + g * xhat * w,  y = norm(h) * w2 * (1 + s2)
+//
+// s, g and s2 have a row per batch item, or, with document ids, per document (a
+// token of no document has s = g = s2 = 0).  With m = 1 + s or g, constant over the
+// tokens of one row, and d the gradient of the normed output, the backward is
+//
+//   dx = rrms * (d*w*m - xhat * mean(d*w*m * xhat))
+//   S[row] = sum over its tokens of d * xhat;  ds = dg = w * S;  dw = sum over rows of m * S
+//
+// so the channel sums need one fp32 accumulator a channel, whatever the documents.
+// All arithmetic is fp32; each output is rounded once.  h enters the second norm
+// unrounded, in the backward too, which forms it again from r and x (it reads as
+// many tensors as with h, and dw2 and ds2 stay fp32-exact).
+//
+// Every kernel is bound by memory: a token's channels are held in registers between
+// the reads and the writes, so each tensor is touched once.
+#include <type_traits>
+
+#include "sage_common.h"
+#include "sage_launch.h"
+
+namespace sage {
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kVec = 8;      // channels of one 16-byte access
+constexpr int kPer = 16;     // channels a thread holds of a token
+
+template <typename T>
+struct Vec8;
+template <>
+struct Vec8<__bf16> {
+  typedef bf16x8 type;
+};
+template <>
+struct Vec8<_Float16> {
+  typedef f16x8 type;
+};
+
+// Sum over the 64 lanes of a wave, in all of them: a fixed tree of lane distances 1,
+// 2, 4, 8 (DPP within rows of 16), 16 and 32.
+__device__ __forceinline__ float wave_sum(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  v += dpp(v, std::integral_constant<int, 0xb1>{});   // quad_perm [1,0,3,2]
+  v += dpp(v, std::integral_constant<int, 0x4e>{});   // quad_perm [2,3,0,1]
+  v += dpp(v, std::integral_constant<int, 0x141>{});  // row_half_mirror: the other quad of eight lanes
+  v += dpp(v, std::integral_constant<int, 0x140>{});  // row_mirror: the other eight of sixteen
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const uint32_t w = __float_as_uint(v);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Sums of K values over the TPR threads of a token, in all of them.  `red`: a slot of
+// (waves of the workgroup) x K floats that no thread of an earlier sum still reads.
+template <int TPR, int K>
+__device__ __forceinline__ void token_sum(float (&v)[K], float* red, int wave) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+  if constexpr (TPR > 64) {
+    constexpr int W = TPR / 64;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) red[wave * K + k] = v[k];
+    }
+    __syncthreads();
+    const int w0 = wave / W * W;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float s = red[w0 * K + k];
+#pragma unroll
+      for (int w = 1; w < W; ++w) s += red[(w0 + w) * K + k];
+      v[k] = s;
+    }
+  }
+}
+
+// The channels a thread holds: with VEC two runs of eight, 16-byte accesses; without
+// (odd widths, misaligned rows), every TPR-th channel, so that a wave's accesses are
+// consecutive.
+template <int TPR, bool VEC>
+struct Cols {
+  static __device__ __forceinline__ int col(int t, int j) {
+    return VEC ? ((j / kVec) * TPR + t) * kVec + j % kVec : j * TPR + t;
+  }
+};
+
+// One thread's channels of a row of T, as they lie in memory (loads issue here, the
+// conversion follows when the values are used).  Channels past c are zeros.
+template <typename T, int TPR, bool VEC>
+struct Raw {
+  using V = typename Vec8<T>::type;
+  V v[kPer / kVec];
+  __device__ __forceinline__ void load(const T* row, int t, int c) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < kPer / kVec; ++i) {
+        const int at = (i * TPR + t) * kVec;
+        v[i] = at < c ? *reinterpret_cast<const V*>(row + at) : V{};
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int at = j * TPR + t;
+        v[j / kVec][j % kVec] = at < c ? row[at] : (T)0.0f;
+      }
+    }
+  }
+  __device__ __forceinline__ float operator[](int j) const { return (float)v[j / kVec][j % kVec]; }
+};
+
+template <typename T, int TPR, bool VEC>
+__device__ __forceinline__ void store_row(T* row, int t, int c, const float (&f)[kPer]) {
+  if constexpr (VEC) {
+    using V = typename Vec8<T>::type;
+#pragma unroll
+    for (int i = 0; i < kPer / kVec; ++i) {
+      const int at = (i * TPR + t) * kVec;
+      V o;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) o[j] = (T)f[i * kVec + j];
+      if (at < c) *reinterpret_cast<V*>(row + at) = o;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int at = j * TPR + t;
+      if (at < c) row[at] = (T)f[j];
+    }
+  }
+}
+
+// A thread's channels of a parameter row (T or fp32, or none: `fill`).
+template <typename T, int TPR, bool VEC>
+__device__ __forceinline__ void load_param(const void* p, bool f32, int64_t off, int t, int c, float fill,
+                                           float (&f)[kPer]) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) f[j] = fill;
+  } else if (f32) {
+    const float* row = static_cast<const float*>(p) + off;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < kPer / 4; ++i) {
+        const int at = Cols<TPR, VEC>::col(t, i * 4);
+        const f32x4 v = at < c ? *reinterpret_cast<const f32x4*>(row + at) : f32x4{};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[i * 4 + j] = v[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int at = Cols<TPR, VEC>::col(t, j);
+        f[j] = at < c ? row[at] : 0.0f;
+      }
+    }
+  } else {
+    Raw<T, TPR, VEC> r;
+    r.load(static_cast<const T*>(p) + off, t, c);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) f[j] = r[j];
+  }
+}
+
+__device__ __forceinline__ float rrms(float sum_sq, int c, float eps) {
+  return 1.0f / sqrtf(sum_sq / (float)c + eps);
+}
+
+// w * (scale ? 1 + s : g) of conditioning row `id` of batch item b (id < 0 or >= groups: no
+// document), of one thread's channels.
+template <typename T, int TPR, bool VEC>
+__device__ __forceinline__ void weight_row(const NormParam& w, const NormCond& k, bool scale, int b, int id, int t,
+                                           int c, float (&wm)[kPer]) {
+  float m[kPer];
+  load_param<T, TPR, VEC>(w.p, w.f32, 0, t, c, 1.0f, wm);
+  const bool live = k.p && id >= 0 && id < k.groups;
+  load_param<T, TPR, VEC>(live ? k.p : nullptr, k.f32, b * k.bs + id * k.gs, t, c, scale || k.p ? 0.0f : 1.0f, m);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) wm[j] *= scale ? 1.0f + m[j] : m[j];
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const NormRows& r, int b, int64_t n) {
+  return static_cast<const T*>(r.p) + b * r.bs + n * r.rs;
+}
+
+// Forward: TPR threads a token, one token a thread group.  All loads of a token, the
+// parameter rows included, are issued before its first sum.
+template <typename T, int OP, int TPR, bool VEC>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(NormArgs a) {
+  constexpr int NT = TPR > 256 ? TPR : 256;
+  constexpr int TOK = NT / TPR;
+  __shared__ float red[NT / 64], red2[NT / 64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * TOK + threadIdx.x / TPR, rows = (int64_t)a.b * a.n;
+  const bool live = row < rows;  // a thread group past the last token takes part in the barriers alone
+  const int b = live ? (int)(row / a.n) : 0;
+  const int64_t n = live ? row - (int64_t)b * a.n : 0;
+  const int c = live ? a.c : 0;
+  Raw<T, TPR, VEC> x, r;
+  x.load(row_of<T>(a.x, b, n), t, c);
+  if constexpr (OP != kNormModulate) r.load(row_of<T>(a.res, b, n), t, c);
+  const int id = a.doc && live ? a.doc[row] : 0;
+  float wm[kPer], wm2[kPer];
+  weight_row<T, TPR, VEC>(a.w, a.cond, OP == kNormModulate, b, id, t, c, wm);
+  if constexpr (OP == kNormGateModulate) weight_row<T, TPR, VEC>(a.w2, a.cond2, true, b, id, t, c, wm2);
+  float s[1] = {0.0f};
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) s[0] += x[j] * x[j];
+  token_sum<TPR>(s, red, wave);
+  const float rr = rrms(s[0], a.c, a.eps);
+  float y[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    y[j] = x[j] * rr * wm[j];
+    if constexpr (OP != kNormModulate) y[j] += r[j];
+  }
+  if constexpr (OP == kNormGateModulate) {
+    if (live) store_row<T, TPR, VEC>(static_cast<T*>(a.hidden) + row * a.c, t, c, y);
+    s[0] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) s[0] += y[j] * y[j];
+    token_sum<TPR>(s, red2, wave);
+    const float r2 = rrms(s[0], a.c, a.eps);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) y[j] = y[j] * r2 * wm2[j];
+  }
+  if (live) store_row<T, TPR, VEC>(static_cast<T*>(a.out) + row * a.c, t, c, y);
+}
+
+constexpr int kBwdNT = 512;  // threads of a backward workgroup; also the most tokens of its chunk
+
+// One token's tensors in the backward.
+template <typename T, int OP, int TPR, bool VEC>
+struct BwdRow {
+  Raw<T, TPR, VEC> x, d, r, dh;  // r, dh: gate_modulate alone
+  __device__ __forceinline__ void load(const NormArgs& a, int b, int64_t n, int t, int c) {
+    x.load(row_of<T>(a.x, b, n), t, c);
+    d.load(row_of<T>(a.dout, b, n), t, c);
+    if constexpr (OP == kNormGateModulate) {
+      r.load(row_of<T>(a.res, b, n), t, c);
+      dh.load(row_of<T>(a.dhidden, b, n), t, c);
+    }
+  }
+};
+
+// Adds the groups' channel sums in order and stores them as one partial row.
+template <int TPR, bool VEC>
+__device__ __forceinline__ void store_partial(float* dst, float* sum, int grp, int t, int c, const float (&acc)[kPer]) {
+  constexpr int G = kBwdNT / TPR;
+  if constexpr (G == 1) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int at = Cols<TPR, VEC>::col(t, j);
+      if (at < c) dst[at] = acc[j];
+    }
+  } else {
+#pragma unroll 1
+    for (int g = 0; g < G; ++g) {
+      if (g == grp) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          // conflict-free order: a thread's value j lies at j * TPR + t
+          const float v = g == 0 ? acc[j] : sum[j * TPR + t] + acc[j];
+          if (g + 1 < G) {
+            sum[j * TPR + t] = v;
+          } else {
+            const int at = Cols<TPR, VEC>::col(t, j);
+            if (at < c) dst[at] = v;
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Backward: a workgroup takes a chunk of consecutive tokens of one batch item, its
+// kBwdNT / TPR thread groups one token each at a time, the next token's loads in flight
+// under the present one's sums.  With document ids the chunk's tokens are taken document
+// by document (ids in order, the tokens of none last), so m is constant over a run and its
+// S is one partial row: part[chunk][slot][set][cp], its id in part_id.  Runs are few (a
+// chunk has as many as it has documents), and the order is fixed by the ids alone.
+template <typename T, int OP, int TPR, bool VEC>
+__global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
+  constexpr int G = kBwdNT / TPR, W = kBwdNT / 64;
+  constexpr int SETS = OP == kNormGateModulate ? 2 : 1;
+  constexpr bool kScale = OP == kNormModulate;
+  __shared__ float red[2][W * 2], red1[W], red3[W];
+  __shared__ float sum[G == 1 ? 1 : TPR * kPer];
+  __shared__ int ids_min[W], counts[W];
+  __shared__ uint16_t list[kBwdNT];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+  const int b = blockIdx.x / a.chunks;
+  const int64_t n0 = (int64_t)(blockIdx.x % a.chunks) * a.chunk;
+  const int len = (int)(a.n - n0 < a.chunk ? a.n - n0 : a.chunk);
+  const int c = a.c;
+  const bool sums = a.part != nullptr;
+
+  int my = 0x7fffffff, prev = -1, slot = 0, done = 0;
+  if (a.doc && (int)threadIdx.x < len) {
+    my = a.doc[(int64_t)b * a.n + n0 + threadIdx.x];
+    if (my < 0 || my >= a.groups) my = a.groups;
+  }
+  while (done < len) {
+    // the next run: its id and its tokens
+    int id = 0, run = len;
+    if (a.doc) {
+      int least = my > prev ? my : 0x7fffffff;
+#pragma unroll
+      for (int s = 1; s < 64; s *= 2) least = min(least, __shfl_xor(least, s));
+      if (lane == 0) ids_min[wave] = least;
+      __syncthreads();
+      id = ids_min[0];
+#pragma unroll
+      for (int w = 1; w < W; ++w) id = min(id, ids_min[w]);
+      const uint64_t mine = __ballot(my == id);
+      if (lane == 0) counts[wave] = __popcll(mine);
+      __syncthreads();
+      int before = 0;
+      run = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        before += w < wave ? counts[w] : 0;
+        run += counts[w];
+      }
+      if (my == id) list[before + __popcll(mine & ((1ull << lane) - 1))] = (uint16_t)threadIdx.x;
+      prev = id;
+      __syncthreads();
+    }
+    float wm[kPer], wm2[kPer], acc[kPer] = {}, acc2[kPer] = {};
+    weight_row<T, TPR, VEC>(a.w, a.cond, kScale, b, id, t, c, wm);
+    if constexpr (SETS == 2) weight_row<T, TPR, VEC>(a.w2, a.cond2, true, b, id, t, c, wm2);
+
+    BwdRow<T, OP, TPR, VEC> cur, next;
+    auto token = [&](int pos) { return n0 + (a.doc ? (int)list[pos] : pos); };
+    // a group past its last token loads nothing (its channels are zeros)
+    cur.load(a, b, grp < run ? token(grp) : n0, t, grp < run ? c : 0);
+    const int iters = (run + G - 1) / G;
+#pragma unroll 1
+    for (int it = 0; it < iters; ++it) {
+      const int pos = it * G + grp, npos = pos + G;
+      const int64_t n = pos < run ? token(pos) : n0;
+      if (it + 1 < iters) next.load(a, b, npos < run ? token(npos) : n0, t, npos < run ? c : 0);
+      const int64_t at = ((int64_t)b * a.n + n) * c;
+      float o[kPer];
+      if constexpr (OP != kNormGateModulate) {
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          s[0] += cur.x[j] * cur.x[j];
+          s[1] += cur.d[j] * wm[j] * cur.x[j];
+        }
+        token_sum<TPR>(s, red[it & 1], wave);
+        const float r = rrms(s[0], c, a.eps), k = s[1] * r / (float)c;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const float xh = cur.x[j] * r;
+          o[j] = r * (cur.d[j] * wm[j] - xh * k);
+          acc[j] += cur.d[j] * xh;
+        }
+      } else {
+        float s1[1] = {0.0f};
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) s1[0] += cur.x[j] * cur.x[j];
+        token_sum<TPR>(s1, red1, wave);
+        const float r1 = rrms(s1[0], c, a.eps);
+        float s[2] = {0.0f, 0.0f};
+        float h[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          h[j] = cur.r[j] + cur.x[j] * r1 * wm[j];
+          s[0] += h[j] * h[j];
+          s[1] += cur.d[j] * wm2[j] * h[j];
+        }
+        token_sum<TPR>(s, red[it & 1], wave);
+        const float r2 = rrms(s[0], c, a.eps), k2 = s[1] * r2 / (float)c;
+        float s3[1] = {0.0f};
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const float hh = h[j] * r2;
+          acc2[j] += cur.d[j] * hh;
+          h[j] = cur.dh[j] + r2 * (cur.d[j] * wm2[j] - hh * k2);  // the gradient of h
+          s3[0] += h[j] * wm[j] * cur.x[j];
+        }
+        if (pos < run) store_row<T, TPR, VEC>(static_cast<T*>(a.dres) + at, t, c, h);
+        token_sum<TPR>(s3, red3, wave);
+        const float k1 = s3[0] * r1 / (float)c;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const float xh = cur.x[j] * r1;
+          o[j] = r1 * (h[j] * wm[j] - xh * k1);
+          acc[j] += h[j] * xh;
+        }
+      }
+      if (pos < run && a.dx) store_row<T, TPR, VEC>(static_cast<T*>(a.dx) + at, t, c, o);
+      cur = next;
+    }
+    if (sums) {
+      const int64_t p = ((int64_t)blockIdx.x * a.slots + slot) * SETS;
+      store_partial<TPR, VEC>(a.part + p * a.cp, sum, grp, t, c, acc);
+      if constexpr (SETS == 2) store_partial<TPR, VEC>(a.part + (p + 1) * a.cp, sum, grp, t, c, acc2);
+      if (a.doc && threadIdx.x == 0) a.part_id[(int64_t)blockIdx.x * a.slots + slot] = id;
+    }
+    done += run;
+    ++slot;
+    // the sums' slots and the list are read no more when the next run writes them
+    __syncthreads();
+  }
+  if (sums && a.doc)
+    for (int s = slot + (int)threadIdx.x; s < a.slots; s += kBwdNT) a.part_id[(int64_t)blockIdx.x * a.slots + s] = -1;
+}
+
+// The parameters' gradients from the partial rows.  blockIdx.y: set * (B * groups + 1) + job;
+// job < B * groups: dcond[b][g] = w * (sum of the partials of its id); the last job: dw =
+// sum over all partials of m * S.  A workgroup takes 64 channels (16 threads of 4), its 16
+// thread rows every 16th partial, added in order at the end.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_param_kernel(NormArgs a, int sets, int modulate) {
+  __shared__ f32x4 sum[16][16];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int jobs = a.b * a.groups + 1;
+  const int set = blockIdx.y / jobs, job = blockIdx.y - set * jobs;
+  const int col = blockIdx.x * 64 + tx * 4;
+  const bool dw = job == jobs - 1;
+  const int b = dw ? 0 : job / a.groups, g = dw ? 0 : job - b * a.groups;
+  const NormParam w = set ? a.w2 : a.w;
+  const NormCond k = set ? a.cond2 : a.cond;
+  void* dst = set ? (dw ? a.dw2 : a.dcond2) : (dw ? a.dw : a.dcond);
+  if (!dst) return;  // uniform over the workgroup
+  const bool scale = set || modulate;
+  auto param = [&](const void* p, bool f32, int64_t at) {
+    return f32 ? static_cast<const float*>(p)[at] : (float)static_cast<const T*>(p)[at];
+  };
+  f32x4 acc = {};
+  if (col < a.cp) {
+    const int64_t first = dw ? 0 : (int64_t)b * a.chunks, last = dw ? (int64_t)a.b * a.chunks : first + a.chunks;
+    for (int64_t q = first + ty; q < last; q += 16) {
+      for (int s = 0; s < a.slots; ++s) {
+        const int id = a.doc ? a.part_id[q * a.slots + s] : 0;
+        if (id < 0) break;
+        if (!dw && id != g) continue;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + ((q * a.slots + s) * sets + set) * a.cp + col);
+        if (!dw) {
+          acc += v;
+        } else {
+          const bool live = k.p && id < k.groups;
+          const int64_t off = live ? (q / a.chunks) * k.bs + id * k.gs : 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float m = live && col + j < a.c ? param(k.p, k.f32, off + col + j) : scale || k.p ? 0.0f : 1.0f;
+            acc[j] += (scale ? 1.0f + m : m) * v[j];
+          }
+        }
+      }
+    }
+  }
+  sum[ty][tx] = acc;
+  __syncthreads();
+  if (ty != 0) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) acc += sum[i][tx];
+  const bool f32 = dw ? w.f32 : k.f32;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int at = col + j;
+    if (at >= a.c) continue;
+    const float v = dw || !w.p ? acc[j] : acc[j] * param(w.p, w.f32, at);
+    const int64_t o = dw ? at : ((int64_t)b * a.groups + g) * a.c + at;
+    if (f32)
+      static_cast<float*>(dst)[o] = v;
+    else
+      static_cast<T*>(dst)[o] = (T)v;
+  }
+}
+
+// Whether every row of the call allows 16-byte accesses.
+bool all_vec(const NormArgs& a) {
+  bool ok = a.c % kVec == 0;
+  auto rows = [&](const NormRows& r) {
+    if (r.p)
+      ok = ok && (reinterpret_cast<uintptr_t>(r.p) & 15) == 0 && (a.b == 1 || r.bs % kVec == 0) &&
+           (a.n == 1 || r.rs % kVec == 0);
+  };
+  auto cond = [&](const NormCond& k) {
+    if (k.p)
+      ok = ok && (reinterpret_cast<uintptr_t>(k.p) & 15) == 0 && (a.b == 1 || k.bs % kVec == 0) &&
+           (k.groups == 1 || k.gs % kVec == 0);
+  };
+  auto ptr = [&](const void* p) { ok = ok && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  rows(a.x), rows(a.res), rows(a.dout), rows(a.dhidden);
+  cond(a.cond), cond(a.cond2);
+  ptr(a.w.p), ptr(a.w2.p);
+  ptr(a.out), ptr(a.hidden), ptr(a.dx), ptr(a.dres);
+  return ok;
+}
+
+template <typename T, int OP, int TPR, bool VEC>
+hipError_t fwd(const NormArgs& a, hipStream_t st) {
+  constexpr int NT = TPR > 256 ? TPR : 256, TOK = NT / TPR;
+  const int64_t rows = (int64_t)a.b * a.n;
+  norm_fwd_kernel<T, OP, TPR, VEC><<<(uint32_t)((rows + TOK - 1) / TOK), NT, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T, int OP, int TPR, bool VEC>
+hipError_t bwd(const NormArgs& a, hipStream_t st) {
+  norm_bwd_kernel<T, OP, TPR, VEC><<<(uint32_t)((int64_t)a.b * a.chunks), kBwdNT, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+template <bool BWD, typename T, int OP, int TPR>
+hipError_t pick_vec(const NormArgs& a, hipStream_t st) {
+  if (all_vec(a)) return BWD ? bwd<T, OP, TPR, true>(a, st) : fwd<T, OP, TPR, true>(a, st);
+  return BWD ? bwd<T, OP, TPR, false>(a, st) : fwd<T, OP, TPR, false>(a, st);
+}
+
+template <bool BWD, typename T, int OP>
+hipError_t pick_width(const NormArgs& a, hipStream_t st) {
+  if (a.c <= 64 * kPer) return pick_vec<BWD, T, OP, 64>(a, st);
+  if (a.c <= 256 * kPer) return pick_vec<BWD, T, OP, 256>(a, st);
+  return pick_vec<BWD, T, OP, 512>(a, st);
+}
+
+template <bool BWD, typename T>
+hipError_t pick_op(int op, const NormArgs& a, hipStream_t st) {
+  if (op == kNormModulate) return pick_width<BWD, T, kNormModulate>(a, st);
+  if (op == kNormGate) return pick_width<BWD, T, kNormGate>(a, st);
+  return pick_width<BWD, T, kNormGateModulate>(a, st);
+}
+
+}  // namespace
+
+NormChunks norm_chunks(int64_t b, int64_t n, int64_t c, int64_t groups, bool doc) {
+  const int64_t g = kBwdNT / (c <= 64 * kPer ? 64 : c <= 256 * kPer ? 256 : 512);
+  NormChunks k{};
+  // one workgroup a CU, at least two tokens a thread group, at most kBwdNT tokens
+  int64_t chunks = (256 + b - 1) / b;
+  if (chunks > (n + 2 * g - 1) / (2 * g)) chunks = (n + 2 * g - 1) / (2 * g);
+  if (chunks < (n + kBwdNT - 1) / kBwdNT) chunks = (n + kBwdNT - 1) / kBwdNT;
+  k.chunk = (n + chunks - 1) / chunks;
+  k.chunks = (n + k.chunk - 1) / k.chunk;
+  k.slots = !doc ? 1 : groups + 1 < k.chunk ? groups + 1 : k.chunk;
+  k.cp = (c + 3) / 4 * 4;
+  return k;
+}
+
+hipError_t launch_norm_fwd(int op, int f16, const NormArgs& a, hipStream_t st) {
+  return f16 ? pick_op<false, _Float16>(op, a, st) : pick_op<false, __bf16>(op, a, st);
+}
+
+hipError_t launch_norm_bwd(int op, int f16, const NormArgs& a, hipStream_t st) {
+  hipError_t e = f16 ? pick_op<true, _Float16>(op, a, st) : pick_op<true, __bf16>(op, a, st);
+  if (e != hipSuccess || !a.part) return e;
+  const int sets = op == kNormGateModulate ? 2 : 1;
+  const dim3 grid((uint32_t)((a.c + 63) / 64), (uint32_t)(sets * (a.b * a.groups + 1)));
+  if (f16)
+    norm_param_kernel<_Float16><<<grid, 256, 0, st>>>(a, sets, op == kNormModulate);
+  else
+    norm_param_kernel<__bf16><<<grid, 256, 0, st>>>(a, sets, op == kNormModulate);
+  return hipGetLastError();
+}
+
+}  // namespace sage

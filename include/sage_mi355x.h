@@ -388,6 +388,88 @@ int sage_attn_qk_accumulators(const void* q_codes, const float* q_scale,
                               void* out, float* lse, int32_t* s_out,
                               hipStream_t stream);
 
+/* ---- The norms around the attention of a transformer block --------------------
+ *
+ * xhat = x / sqrt(mean over c of x^2 + eps), per token of [B, N, C].
+ *   modulate:              out = xhat * weight * (1 + scale)
+ *   gate_residual:         out = residual + gate * xhat * weight
+ *   gate_residual_modulate: hidden = residual + gate * xhat * weight,
+ *                          out = (hidden's xhat) * next_weight * (1 + next_scale),
+ *                          hidden unrounded in the second norm
+ * fp32 arithmetic, one rounding per output.  No reference counterpart in the
+ * attention path (the reference's block applies them beside it).
+ *   dtype         SAGE_DTYPE_BF16 or SAGE_DTYPE_FP16: x, residual, out, hidden and
+ *                 their gradients.
+ *   *_bs, *_rs    element strides per batch item and token; channels contiguous.
+ *                 Outputs and gradients written are contiguous [B, N, C].
+ *   weight        [C] or null (ones).
+ *   scale, gate   rows [B, groups, C] with element strides *_bs, *_gs, or null (scale
+ *                 0, gate 1).  Without doc_ids groups is 1.
+ *   doc_ids       int32 [B, N] or null: the row of each token; a token whose id is
+ *                 below 0 or at least groups has scale 0 and gate 0.
+ *   fp32_params   bits SAGE_FP32_*: which parameters (and their gradients) are fp32;
+ *                 the others are of dtype.
+ *   c             at most 8192; b * n below 2^23, b * groups at most 32767.
+ * Rows from 16-byte boundaries with c a multiple of 8 take wide accesses; any
+ * other alignment is taken too. */
+#define SAGE_DTYPE_BF16 0
+#define SAGE_DTYPE_FP16 1
+#define SAGE_FP32_WEIGHT 1
+#define SAGE_FP32_COND 2
+#define SAGE_FP32_NEXT_WEIGHT 4
+#define SAGE_FP32_NEXT_SCALE 8
+
+int sage_rms_norm_modulate(const void* x, int64_t x_bs, int64_t x_rs, const void* weight,
+                           const void* scale, int64_t scale_bs, int64_t scale_gs, int64_t groups,
+                           const int32_t* doc_ids, int64_t b, int64_t n, int64_t c, int dtype,
+                           int fp32_params, float eps, void* out, hipStream_t stream);
+
+int sage_rms_norm_gate_residual(const void* residual, int64_t r_bs, int64_t r_rs,
+                                const void* x, int64_t x_bs, int64_t x_rs, const void* weight,
+                                const void* gate, int64_t gate_bs, int64_t gate_gs, int64_t groups,
+                                const int32_t* doc_ids, int64_t b, int64_t n, int64_t c, int dtype,
+                                int fp32_params, float eps, void* out, hipStream_t stream);
+
+int sage_rms_norm_gate_residual_modulate(
+    const void* residual, int64_t r_bs, int64_t r_rs, const void* x, int64_t x_bs, int64_t x_rs,
+    const void* weight, const void* gate, int64_t gate_bs, int64_t gate_gs, const void* next_weight,
+    const void* next_scale, int64_t scale_bs, int64_t scale_gs, int64_t groups, const int32_t* doc_ids,
+    int64_t b, int64_t n, int64_t c, int dtype, int fp32_params, float eps, void* hidden, void* out,
+    hipStream_t stream);
+
+/* Bytes of the workspace a backward of these norms needs when it forms gradients of
+ * parameters: fp32 channel sums of each chunk of tokens and document, and the ids they
+ * belong to.  with_doc_ids: whether the call gets document ids; fused: whether it is
+ * sage_rms_norm_gate_residual_modulate_bwd.  0 for sizes it refuses. */
+size_t sage_rms_norm_bwd_workspace_bytes(int64_t b, int64_t n, int64_t c, int64_t groups, int with_doc_ids,
+                                         int fused);
+
+/* Gradients.  dx (and dresidual) contiguous [B, N, C], dweight [C], dscale / dgate
+ * contiguous [B, groups, C].  dx and each parameter's gradient may be null (not wanted);
+ * with all parameters' null no workspace is needed.  The residual's gradient of
+ * gate_residual is dout itself.  Channel sums are added in a fixed order. */
+int sage_rms_norm_modulate_bwd(const void* dout, int64_t d_bs, int64_t d_rs, const void* x, int64_t x_bs,
+                               int64_t x_rs, const void* weight, const void* scale, int64_t scale_bs,
+                               int64_t scale_gs, int64_t groups, const int32_t* doc_ids, int64_t b, int64_t n,
+                               int64_t c, int dtype, int fp32_params, float eps, void* workspace,
+                               size_t workspace_bytes, void* dx, void* dweight, void* dscale, hipStream_t stream);
+
+int sage_rms_norm_gate_residual_bwd(const void* dout, int64_t d_bs, int64_t d_rs, const void* x, int64_t x_bs,
+                                    int64_t x_rs, const void* weight, const void* gate, int64_t gate_bs,
+                                    int64_t gate_gs, int64_t groups, const int32_t* doc_ids, int64_t b,
+                                    int64_t n, int64_t c, int dtype, int fp32_params, float eps, void* workspace,
+                                    size_t workspace_bytes, void* dx, void* dweight, void* dgate,
+                                    hipStream_t stream);
+
+int sage_rms_norm_gate_residual_modulate_bwd(
+    const void* dhidden, int64_t dh_bs, int64_t dh_rs, const void* dout, int64_t d_bs, int64_t d_rs,
+    const void* residual, int64_t r_bs, int64_t r_rs, const void* x, int64_t x_bs, int64_t x_rs,
+    const void* weight, const void* gate, int64_t gate_bs, int64_t gate_gs, const void* next_weight,
+    const void* next_scale, int64_t scale_bs, int64_t scale_gs, int64_t groups, const int32_t* doc_ids,
+    int64_t b, int64_t n, int64_t c, int dtype, int fp32_params, float eps, void* workspace,
+    size_t workspace_bytes, void* dresidual, void* dx, void* dweight, void* dgate, void* dnext_weight,
+    void* dnext_scale, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,317 @@
+"""GPU: the norms around the attention (futudiffu_amd/block_ops.py) against their 64-bit
+definition (oracle/block_oracle.py), outputs and every gradient.
+
+An error is measured in what is allowed: the bound on 32-bit arithmetic in any order, then
+one rounding to the output's type.
+"""
+
+import pytest
+import torch
+
+from oracle import block_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-5
+BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _ids(lengths, n, batch):
+    ids = torch.full((batch, n), -1, dtype=torch.int32)
+    for b in range(batch):
+        at = 0
+        for i, x in enumerate(lengths):
+            ids[b, at:at + x] = (i + b) % len(lengths)
+            at += x
+    return ids
+
+
+def _inputs(op, B, N, C, dtype, params, docs, seed=0):
+    """On the CPU; ``docs``: None, or (rows a batch item, ids [B, N])."""
+    g = torch.Generator().manual_seed(seed)
+
+    def normal(*shape, to=dtype, s=1.0, o=0.0):
+        return (o + s * torch.randn(*shape, generator=g)).to(to)
+
+    rows = (B, C) if docs is None else (B, docs[0], C)
+    v = dict(x=normal(B, N, C, s=1.5), weight=normal(C, to=params, s=0.3, o=1.0), cond=normal(*rows, to=params, s=0.5),
+             dout=normal(B, N, C))
+    if op != "modulate":
+        v["residual"] = normal(B, N, C, s=2.0)
+    if op == "gate_modulate":
+        v["next_weight"] = normal(C, to=params, s=0.3, o=1.0)
+        v["next_scale"] = normal(*rows, to=params, s=0.5)
+        v["dhidden"] = normal(B, N, C)
+    v["doc_ids"] = None if docs is None else docs[1]
+    return v
+
+
+ORDER = {"modulate": ("x", "weight", "cond"), "gate": ("residual", "x", "weight", "cond"),
+         "gate_modulate": ("residual", "x", "weight", "cond", "next_weight", "next_scale")}
+
+
+def _call(op, v, eps=EPS):
+    import futudiffu_amd as F
+    fn = {"modulate": F.rms_norm_modulate, "gate": F.rms_norm_gate_residual,
+          "gate_modulate": F.rms_norm_gate_residual_modulate}[op]
+    got = fn(*(v[k] for k in ORDER[op]), doc_ids=v["doc_ids"], eps=eps)
+    return {"hidden": got[0], "out": got[1]} if op == "gate_modulate" else {"out": got}
+
+
+def _with_grads(op, v, eps=EPS, leaves=None):
+    v = dict(v)
+    leaves = [k for k in (leaves or ORDER[op]) if v[k] is not None]
+    for k in leaves:
+        v[k] = v[k].detach().requires_grad_()
+    out = _call(op, v, eps)
+    names = ["out", "hidden"] if op == "gate_modulate" else ["out"]
+    grads = torch.autograd.grad([out[k] for k in names], [v[k] for k in leaves], [v["d" + k] for k in names])
+    out = {k: t.detach() for k, t in out.items()}
+    out.update({"d" + k: t for k, t in zip(leaves, grads)})
+    return out
+
+
+def _to(v, device):
+    return {k: None if t is None else t.to(device) for k, t in v.items()}
+
+
+def _want(op, v, eps=EPS):
+    want = O.norms(op, v["x"], v["weight"], v["cond"], v["doc_ids"], eps, v.get("residual"), v.get("next_weight"),
+                   v.get("next_scale"), v["dout"], v.get("dhidden"))
+    if op == "gate":
+        want["dresidual"] = (v["dout"].double(), torch.zeros_like(v["dout"], dtype=torch.float64))
+    return want
+
+
+def _check(got, want, case=""):
+    torch.cuda.synchronize()
+    for name, g in got.items():
+        exact, bound = want[name]
+        w = O.worst(g.cpu(), exact.cpu(), bound.cpu())
+        assert w <= 1.0, f"{case} {name}: {w:.3g} of what is allowed"
+
+
+SHAPES = [
+    (1, 1, 8), (1, 1, 1), (2, 3, 7), (1, 33, 64), (3, 17, 1000), (1, 65, 1001), (2, 130, 1024), (1, 9, 1032),
+    (2, 40, 3840), (1, 31, 3841), (1, 5, 4104), (1, 19, 8192), (2, 3, 8191), (1, 700, 72),
+]
+
+
+@pytest.mark.parametrize("B,N,C", SHAPES)
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_outputs_and_gradients(cuda, op, B, N, C):
+    """Every width class (one wave, four and eight a token; runs of eight channels and odd
+    widths), one conditioning row a batch item; both 16-bit types, fp32 parameters too."""
+    for dtype, params in ((BF, BF), (FP, F32)):
+        print(op, B, N, C, dtype, params, flush=True)
+        v = _inputs(op, B, N, C, dtype, params, None, seed=N + C)
+        got = _with_grads(op, _to(v, cuda))
+        assert all(got[k].dtype == dtype for k in ("out", "dx"))
+        assert got["dweight"].dtype == got["dcond"].dtype == params
+        _check(got, _want(op, v))
+        plain = _call(op, _to(v, cuda))  # without gradients: the same bits
+        for k, t in plain.items():
+            assert torch.equal(t.view(torch.int16), got[k].view(torch.int16))
+
+
+DOCS = [
+    (1, 300, 256, (100, 150), "contiguous"),      # 50 tokens of no document at the end
+    (2, 1100, 72, (500, 333, 267), "contiguous"),  # rotated rows in the second batch item
+    (1, 97, 3840, (40, 57), "contiguous"),
+    (1, 600, 136, (600,), "interleaved"),          # 5 documents in turn: every chunk holds them all
+    (1, 50, 1001, (1,) * 50, "contiguous"),        # a document a token
+    (1, 64, 64, (), "contiguous"),                 # no token has a document
+    (1, 64, 64, (64,), "outside"),                 # ids beyond the rows, and below 0
+]
+
+
+@pytest.mark.parametrize("B,N,C,lengths,kind", DOCS)
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_documents(cuda, op, B, N, C, lengths, kind):
+    if kind == "interleaved":
+        rows, ids = 5, (torch.arange(N, dtype=torch.int32) % 5).expand(B, N).contiguous()
+    elif kind == "outside":
+        rows, ids = 2, torch.tensor([0, 5, -7, 1, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32).repeat(B, 11)[:, :N].contiguous()
+    else:
+        rows, ids = max(1, len(lengths)), _ids(lengths, N, B)
+    for dtype, params in ((BF, F32), (FP, FP)):
+        print(op, B, N, C, kind, dtype, flush=True)
+        v = _inputs(op, B, N, C, dtype, params, (rows, ids), seed=C)
+        _check(_with_grads(op, _to(v, cuda)), _want(op, v))
+
+
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_absent_parameters(cuda, op):
+    """No weight (ones), no scale (0), no gate (1); gradients of the rest alone."""
+    for keep in ((), ("weight",), ("cond",), ("next_weight",), ("next_scale",)):
+        if op != "gate_modulate" and keep and keep[0].startswith("next"):
+            continue
+        v = _inputs(op, 2, 21, 520, BF, BF, None, seed=5)
+        want = {k: None if k in ("weight", "cond", "next_weight", "next_scale") and k not in keep else t
+                for k, t in v.items()}
+        print(op, keep, flush=True)
+        _check(_with_grads(op, _to(want, cuda)), _want(op, want))
+
+
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_strides_and_alignment(cuda, op):
+    """Views: a channel slice of a wider tensor, an offset of one element, transposed
+    channels, expanded conditioning rows, chunks of one projection; the rows around the
+    outputs stay as they were (fresh tensors)."""
+    B, N, C = 2, 37, 264
+    v = _to(_inputs(op, B, N, C, BF, BF, None, seed=9), cuda)
+    want = _want(op, {k: None if t is None else t.cpu() for k, t in v.items()})
+    ref = _with_grads(op, v)
+    _check(ref, want)
+
+    def wide(t, off):
+        w = torch.zeros(*t.shape[:-1], C + 40, dtype=t.dtype, device=t.device)
+        w[..., off:off + C] = t
+        return w[..., off:off + C]
+
+    def swapped(t):
+        return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+    tokens = [k for k in ("x", "residual", "dout", "dhidden") if k in v]
+    for name, how in (("wide", lambda t: wide(t, 8)), ("offset", lambda t: wide(t, 1)), ("swapped", swapped),
+                      ("batch-strided", lambda t: torch.stack([t, t], 1)[:, 0])):
+        u = dict(v, **{k: how(v[k]) for k in tokens})
+        got = _with_grads(op, u)
+        print(op, name, flush=True)
+        _check(got, want, name)
+    conds = [k for k in ("cond", "next_scale") if k in v]
+    proj = torch.cat([v[k] for k in conds] * 2, -1)
+    u = dict(v, **dict(zip(conds, proj.chunk(2 * len(conds), -1))))
+    _check(_with_grads(op, u), want, "chunks")
+    u = dict(v, **{k: v[k][:1].expand(B, C) for k in conds})
+    _check(_with_grads(op, u), _want(op, {k: None if t is None else t.cpu() for k, t in u.items()}), "expanded")
+
+
+def test_two_dimensional_and_empty(cuda):
+    import futudiffu_amd as F
+    v = _to(_inputs("gate_modulate", 1, 11, 96, BF, BF, None, seed=2), cuda)
+    three = _call("gate_modulate", v)
+    flat = {k: t[0] if k in ("x", "residual") else t for k, t in v.items() if t is not None}
+    two = _call("gate_modulate", dict(flat, doc_ids=None))
+    assert all(torch.equal(two[k], three[k][0]) for k in two)
+    ids = torch.zeros(11, dtype=torch.int64, device=cuda)
+    got = F.rms_norm_modulate(flat["x"], flat["weight"], v["cond"][:, None], doc_ids=ids)
+    assert torch.equal(got, F.rms_norm_modulate(v["x"], v["weight"], v["cond"])[0])
+    for op in ORDER:
+        for B, N in ((1, 0), (0, 4)):
+            e = _to(_inputs(op, B, N, 96, BF, BF, None), cuda)
+            got = _with_grads(op, e)
+            assert got["out"].shape == (B, N, 96) and got["dx"].shape == (B, N, 96)
+            assert not got["dweight"].any() and got["dcond"].shape == (B, 96) and not got["dcond"].any()
+
+
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_not_finite_and_zero_rows(cuda, op):
+    """A token with an infinity or NaN spoils its own row alone; a row of zeros is fine."""
+    v = _inputs(op, 1, 40, 256, BF, BF, None, seed=3)
+    clean = _call(op, _to(v, cuda))
+    bad = dict(v, x=v["x"].clone())
+    bad["x"][0, 3, 7] = float("inf")
+    bad["x"][0, 5, 9] = float("nan")
+    bad["x"][0, 8] = 0
+    got = _call(op, _to(bad, cuda))
+    for k in got:
+        g, c = got[k][0].float(), clean[k][0].float()
+        assert torch.isnan(g[3]).any() and torch.isnan(g[5]).all()
+        keep = [i for i in range(40) if i not in (3, 5, 8)]
+        assert torch.equal(g[keep], c[keep]) and torch.isfinite(g[8]).all()
+        if k != "out" or op == "gate":
+            assert torch.equal(got[k][0, 8], v["residual"][0, 8].to(got[k].device))
+
+
+def test_gradients_against_differences(cuda):
+    """Central differences of the operator itself along random directions, in fp32 sums of
+    fp16 outputs: the step is 2^-4 of the inputs' scale, so the difference's own error is the
+    outputs' rounding (half a step of 2^-11 each, independent, over a sum of their squares)
+    and the third-order term."""
+    op = "gate_modulate"
+    v = _inputs(op, 1, 64, 128, FP, F32, (2, _ids((30, 30), 64, 1)), seed=11)
+    d = _to(v, cuda)
+    got = _with_grads(op, d)
+    g = torch.Generator().manual_seed(1)
+    for leaf in ("weight", "cond", "next_weight", "next_scale"):
+        step = torch.randn(v[leaf].shape, generator=g).to(cuda) * 2.0 ** -4
+        hi, lo = (_call(op, dict(d, **{leaf: d[leaf] + s * step})) for s in (1, -1))
+        num = sum(((hi[k].double() - lo[k].double()) * d["d" + k].double()).sum() for k in hi) / 2
+        ana = (got["d" + leaf].double() * step.double()).sum()
+        # each output is off by at most 2^-11 of itself (both sides), summed in quadrature x 4
+        noise = 4 * sum(((hi[k].double() * 2.0 ** -11 * d["d" + k].double()) ** 2).sum() for k in hi).sqrt()
+        cubic = 0.0
+        if leaf in ("weight", "cond"):  # out depends on them through the second norm
+            half = [_call(op, dict(d, **{leaf: d[leaf] + s * step / 2})) for s in (1, -1)]
+            num2 = sum(((half[0][k].double() - half[1][k].double()) * d["d" + k].double()).sum() for k in hi)
+            cubic = abs(float(num - num2)) * 4 / 3
+        assert abs(float(num - ana)) <= float(noise) + cubic, (leaf, float(num), float(ana), float(noise), cubic)
+
+
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_repeatable_and_partial_gradients(cuda, op):
+    """The same bits every time, and whichever gradients are asked for."""
+    v = _to(_inputs(op, 2, 333, 1024, BF, F32, (3, _ids((100, 100, 133), 333, 2)), seed=4), cuda)
+    ref = _with_grads(op, v)
+    for _ in range(3):
+        again = _with_grads(op, v)
+        assert all(torch.equal(again[k], ref[k]) for k in ref)
+    for leaf in ORDER[op]:
+        one = _with_grads(op, v, leaves=(leaf,))
+        assert torch.equal(one["d" + leaf], ref["d" + leaf]), leaf
+
+
+def test_other_stream_and_overlapping_calls(cuda):
+    v = _to(_inputs("gate_modulate", 1, 500, 2048, BF, BF, None, seed=6), cuda)
+    u = _to(_inputs("gate_modulate", 1, 480, 1536, BF, BF, None, seed=7), cuda)
+    ref, ref_u = _with_grads("gate_modulate", v), _with_grads("gate_modulate", u)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            a = _with_grads("gate_modulate", v)
+        with torch.cuda.stream(s2):
+            b = _with_grads("gate_modulate", u)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a[k], ref[k]) for k in ref) and all(torch.equal(b[k], ref_u[k]) for k in ref_u)
+
+
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_captured_step_replays(cuda, op):
+    """Forward and backward in one graph, replayed on new inputs between eager work."""
+    ids = _ids((100, 150), 300, 1)
+    v = _to(_inputs(op, 1, 300, 512, BF, BF, (2, ids), seed=8), cuda)
+    static = {k: None if t is None else t.clone() for k, t in v.items()}
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        _with_grads(op, static)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = _with_grads(op, static)
+    for seed in (20, 21, 22):
+        new = _to(_inputs(op, 1, 300, 512, BF, BF, (2, ids), seed=seed), cuda)
+        for k, t in new.items():
+            if t is not None:
+                static[k].copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _with_grads(op, new)
+        assert all(torch.equal(got[k], want[k]) for k in want), [k for k in want if not torch.equal(got[k], want[k])]
+
+
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_ops_check_and_compile(cuda, op):
+    name = {"modulate": "rms_norm_modulate", "gate": "rms_norm_gate_residual",
+            "gate_modulate": "rms_norm_gate_residual_modulate"}[op]
+    v = _to(_inputs(op, 2, 20, 136, BF, F32, (2, _ids((8, 9), 20, 2)), seed=1), cuda)
+    args = [v[k].requires_grad_() for k in ORDER[op]] + [v["doc_ids"], EPS]
+    torch.library.opcheck(getattr(torch.ops.futudiffu_ii, name).default, tuple(args),
+                          test_utils=("test_schema", "test_autograd_registration", "test_faketensor",
+                                      "test_aot_dispatch_static"))
+    want = _with_grads(op, v)
+    compiled = torch.compile(lambda *a: tuple(_call(op, dict(v, **dict(zip(ORDER[op], a)))).values()),
+                             backend="aot_eager", fullgraph=True)
+    got = compiled(*(v[k].detach().requires_grad_() for k in ORDER[op]))
+    assert all(torch.equal(a, b) for a, b in zip(got, (want[k] for k in (["hidden", "out"] if op == "gate_modulate" else ["out"]))))
