@@ -11,14 +11,13 @@ per output.  ``x`` is ``[B, N, C]`` (or ``[N, C]``), bfloat16 or float16, with a
 and ``gate`` have a row per batch item, ``[B, C]``, or with ``doc_ids`` (int32 ``[B, N]``,
 as :func:`futudiffu_amd.build_doc_ids` makes them) a row per document of a packed
 sequence, ``[B, G, C]``: a token whose id is not in ``0 .. G-1`` (padding) has scale 0 and
-gate 0.  Parameters are of ``x``'s type or float32; chunks of one projection's output are
+gate 0, and behind a gate its ``x`` is not read.  Parameters are of ``x``'s type or float32; chunks of one projection's output are
 read in place.
 
-The functions differentiate: where a gradient is wanted, or under ``torch.compile``,
-they go through the custom ops ``futudiffu_ii::rms_norm_modulate``,
-``::rms_norm_gate_residual`` and ``::rms_norm_gate_residual_modulate``, whose gradients
-are ops of their own; channel sums are added in a fixed order, so gradients repeat bit
-for bit.  An empty batch gives empty outputs and zero parameter gradients.
+The functions differentiate.  Under ``torch.compile`` they go through the custom ops
+``futudiffu_ii::rms_norm_modulate``, ``::rms_norm_gate_residual`` and
+``::rms_norm_gate_residual_modulate``, which carry the same gradients.  Channel sums are
+added in a fixed order, so gradients repeat bit for bit.  An empty batch gives empty outputs and zero parameter gradients.
 """
 
 from __future__ import annotations
@@ -27,6 +26,7 @@ import contextlib
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .sage_attention import _ptr, _stream_handle
@@ -35,11 +35,12 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _ops = torch.library.Library("futudiffu_ii", "FRAGMENT")
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """The library launches on the current device: make it ``device``."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _tokens(name: str, t: Tensor, like: Tensor | None = None) -> Tensor:
@@ -109,10 +110,12 @@ def _f32(*params: Tensor | None) -> int:
     return sum(1 << i for i, p in enumerate(params) if p is not None and p.dtype == torch.float32)
 
 
-def _through_op(*tensors: Tensor | None) -> bool:
-    if torch.compiler.is_compiling():
-        return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _wants_grad(*tensors: Tensor | None) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 class _Norm:
@@ -355,21 +358,73 @@ torch.library.register_autograd("futudiffu_ii::rms_norm_gate_residual_modulate",
                                 setup_context=_gate_modulate_setup, lib=_ops)
 
 
+class _Modulate(torch.autograd.Function):
+    """The op and its formula without the dispatch of a Python op, which takes the host longer
+    than a step's kernels take the GPU."""
+
+    @staticmethod
+    def forward(ctx, *inputs):
+        _modulate_setup(ctx, inputs, None)
+        return _modulate_forward(*inputs)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, weight, scale, doc_ids = ctx.saved_tensors
+        return *_norm_backward("sage_rms_norm_modulate_bwd", "scale", dout, x, weight, scale, doc_ids, ctx.eps,
+                               ctx.needs_input_grad[:3]), None, None
+
+
+class _Gate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *inputs):
+        _gate_setup(ctx, inputs, None)
+        return _gate_forward(*inputs)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, weight, gate, doc_ids = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return (dout if need[0] else None, *_norm_backward(
+            "sage_rms_norm_gate_residual_bwd", "gate", dout, x, weight, gate, doc_ids, ctx.eps, need[1:4]), None, None)
+
+
+class _GateModulate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *inputs):
+        _gate_modulate_setup(ctx, inputs, None)
+        return _gate_modulate_forward(*inputs)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dhidden, dout):
+        residual, x, weight, gate, next_weight, next_scale, doc_ids = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        grads = _gate_modulate_backward(dhidden, dout, residual, x, weight, gate, next_weight, next_scale, doc_ids,
+                                        ctx.eps, need[:6])
+        return *_only(grads, need), None, None
+
+
 # ---- the functions ---------------------------------------------------------------------
 
 def rms_norm_modulate(x: Tensor, weight: Tensor | None = None, scale: Tensor | None = None, *,
                       doc_ids: Tensor | None = None, eps: float = 1e-5) -> Tensor:
     """``xhat * weight * (1 + scale)``: the norm before a block with its modulation."""
-    if _through_op(x, weight, scale):
+    if torch.compiler.is_compiling():
         return torch.ops.futudiffu_ii.rms_norm_modulate(x, weight, scale, doc_ids, eps)
+    if _wants_grad(x, weight, scale):
+        return _Modulate.apply(x, weight, scale, doc_ids, eps)
     return _modulate_forward(x, weight, scale, doc_ids, eps)
 
 
 def rms_norm_gate_residual(residual: Tensor, x: Tensor, weight: Tensor | None = None, gate: Tensor | None = None, *,
                            doc_ids: Tensor | None = None, eps: float = 1e-5) -> Tensor:
     """``residual + gate * xhat * weight``: the norm after a block, gated, onto the residual."""
-    if _through_op(residual, x, weight, gate):
+    if torch.compiler.is_compiling():
         return torch.ops.futudiffu_ii.rms_norm_gate_residual(residual, x, weight, gate, doc_ids, eps)
+    if _wants_grad(residual, x, weight, gate):
+        return _Gate.apply(residual, x, weight, gate, doc_ids, eps)
     return _gate_forward(residual, x, weight, gate, doc_ids, eps)
 
 
@@ -383,7 +438,9 @@ def rms_norm_gate_residual_modulate(residual: Tensor, x: Tensor, weight: Tensor 
     The second norm takes ``hidden`` unrounded: ``out`` is nearer the exact value than the
     two calls' one after the other, which normalize the rounded ``hidden``.
     """
-    if _through_op(residual, x, weight, gate, next_weight, next_scale):
+    if torch.compiler.is_compiling():
         return torch.ops.futudiffu_ii.rms_norm_gate_residual_modulate(residual, x, weight, gate, next_weight,
                                                                       next_scale, doc_ids, eps)
+    if _wants_grad(residual, x, weight, gate, next_weight, next_scale):
+        return _GateModulate.apply(residual, x, weight, gate, next_weight, next_scale, doc_ids, eps)
     return _gate_modulate_forward(residual, x, weight, gate, next_weight, next_scale, doc_ids, eps)

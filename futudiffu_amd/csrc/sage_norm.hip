@@ -99,25 +99,24 @@ struct Cols {
   }
 };
 
-// One thread's channels of a row of T, as they lie in memory (loads issue here, the
-// conversion follows when the values are used).  Channels past c are zeros.
+// Rows are read and written through a buffer resource that ends at the row's last
+// channel: reads past it give zeros and writes past it are dropped, so no access is
+// behind a branch.  A row is uniform over a wave.  One thread's channels of a row of T
+// stay as they lie in memory until they are used.
 template <typename T, int TPR, bool VEC>
 struct Raw {
   using V = typename Vec8<T>::type;
   V v[kPer / kVec];
   __device__ __forceinline__ void load(const T* row, int t, int c) {
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(row, (uint32_t)c * 2);
     if constexpr (VEC) {
 #pragma unroll
-      for (int i = 0; i < kPer / kVec; ++i) {
-        const int at = (i * TPR + t) * kVec;
-        v[i] = at < c ? *reinterpret_cast<const V*>(row + at) : V{};
-      }
+      for (int i = 0; i < kPer / kVec; ++i)
+        v[i] = __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(rs, (i * TPR + t) * kVec * 2, 0, 0));
     } else {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int at = j * TPR + t;
-        v[j / kVec][j % kVec] = at < c ? row[at] : (T)0.0f;
-      }
+      for (int j = 0; j < kPer; ++j)
+        v[j / kVec][j % kVec] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(rs, (j * TPR + t) * 2, 0, 0));
     }
   }
   __device__ __forceinline__ float operator[](int j) const { return (float)v[j / kVec][j % kVec]; }
@@ -125,22 +124,20 @@ struct Raw {
 
 template <typename T, int TPR, bool VEC>
 __device__ __forceinline__ void store_row(T* row, int t, int c, const float (&f)[kPer]) {
+  const __amdgpu_buffer_rsrc_t rs = raw_rsrc(row, (uint32_t)c * 2);
   if constexpr (VEC) {
     using V = typename Vec8<T>::type;
 #pragma unroll
     for (int i = 0; i < kPer / kVec; ++i) {
-      const int at = (i * TPR + t) * kVec;
       V o;
 #pragma unroll
       for (int j = 0; j < kVec; ++j) o[j] = (T)f[i * kVec + j];
-      if (at < c) *reinterpret_cast<V*>(row + at) = o;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rs, (i * TPR + t) * kVec * 2, 0, 0);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int at = j * TPR + t;
-      if (at < c) row[at] = (T)f[j];
-    }
+    for (int j = 0; j < kPer; ++j)
+      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (T)f[j]), rs, (j * TPR + t) * 2, 0, 0);
   }
 }
 
@@ -152,21 +149,19 @@ __device__ __forceinline__ void load_param(const void* p, bool f32, int64_t off,
 #pragma unroll
     for (int j = 0; j < kPer; ++j) f[j] = fill;
   } else if (f32) {
-    const float* row = static_cast<const float*>(p) + off;
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(static_cast<const float*>(p) + off, (uint32_t)c * 4);
     if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < kPer / 4; ++i) {
         const int at = Cols<TPR, VEC>::col(t, i * 4);
-        const f32x4 v = at < c ? *reinterpret_cast<const f32x4*>(row + at) : f32x4{};
+        const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at * 4, 0, 0));
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[i * 4 + j] = v[j];
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int at = Cols<TPR, VEC>::col(t, j);
-        f[j] = at < c ? row[at] : 0.0f;
-      }
+      for (int j = 0; j < kPer; ++j)
+        f[j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, Cols<TPR, VEC>::col(t, j) * 4, 0, 0));
     }
   } else {
     Raw<T, TPR, VEC> r;
@@ -198,6 +193,12 @@ __device__ __forceinline__ const T* row_of(const NormRows& r, int b, int64_t n) 
   return static_cast<const T*>(r.p) + b * r.bs + n * r.rs;
 }
 
+// A token of no document behind a gate: its x is not read (whatever padding holds there
+// reaches neither the output nor a gradient), xhat is 0.
+__device__ __forceinline__ bool no_document(const NormArgs& a, int id) {
+  return a.doc && a.cond.p && (id < 0 || id >= a.groups);
+}
+
 // Forward: TPR threads a token, one token a thread group.  All loads of a token, the
 // parameter rows included, are issued before its first sum.
 template <typename T, int OP, int TPR, bool VEC>
@@ -206,15 +207,16 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(NormArg
   constexpr int TOK = NT / TPR;
   __shared__ float red[NT / 64], red2[NT / 64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * TOK + threadIdx.x / TPR, rows = (int64_t)a.b * a.n;
+  const int64_t row = (int64_t)blockIdx.x * TOK + wave / (TPR / 64), rows = (int64_t)a.b * a.n;
   const bool live = row < rows;  // a thread group past the last token takes part in the barriers alone
   const int b = live ? (int)(row / a.n) : 0;
   const int64_t n = live ? row - (int64_t)b * a.n : 0;
   const int c = live ? a.c : 0;
   Raw<T, TPR, VEC> x, r;
-  x.load(row_of<T>(a.x, b, n), t, c);
+  const int id = a.doc && live ? load_uniform(a.doc, row) : 0;
+  const bool gated = OP == kNormModulate || !no_document(a, id);
+  x.load(row_of<T>(a.x, b, n), t, gated ? c : 0);
   if constexpr (OP != kNormModulate) r.load(row_of<T>(a.res, b, n), t, c);
-  const int id = a.doc && live ? a.doc[row] : 0;
   float wm[kPer], wm2[kPer];
   weight_row<T, TPR, VEC>(a.w, a.cond, OP == kNormModulate, b, id, t, c, wm);
   if constexpr (OP == kNormGateModulate) weight_row<T, TPR, VEC>(a.w2, a.cond2, true, b, id, t, c, wm2);
@@ -222,7 +224,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(NormArg
 #pragma unroll
   for (int j = 0; j < kPer; ++j) s[0] += x[j] * x[j];
   token_sum<TPR>(s, red, wave);
-  const float rr = rrms(s[0], a.c, a.eps);
+  const float rr = gated ? rrms(s[0], a.c, a.eps) : 0.0f;
   float y[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
@@ -248,8 +250,8 @@ constexpr int kBwdNT = 512;  // threads of a backward workgroup; also the most t
 template <typename T, int OP, int TPR, bool VEC>
 struct BwdRow {
   Raw<T, TPR, VEC> x, d, r, dh;  // r, dh: gate_modulate alone
-  __device__ __forceinline__ void load(const NormArgs& a, int b, int64_t n, int t, int c) {
-    x.load(row_of<T>(a.x, b, n), t, c);
+  __device__ __forceinline__ void load(const NormArgs& a, int b, int64_t n, int t, int c, bool gated) {
+    x.load(row_of<T>(a.x, b, n), t, gated ? c : 0);
     d.load(row_of<T>(a.dout, b, n), t, c);
     if constexpr (OP == kNormGateModulate) {
       r.load(row_of<T>(a.res, b, n), t, c);
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
   __shared__ int ids_min[W], counts[W];
   __shared__ uint16_t list[kBwdNT];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR, grp = wave / (TPR / 64);
   const int b = blockIdx.x / a.chunks;
   const int64_t n0 = (int64_t)(blockIdx.x % a.chunks) * a.chunk;
   const int len = (int)(a.n - n0 < a.chunk ? a.n - n0 : a.chunk);
@@ -319,7 +321,7 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
   }
   while (done < len) {
     // the next run: its id and its tokens
-    int id = 0, run = len;
+    int id = 0, run = len;  // uniform
     if (a.doc) {
       int least = my > prev ? my : 0x7fffffff;
 #pragma unroll
@@ -329,6 +331,7 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
       id = ids_min[0];
 #pragma unroll
       for (int w = 1; w < W; ++w) id = min(id, ids_min[w]);
+      id = __builtin_amdgcn_readfirstlane(id);
       const uint64_t mine = __ballot(my == id);
       if (lane == 0) counts[wave] = __popcll(mine);
       __syncthreads();
@@ -339,6 +342,7 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
         before += w < wave ? counts[w] : 0;
         run += counts[w];
       }
+      run = __builtin_amdgcn_readfirstlane(run);
       if (my == id) list[before + __popcll(mine & ((1ull << lane) - 1))] = (uint16_t)threadIdx.x;
       prev = id;
       __syncthreads();
@@ -347,17 +351,19 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
     weight_row<T, TPR, VEC>(a.w, a.cond, kScale, b, id, t, c, wm);
     if constexpr (SETS == 2) weight_row<T, TPR, VEC>(a.w2, a.cond2, true, b, id, t, c, wm2);
 
+    const bool gated = kScale || !no_document(a, id);
     BwdRow<T, OP, TPR, VEC> cur, next;
-    auto token = [&](int pos) { return n0 + (a.doc ? (int)list[pos] : pos); };
+    auto token = [&](int pos) { return n0 + (a.doc ? __builtin_amdgcn_readfirstlane(list[pos]) : pos); };
     // a group past its last token loads nothing (its channels are zeros)
-    cur.load(a, b, grp < run ? token(grp) : n0, t, grp < run ? c : 0);
+    cur.load(a, b, grp < run ? token(grp) : n0, t, grp < run ? c : 0, gated);
     const int iters = (run + G - 1) / G;
 #pragma unroll 1
     for (int it = 0; it < iters; ++it) {
       const int pos = it * G + grp, npos = pos + G;
       const int64_t n = pos < run ? token(pos) : n0;
-      if (it + 1 < iters) next.load(a, b, npos < run ? token(npos) : n0, t, npos < run ? c : 0);
+      if (it + 1 < iters) next.load(a, b, npos < run ? token(npos) : n0, t, npos < run ? c : 0, gated);
       const int64_t at = ((int64_t)b * a.n + n) * c;
+      const bool has = gated && pos < run;  // zeros else, whose norm is not formed (infinite where eps is 0)
       float o[kPer];
       if constexpr (OP != kNormGateModulate) {
         float s[2] = {0.0f, 0.0f};
@@ -367,7 +373,7 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
           s[1] += cur.d[j] * wm[j] * cur.x[j];
         }
         token_sum<TPR>(s, red[it & 1], wave);
-        const float r = rrms(s[0], c, a.eps), k = s[1] * r / (float)c;
+        const float r = has ? rrms(s[0], c, a.eps) : 0.0f, k = s[1] * r / (float)c;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
           const float xh = cur.x[j] * r;
@@ -379,7 +385,7 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
 #pragma unroll
         for (int j = 0; j < kPer; ++j) s1[0] += cur.x[j] * cur.x[j];
         token_sum<TPR>(s1, red1, wave);
-        const float r1 = rrms(s1[0], c, a.eps);
+        const float r1 = has ? rrms(s1[0], c, a.eps) : 0.0f;
         float s[2] = {0.0f, 0.0f};
         float h[kPer];
 #pragma unroll
@@ -389,7 +395,7 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
           s[1] += cur.d[j] * wm2[j] * h[j];
         }
         token_sum<TPR>(s, red[it & 1], wave);
-        const float r2 = rrms(s[0], c, a.eps), k2 = s[1] * r2 / (float)c;
+        const float r2 = pos < run ? rrms(s[0], c, a.eps) : 0.0f, k2 = s[1] * r2 / (float)c;
         float s3[1] = {0.0f};
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
@@ -428,11 +434,15 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
 
 // The parameters' gradients from the partial rows.  blockIdx.y: set * (B * groups + 1) + job;
 // job < B * groups: dcond[b][g] = w * (sum of the partials of its id); the last job: dw =
-// sum over all partials of m * S.  A workgroup takes 64 channels (16 threads of 4), its 16
-// thread rows every 16th partial, added in order at the end.
+// sum over all partials of m * S.  A workgroup takes 64 channels (16 threads of 4), its 32
+// thread rows every 32nd chunk, added in order at the end.  The loads of kBatch chunks are
+// in flight together: with one chunk at a time and 16 thread rows the kernel took 22 us
+// at 256 chunks of 3840 channels, all of it latency.
+constexpr int kParamRows = 32, kBatch = 4;
+
 template <typename T>
-__global__ __launch_bounds__(256) void norm_param_kernel(NormArgs a, int sets, int modulate) {
-  __shared__ f32x4 sum[16][16];
+__global__ __launch_bounds__(16 * kParamRows) void norm_param_kernel(NormArgs a, int sets, int modulate) {
+  __shared__ f32x4 sum[kParamRows][16];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int jobs = a.b * a.groups + 1;
   const int set = blockIdx.y / jobs, job = blockIdx.y - set * jobs;
@@ -447,25 +457,53 @@ __global__ __launch_bounds__(256) void norm_param_kernel(NormArgs a, int sets, i
   auto param = [&](const void* p, bool f32, int64_t at) {
     return f32 ? static_cast<const float*>(p)[at] : (float)static_cast<const T*>(p)[at];
   };
+  // what a partial of id at chunk q counts for: its m (dw), or 1 or nothing
+  auto factor = [&](int q, int id) {
+    f32x4 m = {};
+    if (!dw) {
+      m += id == g ? 1.0f : 0.0f;
+    } else {
+      const bool live = k.p && id < k.groups;
+      const int64_t off = live ? (q / a.chunks) * k.bs + id * k.gs : 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m[j] = live && col + j < a.c ? param(k.p, k.f32, off + col + j) : scale || k.p ? 0.0f : 1.0f;
+        if (scale) m[j] += 1.0f;
+      }
+    }
+    return m;
+  };
+  auto partial = [&](int64_t q, int s) {
+    return *reinterpret_cast<const f32x4*>(a.part + ((q * a.slots + s) * sets + set) * a.cp + col);
+  };
   f32x4 acc = {};
   if (col < a.cp) {
-    const int64_t first = dw ? 0 : (int64_t)b * a.chunks, last = dw ? (int64_t)a.b * a.chunks : first + a.chunks;
-    for (int64_t q = first + ty; q < last; q += 16) {
-      for (int s = 0; s < a.slots; ++s) {
-        const int id = a.doc ? a.part_id[q * a.slots + s] : 0;
-        if (id < 0) break;
-        if (!dw && id != g) continue;
-        const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + ((q * a.slots + s) * sets + set) * a.cp + col);
-        if (!dw) {
-          acc += v;
-        } else {
-          const bool live = k.p && id < k.groups;
-          const int64_t off = live ? (q / a.chunks) * k.bs + id * k.gs : 0;
+    const int first = dw ? 0 : b * a.chunks, last = dw ? a.b * a.chunks : first + a.chunks;
+    for (int q0 = first + ty; q0 < last; q0 += kParamRows * kBatch) {
+      int id[kBatch], id1[kBatch];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float m = live && col + j < a.c ? param(k.p, k.f32, off + col + j) : scale || k.p ? 0.0f : 1.0f;
-            acc[j] += (scale ? 1.0f + m : m) * v[j];
-          }
+      for (int i = 0; i < kBatch; ++i) {
+        const int q = q0 + i * kParamRows;
+        id[i] = q >= last ? -1 : a.doc ? a.part_id[(int64_t)q * a.slots] : 0;
+        id1[i] = q < last && a.slots > 1 ? a.part_id[(int64_t)q * a.slots + 1] : -1;
+      }
+      f32x4 v[kBatch], m[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int q = q0 + i * kParamRows;
+        const bool use = id[i] >= 0 && (dw || id[i] == g);
+        v[i] = use ? partial(q, 0) : f32x4{};
+        m[i] = use ? factor(q, id[i]) : f32x4{};
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int q = q0 + i * kParamRows;
+        acc += m[i] * v[i];
+        // the other documents of a chunk that holds several
+        for (int s = 1, d = id1[i]; d >= 0;) {
+          if (dw || d == g) acc += factor(q, d) * partial(q, s);
+          ++s;
+          d = s < a.slots ? a.part_id[(int64_t)q * a.slots + s] : -1;
         }
       }
     }
@@ -474,7 +512,7 @@ __global__ __launch_bounds__(256) void norm_param_kernel(NormArgs a, int sets, i
   __syncthreads();
   if (ty != 0) return;
 #pragma unroll
-  for (int i = 1; i < 16; ++i) acc += sum[i][tx];
+  for (int i = 1; i < kParamRows; ++i) acc += sum[i][tx];
   const bool f32 = dw ? w.f32 : k.f32;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -570,9 +608,9 @@ hipError_t launch_norm_bwd(int op, int f16, const NormArgs& a, hipStream_t st) {
   const int sets = op == kNormGateModulate ? 2 : 1;
   const dim3 grid((uint32_t)((a.c + 63) / 64), (uint32_t)(sets * (a.b * a.groups + 1)));
   if (f16)
-    norm_param_kernel<_Float16><<<grid, 256, 0, st>>>(a, sets, op == kNormModulate);
+    norm_param_kernel<_Float16><<<grid, 16 * kParamRows, 0, st>>>(a, sets, op == kNormModulate);
   else
-    norm_param_kernel<__bf16><<<grid, 256, 0, st>>>(a, sets, op == kNormModulate);
+    norm_param_kernel<__bf16><<<grid, 16 * kParamRows, 0, st>>>(a, sets, op == kNormModulate);
   return hipGetLastError();
 }
 

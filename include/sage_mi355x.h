@@ -406,7 +406,8 @@ int sage_attn_qk_accumulators(const void* q_codes, const float* q_scale,
  *   scale, gate   rows [B, groups, C] with element strides *_bs, *_gs, or null (scale
  *                 0, gate 1).  Without doc_ids groups is 1.
  *   doc_ids       int32 [B, N] or null: the row of each token; a token whose id is
- *                 below 0 or at least groups has scale 0 and gate 0.
+ *                 below 0 or at least groups has scale 0 and gate 0 (and with a
+ *                 gate its x is not read: padding may hold anything).
  *   fp32_params   bits SAGE_FP32_*: which parameters (and their gradients) are fp32;
  *                 the others are of dtype.
  *   c             at most 8192; b * n below 2^23, b * groups at most 32767.

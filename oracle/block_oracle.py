@@ -90,6 +90,9 @@ def norms(op: str, x: Tensor, weight, cond, doc_ids, eps: float, residual=None, 
         m = 1 + m
     xd = x.double()
     xhat, r = _unit(xd, eps)
+    if op != "modulate" and cond is not None and doc_ids is not None:  # tokens of no document: x is not read
+        dead = ((doc_ids < 0) | (doc_ids >= cond.shape[1]))[..., None]
+        xhat, r = xhat.masked_fill(dead, 0.0), r.masked_fill(dead, 0.0)
     p = xhat * w * m
     out = {}
     if op == "modulate":

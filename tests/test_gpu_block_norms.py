@@ -224,6 +224,20 @@ def test_not_finite_and_zero_rows(cuda, op):
             assert torch.equal(got[k][0, 8], v["residual"][0, 8].to(got[k].device))
 
 
+@pytest.mark.parametrize("op", ["gate", "gate_modulate"])
+def test_padding_behind_a_gate_is_not_read(cuda, op):
+    """Whatever x holds in tokens of no document: the output is the residual's, and no
+    gradient sees it."""
+    ids = _ids((70, 50), 150, 1)
+    v = _inputs(op, 1, 150, 1001, BF, F32, (2, ids), seed=12)
+    v["x"][0, 120:130] = float("nan")
+    v["x"][0, 130:140] = float("inf")
+    for eps in (EPS, 0.0):
+        got = _with_grads(op, _to(v, cuda), eps)
+        _check(got, _want(op, v, eps))
+        assert all(torch.isfinite(t).all() for t in got.values()) and not got["dx"][0, 120:].any()
+
+
 def test_gradients_against_differences(cuda):
     """Central differences of the operator itself along random directions, in fp32 sums of
     fp16 outputs: the step is 2^-4 of the inputs' scale, so the difference's own error is the
