@@ -22,6 +22,7 @@ from .attention_srcii import (  # noqa: F401
     sage_bwd_op,
 )
 from .block_ops import (  # noqa: F401  (registers the ops around the attention)
+    fused_linear,
     rms_norm_gate_residual,
     rms_norm_gate_residual_modulate,
     rms_norm_modulate,

@@ -4,6 +4,7 @@
 * :func:`rms_norm_gate_residual` the norm after it: ``residual + gate * xhat * weight``
 * :func:`rms_norm_gate_residual_modulate` the norm after one half of a block and the
   norm before the next, in one pass
+* :func:`fused_linear`           a projection: ``act(x weight^T + bias) + residual``
 
 ``xhat = x / sqrt(mean(x^2) + eps)`` over the channels; arithmetic in fp32, one rounding
 per output.  ``x`` is ``[B, N, C]`` (or ``[N, C]``), bfloat16 or float16, with any strides
@@ -15,9 +16,9 @@ gate 0, and behind a gate its ``x`` is not read.  Parameters are of ``x``'s type
 read in place.
 
 The functions differentiate.  Under ``torch.compile`` they go through the custom ops
-``futudiffu_ii::rms_norm_modulate``, ``::rms_norm_gate_residual`` and
-``::rms_norm_gate_residual_modulate``, which carry the same gradients.  Channel sums are
-added in a fixed order, so gradients repeat bit for bit.  An empty batch gives empty outputs and zero parameter gradients.
+``futudiffu_ii::rms_norm_modulate``, ``::rms_norm_gate_residual``,
+``::rms_norm_gate_residual_modulate`` and ``::fused_linear``, which carry the same
+gradients.  Sums are added in a fixed order, so results and gradients repeat bit for bit.  An empty batch gives empty outputs and zero parameter gradients.
 """
 
 from __future__ import annotations
@@ -248,6 +249,106 @@ def _gate_modulate_backward(dhidden: Tensor, dout: Tensor, residual: Tensor, x: 
     return dr, dx, *params
 
 
+_ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "swiglu": 3}
+
+
+class _Linear:
+    """The checked arguments of a linear call, as the library takes them."""
+
+    def __init__(self, x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str):
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+        if x.ndim < 1 or x.dtype not in _DTYPES:
+            raise ValueError(f"x must be a bfloat16 or float16 tensor [..., K], got {x.dtype} {list(x.shape)}")
+        if not x.is_cuda:
+            raise ValueError(f"x must be a GPU tensor (device {x.device})")
+        self.K = K = x.shape[-1]
+        if (weight.ndim != 2 or weight.shape[1] != K or K < 1 or weight.shape[0] < 1 or weight.dtype != x.dtype
+                or weight.device != x.device):
+            raise ValueError(f"weight must be a {x.dtype} [N, {K}] tensor on {x.device}, got {weight.dtype} "
+                             f"{list(weight.shape)} on {weight.device}")
+        self.rows = rows = weight.shape[0]
+        self.act = _ACTIVATIONS[activation]
+        if self.act == 3 and rows % 2:
+            raise ValueError(f"a swiglu weight has an even number of rows, got {rows}")
+        self.N = N = rows // 2 if self.act == 3 else rows
+        if bias is not None and (bias.shape != (rows,) or bias.device != x.device
+                                 or (bias.dtype != x.dtype and bias.dtype != torch.float32)):
+            raise ValueError(f"bias must be a [{rows}] tensor of {x.dtype} or float32 on {x.device}, got {bias.dtype} "
+                             f"{list(bias.shape)} on {bias.device}")
+        self.shape = (*x.shape[:-1], N)
+        if residual is not None and (residual.shape != self.shape or residual.dtype != x.dtype
+                                     or residual.device != x.device):
+            raise ValueError(f"residual must be a {x.dtype} {list(self.shape)} tensor on {x.device}, got "
+                             f"{residual.dtype} {list(residual.shape)} on {residual.device}")
+        self.x, self.weight = _matrix(x), _matrix(weight)
+        self.bias = None if bias is None else bias.contiguous()
+        self.residual = None if residual is None else _matrix(residual)
+        self.M = self.x.shape[0]
+        self.dtype = _DTYPES[x.dtype]
+        self.f32 = bias is not None and bias.dtype == torch.float32
+
+
+def _matrix(t: Tensor) -> Tensor:
+    """``[..., C]`` as rows ``[M, C]`` the kernels read in place: columns contiguous, rows at
+    least their width apart."""
+    if t.ndim != 2:
+        t = t.reshape(-1, t.shape[-1])
+    M, C = t.shape
+    rs, cs = t.stride()
+    if (cs != 1 and C != 1) or (M > 1 and not C <= rs < 1 << 22):
+        t = t.contiguous()
+    return t
+
+
+def _linear_forward(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str,
+                    keep_z: bool) -> tuple[Tensor, Tensor | None]:
+    a = _Linear(x, weight, bias, residual, activation)
+    out = torch.empty(a.shape, dtype=x.dtype, device=x.device)
+    z = torch.empty((a.M, a.rows), dtype=x.dtype, device=x.device) if keep_z and a.act else None
+    if a.M == 0:
+        return out, z
+    with _on(x.device):
+        lib = _lib.load()
+        xp, xs, wp, ws = a.x.data_ptr(), a.x.stride(0), a.weight.data_ptr(), a.weight.stride(0)
+        size = lib.sage_linear_workspace_bytes(xp, xs, wp, ws, a.M, a.N, a.K, a.act)
+        work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        _lib.check(lib.sage_linear(
+            xp, xs, wp, ws, _ptr(a.bias), a.f32, _ptr(a.residual), 0 if a.residual is None else a.residual.stride(0),
+            a.M, a.N, a.K, a.dtype, a.act, _ptr(work), size, _ptr(z), out.data_ptr(), _stream_handle(x.device)))
+    return out, z
+
+
+def _linear_backward(dout: Tensor, x: Tensor, weight: Tensor, bias: Tensor | None, z: Tensor | None,
+                     activation: str, wanted: list[bool]) -> tuple[Tensor | None, ...]:
+    """dx, dweight, dbias (None where not wanted)."""
+    a = _Linear(x, weight, bias, None, activation)
+    if dout.shape != a.shape or dout.dtype != x.dtype or dout.device != x.device:
+        raise ValueError(f"dout must be a {x.dtype} {list(a.shape)} tensor on {x.device}, got {dout.dtype} "
+                         f"{list(dout.shape)} on {dout.device}")
+    if a.act and (z is None or z.shape != (a.M, a.rows) or z.dtype != x.dtype or not z.is_contiguous()):
+        raise ValueError("the gradient of an activation needs the z that the forward kept (keep_z)")
+    dx, dw, db = _grad(x, wanted[0]), _grad(weight, wanted[1]), _grad(bias, wanted[2])
+    if a.M == 0:
+        for g in (dw, db):
+            if g is not None:
+                g.zero_()
+        return dx, dw, db
+    want = (dx is not None) + 2 * (dw is not None) + 4 * (db is not None)
+    if not want:
+        return dx, dw, db
+    d = _matrix(dout)
+    with _on(x.device):
+        lib = _lib.load()
+        rows = (d.data_ptr(), d.stride(0), a.x.data_ptr(), a.x.stride(0), a.weight.data_ptr(), a.weight.stride(0))
+        size = lib.sage_linear_bwd_workspace_bytes(*rows, a.M, a.N, a.K, a.act, want)
+        work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        _lib.check(lib.sage_linear_bwd(
+            *rows, _ptr(z) if a.act else None, a.M, a.N, a.K, a.dtype, a.act, a.f32, _ptr(work), size, _ptr(dx),
+            _ptr(dw), _ptr(db), _stream_handle(x.device)))
+    return dx, dw, db
+
+
 # ---- ops and their autograd formulas ---------------------------------------------------
 #
 # A gradient op returns an empty tensor in the place of a gradient that is not wanted
@@ -406,6 +507,56 @@ class _GateModulate(torch.autograd.Function):
         return *_only(grads, need), None, None
 
 
+_define("fused_linear(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, str activation, bool keep_z) "
+        "-> (Tensor, Tensor)",
+        lambda x, weight, bias, residual, activation, keep_z: _present(
+            _linear_forward(x, weight, bias, residual, activation, keep_z), x),
+        lambda x, weight, bias, residual, activation, keep_z: (
+            x.new_empty(*x.shape[:-1], weight.shape[0] // (2 if activation == "swiglu" else 1)),
+            x.new_empty(x.numel() // x.shape[-1], weight.shape[0]) if keep_z and activation != "none"
+            else x.new_empty(0)))
+_define("fused_linear_backward(Tensor dout, Tensor x, Tensor weight, Tensor? bias, Tensor? z, str activation, "
+        "bool[] wanted) -> (Tensor, Tensor, Tensor)",
+        lambda dout, x, weight, bias, z, activation, wanted: _present(
+            _linear_backward(dout, x, weight, bias, z, activation, wanted), x),
+        lambda dout, x, weight, bias, z, activation, wanted: _fake_grads(x, *zip((x, weight, bias), wanted)))
+
+
+def _linear_setup(ctx, inputs, output):
+    x, weight, bias, residual, activation, keep_z = inputs
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(x, weight, bias, output[1])
+    ctx.activation = activation
+
+
+def _linear_autograd(ctx, dout, dz):
+    x, weight, bias, z = ctx.saved_tensors
+    wanted = _wanted(ctx, range(3), (x, weight, bias))
+    grads = (None, None, None)
+    if any(wanted):
+        grads = torch.ops.futudiffu_ii.fused_linear_backward(dout, x, weight, bias, z, ctx.activation, wanted)
+    return *_only(grads, wanted), dout if ctx.needs_input_grad[3] else None, None, None
+
+
+torch.library.register_autograd("futudiffu_ii::fused_linear", _linear_autograd, setup_context=_linear_setup, lib=_ops)
+
+
+class _FusedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        out, z = _linear_forward(x, weight, bias, residual, activation, True)
+        ctx.save_for_backward(x, weight, bias, z)
+        ctx.activation = activation
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, weight, bias, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return (*_linear_backward(dout, x, weight, bias, z, ctx.activation, need[:3]), dout if need[3] else None, None)
+
+
 # ---- the functions ---------------------------------------------------------------------
 
 def rms_norm_modulate(x: Tensor, weight: Tensor | None = None, scale: Tensor | None = None, *,
@@ -444,3 +595,25 @@ def rms_norm_gate_residual_modulate(residual: Tensor, x: Tensor, weight: Tensor 
     if _wants_grad(residual, x, weight, gate, next_weight, next_scale):
         return _GateModulate.apply(residual, x, weight, gate, next_weight, next_scale, doc_ids, eps)
     return _gate_modulate_forward(residual, x, weight, gate, next_weight, next_scale, doc_ids, eps)
+
+
+def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual: Tensor | None = None, *,
+                 activation: str = "none") -> Tensor:
+    """``act(x weight^T + bias) + residual`` in one product.
+
+    ``x`` is ``[..., K]``, bfloat16 or float16; ``weight`` ``[N, K]`` of the same type;
+    ``bias`` ``[N]`` of that type or float32; ``residual`` ``[..., N]``.  ``activation`` is
+    "none", "silu", "gelu" (the tanh form) or "swiglu", whose weight and bias have the rows
+    of the gate and then those it multiplies: ``silu(z[..., :N/2]) * z[..., N/2:]``, and the
+    output ``N/2`` columns.  Sums are fp32, the output is rounded once.
+
+    For the gradient of an activation the forward keeps ``z = x weight^T + bias`` rounded to
+    ``x``'s type, and ``dout * act'(z)`` is rounded to it as an operand of the products, each
+    as a 16-bit framework does it; the bias's gradient adds it unrounded.
+    """
+    if torch.compiler.is_compiling():
+        keep = activation != "none" and _wants_grad(x, weight, bias, residual)
+        return torch.ops.futudiffu_ii.fused_linear(x, weight, bias, residual, activation, keep)[0]
+    if _wants_grad(x, weight, bias, residual):
+        return _FusedLinear.apply(x, weight, bias, residual, activation)
+    return _linear_forward(x, weight, bias, residual, activation, False)[0]

@@ -24,7 +24,7 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 # --phase-timing; never loaded by the product path
 PHASE_LIB_PATH = os.path.join(HERE, "libsage_mi355x_phase.so")
 SOURCES = ["sage_quant.hip", "sage_attn.hip", "sage_mask.hip", "sage_bwd.hip", "sage_capi.hip",
-           "sage_norm.hip"]
+           "sage_norm.hip", "sage_linear.hip"]
 ARCH = "gfx950"
 
 

@@ -879,3 +879,262 @@ int sage_rms_norm_gate_residual_modulate_bwd(
 }
 
 }  // extern "C"
+
+namespace {
+
+int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+int check_linear(int64_t m, int64_t n, int64_t k, int64_t w_rs, int dtype, int activation) {
+  if (m <= 0 || n <= 0 || k <= 0)
+    return fail(SAGE_ERR_ARG, "m=%lld, n=%lld and k=%lld must be positive", (long long)m, (long long)n, (long long)k);
+  if (activation < SAGE_ACT_NONE || activation > SAGE_ACT_SWIGLU)
+    return fail(SAGE_ERR_ARG, "unknown activation %d", activation);
+  if (dtype != SAGE_DTYPE_BF16 && dtype != SAGE_DTYPE_FP16) return fail(SAGE_ERR_ARG, "unknown dtype %d", dtype);
+  const int64_t rows = activation == SAGE_ACT_SWIGLU ? 2 * n : n;
+  if (m >= (int64_t)1 << 24 || n >= (int64_t)1 << 22 || k >= (int64_t)1 << 22)
+    return fail(SAGE_ERR_ARG, "m=%lld, n=%lld or k=%lld exceeds 2^24, 2^22, 2^22", (long long)m, (long long)n,
+                (long long)k);
+  if (rows * up8(k) * 2 >= (int64_t)1 << 31 || (rows - 1) * w_rs * 2 + k * 2 >= (int64_t)1 << 31)
+    return fail(SAGE_ERR_ARG, "a weight of %lld x %lld has 2^31 bytes or more", (long long)rows, (long long)k);
+  return SAGE_OK;
+}
+
+// Row strides: at least the columns (one row: anything), and panels of 256 rows under 2^31 bytes.
+int check_rows(int64_t rs, int64_t rows, int64_t cols, const char* what) {
+  if (rows > 1 && rs < cols) return fail(SAGE_ERR_ARG, "%s rows are %lld apart, under %lld", what, (long long)rs, (long long)cols);
+  if (rs >= (int64_t)1 << 22) return fail(SAGE_ERR_ARG, "%s rows are %lld apart, 2^22 or more", what, (long long)rs);
+  return SAGE_OK;
+}
+
+// Rows a product can read in place: from 16-byte boundaries, `cols` a multiple of 8 where the
+// contraction runs along them.
+bool in_place(const void* p, int64_t rs, int64_t rows, int64_t cols) {
+  return aligned16(p) && (rows == 1 || rs % 8 == 0) && cols % 8 == 0;
+}
+
+// An operand in place, or its copy in the workspace (packed on run).
+struct LinearOperand {
+  const void* src;
+  int64_t rs, rows, cols, pc;
+  bool copy;
+  size_t off;
+  LinearOperand(const void* p, int64_t rs_, int64_t rows_, int64_t cols_, size_t& at)
+      : src(p), rs(rs_), rows(rows_), cols(cols_), pc(up8(cols_)), copy(!in_place(p, rs_, rows_, cols_)), off(at) {
+    if (copy) at += up256((size_t)(rows * pc) * 2);
+  }
+  const void* ptr(void* ws) const { return copy ? static_cast<uint8_t*>(ws) + off : src; }
+  int64_t ld() const { return copy ? pc : rows == 1 ? up8(cols) : rs; }
+  hipError_t pack(int dtype, void* ws, hipStream_t st) const {
+    return copy ? sage::launch_pack(dtype, src, rs, rows, cols, static_cast<uint8_t*>(ws) + off, pc, st) : hipSuccess;
+  }
+};
+
+sage::GemmArgs forward_gemm(int64_t m, int64_t n, int64_t k, int act) {
+  sage::GemmArgs g{};
+  g.m = m;
+  g.n = (int)n;
+  g.k = up8(k);
+  g.kv = k;
+  g.a_kc = g.b_kc = 1;
+  g.act = act;
+  sage::gemm_plan(g);
+  return g;
+}
+
+// The backward's steps and their places in its workspace.
+struct LinearBwd {
+  int64_t rows;
+  bool form_dz;     // dz is formed (an activation, or rows that no product can read in place)
+  bool dz_in_place; // dout itself is the products' operand
+  int64_t ldz;
+  size_t dz_off, sum_off, part_off, bytes;
+  int64_t chunks, chunk;
+  sage::GemmArgs gx{}, gw{};
+  // x and weight as rows whose columns the products read 16 bytes at a time
+  size_t x_off, w_off;
+  bool copy_x, copy_w;
+  LinearBwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs, const void* w, int64_t w_rs, int64_t m,
+            int64_t n, int64_t k, int act, int want) {
+    rows = act == SAGE_ACT_SWIGLU ? 2 * n : n;
+    const bool products = want & 3;
+    form_dz = products && (act != SAGE_ACT_NONE || !in_place(dout, d_rs, m, n));
+    dz_in_place = products && !form_dz;
+    ldz = form_dz ? up8(rows) : m == 1 ? up8(rows) : d_rs;
+    size_t at = 0;
+    dz_off = at;
+    if (form_dz) at += up256((size_t)(m * ldz) * 2);
+    // bias: chunks of at least 32 rows, at most 256 of them
+    chunk = (m + 255) / 256 < 32 ? 32 : (m + 255) / 256;
+    chunks = (m + chunk - 1) / chunk;
+    sum_off = at;
+    if (want & 4) at += up256((size_t)(chunks * rows) * 4);
+    copy_x = (want & 2) && !in_place(x, x_rs, m, k);
+    copy_w = (want & 1) && !in_place(w, w_rs, rows, k);
+    x_off = at;
+    if (copy_x) at += up256((size_t)(m * up8(k)) * 2);
+    w_off = at;
+    if (copy_w) at += up256((size_t)(rows * up8(k)) * 2);
+    size_t part = 0;
+    if (want & 1) {
+      gx.m = m;
+      gx.n = (int)k;
+      gx.k = up8(rows);
+      gx.kv = rows;
+      gx.a_kc = 1;
+      gx.lda = ldz;
+      gx.ldb = copy_w ? up8(k) : rows == 1 ? up8(k) : w_rs;
+      sage::gemm_plan(gx);
+      part = (size_t)gx.part_floats * 4;
+    }
+    if (want & 2) {
+      gw.m = rows;
+      gw.n = (int)k;
+      gw.k = gw.kv = m;
+      gw.lda = ldz;
+      gw.ldb = copy_x ? up8(k) : m == 1 ? up8(k) : x_rs;
+      sage::gemm_plan(gw);
+      part = std::max(part, (size_t)gw.part_floats * 4);
+    }
+    part_off = at;
+    bytes = at + up256(part);
+  }
+};
+
+}  // namespace
+
+extern "C" {
+
+size_t sage_linear_workspace_bytes(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, int64_t m,
+                                   int64_t n, int64_t k, int activation) {
+  if (m <= 0 || n <= 0 || k <= 0 || m >= (int64_t)1 << 24 || n >= (int64_t)1 << 22 || k >= (int64_t)1 << 22) return 0;
+  size_t at = 0;
+  const LinearOperand xo(x, x_rs, m, k, at);
+  const LinearOperand wo(weight, w_rs, activation == SAGE_ACT_SWIGLU ? 2 * n : n, k, at);
+  return at + (size_t)forward_gemm(m, n, k, activation).part_floats * 4;
+}
+
+int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, const void* bias, int bias_fp32,
+                const void* residual, int64_t r_rs, int64_t m, int64_t n, int64_t k, int dtype, int activation,
+                void* workspace, size_t workspace_bytes, void* z, void* out, hipStream_t stream) {
+  if (const int e = check_linear(m, n, k, w_rs, dtype, activation)) return e;
+  const int64_t rows = activation == SAGE_ACT_SWIGLU ? 2 * n : n;
+  if (!x || !weight || !out) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  if (const int e = check_rows(x_rs, m, k, "x")) return e;
+  if (const int e = check_rows(w_rs, rows, k, "weight")) return e;
+  if (residual)
+    if (const int e = check_rows(r_rs, m, n, "residual")) return e;
+  for (const void* p : {x, weight, residual, (const void*)z, (const void*)out})
+    if (reinterpret_cast<uintptr_t>(p) & 1u) return fail(SAGE_ERR_ALIGN, "tensor pointers must be aligned to their elements");
+  if (reinterpret_cast<uintptr_t>(bias) & (bias_fp32 ? 3u : 1u))
+    return fail(SAGE_ERR_ALIGN, "bias must be aligned to its elements");
+  size_t at = 0;
+  const LinearOperand xo(x, x_rs, m, k, at);
+  const LinearOperand wo(weight, w_rs, rows, k, at);
+  sage::GemmArgs g = forward_gemm(m, n, k, activation);
+  const size_t need = at + (size_t)g.part_floats * 4;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace_bytes);
+  if (need && !aligned16(workspace)) return fail(SAGE_ERR_ALIGN, "workspace must be 16-byte aligned");
+  hipError_t e = xo.pack(dtype, workspace, stream);
+  if (e == hipSuccess) e = wo.pack(dtype, workspace, stream);
+  if (e != hipSuccess) return launch_status(e, "sage_linear (copy)");
+  g.a = xo.ptr(workspace);
+  g.lda = xo.ld();
+  g.b = wo.ptr(workspace);
+  g.ldb = wo.ld();
+  g.bias = bias;
+  g.bias_f32 = bias_fp32 != 0;
+  g.res = residual;
+  g.ldr = r_rs;
+  g.z = z;
+  g.out = out;
+  g.vec = n % 8 == 0 && aligned16(out) && (!z || aligned16(z)) &&
+          (!residual || (aligned16(residual) && (m == 1 || r_rs % 8 == 0)));
+  g.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at);
+  return launch_status(sage::launch_gemm(g, dtype, stream), "sage_linear");
+}
+
+size_t sage_linear_bwd_workspace_bytes(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
+                                       const void* weight, int64_t w_rs, int64_t m, int64_t n, int64_t k,
+                                       int activation, int want) {
+  if (m <= 0 || n <= 0 || k <= 0 || m >= (int64_t)1 << 24 || n >= (int64_t)1 << 22 || k >= (int64_t)1 << 22) return 0;
+  return LinearBwd(dout, d_rs, x, x_rs, weight, w_rs, m, n, k, activation, want).bytes;
+}
+
+int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs, const void* weight, int64_t w_rs,
+                    const void* z, int64_t m, int64_t n, int64_t k, int dtype, int activation, int bias_fp32,
+                    void* workspace, size_t workspace_bytes, void* dx, void* dweight, void* dbias,
+                    hipStream_t stream) {
+  if (const int e = check_linear(m, n, k, dx ? w_rs : 0, dtype, activation)) return e;
+  const int64_t rows = activation == SAGE_ACT_SWIGLU ? 2 * n : n;
+  const int want = (dx ? 1 : 0) | (dweight ? 2 : 0) | (dbias ? 4 : 0);
+  if (!dout || (dweight && !x) || (dx && !weight) || (activation != SAGE_ACT_NONE && !z))
+    return fail(SAGE_ERR_ARG, "null tensor pointer");
+  if (!want) return SAGE_OK;
+  if (const int e = check_rows(d_rs, m, n, "dout")) return e;
+  if (dweight)
+    if (const int e = check_rows(x_rs, m, k, "x")) return e;
+  if (dx)
+    if (const int e = check_rows(w_rs, rows, k, "weight")) return e;
+  for (const void* p : {dout, x, weight, z, (const void*)dx, (const void*)dweight})
+    if (reinterpret_cast<uintptr_t>(p) & 1u) return fail(SAGE_ERR_ALIGN, "tensor pointers must be aligned to their elements");
+  if (reinterpret_cast<uintptr_t>(dbias) & (bias_fp32 ? 3u : 1u))
+    return fail(SAGE_ERR_ALIGN, "dbias must be aligned to its elements");
+  LinearBwd p(dout, d_rs, x, x_rs, weight, w_rs, m, n, k, activation, want);
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes))
+    return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu", p.bytes, workspace_bytes);
+  if (p.bytes && !aligned16(workspace)) return fail(SAGE_ERR_ALIGN, "workspace must be 16-byte aligned");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (p.form_dz || dbias) {
+    sage::DactArgs d{};
+    d.dout = dout;
+    d.z = z;
+    d.ldd = d_rs;
+    d.m = m;
+    d.n = (int)n;
+    d.act = activation;
+    d.dz = p.form_dz ? ws + p.dz_off : nullptr;
+    d.ldz = p.ldz;
+    d.vec_d = in_place(dout, d_rs, m, n);
+    d.vec_z = n % 8 == 0 && aligned16(z);
+    d.vec_o = n % 8 == 0;
+    d.part = dbias ? reinterpret_cast<float*>(ws + p.sum_off) : nullptr;
+    d.chunks = p.chunks;
+    d.chunk = p.chunk;
+    d.dbias = dbias;
+    d.bias_f32 = bias_fp32 != 0;
+    const hipError_t e = sage::launch_dact(dtype, d, stream);
+    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (activation)");
+  }
+  const void* dz = p.form_dz ? ws + p.dz_off : dout;
+  if (p.copy_x) {
+    const hipError_t e = sage::launch_pack(dtype, x, x_rs, m, k, ws + p.x_off, up8(k), stream);
+    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (copy)");
+  }
+  if (p.copy_w) {
+    const hipError_t e = sage::launch_pack(dtype, weight, w_rs, rows, k, ws + p.w_off, up8(k), stream);
+    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (copy)");
+  }
+  if (dx) {
+    p.gx.a = dz;
+    p.gx.b = p.copy_w ? ws + p.w_off : weight;
+    p.gx.out = dx;
+    p.gx.vec = k % 8 == 0 && aligned16(dx);
+    p.gx.part = reinterpret_cast<float*>(ws + p.part_off);
+    const hipError_t e = sage::launch_gemm(p.gx, dtype, stream);
+    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (dx)");
+  }
+  if (dweight) {
+    p.gw.a = dz;
+    p.gw.b = p.copy_x ? ws + p.x_off : x;
+    p.gw.out = dweight;
+    p.gw.vec = k % 8 == 0 && aligned16(dweight);
+    p.gw.part = reinterpret_cast<float*>(ws + p.part_off);
+    const hipError_t e = sage::launch_gemm(p.gw, dtype, stream);
+    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (dweight)");
+  }
+  return launch_status(hipSuccess, "sage_linear_bwd");
+}
+
+}  // extern "C"

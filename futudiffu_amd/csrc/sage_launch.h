@@ -364,4 +364,49 @@ NormChunks norm_chunks(int64_t b, int64_t n, int64_t c, int64_t groups, bool doc
 hipError_t launch_norm_fwd(int op, int f16, const NormArgs& a, hipStream_t st);
 hipError_t launch_norm_bwd(int op, int f16, const NormArgs& a, hipStream_t st);
 
+// Linear layers (sage_linear.hip).
+constexpr int kActNone = 0, kActSilu = 1, kActGelu = 2, kActSwiglu = 3;
+
+// C[m][n] = sum_k A[m][k] B[n][k] with an epilogue.  A is [m][k] rows lda apart (a_kc) or
+// [k][m]; B likewise.  Rows from 16-byte boundaries, lda and ldb multiples of 8.  An
+// operand with the contraction contiguous has k columns, k a multiple of 8 (zeros behind
+// kv); one without has kv rows.
+struct GemmArgs {
+  const void *a, *b;
+  int64_t lda, ldb;
+  int64_t m, k, kv;
+  int n;  // columns of the output (swiglu: B has 2 n rows, the gates and then the others)
+  int a_kc, b_kc;
+  int act;
+  const void* bias;  // [rows of B], T or fp32; null: none
+  int bias_f32;
+  const void* res;  // T rows ldr apart; null: none
+  int64_t ldr;
+  void* z;    // T [m][rows of B]: acc + bias, for the backward; null: not kept
+  void* out;  // T [m][n]
+  int vec;    // rows of res, z and out take 16-byte accesses
+  // the plan (gemm_plan)
+  int big, skinny, kt, tm, tn;
+  int whole, parts;     // tiles past `whole` run as `parts` pieces of the contraction
+  int64_t part_floats;  // fp32 sums of the pieces
+  float* part;
+};
+void gemm_plan(GemmArgs& a);
+hipError_t launch_gemm(const GemmArgs& a, int f16, hipStream_t st);
+hipError_t launch_pack(int f16, const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t pc,
+                       hipStream_t st);
+struct DactArgs {
+  const void *dout, *z;  // z: act != none
+  int64_t ldd, m;
+  int n, act;
+  void* dz;  // rows ldz apart; null: not formed
+  int64_t ldz;
+  int vec_d, vec_z, vec_o;
+  float* part;  // column sums [chunks][n or 2n]; null: no bias gradient
+  int64_t chunks, chunk;
+  void* dbias;
+  int bias_f32;
+};
+hipError_t launch_dact(int f16, const DactArgs& a, hipStream_t st);
+
 }  // namespace sage

@@ -1,0 +1,756 @@
+// Linear layers of a transformer block for gfx950: out = act(x W^T + b) + r, and its
+// gradients, bf16 or fp16 with fp32 accumulation.
+//
+// One product C[m][n] = sum_k A[m][k] B[n][k] in three operand layouts:
+//   forward  A = x  [M][K],  B = W [N][K]          (both with the contraction contiguous)
+//   dx       A = dz [M][N'], B = W as [N'][K]      (B: the output's columns contiguous)
+//   dW       A = dz as [M][N'], B = x as [M][K]    (both: the contraction strided)
+// and three kernels: tiles through LDS (gemm_kernel), few rows on one side
+// (skinny_kernel), and the sum of a tile's pieces (join_kernel).
+#include <type_traits>
+
+#include "sage_common.h"
+#include "sage_launch.h"
+
+namespace sage {
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+struct Vec8;
+template <>
+struct Vec8<__bf16> {
+  typedef bf16x8 type;
+};
+template <>
+struct Vec8<_Float16> {
+  typedef f16x8 type;
+};
+
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------- activations
+
+constexpr float kGeluA = 0.7978845608028654f;  // sqrt(2/pi)
+
+// 1 / (1 + exp(-z)); exp(-z) may overflow to infinity, which gives 0.
+__device__ __forceinline__ float sigmoidf(float z) { return 1.0f / (1.0f + __expf(-z)); }
+
+__device__ __forceinline__ float act_fwd(int act, float z) {
+  if (act == kActSilu || act == kActSwiglu) return z * sigmoidf(z);
+  if (act == kActGelu)  // 0.5 z (1 + tanh(u)) = z sigmoid(2u), u = a (z + 0.044715 z^3)
+    return z * sigmoidf(2.0f * kGeluA * (z + 0.044715f * z * z * z));
+  return z;
+}
+
+__device__ __forceinline__ float act_grad(int act, float z) {
+  if (act == kActSilu || act == kActSwiglu) {
+    const float s = sigmoidf(z);
+    return s + z * s * (1.0f - s);
+  }
+  if (act == kActGelu) {  // with s = sigmoid(2u): s + z s (1 - s) 2 u'
+    const float s = sigmoidf(2.0f * kGeluA * (z + 0.044715f * z * z * z));
+    return s + z * s * (1.0f - s) * (2.0f * kGeluA * (1.0f + 3.0f * 0.044715f * z * z));
+  }
+  return 1.0f;
+}
+
+// ---------------------------------------------------------------- rows of the epilogue
+
+// Eight consecutive columns of a row of T, at column n of `cols`; past the last: zeros.
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int n, int cols, bool vec, float (&f)[8]) {
+  if (vec) {
+    const auto v = *reinterpret_cast<const typename Vec8<T>::type*>(row + n);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (float)v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = n + j < cols ? (float)row[n + j] : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* row, int n, int cols, bool vec, const float (&f)[8]) {
+  if (vec) {
+    typename Vec8<T>::type v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (T)f[j];
+    *reinterpret_cast<typename Vec8<T>::type*>(row + n) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n + j < cols) row[n + j] = (T)f[j];
+  }
+}
+
+__device__ __forceinline__ float param_at(const void* p, bool f32, bool f16, int64_t i) {
+  if (f32) return static_cast<const float*>(p)[i];
+  return f16 ? (float)static_cast<const _Float16*>(p)[i] : (float)static_cast<const __bf16*>(p)[i];
+}
+
+// Bias of eight columns from row `at` of the weight on (columns past `cols`: zeros).
+template <typename T>
+__device__ __forceinline__ void load_bias(const GemmArgs& a, int at, int n, int cols, float (&f)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    f[j] = a.bias && n + j < cols ? param_at(a.bias, a.bias_f32, std::is_same<T, _Float16>::value, at + n + j) : 0.0f;
+}
+
+// The epilogue of row m, columns n .. n + 7 (n < a.n): z = acc + bias, kept when the backward wants it,
+// out = act(z) + residual, rounded once.  z2 and b2: the second half of a swiglu.
+template <typename T>
+__device__ __forceinline__ void finish8(const GemmArgs& a, int64_t m, int n, float (&z)[8], float (&z2)[8],
+                                        const float (&b)[8], const float (&b2)[8]) {
+  const bool glu = a.act == kActSwiglu;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    z[j] += b[j];
+    if (glu) z2[j] += b2[j];
+  }
+  if (a.z) {
+    T* row = static_cast<T*>(a.z) + m * (glu ? 2 * (int64_t)a.n : a.n);
+    store8<T>(row, n, a.n, a.vec, z);
+    if (glu) store8<T>(row + a.n, n, a.n, a.vec, z2);
+  }
+  float r[8] = {};
+  if (a.res) load8<T>(static_cast<const T*>(a.res) + m * a.ldr, n, a.n, a.vec, r);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float y = act_fwd(a.act, z[j]);
+    if (glu) y *= z2[j];
+    z[j] = y + r[j];
+  }
+  store8<T>(static_cast<T*>(a.out) + m * a.n, n, a.n, a.vec, z);
+}
+
+// ---------------------------------------------------------------- tiles
+
+constexpr int kBK = 64;  // contraction of one LDS stage
+
+// A tile shape: WM x WN waves, each with MI x 2 blocks of 32 x 32.
+template <int WM_, int WN_, int MI_>
+struct Tile {
+  static constexpr int WM = WM_, WN = WN_, MI = MI_, NI = 2;
+  static constexpr int WAVES = WM * WN, NT = 64 * WAVES;
+  static constexpr int BM = WM * MI * 32, BN = WN * NI * 32;
+  static constexpr int A_BYTES = BM * kBK * 2, B_BYTES = BN * kBK * 2, STAGE = A_BYTES + B_BYTES;
+  static constexpr int kPitch = 72;                        // floats of an epilogue row: see epilogue()
+  static constexpr int EPI = WAVES * 32 * kPitch * 4;
+  static constexpr int LDS = 2 * STAGE > EPI ? 2 * STAGE : EPI;
+};
+
+// One direct global -> LDS load of 64 chunks: lane l's 16 bytes land at lds + 16 l; an
+// offset past the resource's end gives zeros.
+__device__ __forceinline__ void dma_16(uint8_t* lds, __amdgpu_buffer_rsrc_t rs, int off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds, 16, off, 0, 0, 0);
+}
+
+// One operand's part of an LDS stage: ROWS rows (of the output's m or n) by kBK.
+//
+// KC (contraction contiguous in memory): 128-byte rows, row r's 16-byte chunk c at
+// c ^ ((r >> 1) & 7): the 16 rows that a fragment read touches at a time lie on 16
+// different 16-byte columns of the 256 bytes of banks.
+// Not KC: the kBK contraction rows of ROWS * 2 bytes, 64-byte runs u at u ^ (k & 3), so
+// that the 4 rows of a transposing read (ds_read_b64_tr_b16: 16 lanes read 4 rows by 16
+// columns, each lane gets one column's 4 rows) lie on different banks.
+// Every load is a direct global -> LDS load of 1 KiB by one wave, whose lanes choose
+// their source accordingly.
+template <int ROWS, bool KC, int WAVES>
+struct Operand {
+  static constexpr int LOADS = ROWS * kBK * 2 / 1024 / WAVES;  // of one wave
+  const uint8_t* base;
+  int64_t ld2;  // bytes between rows in memory
+  int valid;    // rows (KC) or columns (not KC) of this tile that exist
+  int off[LOADS];
+  int kpos;     // KC: first contraction index of the lane's chunk (the same in every load)
+
+  // glu: tile row j is row (j / 64) * 32 + j % 32 of half (j / 32) % 2, the halves `half`
+  // rows apart.
+  __device__ __forceinline__ void init(const void* p, int64_t ld, int64_t row0, int64_t rows, int wave, int lane,
+                                       bool glu, int64_t half) {
+    ld2 = ld * 2;
+    base = static_cast<const uint8_t*>(p) + row0 * (KC ? ld2 : 2);
+    const int64_t left = rows - row0;
+    valid = (int)(left < ROWS ? left : ROWS);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int q = i * WAVES + wave;
+      if constexpr (KC) {
+        int r = q * 8 + (lane >> 3);
+        const int c = (lane & 7) ^ ((r >> 1) & 7);
+        kpos = c * 8;
+        const bool up = glu && ((r >> 5) & 1);
+        if (glu) r = (r >> 6) * 32 + (r & 31);
+        off[i] = r < valid ? (int)(r * ld2 + (up ? half * ld2 : 0)) + c * 16 : (int)0x80000000;
+      } else {
+        const int at = q * 1024 + lane * 16, k = at / (ROWS * 2), in = at % (ROWS * 2);
+        off[i] = (int)(k * ld2) + ((((in >> 6) ^ (k & 3)) << 6) | (in & 63));
+      }
+    }
+  }
+  // Issues the loads of contraction k0 .. k0 + kBK - 1 of K into `lds`.
+  __device__ __forceinline__ void issue(uint8_t* lds, int64_t k0, int64_t K, int wave) const {
+    const int left = (int)(K - k0 < kBK ? K - k0 : kBK);
+    if constexpr (KC) {
+      // rows past the last have an offset past any size; so get chunks past K
+      const __amdgpu_buffer_rsrc_t rs = raw_rsrc(base + k0 * 2, 0x7fffffff);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int o = kpos < left ? off[i] : (int)0x80000000;
+        dma_16(lds + (i * WAVES + wave) * 1024, rs, o);
+      }
+    } else {
+      // columns past the last read what follows in memory (they reach outputs that are
+      // not stored alone), up to the end of the last row, in whole 4 bytes; rows past K
+      // read zeros
+      const __amdgpu_buffer_rsrc_t rs =
+          raw_rsrc(base + k0 * ld2, left > 0 ? (uint32_t)((left - 1) * ld2 + (valid + 1) / 2 * 4) : 0u);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+        dma_16(lds + (i * WAVES + wave) * 1024, rs, off[i]);
+    }
+  }
+};
+
+// Byte offset in an operand's stage of the fragment of 32 rows from `row` on: lane (h, r)
+// gets row r, contraction 16 s + 8 h .. + 7.
+template <int ROWS, bool KC>
+struct FragAddr {
+  int at[KC ? kBK / 16 : 1];
+  __device__ __forceinline__ void init(int row, int lane) {
+    const int h = lane >> 5, r = row + (lane & 31);
+    if constexpr (KC) {
+#pragma unroll
+      for (int s = 0; s < kBK / 16; ++s) at[s] = r * 128 + (((2 * s + h) ^ ((r >> 1) & 7)) << 4);
+    } else {
+      const int l = lane & 15, g = (lane >> 4) & 1, k = 8 * h + (l >> 2);
+      const int col = (row + 16 * g + 4 * (l & 3)) * 2;
+      at[0] = k * (ROWS * 2) + ((((col >> 6) ^ (k & 3)) << 6) | (col & 63));
+    }
+  }
+};
+
+// A transposing read of 8 bytes a lane.  `p` is restrict so that the read carries alias
+// information: without any, the compiler waits for the direct loads in flight before it.
+__device__ __forceinline__ s16x4 read_tr(const uint8_t* __restrict__ p) {
+  typedef __attribute__((address_space(3))) s16x4* LdsPtr;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p));
+}
+
+template <typename T, int ROWS, bool KC>
+__device__ __forceinline__ typename Vec8<T>::type frag(const uint8_t* __restrict__ stage, const FragAddr<ROWS, KC>& f,
+                                                       int s) {
+  if constexpr (KC) {
+    return *reinterpret_cast<const typename Vec8<T>::type*>(stage + f.at[s]);
+  } else {
+    const uint8_t* p = stage + f.at[0] + s * 16 * (ROWS * 2);
+    const s16x4 a = read_tr(p), b = read_tr(p + 4 * (ROWS * 2));
+    return __builtin_bit_cast(typename Vec8<T>::type, s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+  }
+}
+
+// A 32 x 64 block of one wave's sums (two accumulators, or the two halves of a swiglu)
+// through its own part of LDS to rows of eight columns a lane.  The pitch of 72 floats
+// puts the two rows a store instruction writes (4 apart) on different banks.
+template <typename T>
+__device__ __forceinline__ void epilogue(const GemmArgs& a, float* lds, int lane, int64_t m0, int n0, f32x16 c0,
+                                         f32x16 c1) {
+  constexpr int P = 72;
+  const bool glu = a.act == kActSwiglu;
+  const int h = lane >> 5, r = lane & 31;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = 8 * (i >> 2) + 4 * h + (i & 3);
+    lds[row * P + r] = c0[i];
+    lds[row * P + 32 + r] = c1[i];
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  // glu: 4 lanes a row of 32 columns; else 8 lanes a row of 64
+  const int per = glu ? 4 : 8, rows = 64 / per;
+  const int lr = lane / per, n = n0 + lane % per * 8;
+  if (n < a.n) {
+    float b[8], b2[8] = {};
+    load_bias<T>(a, 0, n, a.n, b);
+    if (glu) load_bias<T>(a, a.n, n, a.n, b2);
+    for (int row = lr; row < 32; row += rows) {
+      const int64_t m = m0 + row;
+      if (m < a.m) {
+        float z[8], z2[8] = {};
+        const float* src = lds + row * P + lane % per * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          z[j] = src[j];
+          if (glu) z2[j] = src[32 + j];
+        }
+        finish8<T>(a, m, n, z, z2, b, b2);
+      }
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Tile t of the schedule: groups of 4 tile rows, column by column inside, so that the 32
+// tiles an XCD runs together share 4 row panels and 8 column panels.
+__device__ __forceinline__ void tile_at(const GemmArgs& a, int t, int& tm, int& tn) {
+  constexpr int G = 4;
+  const int g = t / (G * a.tn), in = t - g * G * a.tn;
+  const int rows = min(G, a.tm - g * G);
+  tn = in / rows;
+  tm = g * G + in - tn * rows;
+}
+
+// Work unit of workgroup `b`: the hardware hands workgroup b to XCD b % 8; every XCD takes
+// a contiguous range of the whole tiles, then of the cut ones' pieces.
+__device__ __forceinline__ int xcd_share(int b, int total) {
+  const int x = b % 8, local = b / 8, per = total / 8, rem = total % 8;
+  return x * per + min(x, rem) + local;
+}
+
+template <typename T, bool AK, bool BKC, typename TL>
+__global__ __launch_bounds__(TL::NT, 2) void gemm_kernel(GemmArgs a) {
+  __shared__ __align__(1024) uint8_t lds[TL::LDS];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const bool glu = BKC && a.act == kActSwiglu;
+  const int bid = blockIdx.x;
+  int t, piece = 0;
+  int kt0 = 0, kt1 = a.kt;
+  const bool cut = bid >= a.whole;
+  if (!cut) {
+    t = xcd_share(bid, a.whole);
+  } else {
+    const int u = xcd_share(bid - a.whole, ((int)gridDim.x - a.whole));
+    t = a.whole + u / a.parts;
+    piece = u - (t - a.whole) * a.parts;
+    kt0 = (int)((int64_t)a.kt * piece / a.parts);
+    kt1 = (int)((int64_t)a.kt * (piece + 1) / a.parts);
+  }
+  int tm, tn;
+  tile_at(a, t, tm, tn);
+  const int64_t m0 = (int64_t)tm * TL::BM;
+  const int n0 = tn * (glu ? TL::BN / 2 : TL::BN);
+
+  Operand<TL::BM, AK, TL::WAVES> A;
+  Operand<TL::BN, BKC, TL::WAVES> B;
+  A.init(a.a, a.lda, m0, a.m, wave, lane, false, 0);
+  B.init(a.b, a.ldb, n0, a.n, wave, lane, glu, a.n);
+  const int wm = wave / TL::WN, wn = wave % TL::WN;
+  FragAddr<TL::BM, AK> fa[TL::MI];
+  FragAddr<TL::BN, BKC> fb[TL::NI];
+#pragma unroll
+  for (int i = 0; i < TL::MI; ++i) fa[i].init((wm * TL::MI + i) * 32, lane);
+#pragma unroll
+  for (int i = 0; i < TL::NI; ++i) fb[i].init((wn * TL::NI + i) * 32, lane);
+
+  f32x16 acc[TL::MI][TL::NI] = {};
+  A.issue(lds, (int64_t)kt0 * kBK, AK ? a.k : a.kv, wave);
+  B.issue(lds + TL::A_BYTES, (int64_t)kt0 * kBK, BKC ? a.k : a.kv, wave);
+  for (int kt = kt0; kt < kt1; ++kt) {
+    wait_vmem();
+    __syncthreads();
+    if (kt + 1 < kt1) {
+      uint8_t* next = lds + ((kt + 1 - kt0) & 1) * TL::STAGE;
+      A.issue(next, (int64_t)(kt + 1) * kBK, AK ? a.k : a.kv, wave);
+      B.issue(next + TL::A_BYTES, (int64_t)(kt + 1) * kBK, BKC ? a.k : a.kv, wave);
+    }
+    const uint8_t* sa = lds + ((kt - kt0) & 1) * TL::STAGE;
+    const uint8_t* sb = sa + TL::A_BYTES;
+#pragma unroll
+    for (int s = 0; s < kBK / 16; ++s) {
+      typename Vec8<T>::type va[TL::MI], vb[TL::NI];
+#pragma unroll
+      for (int i = 0; i < TL::MI; ++i) va[i] = frag<T>(sa, fa[i], s);
+#pragma unroll
+      for (int i = 0; i < TL::NI; ++i) vb[i] = frag<T>(sb, fb[i], s);
+#pragma unroll
+      for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < TL::NI; ++j) acc[i][j] = mfma32(va[i], vb[j], acc[i][j]);
+    }
+  }
+  __syncthreads();
+  if (cut) {
+    // the piece's sums, in the order the lanes hold them
+    float* dst = a.part + ((int64_t)(t - a.whole) * a.parts + piece) * (TL::BM * TL::BN) +
+                 wave * (TL::MI * TL::NI * 1024);
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::NI; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4*>(dst + ((i * TL::NI + j) * 4 + q) * 256 + lane * 4) =
+              f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    return;
+  }
+  float* mine = reinterpret_cast<float*>(lds) + wave * 32 * TL::kPitch;
+#pragma unroll
+  for (int i = 0; i < TL::MI; ++i)
+    epilogue<T>(a, mine, lane, m0 + (wm * TL::MI + i) * 32, n0 + wn * (glu ? 32 : 64), acc[i][0], acc[i][1]);
+}
+
+// Adds the pieces of the cut tiles in order and finishes them: a wave takes one 32 x 64
+// block of a tile.
+template <typename T, typename TL>
+__global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
+  __shared__ float lds[4][32 * TL::kPitch];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  constexpr int BLOCKS = TL::WAVES * TL::MI;
+  const int u = blockIdx.x * 4 + wave, t = u / BLOCKS, blk = u - t * BLOCKS;
+  const float* src = a.part + (int64_t)t * a.parts * (TL::BM * TL::BN) + blk * (TL::NI * 1024) + lane * 4;
+  f32x16 c[2] = {};
+  for (int p = 0; p < a.parts; ++p) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(src + (j * 4 + q) * 256);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[j][4 * q + e] += v[e];
+      }
+    src += TL::BM * TL::BN;
+  }
+  int tm, tn;
+  tile_at(a, a.whole + t, tm, tn);
+  const int w = blk / TL::MI, wm = w / TL::WN, wn = w % TL::WN;
+  const bool glu = a.act == kActSwiglu;
+  epilogue<T>(a, lds[wave], lane, (int64_t)tm * TL::BM + (wm * TL::MI + blk % TL::MI) * 32,
+              tn * (glu ? TL::BN / 2 : TL::BN) + wn * (glu ? 32 : 64), c[0], c[1]);
+}
+
+// ---------------------------------------------------------------- few rows
+
+constexpr int kSkinnyWaves = 8;
+
+// out for at most 16 * MT rows on the short side: a workgroup takes 16 rows of the long
+// side and reads them once, straight into the matrix operand's registers (lane (q, r): row
+// r, contraction 8 q .. 8 q + 7 of a step of 32); its waves share the contraction, 64 at a
+// time in turn, and their sums are added in order.  swap: the long side is x (m), not W (n).
+template <typename T, int MT, bool GLU>
+__global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(GemmArgs a, int swap) {
+  using V = typename Vec8<T>::type;
+  constexpr int H = GLU ? 2 : 1;
+  __shared__ f32x4 part[kSkinnyWaves][H][MT][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int q = lane >> 4, r = lane & 15;
+  const uint8_t* lp = static_cast<const uint8_t*>(swap ? a.a : a.b);
+  const uint8_t* sp = static_cast<const uint8_t*>(swap ? a.b : a.a);
+  const int64_t lld = (swap ? a.lda : a.ldb) * 2, sld = (swap ? a.ldb : a.lda) * 2;
+  const int64_t llen = swap ? a.m : a.n, slen = swap ? a.n : a.m;
+  const int64_t l0 = (int64_t)blockIdx.x * 16;
+  // rows past the last read the last one again; what they give is not stored
+  const uint8_t* lrow[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h) lrow[h] = lp + (min(l0 + r, llen - 1) + h * llen) * lld;
+  const uint8_t* srow[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) srow[i] = sp + min((int64_t)(i * 16 + r), slen - 1) * sld;
+  f32x4 acc[H][MT] = {};
+  auto step = [&](int64_t k, bool tail) {
+    // two steps of 32; a tail's lanes past the end take zeros
+    V l[2][H], s[2][MT];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t at = k + 32 * u + 8 * q;
+      const bool in = !tail || at < a.k;
+#pragma unroll
+      for (int h = 0; h < H; ++h) l[u][h] = in ? *reinterpret_cast<const V*>(lrow[h] + at * 2) : V{};
+#pragma unroll
+      for (int i = 0; i < MT; ++i) s[u][i] = in ? *reinterpret_cast<const V*>(srow[i] + at * 2) : V{};
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[h][i] = mfma16(l[u][h], s[u][i], acc[h][i]);
+  };
+  const int64_t whole = a.k / 64;
+  int64_t k = wave;
+#pragma unroll 4
+  for (; k < whole; k += kSkinnyWaves) step(k * 64, false);
+  if (k == whole && whole * 64 < a.k) step(k * 64, true);
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) part[wave][h][i][lane] = acc[h][i];
+  __syncthreads();
+  // lane (q, r) of tile i holds long rows 4 q .. + 3 of short row r
+  for (int u = threadIdx.x; u < MT * 64; u += 64 * kSkinnyWaves) {
+    const int i = u >> 6, ln = u & 63;
+    f32x4 z = {}, z2 = {};
+#pragma unroll
+    for (int w = 0; w < kSkinnyWaves; ++w) {
+      z += part[w][0][i][ln];
+      if (GLU) z2 += part[w][H - 1][i][ln];
+    }
+    const int64_t srow_i = i * 16 + (ln & 15);
+    if (srow_i >= slen) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t lrow_j = l0 + 4 * (ln >> 4) + j;
+      if (lrow_j >= llen) continue;
+      const int64_t m = swap ? lrow_j : srow_i, n = swap ? srow_i : lrow_j;
+      float v = z[j], v2 = z2[j];
+      if (a.bias) {
+        v += param_at(a.bias, a.bias_f32, std::is_same<T, _Float16>::value, n);
+        if (GLU) v2 += param_at(a.bias, a.bias_f32, std::is_same<T, _Float16>::value, a.n + n);
+      }
+      if (a.z) {
+        T* row = static_cast<T*>(a.z) + m * a.n * H;
+        row[n] = (T)v;
+        if (GLU) row[a.n + n] = (T)v2;
+      }
+      float y = act_fwd(a.act, v);
+      if (GLU) y *= v2;
+      if (a.res) y += (float)static_cast<const T*>(a.res)[m * a.ldr + n];
+      static_cast<T*>(a.out)[m * a.n + n] = (T)y;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- operands and gradients beside the products
+
+// Rows [rows][cols] at any alignment into 16-byte aligned rows of `pc` columns (a multiple
+// of 8), zeros behind the last column: what the products read.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t ld, int64_t rows, int64_t cols, T* dst,
+                                                   int64_t pc) {
+  const int64_t chunks = pc / 8, total = rows * chunks;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
+    const int64_t r = u / chunks;
+    const int c = (int)(u - r * chunks) * 8;
+    typename Vec8<T>::type v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? src[r * ld + c + j] : (T)0.0f;
+    *reinterpret_cast<typename Vec8<T>::type*>(dst + r * pc + c) = v;
+  }
+}
+
+// The gradient of z: dz = dout * act'(z) (swiglu: both halves), rounded to T as the
+// products' operand, into rows of `ldz` (zeros behind the last column); with `part` the
+// column sums of the unrounded values over each chunk of rows, for the bias.  A workgroup
+// takes 512 columns (64 lanes of 8) of a chunk, a wave every fourth row.
+template <typename T>
+__global__ __launch_bounds__(256) void dact_kernel(DactArgs a) {
+  __shared__ float sum[2][4][512];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const bool glu = a.act == kActSwiglu;
+  const int n = blockIdx.x * 512 + lane * 8;
+  const int64_t r0 = (int64_t)blockIdx.y * a.chunk, r1 = r0 + a.chunk < a.m ? r0 + a.chunk : a.m;
+  float s1[8] = {}, s2[8] = {};
+  if (n < a.n) {
+#pragma unroll 2
+    for (int64_t m = r0 + wave; m < r1; m += 4) {
+      float d[8], z[8], z2[8];
+      load8<T>(static_cast<const T*>(a.dout) + m * a.ldd, n, a.n, a.vec_d, d);
+      if (a.act != kActNone) {
+        const T* zr = static_cast<const T*>(a.z) + m * (glu ? 2 * a.n : a.n);
+        load8<T>(zr, n, a.n, a.vec_z, z);
+        if (glu) load8<T>(zr + a.n, n, a.n, a.vec_z, z2);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (glu) {
+          const float up = d[j] * act_fwd(a.act, z[j]);
+          d[j] = d[j] * z2[j] * act_grad(a.act, z[j]);
+          z2[j] = up;
+          s2[j] += up;
+        } else if (a.act != kActNone) {
+          d[j] *= act_grad(a.act, z[j]);
+        }
+        s1[j] += d[j];
+      }
+      if (a.dz) {
+        T* row = static_cast<T*>(a.dz) + m * a.ldz;
+        store8<T>(row, n, a.n, a.vec_o, d);
+        if (glu) store8<T>(row + a.n, n, a.n, a.vec_o, z2);
+      }
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    sum[0][wave][j * 64 + lane] = s1[j];
+    if (glu) sum[1][wave][j * 64 + lane] = s2[j];
+  }
+  __syncthreads();
+  for (int u = threadIdx.x; u < (glu ? 1024 : 512); u += 256) {
+    const int half = u >> 9, at = u & 511, col = blockIdx.x * 512 + at;
+    const int v = (at & 7) * 64 + (at >> 3);
+    if (col < a.n)
+      a.part[(int64_t)blockIdx.y * (glu ? 2 * a.n : a.n) + half * a.n + col] =
+          sum[half][0][v] + sum[half][1][v] + sum[half][2][v] + sum[half][3][v];
+  }
+}
+
+// Zeros behind the last column of packed gradient rows.
+template <typename T>
+__global__ __launch_bounds__(256) void clear_tail_kernel(T* p, int64_t rows, int64_t ld, int cols) {
+  const int w = (int)(ld - cols);
+  const int64_t total = rows * w;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
+    const int64_t r = u / w;
+    p[r * ld + cols + (u - r * w)] = (T)0.0f;
+  }
+}
+
+// The bias's gradient: the chunks' column sums, added in order by 16 thread rows.
+template <typename T>
+__global__ __launch_bounds__(256) void dbias_kernel(const float* part, int chunks, int n, void* dst, int f32) {
+  __shared__ float sum[16][16];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, col = blockIdx.x * 16 + tx;
+  float s = 0.0f;
+  if (col < n)
+    for (int q = ty; q < chunks; q += 16) s += part[(int64_t)q * n + col];
+  sum[ty][tx] = s;
+  __syncthreads();
+  if (ty != 0 || col >= n) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += sum[i][tx];
+  if (f32)
+    static_cast<float*>(dst)[col] = s;
+  else
+    static_cast<T*>(dst)[col] = (T)s;
+}
+
+using Big = Tile<2, 4, 4>;    // 256 x 256, 8 waves of 128 x 64, one workgroup a CU
+using Small = Tile<2, 2, 2>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
+
+template <typename T, bool AK, bool BKC, typename TL>
+hipError_t run_tiles(const GemmArgs& a, hipStream_t st) {
+  const int tiles = a.tm * a.tn, rest = tiles - a.whole;
+  gemm_kernel<T, AK, BKC, TL><<<a.whole + rest * a.parts, TL::NT, 0, st>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || rest == 0) return e;
+  join_kernel<T, TL><<<rest * TL::WAVES * TL::MI / 4, 256, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T, bool AK, bool BKC>
+hipError_t run_shape(const GemmArgs& a, hipStream_t st) {
+  return a.big ? run_tiles<T, AK, BKC, Big>(a, st) : run_tiles<T, AK, BKC, Small>(a, st);
+}
+
+template <typename T>
+hipError_t run_skinny(const GemmArgs& a, hipStream_t st) {
+  const int swap = a.skinny == 2;
+  const int64_t len = swap ? a.m : a.n, s = swap ? a.n : a.m;
+  const uint32_t grid = (uint32_t)((len + 15) / 16);
+  constexpr int NT = 64 * kSkinnyWaves;
+  if (a.act == kActSwiglu) {
+    if (s <= 16) skinny_kernel<T, 1, true><<<grid, NT, 0, st>>>(a, swap);
+    else skinny_kernel<T, 2, true><<<grid, NT, 0, st>>>(a, swap);
+  } else if (s <= 16) skinny_kernel<T, 1, false><<<grid, NT, 0, st>>>(a, swap);
+  else if (s <= 32) skinny_kernel<T, 2, false><<<grid, NT, 0, st>>>(a, swap);
+  else skinny_kernel<T, 4, false><<<grid, NT, 0, st>>>(a, swap);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run(const GemmArgs& a, hipStream_t st) {
+  if (a.skinny) return run_skinny<T>(a, st);
+  if (a.a_kc && a.b_kc) return run_shape<T, true, true>(a, st);
+  if (a.a_kc) return run_shape<T, true, false>(a, st);
+  return run_shape<T, false, false>(a, st);
+}
+
+}  // namespace
+
+void gemm_plan(GemmArgs& a) {
+  const bool glu = a.act == kActSwiglu;
+  a.kt = (int)((a.k + kBK - 1) / kBK);
+  a.skinny = 0;
+  if (a.a_kc && a.b_kc) {
+    const int64_t most = glu ? 32 : 64;
+    if (a.m <= most) a.skinny = 1;
+    else if (a.n <= 64 && !glu) a.skinny = 2;
+  }
+  a.part_floats = 0;
+  a.parts = 1;
+  a.tm = a.tn = a.whole = 0;
+  if (a.skinny) return;
+  // the tile shape and the split of the last round's tiles with the least estimated time,
+  // in stages of a 256 x 256 tile (about 1 us); see the measurements there
+  double best = 1e30;
+  for (int big = 1; big >= 0; --big) {
+    const int bm = big ? Big::BM : Small::BM, bn = (big ? Big::BN : Small::BN) / (glu ? 2 : 1);
+    const int64_t tm = (a.m + bm - 1) / bm, tn = (a.n + bn - 1) / bn, tiles = tm * tn;
+    const int slots = big ? 256 : 512;
+    const double stage = big ? 1.0 : 0.75, start = 4.0;  // two small tiles share a CU
+    for (int p = 1; p <= 16; ++p) {
+      const int64_t rest = p == 1 ? 0 : tiles % slots;
+      if (p > 1 && (rest == 0 || a.kt / p < 4)) continue;
+      const int64_t whole = tiles - rest;
+      double cost = (double)((whole + slots - 1) / slots) * (a.kt * stage + start);
+      if (rest) {
+        const double bytes = (double)rest * p * bm * (big ? Big::BN : Small::BN) * 4;
+        cost += (double)((rest * p + slots - 1) / slots) * ((a.kt + p - 1) / p * stage + start) + 6.0 + bytes * 2 / 4e6;
+      }
+      if (cost < best) {
+        best = cost;
+        a.big = big;
+        a.tm = (int)tm;
+        a.tn = (int)tn;
+        a.whole = (int)whole;
+        a.parts = p;
+        a.part_floats = rest * p * bm * (big ? Big::BN : Small::BN);
+      }
+    }
+  }
+}
+
+hipError_t launch_gemm(const GemmArgs& a, int f16, hipStream_t st) {
+  return f16 ? run<_Float16>(a, st) : run<__bf16>(a, st);
+}
+
+hipError_t launch_pack(int f16, const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t pc,
+                       hipStream_t st) {
+  const int64_t units = rows * (pc / 8), blocks = (units + 255) / 256;
+  const uint32_t grid = (uint32_t)(blocks < 4096 ? blocks : 4096);
+  // both types are 16 bits wide and copied as they are
+  (void)f16;
+  pack_kernel<__bf16><<<grid, 256, 0, st>>>(static_cast<const __bf16*>(src), ld, rows, cols, static_cast<__bf16*>(dst), pc);
+  return hipGetLastError();
+}
+
+hipError_t launch_dact(int f16, const DactArgs& a, hipStream_t st) {
+  const dim3 grid((uint32_t)((a.n + 511) / 512), (uint32_t)a.chunks);
+  const int64_t rows = a.act == kActSwiglu ? 2 * a.n : a.n;
+  if (a.dz && a.ldz > rows) {
+    const int64_t blocks = (a.m * (a.ldz - rows) + 255) / 256;
+    clear_tail_kernel<__bf16><<<(uint32_t)(blocks < 1024 ? blocks : 1024), 256, 0, st>>>(
+        static_cast<__bf16*>(a.dz), a.m, a.ldz, (int)rows);
+  }
+  if (f16)
+    dact_kernel<_Float16><<<grid, 256, 0, st>>>(a);
+  else
+    dact_kernel<__bf16><<<grid, 256, 0, st>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !a.part) return e;
+  if (f16)
+    dbias_kernel<_Float16><<<(uint32_t)((rows + 15) / 16), 256, 0, st>>>(a.part, (int)a.chunks, (int)rows, a.dbias, a.bias_f32);
+  else
+    dbias_kernel<__bf16><<<(uint32_t)((rows + 15) / 16), 256, 0, st>>>(a.part, (int)a.chunks, (int)rows, a.dbias, a.bias_f32);
+  return hipGetLastError();
+}
+
+}  // namespace sage

@@ -260,33 +260,29 @@ struct BwdRow {
   }
 };
 
-// Adds the groups' channel sums in order and stores them as one partial row.
+// Adds the groups' channel sums (halves of the groups at a time, a fixed tree) and stores
+// them as one partial row.  `sum`: G / 2 rows of TPR * kPer floats.
 template <int TPR, bool VEC>
-__device__ __forceinline__ void store_partial(float* dst, float* sum, int grp, int t, int c, const float (&acc)[kPer]) {
-  constexpr int G = kBwdNT / TPR;
-  if constexpr (G == 1) {
+__device__ __forceinline__ void store_partial(float* dst, float* sum, int grp, int t, int c, float (&acc)[kPer]) {
+#pragma unroll
+  for (int half = kBwdNT / TPR / 2; half > 0; half /= 2) {
+    // a thread's value j lies at j * TPR + t: no bank conflicts
+    if (grp >= half && grp < 2 * half) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) sum[((grp - half) * kPer + j) * TPR + t] = acc[j];
+    }
+    __syncthreads();
+    if (grp < half) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) acc[j] += sum[(grp * kPer + j) * TPR + t];
+    }
+    __syncthreads();
+  }
+  if (grp == 0) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int at = Cols<TPR, VEC>::col(t, j);
       if (at < c) dst[at] = acc[j];
-    }
-  } else {
-#pragma unroll 1
-    for (int g = 0; g < G; ++g) {
-      if (g == grp) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          // conflict-free order: a thread's value j lies at j * TPR + t
-          const float v = g == 0 ? acc[j] : sum[j * TPR + t] + acc[j];
-          if (g + 1 < G) {
-            sum[j * TPR + t] = v;
-          } else {
-            const int at = Cols<TPR, VEC>::col(t, j);
-            if (at < c) dst[at] = v;
-          }
-        }
-      }
-      __syncthreads();
     }
   }
 }
@@ -303,7 +299,7 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
   constexpr int SETS = OP == kNormGateModulate ? 2 : 1;
   constexpr bool kScale = OP == kNormModulate;
   __shared__ float red[2][W * 2], red1[W], red3[W];
-  __shared__ float sum[G == 1 ? 1 : TPR * kPer];
+  __shared__ float sum[G == 1 ? 1 : G / 2 * TPR * kPer];
   __shared__ int ids_min[W], counts[W];
   __shared__ uint16_t list[kBwdNT];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -347,15 +343,15 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
       prev = id;
       __syncthreads();
     }
-    float wm[kPer], wm2[kPer], acc[kPer] = {}, acc2[kPer] = {};
-    weight_row<T, TPR, VEC>(a.w, a.cond, kScale, b, id, t, c, wm);
-    if constexpr (SETS == 2) weight_row<T, TPR, VEC>(a.w2, a.cond2, true, b, id, t, c, wm2);
-
+    // the first tokens' loads, then the parameters', in flight together
     const bool gated = kScale || !no_document(a, id);
     BwdRow<T, OP, TPR, VEC> cur, next;
     auto token = [&](int pos) { return n0 + (a.doc ? __builtin_amdgcn_readfirstlane(list[pos]) : pos); };
     // a group past its last token loads nothing (its channels are zeros)
     cur.load(a, b, grp < run ? token(grp) : n0, t, grp < run ? c : 0, gated);
+    float wm[kPer], wm2[kPer], acc[kPer] = {}, acc2[kPer] = {};
+    weight_row<T, TPR, VEC>(a.w, a.cond, kScale, b, id, t, c, wm);
+    if constexpr (SETS == 2) weight_row<T, TPR, VEC>(a.w2, a.cond2, true, b, id, t, c, wm2);
     const int iters = (run + G - 1) / G;
 #pragma unroll 1
     for (int it = 0; it < iters; ++it) {
@@ -438,7 +434,7 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
 // thread rows every 32nd chunk, added in order at the end.  The loads of kBatch chunks are
 // in flight together: with one chunk at a time and 16 thread rows the kernel took 22 us
 // at 256 chunks of 3840 channels, all of it latency.
-constexpr int kParamRows = 32, kBatch = 4;
+constexpr int kParamRows = 32, kBatch = 8;
 
 template <typename T>
 __global__ __launch_bounds__(16 * kParamRows) void norm_param_kernel(NormArgs a, int sets, int modulate) {
@@ -491,9 +487,13 @@ __global__ __launch_bounds__(16 * kParamRows) void norm_param_kernel(NormArgs a,
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int q = q0 + i * kParamRows;
+        v[i] = q < last ? partial(q, 0) : f32x4{};  // the loads do not wait for the ids
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
         const bool use = id[i] >= 0 && (dw || id[i] == g);
-        v[i] = use ? partial(q, 0) : f32x4{};
-        m[i] = use ? factor(q, id[i]) : f32x4{};
+        m[i] = use ? factor(q0 + i * kParamRows, id[i]) : f32x4{};
+        if (!use) v[i] = f32x4{};
       }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {

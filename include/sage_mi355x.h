@@ -471,6 +471,49 @@ int sage_rms_norm_gate_residual_modulate_bwd(
     size_t workspace_bytes, void* dresidual, void* dx, void* dweight, void* dgate, void* dnext_weight,
     void* dnext_scale, hipStream_t stream);
 
+/* ---- Linear layers ------------------------------------------------------------
+ *
+ * out = act(x weight^T + bias) + residual, bf16 or fp16, fp32 accumulation, one rounding.
+ *   x            [m][k] rows x_rs elements apart; weight [rows][k] rows w_rs apart, rows =
+ *                n, or 2 n for SAGE_ACT_SWIGLU (z has 2 n columns and
+ *                out = silu(z[:, :n]) * z[:, n:] + residual).  Columns contiguous.
+ *   bias         [rows] of dtype, or fp32 (bias_fp32), or null.
+ *   residual     [m][n] rows r_rs apart, or null.
+ *   activation   SAGE_ACT_*; gelu is the tanh form.
+ *   z            [m][rows] contiguous or null: x weight^T + bias rounded to dtype, which
+ *                the gradient of an activation needs.
+ *   out          [m][n] contiguous.
+ *   workspace    sage_linear_workspace_bytes(...) bytes, 16-byte aligned; needs no clearing.
+ * m, n, k at least 1; a weight or a row panel of 256 rows has under 2^31 bytes.  Rows of x
+ * and weight that do not start on 16-byte boundaries, or a k that is no multiple of 8, are
+ * copied into the workspace first. */
+#define SAGE_ACT_NONE 0
+#define SAGE_ACT_SILU 1
+#define SAGE_ACT_GELU 2
+#define SAGE_ACT_SWIGLU 3
+
+size_t sage_linear_workspace_bytes(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, int64_t m,
+                                   int64_t n, int64_t k, int activation);
+int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, const void* bias, int bias_fp32,
+                const void* residual, int64_t r_rs, int64_t m, int64_t n, int64_t k, int dtype, int activation,
+                void* workspace, size_t workspace_bytes, void* z, void* out, hipStream_t stream);
+
+/* Gradients of sage_linear: dx [m][k], dweight [rows][k], dbias [rows] (dtype or fp32), each
+ * null if not wanted; the residual's is dout itself.  dz = dout * act'(z) is rounded to dtype
+ * as the products' operand (the bias's gradient adds it unrounded); sums are in a fixed order.
+ *   dout         [m][n] rows d_rs apart.
+ *   z            what sage_linear kept; null with SAGE_ACT_NONE.
+ *   x            null if dweight is; weight null if dx is.
+ *   workspace    sage_linear_bwd_workspace_bytes(...) bytes for the same arguments (want: bit
+ *                0 dx, 1 dweight, 2 dbias). */
+size_t sage_linear_bwd_workspace_bytes(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
+                                       const void* weight, int64_t w_rs, int64_t m, int64_t n, int64_t k,
+                                       int activation, int want);
+int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs, const void* weight, int64_t w_rs,
+                    const void* z, int64_t m, int64_t n, int64_t k, int dtype, int activation, int bias_fp32,
+                    void* workspace, size_t workspace_bytes, void* dx, void* dweight, void* dbias,
+                    hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

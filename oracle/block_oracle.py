@@ -135,3 +135,83 @@ def norms(op: str, x: Tensor, weight, cond, doc_ids, eps: float, residual=None, 
         out["dcond"] = (_row_sums(d * xhat * w, cond, doc_ids),
                         _row_sums((700 * U32 * d.abs() + derr) * (xhat * w).abs(), cond, doc_ids))
     return out
+
+
+def _act(kind: str, z: Tensor):
+    """The activation, its derivative, and bounds on both: how far 32-bit arithmetic is off."""
+    if kind == "none":
+        return z, torch.ones_like(z), torch.zeros_like(z), torch.zeros_like(z)
+    if kind in ("silu", "swiglu"):
+        u, up = z, torch.ones_like(z)
+    else:
+        a = math.sqrt(8 / math.pi)
+        u, up = a * (z + 0.044715 * z ** 3), a * (1 + 3 * 0.044715 * z * z)
+    s = torch.sigmoid(u)
+    # exp(-u) by way of 2^: the exponent's rounding is |u| steps, the rest a few; s (1 - s) of
+    # it reaches s; 1 - s cancels to half a step of 1
+    serr = U32 * (s * (1 - s) * (2 * u.abs() + 4) + 4 * s)
+    f, d = z * s, s + z * s * (1 - s) * up
+    ferr = z.abs() * serr + 2 * U32 * f.abs()
+    derr = serr + (z * up).abs() * (serr * (1 - 2 * s).abs() + U32 * s + 8 * U32 * s * (1 - s)) + 4 * U32 * d.abs()
+    return f, d, ferr, derr
+
+
+def linear(x: Tensor, weight: Tensor, bias, residual, activation: str, dout=None) -> dict[str, tuple[Tensor, Tensor]]:
+    """``{name: (exact, bound)}`` of fused_linear's output, and with ``dout`` its gradients.
+
+    A product of K terms is summed in any order: K roundings of at most the sum of the
+    terms' sizes.  The gradient of an activation takes the rounded z, and its own rounding
+    as the products' operand: half a step of the type each.
+    """
+    eps = torch.finfo(x.dtype).eps
+    xd, wd = x.double().reshape(-1, x.shape[-1]), weight.double()
+    M, K = xd.shape
+    z = xd @ wd.T
+    zerr = (K + 2) * U32 * (xd.abs() @ wd.abs().T)
+    if bias is not None:
+        z = z + bias.double()
+        zerr = zerr + U32 * (z.abs() + bias.double().abs())
+    N = wd.shape[0]
+    if activation == "swiglu":
+        z1, z2 = z.chunk(2, -1)
+        e1, e2 = zerr.chunk(2, -1)
+        f, d, ferr, derr = _act(activation, z1)
+        out, oerr = f * z2, (ferr + e1 * 1.1) * (z2.abs() + e2) + f.abs() * e2 + U32 * (f * z2).abs()
+    else:
+        f, d, ferr, derr = _act(activation, z)
+        out, oerr = f, ferr + zerr * (1.0 if activation == "none" else 1.2)
+    if residual is not None:
+        out = out + residual.double().reshape(M, -1)
+        oerr = oerr + U32 * out.abs()
+    shape = (*x.shape[:-1], out.shape[-1])
+    r = {"out": (out.reshape(shape), oerr.reshape(shape))}
+    if dout is None:
+        return r
+    g = dout.double().reshape(M, -1)
+
+    def kept(zz, ee):  # z as the backward has it: half a step off
+        return ee + eps / 2 * (zz.abs() + ee).clamp_min(torch.finfo(x.dtype).tiny)
+
+    if activation == "none":
+        dz, unrounded, rounded = g, torch.zeros_like(g), torch.zeros_like(g)
+    else:
+        # |act''| is at most 0.5 (silu) and 1.13 (gelu)
+        curve = 0.5 if activation in ("silu", "swiglu") else 1.13
+        if activation == "swiglu":
+            k1, k2 = kept(z1, e1), kept(z2, e2)
+            a, b = g * z2 * d, g * f
+            ae = g.abs() * (k2 * (d.abs() + derr) + z2.abs() * (curve * k1 + derr)) + g.abs() * k2 * curve * k1
+            be = g.abs() * (1.1 * k1 + ferr)
+            dz, unrounded = torch.cat([a, b], -1), torch.cat([ae, be], -1)
+        else:
+            dz, unrounded = g * d, g.abs() * (curve * kept(z, zerr) + derr)
+        unrounded = unrounded + 4 * U32 * dz.abs()
+        rounded = unrounded + eps / 2 * (dz.abs() + unrounded).clamp_min(torch.finfo(x.dtype).tiny)
+    mag = dz.abs() + rounded
+    r["dx"] = ((dz @ wd).reshape(x.shape), (rounded @ wd.abs() + (N + 2) * U32 * (mag @ wd.abs())).reshape(x.shape))
+    r["dweight"] = (dz.T @ xd, rounded.T @ xd.abs() + (M + 2) * U32 * (mag.T @ xd.abs()))
+    if bias is not None:
+        r["dbias"] = (dz.sum(0), (unrounded + (M + 2) * U32 * (dz.abs() + unrounded)).sum(0))
+    if residual is not None:
+        r["dresidual"] = (dout.double(), torch.zeros_like(dout.double()))
+    return r
