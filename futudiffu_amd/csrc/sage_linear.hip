@@ -207,7 +207,7 @@ struct Operand {
   }
   // Issues the loads of contraction k0 .. k0 + kBK - 1 of K into `lds`.
   __device__ __forceinline__ void issue(uint8_t* lds, int64_t k0, int64_t K, int wave) const {
-    const int left = (int)(K - k0 < kBK ? K - k0 : kBK);
+    const int left = (int)(K - k0 < kBK ? K - k0 : kBK);  // 0 or less behind the end
     if constexpr (KC) {
       // rows past the last have an offset past any size; so get chunks past K
       const __amdgpu_buffer_rsrc_t rs = raw_rsrc(base + k0 * 2, 0x7fffffff);
@@ -325,6 +325,10 @@ __device__ __forceinline__ int xcd_share(int b, int total) {
   return x * per + min(x, rem) + local;
 }
 
+// The scheduler's next instruction of a kind.
+__device__ __forceinline__ void order_mfma() { __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
+__device__ __forceinline__ void order_read() { __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
+
 template <typename T, bool AK, bool BKC, typename TL>
 __global__ __launch_bounds__(TL::NT, 2) void gemm_kernel(GemmArgs a) {
   __shared__ __align__(1024) uint8_t lds[TL::LDS];
@@ -360,32 +364,74 @@ __global__ __launch_bounds__(TL::NT, 2) void gemm_kernel(GemmArgs a) {
 #pragma unroll
   for (int i = 0; i < TL::NI; ++i) fb[i].init((wn * TL::NI + i) * 32, lane);
 
+  // A stage's four steps of 16, the next step's fragments read under this one's products.
+  // Before a stage's last step the next stage's loads have arrived and every wave has read
+  // this one's last fragments: behind that barrier the loads after next go into its place,
+  // and the last products run beside the next stage's first reads.  Loads past the last
+  // stage read nothing or are not used.
+  using V = typename Vec8<T>::type;
   f32x16 acc[TL::MI][TL::NI] = {};
-  A.issue(lds, (int64_t)kt0 * kBK, AK ? a.k : a.kv, wave);
-  B.issue(lds + TL::A_BYTES, (int64_t)kt0 * kBK, BKC ? a.k : a.kv, wave);
-  for (int kt = kt0; kt < kt1; ++kt) {
-    wait_vmem();
+  V va[2][TL::MI], vb[2][TL::NI];
+  const int64_t ka = AK ? a.k : a.kv, kb = BKC ? a.k : a.kv;
+  auto read = [&](const uint8_t* sa, int s, int to) {
+#pragma unroll
+    for (int i = 0; i < TL::NI; ++i) vb[to][i] = frag<T>(sa + TL::A_BYTES, fb[i], s);
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i) va[to][i] = frag<T>(sa, fa[i], s);
+  };
+  auto products = [&](int from) {
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::NI; ++j) acc[i][j] = mfma32(va[from][i], vb[from][j], acc[i][j]);
+  };
+  // the order of one step: a product, then reads of the next step, and so on
+  auto order = [&]() {
+    constexpr int M = TL::MI * TL::NI, R = TL::MI * (AK ? 1 : 2) + TL::NI * (BKC ? 1 : 2);
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      order_mfma();
+      if constexpr (R > M) order_read();
+      order_read();
+    }
+  };
+  A.issue(lds, (int64_t)kt0 * kBK, ka, wave);
+  B.issue(lds + TL::A_BYTES, (int64_t)kt0 * kBK, kb, wave);
+  wait_vmem();
+  __syncthreads();
+  A.issue(lds + TL::STAGE, (int64_t)(kt0 + 1) * kBK, ka, wave);
+  B.issue(lds + TL::STAGE + TL::A_BYTES, (int64_t)(kt0 + 1) * kBK, kb, wave);
+  read(lds, 0, 0);
+  for (int kt = kt0; kt + 1 < kt1; ++kt) {
+    uint8_t* here = lds + ((kt - kt0) & 1) * TL::STAGE;
+    read(here, 1, 1);
+    products(0);
+    order();
+    read(here, 2, 0);
+    products(1);
+    order();
+    read(here, 3, 1);
+    products(0);
+    order();
+    __builtin_amdgcn_s_waitcnt(0x0070);  // every load and LDS read
     __syncthreads();
-    if (kt + 1 < kt1) {
-      uint8_t* next = lds + ((kt + 1 - kt0) & 1) * TL::STAGE;
-      A.issue(next, (int64_t)(kt + 1) * kBK, AK ? a.k : a.kv, wave);
-      B.issue(next + TL::A_BYTES, (int64_t)(kt + 1) * kBK, BKC ? a.k : a.kv, wave);
-    }
-    const uint8_t* sa = lds + ((kt - kt0) & 1) * TL::STAGE;
-    const uint8_t* sb = sa + TL::A_BYTES;
-#pragma unroll
-    for (int s = 0; s < kBK / 16; ++s) {
-      typename Vec8<T>::type va[TL::MI], vb[TL::NI];
-#pragma unroll
-      for (int i = 0; i < TL::MI; ++i) va[i] = frag<T>(sa, fa[i], s);
-#pragma unroll
-      for (int i = 0; i < TL::NI; ++i) vb[i] = frag<T>(sb, fb[i], s);
-#pragma unroll
-      for (int i = 0; i < TL::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < TL::NI; ++j) acc[i][j] = mfma32(va[i], vb[j], acc[i][j]);
-    }
+    A.issue(here, (int64_t)(kt + 2) * kBK, ka, wave);
+    B.issue(here + TL::A_BYTES, (int64_t)(kt + 2) * kBK, kb, wave);
+    read(lds + ((kt + 1 - kt0) & 1) * TL::STAGE, 0, 0);
+    products(1);
+    order();
   }
+  {
+    const uint8_t* here = lds + ((kt1 - 1 - kt0) & 1) * TL::STAGE;
+    read(here, 1, 1);
+    products(0);
+    read(here, 2, 0);
+    products(1);
+    read(here, 3, 1);
+    products(0);
+    products(1);
+  }
+  wait_vmem();
   __syncthreads();
   if (cut) {
     // the piece's sums, in the order the lanes hold them
