@@ -1051,6 +1051,7 @@ int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, c
   g.out = out;
   g.vec = n % 8 == 0 && aligned16(out) && (!z || aligned16(z)) &&
           (!residual || (aligned16(residual) && (m == 1 || r_rs % 8 == 0)));
+  g.vec_b = n % 8 == 0 && aligned16(bias);
   g.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at);
   return launch_status(sage::launch_gemm(g, dtype, stream), "sage_linear");
 }

@@ -385,6 +385,7 @@ struct GemmArgs {
   void* z;    // T [m][rows of B]: acc + bias, for the backward; null: not kept
   void* out;  // T [m][n]
   int vec;    // rows of res, z and out take 16-byte accesses
+  int vec_b;  // so does the bias
   // the plan (gemm_plan)
   int big, skinny, kt, tm, tn;
   int whole, parts;     // tiles past `whole` run as `parts` pieces of the contraction

@@ -105,55 +105,121 @@ __device__ __forceinline__ float param_at(const void* p, bool f32, bool f16, int
   return f16 ? (float)static_cast<const _Float16*>(p)[i] : (float)static_cast<const __bf16*>(p)[i];
 }
 
-// Bias of eight columns from row `at` of the weight on (columns past `cols`: zeros).
+// Bias of eight columns, `at` rows into the weight (columns past `cols`: zeros).
 template <typename T>
 __device__ __forceinline__ void load_bias(const GemmArgs& a, int at, int n, int cols, float (&f)[8]) {
+  if (a.bias_f32) {
+    const float* b = static_cast<const float*>(a.bias) + at;
+    if (a.vec_b) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    f[j] = a.bias && n + j < cols ? param_at(a.bias, a.bias_f32, std::is_same<T, _Float16>::value, at + n + j) : 0.0f;
+      for (int q = 0; q < 2; ++q) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(b + n + 4 * q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[4 * q + j] = v[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = n + j < cols ? b[n + j] : 0.0f;
+    }
+  } else {
+    load8<T>(static_cast<const T*>(a.bias) + at, n, cols, a.vec_b, f);
+  }
 }
 
-// The epilogue of row m, columns n .. n + 7 (n < a.n): z = acc + bias, kept when the backward wants it,
-// out = act(z) + residual, rounded once.  z2 and b2: the second half of a swiglu.
-template <typename T>
-__device__ __forceinline__ void finish8(const GemmArgs& a, int64_t m, int n, float (&z)[8], float (&z2)[8],
-                                        const float (&b)[8], const float (&b2)[8]) {
-  const bool glu = a.act == kActSwiglu;
+// The epilogue of row m, columns n .. n + 7 (n < a.n): z = acc + bias, kept when the backward
+// wants it, out = act(z) + residual, rounded once.  z2: the second half of a swiglu.
+template <typename T, int ACT>
+__device__ __forceinline__ void finish8(const GemmArgs& a, int64_t m, int n, float (&z)[8], float (&z2)[8]) {
+  constexpr bool kGlu = ACT == kActSwiglu;
+  if (a.bias) {
+    float b[8];
+    load_bias<T>(a, 0, n, a.n, b);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    z[j] += b[j];
-    if (glu) z2[j] += b2[j];
+    for (int j = 0; j < 8; ++j) z[j] += b[j];
+    if constexpr (kGlu) {
+      load_bias<T>(a, a.n, n, a.n, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z2[j] += b[j];
+    }
   }
-  if (a.z) {
-    T* row = static_cast<T*>(a.z) + m * (glu ? 2 * (int64_t)a.n : a.n);
+  if (ACT != kActNone && a.z) {
+    T* row = static_cast<T*>(a.z) + m * (kGlu ? 2 * (int64_t)a.n : a.n);
     store8<T>(row, n, a.n, a.vec, z);
-    if (glu) store8<T>(row + a.n, n, a.n, a.vec, z2);
+    if constexpr (kGlu) store8<T>(row + a.n, n, a.n, a.vec, z2);
   }
-  float r[8] = {};
-  if (a.res) load8<T>(static_cast<const T*>(a.res) + m * a.ldr, n, a.n, a.vec, r);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    float y = act_fwd(a.act, z[j]);
-    if (glu) y *= z2[j];
-    z[j] = y + r[j];
+    z[j] = act_fwd(ACT, z[j]);
+    if constexpr (kGlu) z[j] *= z2[j];
+  }
+  if (a.res) {
+    float r[8];
+    load8<T>(static_cast<const T*>(a.res) + m * a.ldr, n, a.n, a.vec, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z[j] += r[j];
   }
   store8<T>(static_cast<T*>(a.out) + m * a.n, n, a.n, a.vec, z);
+}
+
+// A 32 x 32 block of the output (or its two halves of a swiglu) from the accumulators of
+// the transposed product, in which lane (h, r) holds row r, columns 8 J + 4 h + i: swapping
+// J = 1 of the lower lanes with J = 0 of the upper gives each lane eight consecutive columns,
+// one 16-byte store, with no pass through LDS.
+template <typename T, int ACT>
+__device__ __forceinline__ void finish_block(const GemmArgs& a, int lane, int64_t m0, int n0, f32x16 c, f32x16 c2) {
+  const int64_t m = m0 + (lane & 31);
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    float z[8], z2[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(c[8 * p + i]), __float_as_uint(c[8 * p + 4 + i]),
+                                                      false, false);
+      z[i] = __uint_as_float(s[0]);
+      z[4 + i] = __uint_as_float(s[1]);
+      if constexpr (ACT == kActSwiglu) {
+        const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(c2[8 * p + i]),
+                                                        __float_as_uint(c2[8 * p + 4 + i]), false, false);
+        z2[i] = __uint_as_float(u[0]);
+        z2[4 + i] = __uint_as_float(u[1]);
+      }
+    }
+    const int n = n0 + 16 * p + 8 * (lane >> 5);
+    if (m < a.m && n < a.n) finish8<T, ACT>(a, m, n, z, z2);
+  }
+}
+
+// A wave's MI x NI blocks from row m0 and tile column n0 on.
+template <typename T, int ACT, int MI, int NI>
+__device__ __forceinline__ void finish_wave(const GemmArgs& a, int lane, int64_t m0, int n0, f32x16 (&c)[MI][NI]) {
+  constexpr bool kGlu = ACT == kActSwiglu;
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; j += kGlu ? 2 : 1)
+      finish_block<T, ACT>(a, lane, m0 + 32 * i, n0 + (kGlu ? 16 : 32) * j, c[i][j], c[i][kGlu ? j + 1 : j]);
+}
+
+template <typename T, int MI, int NI>
+__device__ __forceinline__ void finish(const GemmArgs& a, int lane, int64_t m0, int n0, f32x16 (&c)[MI][NI]) {
+  if (a.act == kActSwiglu) finish_wave<T, kActSwiglu>(a, lane, m0, n0, c);
+  else if (a.act == kActSilu) finish_wave<T, kActSilu>(a, lane, m0, n0, c);
+  else if (a.act == kActGelu) finish_wave<T, kActGelu>(a, lane, m0, n0, c);
+  else finish_wave<T, kActNone>(a, lane, m0, n0, c);
 }
 
 // ---------------------------------------------------------------- tiles
 
 constexpr int kBK = 64;  // contraction of one LDS stage
 
-// A tile shape: WM x WN waves, each with MI x 2 blocks of 32 x 32.
-template <int WM_, int WN_, int MI_>
+// A tile shape: WM x WN waves, each with MI x NI blocks of 32 x 32, `SIMD` waves a SIMD.
+template <int WM_, int WN_, int MI_, int NI_, int SIMD_>
 struct Tile {
-  static constexpr int WM = WM_, WN = WN_, MI = MI_, NI = 2;
+  static constexpr int WM = WM_, WN = WN_, MI = MI_, NI = NI_, SIMD = SIMD_;
   static constexpr int WAVES = WM * WN, NT = 64 * WAVES;
   static constexpr int BM = WM * MI * 32, BN = WN * NI * 32;
-  static constexpr int A_BYTES = BM * kBK * 2, B_BYTES = BN * kBK * 2, STAGE = A_BYTES + B_BYTES;
-  static constexpr int kPitch = 72;                        // floats of an epilogue row: see epilogue()
-  static constexpr int EPI = WAVES * 32 * kPitch * 4;
-  static constexpr int LDS = 2 * STAGE > EPI ? 2 * STAGE : EPI;
+  static constexpr int A_BYTES = BM * kBK * 2, B_BYTES = BN * kBK * 2, B_AT = 3 * A_BYTES;
+  static constexpr int LDS = 3 * A_BYTES + 2 * B_BYTES;
 };
 
 // One direct global -> LDS load of 64 chunks: lane l's 16 bytes land at lds + 16 l; an
@@ -205,27 +271,19 @@ struct Operand {
       }
     }
   }
-  // Issues the loads of contraction k0 .. k0 + kBK - 1 of K into `lds`.
+  // Issues loads FIRST .. FIRST + COUNT - 1 of contraction k0 .. k0 + kBK - 1 of K into `lds`.
+  template <int FIRST, int COUNT>
   __device__ __forceinline__ void issue(uint8_t* lds, int64_t k0, int64_t K, int wave) const {
     const int left = (int)(K - k0 < kBK ? K - k0 : kBK);  // 0 or less behind the end
-    if constexpr (KC) {
-      // rows past the last have an offset past any size; so get chunks past K
-      const __amdgpu_buffer_rsrc_t rs = raw_rsrc(base + k0 * 2, 0x7fffffff);
+    // KC: rows past the last have an offset past any size, and so get chunks past K.  Not
+    // KC: columns past the last read what follows in memory (they reach outputs that are not
+    // stored alone), up to the end of the last row, in whole 4 bytes; rows past K read zeros.
+    const __amdgpu_buffer_rsrc_t rs =
+        KC ? raw_rsrc(base + k0 * 2, 0x7fffffff)
+           : raw_rsrc(base + k0 * ld2, left > 0 ? (uint32_t)((left - 1) * ld2 + (valid + 1) / 2 * 4) : 0u);
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int o = kpos < left ? off[i] : (int)0x80000000;
-        dma_16(lds + (i * WAVES + wave) * 1024, rs, o);
-      }
-    } else {
-      // columns past the last read what follows in memory (they reach outputs that are
-      // not stored alone), up to the end of the last row, in whole 4 bytes; rows past K
-      // read zeros
-      const __amdgpu_buffer_rsrc_t rs =
-          raw_rsrc(base + k0 * ld2, left > 0 ? (uint32_t)((left - 1) * ld2 + (valid + 1) / 2 * 4) : 0u);
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i)
-        dma_16(lds + (i * WAVES + wave) * 1024, rs, off[i]);
-    }
+    for (int i = FIRST; i < FIRST + COUNT; ++i)
+      dma_16(lds + (i * WAVES + wave) * 1024, rs, !KC || kpos < left ? off[i] : (int)0x80000000);
   }
 };
 
@@ -266,48 +324,6 @@ __device__ __forceinline__ typename Vec8<T>::type frag(const uint8_t* __restrict
   }
 }
 
-// A 32 x 64 block of one wave's sums (two accumulators, or the two halves of a swiglu)
-// through its own part of LDS to rows of eight columns a lane.  The pitch of 72 floats
-// puts the two rows a store instruction writes (4 apart) on different banks.
-template <typename T>
-__device__ __forceinline__ void epilogue(const GemmArgs& a, float* lds, int lane, int64_t m0, int n0, f32x16 c0,
-                                         f32x16 c1) {
-  constexpr int P = 72;
-  const bool glu = a.act == kActSwiglu;
-  const int h = lane >> 5, r = lane & 31;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int row = 8 * (i >> 2) + 4 * h + (i & 3);
-    lds[row * P + r] = c0[i];
-    lds[row * P + 32 + r] = c1[i];
-  }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  // glu: 4 lanes a row of 32 columns; else 8 lanes a row of 64
-  const int per = glu ? 4 : 8, rows = 64 / per;
-  const int lr = lane / per, n = n0 + lane % per * 8;
-  if (n < a.n) {
-    float b[8], b2[8] = {};
-    load_bias<T>(a, 0, n, a.n, b);
-    if (glu) load_bias<T>(a, a.n, n, a.n, b2);
-    for (int row = lr; row < 32; row += rows) {
-      const int64_t m = m0 + row;
-      if (m < a.m) {
-        float z[8], z2[8] = {};
-        const float* src = lds + row * P + lane % per * 8;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          z[j] = src[j];
-          if (glu) z2[j] = src[32 + j];
-        }
-        finish8<T>(a, m, n, z, z2, b, b2);
-      }
-    }
-  }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 // Tile t of the schedule: groups of 4 tile rows, column by column inside, so that the 32
 // tiles an XCD runs together share 4 row panels and 8 column panels.
 __device__ __forceinline__ void tile_at(const GemmArgs& a, int t, int& tm, int& tn) {
@@ -325,12 +341,34 @@ __device__ __forceinline__ int xcd_share(int b, int total) {
   return x * per + min(x, rem) + local;
 }
 
+// Waits for every LDS read and for all but the last LEFT direct loads.
+template <int LEFT>
+__device__ __forceinline__ void wait_loads();
+template <>
+__device__ __forceinline__ void wait_loads<4>() { __builtin_amdgcn_s_waitcnt(0x0074); }
+template <>
+__device__ __forceinline__ void wait_loads<6>() { __builtin_amdgcn_s_waitcnt(0x0076); }
+template <>
+__device__ __forceinline__ void wait_loads<8>() { __builtin_amdgcn_s_waitcnt(0x0078); }
+template <>
+__device__ __forceinline__ void wait_loads<12>() { __builtin_amdgcn_s_waitcnt(0x007c); }
+
+// A workgroup barrier that waits for no load (__syncthreads waits for all of them); no
+// memory access moves across it.
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // The scheduler's next instruction of a kind.
 __device__ __forceinline__ void order_mfma() { __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
 __device__ __forceinline__ void order_read() { __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
 
+__device__ __forceinline__ void order_load() { __builtin_amdgcn_sched_group_barrier(0x020, 1, 0); }
+
 template <typename T, bool AK, bool BKC, typename TL>
-__global__ __launch_bounds__(TL::NT, 2) void gemm_kernel(GemmArgs a) {
+__global__ __launch_bounds__(TL::NT, TL::SIMD) void gemm_kernel(GemmArgs a) {
   __shared__ __align__(1024) uint8_t lds[TL::LDS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const bool glu = BKC && a.act == kActSwiglu;
@@ -365,17 +403,21 @@ __global__ __launch_bounds__(TL::NT, 2) void gemm_kernel(GemmArgs a) {
   for (int i = 0; i < TL::NI; ++i) fb[i].init((wn * TL::NI + i) * 32, lane);
 
   // A stage's four steps of 16, the next step's fragments read under this one's products.
-  // Before a stage's last step the next stage's loads have arrived and every wave has read
-  // this one's last fragments: behind that barrier the loads after next go into its place,
-  // and the last products run beside the next stage's first reads.  Loads past the last
-  // stage read nothing or are not used.
+  // Before a stage's last step the next stage has arrived and every wave has read this
+  // one's last fragments: behind that barrier later loads go into its place, and the last
+  // products run beside the next stage's first reads.  LDS holds three stages of A and two
+  // of B.  A wave's eight loads of a stage are spread over the four steps (B's, which the
+  // next barrier waits for, first): issued together behind the barrier they hold the
+  // waves up, 64 loads at 16 cycles of the address unit each, and the matrix cores were
+  // busy 65 % of the time.  Loads past the last stage, and the
+  // reads of it in the last round, give nothing that is used.
   using V = typename Vec8<T>::type;
   f32x16 acc[TL::MI][TL::NI] = {};
   V va[2][TL::MI], vb[2][TL::NI];
   const int64_t ka = AK ? a.k : a.kv, kb = BKC ? a.k : a.kv;
-  auto read = [&](const uint8_t* sa, int s, int to) {
+  auto read = [&](const uint8_t* sa, const uint8_t* sb, int s, int to) {
 #pragma unroll
-    for (int i = 0; i < TL::NI; ++i) vb[to][i] = frag<T>(sa + TL::A_BYTES, fb[i], s);
+    for (int i = 0; i < TL::NI; ++i) vb[to][i] = frag<T>(sb, fb[i], s);
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i) va[to][i] = frag<T>(sa, fa[i], s);
   };
@@ -383,9 +425,11 @@ __global__ __launch_bounds__(TL::NT, 2) void gemm_kernel(GemmArgs a) {
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i)
 #pragma unroll
-      for (int j = 0; j < TL::NI; ++j) acc[i][j] = mfma32(va[from][i], vb[from][j], acc[i][j]);
+      for (int j = 0; j < TL::NI; ++j) acc[i][j] = mfma32(vb[from][j], va[from][i], acc[i][j]);
   };
-  // the order of one step: a product, then reads of the next step, and so on
+  constexpr int H = decltype(A)::LOADS / 2;
+  static_assert(H * 2 == decltype(B)::LOADS, "as many loads of A as of B");
+  // the order of one step: a product, then reads of the next step and loads, and so on
   auto order = [&]() {
     constexpr int M = TL::MI * TL::NI, R = TL::MI * (AK ? 1 : 2) + TL::NI * (BKC ? 1 : 2);
 #pragma unroll
@@ -393,46 +437,45 @@ __global__ __launch_bounds__(TL::NT, 2) void gemm_kernel(GemmArgs a) {
       order_mfma();
       if constexpr (R > M) order_read();
       order_read();
+      if (i % (M / H) == M / H / 2) order_load();
     }
   };
-  A.issue(lds, (int64_t)kt0 * kBK, ka, wave);
-  B.issue(lds + TL::A_BYTES, (int64_t)kt0 * kBK, kb, wave);
-  wait_vmem();
-  __syncthreads();
-  A.issue(lds + TL::STAGE, (int64_t)(kt0 + 1) * kBK, ka, wave);
-  B.issue(lds + TL::STAGE + TL::A_BYTES, (int64_t)(kt0 + 1) * kBK, kb, wave);
-  read(lds, 0, 0);
-  for (int kt = kt0; kt + 1 < kt1; ++kt) {
-    uint8_t* here = lds + ((kt - kt0) & 1) * TL::STAGE;
-    read(here, 1, 1);
+  uint8_t* const lb = lds + TL::B_AT;
+  A.template issue<0, 2 * H>(lds, (int64_t)kt0 * kBK, ka, wave);
+  B.template issue<0, 2 * H>(lb, (int64_t)kt0 * kBK, kb, wave);
+  A.template issue<0, 2 * H>(lds + TL::A_BYTES, (int64_t)(kt0 + 1) * kBK, ka, wave);
+  B.template issue<0, H>(lb + TL::B_BYTES, (int64_t)(kt0 + 1) * kBK, kb, wave);
+  wait_loads<3 * H>();
+  barrier();
+  read(lds, lb, 0, 0);
+  int a0 = 0, b0 = 0;             // the present stage's place
+  int a2 = 2 * TL::A_BYTES;       // the place of the stage after next
+  for (int kt = kt0; kt < kt1; ++kt) {
+    uint8_t* const sa = lds + a0;
+    uint8_t* const sb = lb + b0;
+    read(sa, sb, 1, 1);
     products(0);
+    B.template issue<H, H>(lb + (b0 ^ TL::B_BYTES), (int64_t)(kt + 1) * kBK, kb, wave);
     order();
-    read(here, 2, 0);
+    read(sa, sb, 2, 0);
     products(1);
+    A.template issue<0, H>(lds + a2, (int64_t)(kt + 2) * kBK, ka, wave);
     order();
-    read(here, 3, 1);
+    read(sa, sb, 3, 1);
     products(0);
+    A.template issue<H, H>(lds + a2, (int64_t)(kt + 2) * kBK, ka, wave);
     order();
-    __builtin_amdgcn_s_waitcnt(0x0070);  // every load and LDS read
-    __syncthreads();
-    A.issue(here, (int64_t)(kt + 2) * kBK, ka, wave);
-    B.issue(here + TL::A_BYTES, (int64_t)(kt + 2) * kBK, kb, wave);
-    read(lds + ((kt + 1 - kt0) & 1) * TL::STAGE, 0, 0);
+    wait_loads<2 * H>();
+    barrier();
+    a2 = a0;
+    a0 = a0 == 2 * TL::A_BYTES ? 0 : a0 + TL::A_BYTES;
+    b0 ^= TL::B_BYTES;
+    read(lds + a0, lb + b0, 0, 0);
     products(1);
+    B.template issue<0, H>(sb, (int64_t)(kt + 2) * kBK, kb, wave);
     order();
   }
-  {
-    const uint8_t* here = lds + ((kt1 - 1 - kt0) & 1) * TL::STAGE;
-    read(here, 1, 1);
-    products(0);
-    read(here, 2, 0);
-    products(1);
-    read(here, 3, 1);
-    products(0);
-    products(1);
-  }
-  wait_vmem();
-  __syncthreads();
+  wait_vmem();  // the loads in flight write this workgroup's LDS
   if (cut) {
     // the piece's sums, in the order the lanes hold them
     float* dst = a.part + ((int64_t)(t - a.whole) * a.parts + piece) * (TL::BM * TL::BN) +
@@ -447,22 +490,24 @@ __global__ __launch_bounds__(TL::NT, 2) void gemm_kernel(GemmArgs a) {
               f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
     return;
   }
-  float* mine = reinterpret_cast<float*>(lds) + wave * 32 * TL::kPitch;
-#pragma unroll
-  for (int i = 0; i < TL::MI; ++i)
-    epilogue<T>(a, mine, lane, m0 + (wm * TL::MI + i) * 32, n0 + wn * (glu ? 32 : 64), acc[i][0], acc[i][1]);
+  const int64_t mw = m0 + wm * TL::MI * 32;
+  const int nw = n0 + wn * TL::NI * (glu ? 16 : 32);
+  if constexpr (AK && BKC)
+    finish<T>(a, lane, mw, nw, acc);
+  else
+    finish_wave<T, kActNone>(a, lane, mw, nw, acc);
 }
 
 // Adds the pieces of the cut tiles in order and finishes them: a wave takes one 32 x 64
 // block of a tile.
 template <typename T, typename TL>
 __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
-  __shared__ float lds[4][32 * TL::kPitch];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  constexpr int BLOCKS = TL::WAVES * TL::MI;
+  constexpr int PAIRS = TL::NI / 2, BLOCKS = TL::WAVES * TL::MI * PAIRS;
   const int u = blockIdx.x * 4 + wave, t = u / BLOCKS, blk = u - t * BLOCKS;
-  const float* src = a.part + (int64_t)t * a.parts * (TL::BM * TL::BN) + blk * (TL::NI * 1024) + lane * 4;
-  f32x16 c[2] = {};
+  const float* src = a.part + (int64_t)t * a.parts * (TL::BM * TL::BN) + blk * 2048 + lane * 4;
+  f32x16 c[1][2] = {};
+#pragma unroll 2
   for (int p = 0; p < a.parts; ++p) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -470,16 +515,17 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
       for (int q = 0; q < 4; ++q) {
         const f32x4 v = *reinterpret_cast<const f32x4*>(src + (j * 4 + q) * 256);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[j][4 * q + e] += v[e];
+        for (int e = 0; e < 4; ++e) c[0][j][4 * q + e] += v[e];
       }
     src += TL::BM * TL::BN;
   }
   int tm, tn;
   tile_at(a, a.whole + t, tm, tn);
-  const int w = blk / TL::MI, wm = w / TL::WN, wn = w % TL::WN;
+  const int w = blk / (TL::MI * PAIRS), wm = w / TL::WN, wn = w % TL::WN;
+  const int i = blk / PAIRS % TL::MI, j = blk % PAIRS * 2;
   const bool glu = a.act == kActSwiglu;
-  epilogue<T>(a, lds[wave], lane, (int64_t)tm * TL::BM + (wm * TL::MI + blk % TL::MI) * 32,
-              tn * (glu ? TL::BN / 2 : TL::BN) + wn * (glu ? 32 : 64), c[0], c[1]);
+  finish<T>(a, lane, (int64_t)tm * TL::BM + (wm * TL::MI + i) * 32,
+            tn * (glu ? TL::BN / 2 : TL::BN) + (wn * TL::NI + j) * (glu ? 16 : 32), c);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -678,8 +724,8 @@ __global__ __launch_bounds__(256) void dbias_kernel(const float* part, int chunk
     static_cast<T*>(dst)[col] = (T)s;
 }
 
-using Big = Tile<2, 4, 4>;    // 256 x 256, 8 waves of 128 x 64, one workgroup a CU
-using Small = Tile<2, 2, 2>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
+using Big = Tile<2, 2, 4, 4, 1>;    // 256 x 256, 4 waves of 128 x 128, one workgroup a CU
+using Small = Tile<2, 2, 2, 2, 2>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
 
 template <typename T, bool AK, bool BKC, typename TL>
 hipError_t run_tiles(const GemmArgs& a, hipStream_t st) {
@@ -687,7 +733,7 @@ hipError_t run_tiles(const GemmArgs& a, hipStream_t st) {
   gemm_kernel<T, AK, BKC, TL><<<a.whole + rest * a.parts, TL::NT, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || rest == 0) return e;
-  join_kernel<T, TL><<<rest * TL::WAVES * TL::MI / 4, 256, 0, st>>>(a);
+  join_kernel<T, TL><<<rest * (TL::WAVES * TL::MI * TL::NI / 2) / 4, 256, 0, st>>>(a);
   return hipGetLastError();
 }
 
