@@ -75,7 +75,7 @@ SIGNATURES = {
     "sage_rms_norm_gate_residual_modulate_bwd": (_c.c_int, [
         _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _I64,
         _I64, _P, _I64, _I64, _I64, _c.c_int, _c.c_int, _c.c_float, _P, _c.c_size_t, _P, _P, _P, _P, _P, _P, _P]),
-    "sage_linear_workspace_bytes": (_c.c_size_t, [_P, _I64, _P, _I64, _I64, _I64, _I64, _c.c_int]),
+    "sage_linear_workspace_bytes": (_c.c_size_t, [_P, _I64, _P, _I64, _I64, _I64, _I64, _c.c_int, _c.c_int]),
     "sage_linear": (_c.c_int, [
         _P, _I64, _P, _I64, _P, _c.c_int, _P, _I64, _I64, _I64, _I64, _c.c_int, _c.c_int, _P, _c.c_size_t, _P, _P,
         _P]),

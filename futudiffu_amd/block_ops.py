@@ -311,11 +311,13 @@ def _linear_forward(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Te
     with _on(x.device):
         lib = _lib.load()
         xp, xs, wp, ws = a.x.data_ptr(), a.x.stride(0), a.weight.data_ptr(), a.weight.stride(0)
-        size = lib.sage_linear_workspace_bytes(xp, xs, wp, ws, a.M, a.N, a.K, a.act)
+        rp, rs = (0, 0) if a.residual is None else (a.residual.data_ptr(), a.residual.stride(0))
+        bp = 0 if a.bias is None else a.bias.data_ptr()
+        size = lib.sage_linear_workspace_bytes(xp, xs, wp, ws, a.M, a.N, a.K, a.act, (rp | bp) % 16 != 0 or rs % 8 != 0)
         work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         _lib.check(lib.sage_linear(
-            xp, xs, wp, ws, _ptr(a.bias), a.f32, _ptr(a.residual), 0 if a.residual is None else a.residual.stride(0),
-            a.M, a.N, a.K, a.dtype, a.act, _ptr(work), size, _ptr(z), out.data_ptr(), _stream_handle(x.device)))
+            xp, xs, wp, ws, bp, a.f32, rp, rs, a.M, a.N, a.K, a.dtype, a.act, _ptr(work), size, _ptr(z),
+            out.data_ptr(), _stream_handle(x.device)))
     return out, z
 
 

@@ -930,8 +930,9 @@ struct LinearOperand {
   }
 };
 
-sage::GemmArgs forward_gemm(int64_t m, int64_t n, int64_t k, int act) {
+sage::GemmArgs forward_gemm(int64_t m, int64_t n, int64_t k, int act, bool vec) {
   sage::GemmArgs g{};
+  g.vec = vec;
   g.m = m;
   g.n = (int)n;
   g.k = up8(k);
@@ -984,6 +985,7 @@ struct LinearBwd {
       gx.a_kc = 1;
       gx.lda = ldz;
       gx.ldb = copy_w ? up8(k) : rows == 1 ? up8(k) : w_rs;
+      gx.vec = k % 8 == 0;  // dx and dweight start on 16-byte boundaries
       sage::gemm_plan(gx);
       part = (size_t)gx.part_floats * 4;
     }
@@ -993,6 +995,7 @@ struct LinearBwd {
       gw.k = gw.kv = m;
       gw.lda = ldz;
       gw.ldb = copy_x ? up8(k) : m == 1 ? up8(k) : x_rs;
+      gw.vec = k % 8 == 0;
       sage::gemm_plan(gw);
       part = std::max(part, (size_t)gw.part_floats * 4);
     }
@@ -1006,12 +1009,14 @@ struct LinearBwd {
 extern "C" {
 
 size_t sage_linear_workspace_bytes(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, int64_t m,
-                                   int64_t n, int64_t k, int activation) {
+                                   int64_t n, int64_t k, int activation, int other_rows) {
   if (m <= 0 || n <= 0 || k <= 0 || m >= (int64_t)1 << 24 || n >= (int64_t)1 << 22 || k >= (int64_t)1 << 22) return 0;
   size_t at = 0;
   const LinearOperand xo(x, x_rs, m, k, at);
   const LinearOperand wo(weight, w_rs, activation == SAGE_ACT_SWIGLU ? 2 * n : n, k, at);
-  return at + (size_t)forward_gemm(m, n, k, activation).part_floats * 4;
+  // outputs, residual and bias on 16-byte boundaries or not: room for either
+  return at + (size_t)std::max(forward_gemm(m, n, k, activation, n % 8 == 0).part_floats,
+                               other_rows ? forward_gemm(m, n, k, activation, false).part_floats : 0) * 4;
 }
 
 int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, const void* bias, int bias_fp32,
@@ -1031,7 +1036,9 @@ int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, c
   size_t at = 0;
   const LinearOperand xo(x, x_rs, m, k, at);
   const LinearOperand wo(weight, w_rs, rows, k, at);
-  sage::GemmArgs g = forward_gemm(m, n, k, activation);
+  const bool vec = n % 8 == 0 && aligned16(out) && aligned16(z) && aligned16(bias) && aligned16(residual) &&
+                   (!residual || m == 1 || r_rs % 8 == 0);
+  sage::GemmArgs g = forward_gemm(m, n, k, activation, vec);
   const size_t need = at + (size_t)g.part_floats * 4;
   if (need && (!workspace || workspace_bytes < need))
     return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace_bytes);
@@ -1049,8 +1056,6 @@ int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, c
   g.ldr = r_rs;
   g.z = z;
   g.out = out;
-  g.vec = n % 8 == 0 && aligned16(out) && (!z || aligned16(z)) &&
-          (!residual || (aligned16(residual) && (m == 1 || r_rs % 8 == 0)));
   g.vec_b = n % 8 == 0 && aligned16(bias);
   g.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at);
   return launch_status(sage::launch_gemm(g, dtype, stream), "sage_linear");
@@ -1082,6 +1087,7 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
     if (reinterpret_cast<uintptr_t>(p) & 1u) return fail(SAGE_ERR_ALIGN, "tensor pointers must be aligned to their elements");
   if (reinterpret_cast<uintptr_t>(dbias) & (bias_fp32 ? 3u : 1u))
     return fail(SAGE_ERR_ALIGN, "dbias must be aligned to its elements");
+  if (!aligned16(dx) || !aligned16(dweight)) return fail(SAGE_ERR_ALIGN, "dx and dweight must be 16-byte aligned");
   LinearBwd p(dout, d_rs, x, x_rs, weight, w_rs, m, n, k, activation, want);
   if (p.bytes && (!workspace || workspace_bytes < p.bytes))
     return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu", p.bytes, workspace_bytes);
@@ -1121,7 +1127,6 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
     p.gx.a = dz;
     p.gx.b = p.copy_w ? ws + p.w_off : weight;
     p.gx.out = dx;
-    p.gx.vec = k % 8 == 0 && aligned16(dx);
     p.gx.part = reinterpret_cast<float*>(ws + p.part_off);
     const hipError_t e = sage::launch_gemm(p.gx, dtype, stream);
     if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (dx)");
@@ -1130,7 +1135,6 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
     p.gw.a = dz;
     p.gw.b = p.copy_x ? ws + p.x_off : x;
     p.gw.out = dweight;
-    p.gw.vec = k % 8 == 0 && aligned16(dweight);
     p.gw.part = reinterpret_cast<float*>(ws + p.part_off);
     const hipError_t e = sage::launch_gemm(p.gw, dtype, stream);
     if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (dweight)");

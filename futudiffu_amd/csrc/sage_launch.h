@@ -384,7 +384,7 @@ struct GemmArgs {
   int64_t ldr;
   void* z;    // T [m][rows of B]: acc + bias, for the backward; null: not kept
   void* out;  // T [m][n]
-  int vec;    // rows of res, z and out take 16-byte accesses
+  int vec;    // rows of res, z and out, and the bias, take 16-byte accesses (known to the plan)
   int vec_b;  // so does the bias
   // the plan (gemm_plan)
   int big, skinny, kt, tm, tn;

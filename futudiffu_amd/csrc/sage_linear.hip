@@ -161,51 +161,119 @@ __device__ __forceinline__ void finish8(const GemmArgs& a, int64_t m, int n, flo
   store8<T>(static_cast<T*>(a.out) + m * a.n, n, a.n, a.vec, z);
 }
 
-// A 32 x 32 block of the output (or its two halves of a swiglu) from the accumulators of
-// the transposed product, in which lane (h, r) holds row r, columns 8 J + 4 h + i: swapping
-// J = 1 of the lower lanes with J = 0 of the upper gives each lane eight consecutive columns,
-// one 16-byte store, with no pass through LDS.
-template <typename T, int ACT>
-__device__ __forceinline__ void finish_block(const GemmArgs& a, int lane, int64_t m0, int n0, f32x16 c, f32x16 c2) {
-  const int64_t m = m0 + (lane & 31);
+// Columns 8 h .. + 7 of half p (16 columns) of a 32 x 32 accumulator of the transposed
+// product, in which lane (h, r) holds row r, columns 8 J + 4 h + i: swapping J = 2 p + 1 of the
+// lower lanes with J = 2 p of the upper gives each lane eight consecutive columns.
+__device__ __forceinline__ void eight_of(const f32x16& c, int p, float (&z)[8]) {
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    float z[8], z2[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(c[8 * p + i]), __float_as_uint(c[8 * p + 4 + i]),
-                                                      false, false);
-      z[i] = __uint_as_float(s[0]);
-      z[4 + i] = __uint_as_float(s[1]);
-      if constexpr (ACT == kActSwiglu) {
-        const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(c2[8 * p + i]),
-                                                        __float_as_uint(c2[8 * p + 4 + i]), false, false);
-        z2[i] = __uint_as_float(u[0]);
-        z2[4 + i] = __uint_as_float(u[1]);
-      }
-    }
-    const int n = n0 + 16 * p + 8 * (lane >> 5);
-    if (m < a.m && n < a.n) finish8<T, ACT>(a, m, n, z, z2);
+  for (int i = 0; i < 4; ++i) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(c[8 * p + i]), __float_as_uint(c[8 * p + 4 + i]),
+                                                    false, false);
+    z[i] = __uint_as_float(s[0]);
+    z[4 + i] = __uint_as_float(s[1]);
   }
 }
 
-// A wave's MI x NI blocks from row m0 and tile column n0 on.
-template <typename T, int ACT, int MI, int NI>
+__device__ __forceinline__ u32x4 load_16(__amdgpu_buffer_rsrc_t rs, int off) {
+  return __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0);
+}
+__device__ __forceinline__ void store_16(u32x4 v, __amdgpu_buffer_rsrc_t rs, int off) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, rs, off, 0, 0);
+}
+
+// finish8 for a wave's MI x NI blocks from row m0 and column n0 on, every access 16 bytes
+// through a buffer resource over the rows that exist, straight from the accumulators with no
+// pass through LDS.  What a call does not have (bias, residual, z) has a resource of no
+// bytes, so there is no branch.  PLAIN: out alone.
+template <typename T, int ACT, bool PLAIN, int MI, int NI>
 __device__ __forceinline__ void finish_wave(const GemmArgs& a, int lane, int64_t m0, int n0, f32x16 (&c)[MI][NI]) {
+  using V = typename Vec8<T>::type;
   constexpr bool kGlu = ACT == kActSwiglu;
+  constexpr int kStep = kGlu ? 2 : 1;
+  const int64_t left = a.m - m0;
+  if (left <= 0) return;
+  const int rows = left < 32 * MI ? (int)left : 32 * MI, r = lane & 31, h = lane >> 5;
+  const int wide = kGlu ? 2 * a.n : a.n;
+  const __amdgpu_buffer_rsrc_t out = raw_rsrc(static_cast<T*>(a.out) + m0 * a.n, (uint32_t)rows * a.n * 2);
+  const __amdgpu_buffer_rsrc_t res = raw_rsrc(static_cast<const T*>(a.res) + m0 * a.ldr,
+                                              a.res ? (uint32_t)(((rows - 1) * a.ldr + a.n) * 2) : 0u);
+  const __amdgpu_buffer_rsrc_t zs = raw_rsrc(static_cast<T*>(a.z) + m0 * wide, a.z ? (uint32_t)rows * wide * 2 : 0u);
+  const __amdgpu_buffer_rsrc_t b16 = raw_rsrc(a.bias, a.bias && !a.bias_f32 ? (uint32_t)wide * 2 : 0u);
+  const __amdgpu_buffer_rsrc_t b32 = raw_rsrc(a.bias, a.bias && a.bias_f32 ? (uint32_t)wide * 4 : 0u);
+  auto bias_at = [&](int n, float (&b)[8]) {  // one of the two reads zeros
+    const V v = __builtin_bit_cast(V, load_16(b16, n * 2));
+    const f32x4 lo = __builtin_bit_cast(f32x4, load_16(b32, n * 4)), hi = __builtin_bit_cast(f32x4, load_16(b32, n * 4 + 16));
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+    for (int e = 0; e < 8; ++e) b[e] = (float)v[e] + (e < 4 ? lo[e & 3] : hi[e & 3]);
+  };
 #pragma unroll
-    for (int j = 0; j < NI; j += kGlu ? 2 : 1)
-      finish_block<T, ACT>(a, lane, m0 + 32 * i, n0 + (kGlu ? 16 : 32) * j, c[i][j], c[i][kGlu ? j + 1 : j]);
+  for (int j = 0; j < NI; j += kStep)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int n = n0 + (32 / kStep) * j + 16 * p + 8 * h;
+      const int none = n < a.n ? 0 : (int)0x80000000;  // past the last column: an offset past any size
+      float b[8], b2[8];
+      if constexpr (!PLAIN) {
+        bias_at(n | none, b);
+        if constexpr (kGlu) bias_at((n + a.n) | none, b2);
+      }
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        float z[8], z2[8];
+        eight_of(c[i][j], p, z);
+        if constexpr (kGlu) eight_of(c[i][j + 1], p, z2);
+        const int row = 32 * i + r;
+        if constexpr (!PLAIN) {
+          const V rv = __builtin_bit_cast(V, load_16(res, (int)(row * a.ldr + n) * 2 | none));
+          V zv, zv2;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            z[e] += b[e];
+            zv[e] = (T)z[e];
+            if constexpr (kGlu) {
+              z2[e] += b2[e];
+              zv2[e] = (T)z2[e];
+            }
+            z[e] = act_fwd(ACT, z[e]);
+            if constexpr (kGlu) z[e] *= z2[e];
+            z[e] += (float)rv[e];
+          }
+          if constexpr (ACT != kActNone) {
+            store_16(__builtin_bit_cast(u32x4, zv), zs, (row * wide + n) * 2 | none);
+            if constexpr (kGlu) store_16(__builtin_bit_cast(u32x4, zv2), zs, (row * wide + a.n + n) * 2 | none);
+          }
+        }
+        V o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = (T)z[e];
+        store_16(__builtin_bit_cast(u32x4, o), out, (row * a.n + n) * 2 | none);
+      }
+    }
 }
 
 template <typename T, int MI, int NI>
 __device__ __forceinline__ void finish(const GemmArgs& a, int lane, int64_t m0, int n0, f32x16 (&c)[MI][NI]) {
-  if (a.act == kActSwiglu) finish_wave<T, kActSwiglu>(a, lane, m0, n0, c);
-  else if (a.act == kActSilu) finish_wave<T, kActSilu>(a, lane, m0, n0, c);
-  else if (a.act == kActGelu) finish_wave<T, kActGelu>(a, lane, m0, n0, c);
-  else finish_wave<T, kActNone>(a, lane, m0, n0, c);
+  if (a.act == kActSwiglu) finish_wave<T, kActSwiglu, false>(a, lane, m0, n0, c);
+  else if (a.act == kActSilu) finish_wave<T, kActSilu, false>(a, lane, m0, n0, c);
+  else if (a.act == kActGelu) finish_wave<T, kActGelu, false>(a, lane, m0, n0, c);
+  else finish_wave<T, kActNone, false>(a, lane, m0, n0, c);
+}
+
+// The same for one row of blocks with rows of any alignment, element by element.
+template <typename T, int ACT>
+__device__ __forceinline__ void finish_any(const GemmArgs& a, int lane, int64_t m0, int n0, f32x16 (&c)[1][2]) {
+  constexpr bool kGlu = ACT == kActSwiglu;
+  const int64_t m = m0 + (lane & 31);
+#pragma unroll
+  for (int j = 0; j < 2; j += kGlu ? 2 : 1)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      float z[8], z2[8];
+      eight_of(c[0][j], p, z);
+      eight_of(c[0][1], p, z2);
+      const int n = n0 + 32 * j + 16 * p + 8 * (lane >> 5);
+      if (m < a.m && n < a.n) finish8<T, ACT>(a, m, n, z, z2);
+    }
 }
 
 // ---------------------------------------------------------------- tiles
@@ -495,11 +563,11 @@ __global__ __launch_bounds__(TL::NT, TL::SIMD) void gemm_kernel(GemmArgs a) {
   if constexpr (AK && BKC)
     finish<T>(a, lane, mw, nw, acc);
   else
-    finish_wave<T, kActNone>(a, lane, mw, nw, acc);
+    finish_wave<T, kActNone, true>(a, lane, mw, nw, acc);
 }
 
 // Adds the pieces of the cut tiles in order and finishes them: a wave takes one 32 x 64
-// block of a tile.
+// block of a tile.  Outputs whose rows take no 16-byte accesses all come through here.
 template <typename T, typename TL>
 __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -524,8 +592,13 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
   const int w = blk / (TL::MI * PAIRS), wm = w / TL::WN, wn = w % TL::WN;
   const int i = blk / PAIRS % TL::MI, j = blk % PAIRS * 2;
   const bool glu = a.act == kActSwiglu;
-  finish<T>(a, lane, (int64_t)tm * TL::BM + (wm * TL::MI + i) * 32,
-            tn * (glu ? TL::BN / 2 : TL::BN) + (wn * TL::NI + j) * (glu ? 16 : 32), c);
+  const int64_t m0 = (int64_t)tm * TL::BM + (wm * TL::MI + i) * 32;
+  const int n0 = tn * (glu ? TL::BN / 2 : TL::BN) + (wn * TL::NI + j) * (glu ? 16 : 32);
+  if (a.vec) finish<T>(a, lane, m0, n0, c);
+  else if (a.act == kActSwiglu) finish_any<T, kActSwiglu>(a, lane, m0, n0, c);
+  else if (a.act == kActSilu) finish_any<T, kActSilu>(a, lane, m0, n0, c);
+  else if (a.act == kActGelu) finish_any<T, kActGelu>(a, lane, m0, n0, c);
+  else finish_any<T, kActNone>(a, lane, m0, n0, c);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -789,7 +862,7 @@ void gemm_plan(GemmArgs& a) {
     const int slots = big ? 256 : 512;
     const double stage = big ? 1.0 : 0.75, start = 4.0;  // two small tiles share a CU
     for (int p = 1; p <= 16; ++p) {
-      const int64_t rest = p == 1 ? 0 : tiles % slots;
+      const int64_t rest = !a.vec ? tiles : p == 1 ? 0 : tiles % slots;
       if (p > 1 && (rest == 0 || a.kt / p < 4)) continue;
       const int64_t whole = tiles - rest;
       double cost = (double)((whole + slots - 1) / slots) * (a.kt * stage + start);

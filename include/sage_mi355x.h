@@ -484,6 +484,8 @@ int sage_rms_norm_gate_residual_modulate_bwd(
  *                the gradient of an activation needs.
  *   out          [m][n] contiguous.
  *   workspace    sage_linear_workspace_bytes(...) bytes, 16-byte aligned; needs no clearing.
+ *                other_rows: whether the residual, bias, z or out may start off 16-byte
+ *                boundaries, or the residual's rows (r_rs no multiple of 8).
  * m, n, k at least 1; a weight or a row panel of 256 rows has under 2^31 bytes.  Rows of x
  * and weight that do not start on 16-byte boundaries, or a k that is no multiple of 8, are
  * copied into the workspace first. */
@@ -493,13 +495,13 @@ int sage_rms_norm_gate_residual_modulate_bwd(
 #define SAGE_ACT_SWIGLU 3
 
 size_t sage_linear_workspace_bytes(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, int64_t m,
-                                   int64_t n, int64_t k, int activation);
+                                   int64_t n, int64_t k, int activation, int other_rows);
 int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, const void* bias, int bias_fp32,
                 const void* residual, int64_t r_rs, int64_t m, int64_t n, int64_t k, int dtype, int activation,
                 void* workspace, size_t workspace_bytes, void* z, void* out, hipStream_t stream);
 
-/* Gradients of sage_linear: dx [m][k], dweight [rows][k], dbias [rows] (dtype or fp32), each
- * null if not wanted; the residual's is dout itself.  dz = dout * act'(z) is rounded to dtype
+/* Gradients of sage_linear: dx [m][k], dweight [rows][k] (both from 16-byte boundaries), dbias
+ * [rows] (dtype or fp32), each null if not wanted; the residual's is dout itself.  dz = dout * act'(z) is rounded to dtype
  * as the products' operand (the bias's gradient adds it unrounded); sums are in a fixed order.
  *   dout         [m][n] rows d_rs apart.
  *   z            what sage_linear kept; null with SAGE_ACT_NONE.
