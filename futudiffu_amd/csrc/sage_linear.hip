@@ -49,8 +49,9 @@ __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
 
 constexpr float kGeluA = 0.7978845608028654f;  // sqrt(2/pi)
 
-// 1 / (1 + exp(-z)); exp(-z) may overflow to infinity, which gives 0.
-__device__ __forceinline__ float sigmoidf(float z) { return 1.0f / (1.0f + __expf(-z)); }
+// 1 / (1 + exp(-z)), the quotient by v_rcp_f32 (within one step of fp32, as the exponential
+// is: far below the 16-bit results' rounding); exp(-z) may overflow to infinity, which gives 0.
+__device__ __forceinline__ float sigmoidf(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
 __device__ __forceinline__ float act_fwd(int act, float z) {
   if (act == kActSilu || act == kActSwiglu) return z * sigmoidf(z);
@@ -181,6 +182,20 @@ __device__ __forceinline__ void store_16(u32x4 v, __amdgpu_buffer_rsrc_t rs, int
   __builtin_amdgcn_raw_buffer_store_b128(v, rs, off, 0, 0);
 }
 
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// The two halves' packed columns of a 32 x 32 block (lane (h, r): row r, columns 16 p + 8 h of
+// half p) to rows: x: row lane % 16, y: row 16 + lane % 16, both with columns 16 g + 8 h (g:
+// lane bit 4), so that a store's four lanes of a row write 64 bytes together.  Its own inverse.
+__device__ __forceinline__ void halves_to_rows(u32x4& x, u32x4& y) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto s = __builtin_amdgcn_permlane16_swap(x[i], y[i], false, false);
+    x[i] = s[0];
+    y[i] = s[1];
+  }
+}
+
 // finish8 for a wave's MI x NI blocks from row m0 and column n0 on, every access 16 bytes
 // through a buffer resource over the rows that exist, straight from the accumulators with no
 // pass through LDS.  What a call does not have (bias, residual, z) has a resource of no
@@ -192,7 +207,7 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int lane, int64_t
   constexpr int kStep = kGlu ? 2 : 1;
   const int64_t left = a.m - m0;
   if (left <= 0) return;
-  const int rows = left < 32 * MI ? (int)left : 32 * MI, r = lane & 31, h = lane >> 5;
+  const int rows = left < 32 * MI ? (int)left : 32 * MI, h = lane >> 5, row = lane & 15;
   const int wide = kGlu ? 2 * a.n : a.n;
   const __amdgpu_buffer_rsrc_t out = raw_rsrc(static_cast<T*>(a.out) + m0 * a.n, (uint32_t)rows * a.n * 2);
   const __amdgpu_buffer_rsrc_t res = raw_rsrc(static_cast<const T*>(a.res) + m0 * a.ldr,
@@ -206,49 +221,75 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int lane, int64_t
 #pragma unroll
     for (int e = 0; e < 8; ++e) b[e] = (float)v[e] + (e < 4 ? lo[e & 3] : hi[e & 3]);
   };
+  // the columns of block column j that this lane loads and stores, and whether they exist
+  // (else an offset past any size)
+  auto column = [&](int j) { return n0 + (32 / kStep) * j + 16 * ((lane >> 4) & 1) + 8 * h; };
+  auto beyond = [&](int n) { return n < a.n ? 0 : (int)0x80000000; };
+  // a block column's residual is read one block column ahead; the scheduling barriers keep
+  // the rest of the loads where they are, or registers run out
+  u32x4 ahead[2][MI][2];
+  auto residual = [&](int j, int to) {
+    const int n = column(j), none = beyond(n);
 #pragma unroll
-  for (int j = 0; j < NI; j += kStep)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int n = n0 + (32 / kStep) * j + 16 * p + 8 * h;
-      const int none = n < a.n ? 0 : (int)0x80000000;  // past the last column: an offset past any size
-      float b[8], b2[8];
-      if constexpr (!PLAIN) {
-        bias_at(n | none, b);
-        if constexpr (kGlu) bias_at((n + a.n) | none, b2);
+      for (int q = 0; q < 2; ++q) ahead[to][i][q] = load_16(res, (int)((32 * i + 16 * q + row) * a.ldr + n) * 2 | none);
+  };
+  auto store = [&](__amdgpu_buffer_rsrc_t rs, int i, int width, int n, int none, V v0, V v1) {
+    u32x4 x = __builtin_bit_cast(u32x4, v0), y = __builtin_bit_cast(u32x4, v1);
+    halves_to_rows(x, y);
+    store_16(x, rs, ((32 * i + row) * width + n) * 2 | none);
+    store_16(y, rs, ((32 * i + 16 + row) * width + n) * 2 | none);
+  };
+  if constexpr (!PLAIN) residual(0, 0);
+#pragma unroll
+  for (int j = 0; j < NI; j += kStep) {
+    const int n = column(j), none = beyond(n);
+    float b[2][8], b2[2][8];
+    if constexpr (!PLAIN) {
+      if (j + kStep < NI) residual(j + kStep, (j / kStep + 1) & 1);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int nb = n0 + (32 / kStep) * j + 16 * p + 8 * h, nob = beyond(nb);
+        bias_at(nb | nob, b[p]);
+        if constexpr (kGlu) bias_at((nb + a.n) | nob, b2[p]);
       }
+    }
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
+    for (int i = 0; i < MI; ++i) {
+      V o[2], zv[2], zv2[2];
+      if constexpr (!PLAIN) halves_to_rows(ahead[j / kStep & 1][i][0], ahead[j / kStep & 1][i][1]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
         float z[8], z2[8];
         eight_of(c[i][j], p, z);
         if constexpr (kGlu) eight_of(c[i][j + 1], p, z2);
-        const int row = 32 * i + r;
         if constexpr (!PLAIN) {
-          const V rv = __builtin_bit_cast(V, load_16(res, (int)(row * a.ldr + n) * 2 | none));
-          V zv, zv2;
+          const V rv = __builtin_bit_cast(V, ahead[j / kStep & 1][i][p]);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            z[e] += b[e];
-            zv[e] = (T)z[e];
+            z[e] += b[p][e];
+            zv[p][e] = (T)z[e];
             if constexpr (kGlu) {
-              z2[e] += b2[e];
-              zv2[e] = (T)z2[e];
+              z2[e] += b2[p][e];
+              zv2[p][e] = (T)z2[e];
             }
             z[e] = act_fwd(ACT, z[e]);
             if constexpr (kGlu) z[e] *= z2[e];
             z[e] += (float)rv[e];
           }
-          if constexpr (ACT != kActNone) {
-            store_16(__builtin_bit_cast(u32x4, zv), zs, (row * wide + n) * 2 | none);
-            if constexpr (kGlu) store_16(__builtin_bit_cast(u32x4, zv2), zs, (row * wide + a.n + n) * 2 | none);
-          }
         }
-        V o;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = (T)z[e];
-        store_16(__builtin_bit_cast(u32x4, o), out, (row * a.n + n) * 2 | none);
+        for (int e = 0; e < 8; ++e) o[p][e] = (T)z[e];
       }
+      if constexpr (!PLAIN && ACT != kActNone) {
+        store(zs, i, wide, n, none, zv[0], zv[1]);
+        if constexpr (kGlu) store(zs, i, wide, n + a.n, none, zv2[0], zv2[1]);
+      }
+      store(out, i, a.n, n, none, o[0], o[1]);
     }
+    keep_order();
+  }
 }
 
 template <typename T, int MI, int NI>
