@@ -523,7 +523,8 @@ __global__ __launch_bounds__(TL::NT, TL::SIMD) void gemm_kernel(GemmArgs a) {
   using V = typename Vec8<T>::type;
   f32x16 acc[TL::MI][TL::NI] = {};
   V va[2][TL::MI], vb[2][TL::NI];
-  const int64_t ka = AK ? a.k : a.kv, kb = BKC ? a.k : a.kv;
+  // nothing is read past the piece's last stage
+  const int64_t end = (int64_t)kt1 * kBK, ka = min(AK ? a.k : a.kv, end), kb = min(BKC ? a.k : a.kv, end);
   auto read = [&](const uint8_t* sa, const uint8_t* sb, int s, int to) {
 #pragma unroll
     for (int i = 0; i < TL::NI; ++i) vb[to][i] = frag<T>(sb, fb[i], s);
