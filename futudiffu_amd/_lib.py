@@ -93,6 +93,8 @@ _lib = None
 def load() -> ctypes.CDLL:
     """Load the library and attach prototypes (no GPU needed)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):

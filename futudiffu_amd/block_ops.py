@@ -23,92 +23,75 @@ gradients.  Sums are added in a fixed order, so results and gradients repeat bit
 
 from __future__ import annotations
 
-import contextlib
+import functools
 
 import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .sage_attention import _ptr, _stream_handle
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _ops = torch.library.Library("futudiffu_ii", "FRAGMENT")
 
 
-_HERE = contextlib.nullcontext()
+# The host's time is a large part of a small call, and all of a small training step, whose
+# halves run on two threads: hence one pass over the arguments, sizes that depend on sizes
+# alone kept, and no second look in the backward at what the forward checked.
+
+def _launch(device: int, fn, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of ``device``, made the current device (the
+    library launches there)."""
+    if device == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        _lib.check(status)
 
 
-def _on(device: torch.device):
-    """The library launches on the current device: make it ``device``."""
-    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+def _describe(t: Tensor) -> str:
+    return f"{t.dtype} {list(t.shape)} on {t.device}"
 
 
 def _tokens(name: str, t: Tensor, like: Tensor | None = None) -> Tensor:
     """A token tensor the kernels read in place: channels contiguous."""
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name} must be a {like.dtype} {list(like.shape)} tensor on {like.device}, got "
-                         f"{t.dtype} {list(t.shape)} on {t.device}")
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.get_device() != like.get_device()):
+        raise ValueError(f"{name} must be a {_describe(like)} tensor, got {_describe(t)}")
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _dims(t: Tensor) -> tuple[int, int]:
-    """Element strides per batch item and token."""
+def _rows3(t: Tensor) -> tuple[int, int, int]:
+    """Address and element strides per batch item and token."""
     s = t.stride()
-    return (s[0], s[1]) if len(s) == 3 else (0, s[0])
+    return (t.data_ptr(), s[0], s[1]) if len(s) == 3 else (t.data_ptr(), 0, s[0])
 
 
-def _check_x(x: Tensor, eps: float) -> tuple[int, int, int]:
-    if x.ndim not in (2, 3):
-        raise ValueError(f"x must be [B, N, C] or [N, C], got {list(x.shape)}")
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
-    if not x.is_cuda:
-        raise ValueError(f"x must be a GPU tensor (device {x.device})")
-    if not eps >= 0:
-        raise ValueError(f"eps must be >= 0, got {eps}")
-    B, N, C = x.shape if x.ndim == 3 else (1, *x.shape)
-    if C < 1:
-        raise ValueError(f"x needs at least one channel, got {list(x.shape)}")
-    return B, N, C
-
-
-def _check_weight(name: str, w: Tensor | None, x: Tensor, C: int) -> Tensor | None:
-    if w is None:
-        return None
-    if w.shape != (C,) or w.device != x.device or (w.dtype != x.dtype and w.dtype != torch.float32):
-        raise ValueError(f"{name} must be a [{C}] tensor of {x.dtype} or float32 on {x.device}, got {w.dtype} "
-                         f"{list(w.shape)} on {w.device}")
+def _check_weight(name: str, w: Tensor, x: Tensor, C: int) -> Tensor:
+    if w.shape != (C,) or w.get_device() != x.get_device() or (w.dtype != torch.float32 and w.dtype != x.dtype):
+        raise ValueError(f"{name} must be a [{C}] tensor of {x.dtype} or float32 on {x.device}, got {_describe(w)}")
     return w.contiguous()
 
 
-def _check_cond(name: str, k: Tensor | None, x: Tensor, B: int, C: int, docs: bool):
-    """A conditioning tensor and its (batch, row) strides and rows."""
-    if k is None:
-        return None, 0, 0, 0
-    want = f"[{B}, G, {C}] (with doc_ids)" if docs else f"[{B}, {C}]"
-    ok = (k.ndim == 3 and k.shape[0] == B and k.shape[1] >= 1 and k.shape[2] == C) if docs else k.shape == (B, C)
-    if not ok or k.device != x.device or (k.dtype != x.dtype and k.dtype != torch.float32):
-        raise ValueError(f"{name} must be a {want} tensor of {x.dtype} or float32 on {x.device}, got {k.dtype} "
-                         f"{list(k.shape)} on {k.device}")
-    if k.stride(-1) != 1 and C != 1:
+def _check_cond(name: str, k: Tensor, x: Tensor, B: int, C: int, docs: bool) -> tuple[Tensor, int, int, int]:
+    """A conditioning tensor, its (batch, row) strides and its rows a batch item."""
+    shape = k.shape
+    ok = len(shape) == 3 and shape[0] == B and shape[1] >= 1 and shape[2] == C if docs else shape == (B, C)
+    if not ok or k.get_device() != x.get_device() or (k.dtype != torch.float32 and k.dtype != x.dtype):
+        want = f"[{B}, G, {C}] (with doc_ids)" if docs else f"[{B}, {C}]"
+        raise ValueError(f"{name} must be a {want} tensor of {x.dtype} or float32 on {x.device}, got {_describe(k)}")
+    if C != 1 and k.stride(-1) != 1:
         k = k.contiguous()
-    return (k, k.stride(0), k.stride(1), k.shape[1]) if docs else (k, k.stride(0), 0, 1)
+    return (k, k.stride(0), k.stride(1), shape[1]) if docs else (k, k.stride(0), 0, 1)
 
 
-def _check_docs(doc_ids: Tensor | None, x: Tensor, B: int, N: int) -> Tensor | None:
-    if doc_ids is None:
-        return None
-    if doc_ids.shape != ((B, N) if x.ndim == 3 else (N,)) and doc_ids.shape != (B, N):
+def _check_docs(doc_ids: Tensor, x: Tensor, B: int, N: int) -> Tensor:
+    if doc_ids.shape != (B, N) and (x.ndim == 3 or doc_ids.shape != (N,)):
         raise ValueError(f"doc_ids must be [B, N] = [{B}, {N}], got {list(doc_ids.shape)}")
     if doc_ids.dtype.is_floating_point or doc_ids.dtype == torch.bool:
         raise ValueError(f"doc_ids must hold integers, got {doc_ids.dtype}")
     return doc_ids.to(device=x.device, dtype=torch.int32).contiguous()
-
-
-def _f32(*params: Tensor | None) -> int:
-    """Bit i: parameter i is fp32."""
-    return sum(1 << i for i, p in enumerate(params) if p is not None and p.dtype == torch.float32)
 
 
 def _wants_grad(*tensors: Tensor | None) -> bool:
@@ -122,58 +105,97 @@ def _wants_grad(*tensors: Tensor | None) -> bool:
 class _Norm:
     """The checked arguments of a norm call, as the library takes them."""
 
+    __slots__ = ("x", "device", "dims", "doc", "weight", "cond", "next_weight", "next_scale", "head", "next", "tail",
+                 "empty", "sizes")
+
     def __init__(self, x: Tensor, weight, cond_name: str, cond, doc_ids, eps: float, next_weight=None,
                  next_scale=None):
-        self.B, self.N, self.C = B, N, C = _check_x(x, eps)
-        self.x = x = _tokens("x", x)
-        if cond is None and next_scale is None:
-            if doc_ids is not None:
-                _check_docs(doc_ids, x, B, N)
-            doc_ids = None  # nothing differs between documents
-        self.doc = _check_docs(doc_ids, x, B, N)
-        self.weight = _check_weight("weight", weight, x, C)
-        docs = self.doc is not None
-        self.cond, self.cbs, self.cgs, g1 = _check_cond(cond_name, cond, x, B, C, docs)
-        self.next_weight = _check_weight("next_weight", next_weight, x, C)
-        self.next_scale, self.sbs, self.sgs, g2 = _check_cond("next_scale", next_scale, x, B, C, docs)
-        if g1 and g2 and g1 != g2:
-            raise ValueError(f"{cond_name} and next_scale must have a row for the same documents, got {g1} and {g2}")
-        self.groups = g1 or g2 or 1
-        self.f32 = _f32(self.weight, self.cond, self.next_weight, self.next_scale)
+        shape = x.shape
+        if len(shape) == 3:
+            B, N, C = shape
+        elif len(shape) == 2:
+            B, (N, C) = 1, shape
+        else:
+            raise ValueError(f"x must be [B, N, C] or [N, C], got {list(shape)}")
+        dtype = _DTYPES.get(x.dtype)
+        if dtype is None:
+            raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
+        if not x.is_cuda:
+            raise ValueError(f"x must be a GPU tensor (device {x.device})")
+        if not eps >= 0:
+            raise ValueError(f"eps must be >= 0, got {eps}")
+        if C < 1:
+            raise ValueError(f"x needs at least one channel, got {list(shape)}")
+        self.device = x.get_device()
+        self.x = x = x if C == 1 or x.stride(-1) == 1 else x.contiguous()
+        # tensors made for the call stay referenced until it is launched
+        self.weight, self.cond, self.next_weight, self.next_scale, self.doc = weight, cond, next_weight, next_scale, None
+        doc = 0
+        if doc_ids is not None:
+            self.doc = _check_docs(doc_ids, x, B, N)
+            if cond is None and next_scale is None:
+                self.doc = None  # nothing differs between documents
+            else:
+                doc = self.doc.data_ptr()
+        f32 = wp = kp = kb = kg = 0
+        groups = 0
+        if weight is not None:
+            self.weight = weight = _check_weight("weight", weight, x, C)
+            wp, f32 = weight.data_ptr(), weight.dtype == torch.float32
+        if cond is not None:
+            self.cond, kb, kg, groups = _check_cond(cond_name, cond, x, B, C, self.doc is not None)
+            kp = self.cond.data_ptr()
+            f32 |= 2 * (cond.dtype == torch.float32)
+        self.head = (wp, kp, kb, kg)
+        w2 = sp = sb = sg = 0
+        if next_weight is not None:
+            self.next_weight = next_weight = _check_weight("next_weight", next_weight, x, C)
+            w2 = next_weight.data_ptr()
+            f32 |= 4 * (next_weight.dtype == torch.float32)
+        if next_scale is not None:
+            self.next_scale, sb, sg, rows = _check_cond("next_scale", next_scale, x, B, C, self.doc is not None)
+            sp = self.next_scale.data_ptr()
+            f32 |= 8 * (next_scale.dtype == torch.float32)
+            if groups and groups != rows:
+                raise ValueError(f"{cond_name} and next_scale must have a row for the same documents, got {groups} and "
+                                 f"{rows}")
+            groups = rows
+        self.next = (w2, sp, sb, sg)
+        groups = groups or 1
+        self.sizes = (B, N, C, groups, doc != 0)
+        self.tail = (groups, doc, B, N, C, dtype, int(f32), eps)
         self.empty = B == 0 or N == 0
-        self.eps = eps
 
-    def tail(self):
-        return (self.groups, _ptr(self.doc), self.B, self.N, self.C, _DTYPES[self.x.dtype], self.f32, self.eps)
+    def workspace(self, fused: bool) -> Tensor:
+        return torch.empty(_norm_workspace_bytes(*self.sizes, fused), dtype=torch.uint8, device=self.x.device)
 
-    def workspace(self, wanted: bool, fused: bool):
-        if not wanted:
-            return None, 0
-        size = _lib.load().sage_rms_norm_bwd_workspace_bytes(self.B, self.N, self.C, self.groups,
-                                                             self.doc is not None, fused)
-        return torch.empty(size, dtype=torch.uint8, device=self.x.device), size
 
-    def zeros(self, *grads: Tensor | None):
-        """The gradients of an empty batch."""
-        for g in grads:
-            if g is not None:
-                g.zero_()
+@functools.lru_cache(maxsize=256)
+def _norm_workspace_bytes(B: int, N: int, C: int, groups: int, docs: bool, fused: bool) -> int:
+    return _lib.load().sage_rms_norm_bwd_workspace_bytes(B, N, C, groups, docs, fused)
 
 
 def _grad(t: Tensor | None, wanted: bool) -> Tensor | None:
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted and t is not None else None
+    return t.new_empty(t.shape) if wanted and t is not None else None
+
+
+def _addr(t: Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _zero(*grads: Tensor | None) -> None:
+    """The parameters' gradients of an empty batch."""
+    for g in grads:
+        if g is not None:
+            g.zero_()
 
 
 def _modulate_forward(x: Tensor, weight: Tensor | None, scale: Tensor | None, doc_ids: Tensor | None,
                       eps: float) -> Tensor:
     a = _Norm(x, weight, "scale", scale, doc_ids, eps)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if a.empty:
-        return out
-    with _on(x.device):
-        _lib.check(_lib.load().sage_rms_norm_modulate(
-            a.x.data_ptr(), *_dims(a.x), _ptr(a.weight), _ptr(a.cond), a.cbs, a.cgs, *a.tail(), out.data_ptr(),
-            _stream_handle(x.device)))
+    out = x.new_empty(x.shape)
+    if not a.empty:
+        _launch(a.device, _lib.load().sage_rms_norm_modulate, *_rows3(a.x), *a.head, *a.tail, out.data_ptr())
     return out
 
 
@@ -181,13 +203,10 @@ def _gate_forward(residual: Tensor, x: Tensor, weight: Tensor | None, gate: Tens
                   doc_ids: Tensor | None, eps: float) -> Tensor:
     a = _Norm(x, weight, "gate", gate, doc_ids, eps)
     r = _tokens("residual", residual, x)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if a.empty:
-        return out
-    with _on(x.device):
-        _lib.check(_lib.load().sage_rms_norm_gate_residual(
-            r.data_ptr(), *_dims(r), a.x.data_ptr(), *_dims(a.x), _ptr(a.weight), _ptr(a.cond), a.cbs, a.cgs,
-            *a.tail(), out.data_ptr(), _stream_handle(x.device)))
+    out = x.new_empty(x.shape)
+    if not a.empty:
+        _launch(a.device, _lib.load().sage_rms_norm_gate_residual, *_rows3(r), *_rows3(a.x), *a.head, *a.tail,
+                out.data_ptr())
     return out
 
 
@@ -196,57 +215,46 @@ def _gate_modulate_forward(residual: Tensor, x: Tensor, weight: Tensor | None, g
                            eps: float) -> tuple[Tensor, Tensor]:
     a = _Norm(x, weight, "gate", gate, doc_ids, eps, next_weight, next_scale)
     r = _tokens("residual", residual, x)
-    hidden = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if a.empty:
-        return hidden, out
-    with _on(x.device):
-        _lib.check(_lib.load().sage_rms_norm_gate_residual_modulate(
-            r.data_ptr(), *_dims(r), a.x.data_ptr(), *_dims(a.x), _ptr(a.weight), _ptr(a.cond), a.cbs, a.cgs,
-            _ptr(a.next_weight), _ptr(a.next_scale), a.sbs, a.sgs, *a.tail(), hidden.data_ptr(), out.data_ptr(),
-            _stream_handle(x.device)))
+    hidden, out = x.new_empty(x.shape), x.new_empty(x.shape)
+    if not a.empty:
+        _launch(a.device, _lib.load().sage_rms_norm_gate_residual_modulate, *_rows3(r), *_rows3(a.x), *a.head,
+                *a.next, *a.tail, hidden.data_ptr(), out.data_ptr())
     return hidden, out
 
 
 def _norm_backward(name: str, cond_name: str, dout: Tensor, x: Tensor, weight: Tensor | None, cond: Tensor | None,
-                   doc_ids: Tensor | None, eps: float, wanted: list[bool]) -> tuple[Tensor | None, ...]:
+                   doc_ids: Tensor | None, eps: float, wanted) -> tuple[Tensor | None, ...]:
     """dx, dweight and the conditioning's gradient (None where not wanted)."""
     a = _Norm(x, weight, cond_name, cond, doc_ids, eps)
     d = _tokens("dout", dout, x)
     dx, dw, dc = _grad(x, wanted[0]), _grad(weight, wanted[1]), _grad(cond, wanted[2])
     if a.empty:
-        a.zeros(dw, dc)
-        return dx, dw, dc
-    if dx is None and dw is None and dc is None:
-        return dx, dw, dc
-    with _on(x.device):
-        ws, wsb = a.workspace(dw is not None or dc is not None, False)
-        _lib.check(getattr(_lib.load(), name)(
-            d.data_ptr(), *_dims(d), a.x.data_ptr(), *_dims(a.x), _ptr(a.weight), _ptr(a.cond), a.cbs, a.cgs,
-            *a.tail(), _ptr(ws), wsb, _ptr(dx), _ptr(dw), _ptr(dc), _stream_handle(x.device)))
+        _zero(dw, dc)
+    elif dx is not None or dw is not None or dc is not None:
+        ws = a.workspace(False) if dw is not None or dc is not None else None
+        _launch(a.device, getattr(_lib.load(), name), *_rows3(d), *_rows3(a.x), *a.head, *a.tail, _addr(ws),
+                0 if ws is None else ws.numel(), _addr(dx), _addr(dw), _addr(dc))
     return dx, dw, dc
 
 
 def _gate_modulate_backward(dhidden: Tensor, dout: Tensor, residual: Tensor, x: Tensor, weight: Tensor | None,
                             gate: Tensor | None, next_weight: Tensor | None, next_scale: Tensor | None,
-                            doc_ids: Tensor | None, eps: float, wanted: list[bool]) -> tuple[Tensor | None, ...]:
+                            doc_ids: Tensor | None, eps: float, wanted) -> tuple[Tensor | None, ...]:
     """Gradients of residual, x, weight, gate, next_weight, next_scale (None where not
     wanted; the residual's, which the others come from, is always formed)."""
     a = _Norm(x, weight, "gate", gate, doc_ids, eps, next_weight, next_scale)
     r, d, dh = _tokens("residual", residual, x), _tokens("dout", dout, x), _tokens("dhidden", dhidden, x)
-    dr, dx = _grad(x, True), _grad(x, wanted[1])
-    params = [_grad(p, w) for p, w in zip((weight, gate, next_weight, next_scale), wanted[2:])]
+    dr, dx = x.new_empty(x.shape), _grad(x, wanted[1])
+    dw, dg, dw2, ds = (_grad(p, w) for p, w in zip((weight, gate, next_weight, next_scale), wanted[2:]))
     if a.empty:
-        a.zeros(*params)
-        return dr, dx, *params
-    with _on(x.device):
-        ws, wsb = a.workspace(any(p is not None for p in params), True)
-        _lib.check(_lib.load().sage_rms_norm_gate_residual_modulate_bwd(
-            dh.data_ptr(), *_dims(dh), d.data_ptr(), *_dims(d), r.data_ptr(), *_dims(r), a.x.data_ptr(),
-            *_dims(a.x), _ptr(a.weight), _ptr(a.cond), a.cbs, a.cgs, _ptr(a.next_weight), _ptr(a.next_scale),
-            a.sbs, a.sgs, *a.tail(), _ptr(ws), wsb, dr.data_ptr(), _ptr(dx), *map(_ptr, params),
-            _stream_handle(x.device)))
-    return dr, dx, *params
+        _zero(dw, dg, dw2, ds)
+    else:
+        some = dw is not None or dg is not None or dw2 is not None or ds is not None
+        ws = a.workspace(True) if some else None
+        _launch(a.device, _lib.load().sage_rms_norm_gate_residual_modulate_bwd, *_rows3(dh), *_rows3(d), *_rows3(r),
+                *_rows3(a.x), *a.head, *a.next, *a.tail, _addr(ws), 0 if ws is None else ws.numel(), dr.data_ptr(),
+                _addr(dx), _addr(dw), _addr(dg), _addr(dw2), _addr(ds))
+    return dr, dx, dw, dg, dw2, ds
 
 
 _ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "swiglu": 3}
@@ -255,38 +263,42 @@ _ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2, "swiglu": 3}
 class _Linear:
     """The checked arguments of a linear call, as the library takes them."""
 
+    __slots__ = ("x", "weight", "bias", "residual", "device", "shape", "M", "N", "K", "rows", "act", "dtype", "f32")
+
     def __init__(self, x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str):
-        if activation not in _ACTIVATIONS:
+        self.act = act = _ACTIVATIONS.get(activation)
+        if act is None:
             raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
-        if x.ndim < 1 or x.dtype not in _DTYPES:
+        self.dtype = _DTYPES.get(x.dtype)
+        if self.dtype is None or x.ndim < 1:
             raise ValueError(f"x must be a bfloat16 or float16 tensor [..., K], got {x.dtype} {list(x.shape)}")
         if not x.is_cuda:
             raise ValueError(f"x must be a GPU tensor (device {x.device})")
-        self.K = K = x.shape[-1]
-        if (weight.ndim != 2 or weight.shape[1] != K or K < 1 or weight.shape[0] < 1 or weight.dtype != x.dtype
-                or weight.device != x.device):
-            raise ValueError(f"weight must be a {x.dtype} [N, {K}] tensor on {x.device}, got {weight.dtype} "
-                             f"{list(weight.shape)} on {weight.device}")
-        self.rows = rows = weight.shape[0]
-        self.act = _ACTIVATIONS[activation]
-        if self.act == 3 and rows % 2:
+        self.device = device = x.get_device()
+        lead = x.shape
+        self.K = K = lead[-1]
+        ws = weight.shape
+        if len(ws) != 2 or ws[1] != K or K < 1 or ws[0] < 1 or weight.dtype != x.dtype or weight.get_device() != device:
+            raise ValueError(f"weight must be a {x.dtype} [N, {K}] tensor on {x.device}, got {_describe(weight)}")
+        self.rows = rows = ws[0]
+        if act == 3 and rows % 2:
             raise ValueError(f"a swiglu weight has an even number of rows, got {rows}")
-        self.N = N = rows // 2 if self.act == 3 else rows
-        if bias is not None and (bias.shape != (rows,) or bias.device != x.device
-                                 or (bias.dtype != x.dtype and bias.dtype != torch.float32)):
-            raise ValueError(f"bias must be a [{rows}] tensor of {x.dtype} or float32 on {x.device}, got {bias.dtype} "
-                             f"{list(bias.shape)} on {bias.device}")
-        self.shape = (*x.shape[:-1], N)
-        if residual is not None and (residual.shape != self.shape or residual.dtype != x.dtype
-                                     or residual.device != x.device):
-            raise ValueError(f"residual must be a {x.dtype} {list(self.shape)} tensor on {x.device}, got "
-                             f"{residual.dtype} {list(residual.shape)} on {residual.device}")
-        self.x, self.weight = _matrix(x), _matrix(weight)
-        self.bias = None if bias is None else bias.contiguous()
-        self.residual = None if residual is None else _matrix(residual)
+        self.N = N = rows // 2 if act == 3 else rows
+        self.f32 = 0
+        if bias is not None:
+            self.f32 = int(bias.dtype == torch.float32)
+            if bias.shape != (rows,) or bias.get_device() != device or not (self.f32 or bias.dtype == x.dtype):
+                raise ValueError(f"bias must be a [{rows}] tensor of {x.dtype} or float32 on {x.device}, got "
+                                 f"{_describe(bias)}")
+            bias = bias.contiguous()
+        self.shape = shape = (*lead[:-1], N)
+        if residual is not None:
+            if residual.shape != shape or residual.dtype != x.dtype or residual.get_device() != device:
+                raise ValueError(f"residual must be a {x.dtype} {list(shape)} tensor on {x.device}, got "
+                                 f"{_describe(residual)}")
+            residual = _matrix(residual)
+        self.x, self.weight, self.bias, self.residual = _matrix(x), _matrix(weight), bias, residual
         self.M = self.x.shape[0]
-        self.dtype = _DTYPES[x.dtype]
-        self.f32 = bias is not None and bias.dtype == torch.float32
 
 
 def _matrix(t: Tensor) -> Tensor:
@@ -301,53 +313,55 @@ def _matrix(t: Tensor) -> Tensor:
     return t
 
 
+# the library takes addresses for their place within 16 bytes alone
+@functools.lru_cache(maxsize=256)
+def _linear_workspace_bytes(*args: int) -> int:
+    return _lib.load().sage_linear_workspace_bytes(*args)
+
+
+@functools.lru_cache(maxsize=256)
+def _linear_bwd_workspace_bytes(*args: int) -> int:
+    return _lib.load().sage_linear_bwd_workspace_bytes(*args)
+
+
 def _linear_forward(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str,
                     keep_z: bool) -> tuple[Tensor, Tensor | None]:
     a = _Linear(x, weight, bias, residual, activation)
-    out = torch.empty(a.shape, dtype=x.dtype, device=x.device)
-    z = torch.empty((a.M, a.rows), dtype=x.dtype, device=x.device) if keep_z and a.act else None
+    out = x.new_empty(a.shape)
+    z = x.new_empty((a.M, a.rows)) if keep_z and a.act else None
     if a.M == 0:
         return out, z
-    with _on(x.device):
-        lib = _lib.load()
-        xp, xs, wp, ws = a.x.data_ptr(), a.x.stride(0), a.weight.data_ptr(), a.weight.stride(0)
-        rp, rs = (0, 0) if a.residual is None else (a.residual.data_ptr(), a.residual.stride(0))
-        bp = 0 if a.bias is None else a.bias.data_ptr()
-        size = lib.sage_linear_workspace_bytes(xp, xs, wp, ws, a.M, a.N, a.K, a.act, (rp | bp) % 16 != 0 or rs % 8 != 0)
-        work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        _lib.check(lib.sage_linear(
-            xp, xs, wp, ws, bp, a.f32, rp, rs, a.M, a.N, a.K, a.dtype, a.act, _ptr(work), size, _ptr(z),
-            out.data_ptr(), _stream_handle(x.device)))
+    xp, xs, wp, ws = a.x.data_ptr(), a.x.stride(0), a.weight.data_ptr(), a.weight.stride(0)
+    rp, rs = (0, 0) if a.residual is None else (a.residual.data_ptr(), a.residual.stride(0))
+    bp = _addr(a.bias)
+    size = _linear_workspace_bytes(xp & 15, xs, wp & 15, ws, a.M, a.N, a.K, a.act, (rp | bp) & 15 != 0 or rs & 7 != 0)
+    work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    _launch(a.device, _lib.load().sage_linear, xp, xs, wp, ws, bp, a.f32, rp, rs, a.M, a.N, a.K, a.dtype, a.act,
+            _addr(work), size, _addr(z), out.data_ptr())
     return out, z
 
 
 def _linear_backward(dout: Tensor, x: Tensor, weight: Tensor, bias: Tensor | None, z: Tensor | None,
-                     activation: str, wanted: list[bool]) -> tuple[Tensor | None, ...]:
+                     activation: str, wanted) -> tuple[Tensor | None, ...]:
     """dx, dweight, dbias (None where not wanted)."""
     a = _Linear(x, weight, bias, None, activation)
-    if dout.shape != a.shape or dout.dtype != x.dtype or dout.device != x.device:
-        raise ValueError(f"dout must be a {x.dtype} {list(a.shape)} tensor on {x.device}, got {dout.dtype} "
-                         f"{list(dout.shape)} on {dout.device}")
+    if dout.shape != a.shape or dout.dtype != x.dtype or dout.get_device() != a.device:
+        raise ValueError(f"dout must be a {x.dtype} {list(a.shape)} tensor on {x.device}, got {_describe(dout)}")
     if a.act and (z is None or z.shape != (a.M, a.rows) or z.dtype != x.dtype or not z.is_contiguous()):
         raise ValueError("the gradient of an activation needs the z that the forward kept (keep_z)")
     dx, dw, db = _grad(x, wanted[0]), _grad(weight, wanted[1]), _grad(bias, wanted[2])
     if a.M == 0:
-        for g in (dw, db):
-            if g is not None:
-                g.zero_()
+        _zero(dw, db)
         return dx, dw, db
     want = (dx is not None) + 2 * (dw is not None) + 4 * (db is not None)
-    if not want:
-        return dx, dw, db
-    d = _matrix(dout)
-    with _on(x.device):
-        lib = _lib.load()
-        rows = (d.data_ptr(), d.stride(0), a.x.data_ptr(), a.x.stride(0), a.weight.data_ptr(), a.weight.stride(0))
-        size = lib.sage_linear_bwd_workspace_bytes(*rows, a.M, a.N, a.K, a.act, want)
+    if want:
+        d = _matrix(dout)
+        dp, ds, xp, xs, wp, ws = (d.data_ptr(), d.stride(0), a.x.data_ptr(), a.x.stride(0), a.weight.data_ptr(),
+                                  a.weight.stride(0))
+        size = _linear_bwd_workspace_bytes(dp & 15, ds, xp & 15, xs, wp & 15, ws, a.M, a.N, a.K, a.act, want)
         work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        _lib.check(lib.sage_linear_bwd(
-            *rows, _ptr(z) if a.act else None, a.M, a.N, a.K, a.dtype, a.act, a.f32, _ptr(work), size, _ptr(dx),
-            _ptr(dw), _ptr(db), _stream_handle(x.device)))
+        _launch(a.device, _lib.load().sage_linear_bwd, dp, ds, xp, xs, wp, ws, _addr(z) if a.act else 0, a.M, a.N,
+                a.K, a.dtype, a.act, a.f32, _addr(work), size, _addr(dx), _addr(dw), _addr(db))
     return dx, dw, db
 
 

@@ -1056,7 +1056,6 @@ int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, c
   g.ldr = r_rs;
   g.z = z;
   g.out = out;
-  g.vec_b = n % 8 == 0 && aligned16(bias);
   g.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at);
   return launch_status(sage::launch_gemm(g, dtype, stream), "sage_linear");
 }
@@ -1103,9 +1102,7 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
     d.act = activation;
     d.dz = p.form_dz ? ws + p.dz_off : nullptr;
     d.ldz = p.ldz;
-    d.vec_d = in_place(dout, d_rs, m, n);
-    d.vec_z = n % 8 == 0 && aligned16(z);
-    d.vec_o = n % 8 == 0;
+    d.vec = in_place(dout, d_rs, m, n) && aligned16(z);
     d.part = dbias ? reinterpret_cast<float*>(ws + p.sum_off) : nullptr;
     d.chunks = p.chunks;
     d.chunk = p.chunk;

@@ -384,8 +384,7 @@ struct GemmArgs {
   int64_t ldr;
   void* z;    // T [m][rows of B]: acc + bias, for the backward; null: not kept
   void* out;  // T [m][n]
-  int vec;    // rows of res, z and out, and the bias, take 16-byte accesses (known to the plan)
-  int vec_b;  // so does the bias
+  int vec;    // rows of res, z and out, and the bias, take 16-byte accesses
   // the plan (gemm_plan)
   int big, skinny, kt, tm, tn;
   int whole, parts;     // tiles past `whole` run as `parts` pieces of the contraction
@@ -402,7 +401,7 @@ struct DactArgs {
   int n, act;
   void* dz;  // rows ldz apart; null: not formed
   int64_t ldz;
-  int vec_d, vec_z, vec_o;
+  int vec;  // every row takes 16-byte accesses (n a multiple of 8)
   float* part;  // column sums [chunks][n or 2n]; null: no bias gradient
   int64_t chunks, chunk;
   void* dbias;

@@ -72,94 +72,11 @@ __device__ __forceinline__ float act_grad(int act, float z) {
   return 1.0f;
 }
 
-// ---------------------------------------------------------------- rows of the epilogue
-
-// Eight consecutive columns of a row of T, at column n of `cols`; past the last: zeros.
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int n, int cols, bool vec, float (&f)[8]) {
-  if (vec) {
-    const auto v = *reinterpret_cast<const typename Vec8<T>::type*>(row + n);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = (float)v[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = n + j < cols ? (float)row[n + j] : 0.0f;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(T* row, int n, int cols, bool vec, const float (&f)[8]) {
-  if (vec) {
-    typename Vec8<T>::type v;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (T)f[j];
-    *reinterpret_cast<typename Vec8<T>::type*>(row + n) = v;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (n + j < cols) row[n + j] = (T)f[j];
-  }
-}
+// ---------------------------------------------------------------- epilogues
 
 __device__ __forceinline__ float param_at(const void* p, bool f32, bool f16, int64_t i) {
   if (f32) return static_cast<const float*>(p)[i];
   return f16 ? (float)static_cast<const _Float16*>(p)[i] : (float)static_cast<const __bf16*>(p)[i];
-}
-
-// Bias of eight columns, `at` rows into the weight (columns past `cols`: zeros).
-template <typename T>
-__device__ __forceinline__ void load_bias(const GemmArgs& a, int at, int n, int cols, float (&f)[8]) {
-  if (a.bias_f32) {
-    const float* b = static_cast<const float*>(a.bias) + at;
-    if (a.vec_b) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(b + n + 4 * q);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[4 * q + j] = v[j];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = n + j < cols ? b[n + j] : 0.0f;
-    }
-  } else {
-    load8<T>(static_cast<const T*>(a.bias) + at, n, cols, a.vec_b, f);
-  }
-}
-
-// The epilogue of row m, columns n .. n + 7 (n < a.n): z = acc + bias, kept when the backward
-// wants it, out = act(z) + residual, rounded once.  z2: the second half of a swiglu.
-template <typename T, int ACT>
-__device__ __forceinline__ void finish8(const GemmArgs& a, int64_t m, int n, float (&z)[8], float (&z2)[8]) {
-  constexpr bool kGlu = ACT == kActSwiglu;
-  if (a.bias) {
-    float b[8];
-    load_bias<T>(a, 0, n, a.n, b);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) z[j] += b[j];
-    if constexpr (kGlu) {
-      load_bias<T>(a, a.n, n, a.n, b);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) z2[j] += b[j];
-    }
-  }
-  if (ACT != kActNone && a.z) {
-    T* row = static_cast<T*>(a.z) + m * (kGlu ? 2 * (int64_t)a.n : a.n);
-    store8<T>(row, n, a.n, a.vec, z);
-    if constexpr (kGlu) store8<T>(row + a.n, n, a.n, a.vec, z2);
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    z[j] = act_fwd(ACT, z[j]);
-    if constexpr (kGlu) z[j] *= z2[j];
-  }
-  if (a.res) {
-    float r[8];
-    load8<T>(static_cast<const T*>(a.res) + m * a.ldr, n, a.n, a.vec, r);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) z[j] += r[j];
-  }
-  store8<T>(static_cast<T*>(a.out) + m * a.n, n, a.n, a.vec, z);
 }
 
 // Columns 8 h .. + 7 of half p (16 columns) of a 32 x 32 accumulator of the transposed
@@ -196,7 +113,8 @@ __device__ __forceinline__ void halves_to_rows(u32x4& x, u32x4& y) {
   }
 }
 
-// finish8 for a wave's MI x NI blocks from row m0 and column n0 on, every access 16 bytes
+// The epilogue of a wave's MI x NI blocks from row m0 and column n0 on: z = acc + bias, kept
+// when the backward wants it, out = act(z) + residual, rounded once.  Every access is 16 bytes
 // through a buffer resource over the rows that exist, straight from the accumulators with no
 // pass through LDS.  What a call does not have (bias, residual, z) has a resource of no
 // bytes, so there is no branch.  PLAIN: out alone.
@@ -300,21 +218,42 @@ __device__ __forceinline__ void finish(const GemmArgs& a, int lane, int64_t m0, 
   else finish_wave<T, kActNone, false>(a, lane, m0, n0, c);
 }
 
-// The same for one row of blocks with rows of any alignment, element by element.
+// The same for one row of blocks (a 32 x 64 part of a tile) whose rows have any alignment: by
+// way of LDS, so that a wave's lanes take consecutive elements of a row (of two rows for a
+// swiglu, which has 32 columns here).  `lds`: 32 x kAnyPitch floats of this wave.
+constexpr int kAnyPitch = 65;
+
 template <typename T, int ACT>
-__device__ __forceinline__ void finish_any(const GemmArgs& a, int lane, int64_t m0, int n0, f32x16 (&c)[1][2]) {
+__device__ __forceinline__ void finish_any(const GemmArgs& a, float* lds, int lane, int64_t m0, int n0,
+                                           f32x16 (&c)[1][2]) {
   constexpr bool kGlu = ACT == kActSwiglu;
-  const int64_t m = m0 + (lane & 31);
+  constexpr int kCols = kGlu ? 32 : 64;
 #pragma unroll
-  for (int j = 0; j < 2; j += kGlu ? 2 : 1)
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      float z[8], z2[8];
-      eight_of(c[0][j], p, z);
-      eight_of(c[0][1], p, z2);
-      const int n = n0 + 32 * j + 16 * p + 8 * (lane >> 5);
-      if (m < a.m && n < a.n) finish8<T, ACT>(a, m, n, z, z2);
+  for (int i = 0; i < 16; ++i) {
+    const int col = 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+    lds[(lane & 31) * kAnyPitch + col] = c[0][0][i];
+    lds[(lane & 31) * kAnyPitch + 32 + col] = c[0][1][i];
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int col = lane % kCols, n = n0 + col;
+  if (n >= a.n) return;
+  const bool f16 = std::is_same<T, _Float16>::value;
+  const float b = a.bias ? param_at(a.bias, a.bias_f32, f16, n) : 0.0f;
+  const float b2 = kGlu && a.bias ? param_at(a.bias, a.bias_f32, f16, a.n + n) : 0.0f;
+  const int64_t wide = kGlu ? 2 * (int64_t)a.n : a.n;
+#pragma unroll 4
+  for (int row = lane / kCols; row < 32; row += 64 / kCols) {
+    const int64_t m = m0 + row;
+    if (m >= a.m) break;
+    const float r = a.res ? (float)static_cast<const T*>(a.res)[m * a.ldr + n] : 0.0f;
+    const float z = lds[row * kAnyPitch + col] + b, z2 = kGlu ? lds[row * kAnyPitch + 32 + col] + b2 : 1.0f;
+    if (ACT != kActNone && a.z) {
+      static_cast<T*>(a.z)[m * wide + n] = (T)z;
+      if constexpr (kGlu) static_cast<T*>(a.z)[m * wide + a.n + n] = (T)z2;
     }
+    static_cast<T*>(a.out)[m * a.n + n] = (T)(act_fwd(ACT, z) * z2 + r);
+  }
 }
 
 // ---------------------------------------------------------------- tiles
@@ -636,11 +575,12 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
   const bool glu = a.act == kActSwiglu;
   const int64_t m0 = (int64_t)tm * TL::BM + (wm * TL::MI + i) * 32;
   const int n0 = tn * (glu ? TL::BN / 2 : TL::BN) + (wn * TL::NI + j) * (glu ? 16 : 32);
+  __shared__ float any[4][32 * kAnyPitch];
   if (a.vec) finish<T>(a, lane, m0, n0, c);
-  else if (a.act == kActSwiglu) finish_any<T, kActSwiglu>(a, lane, m0, n0, c);
-  else if (a.act == kActSilu) finish_any<T, kActSilu>(a, lane, m0, n0, c);
-  else if (a.act == kActGelu) finish_any<T, kActGelu>(a, lane, m0, n0, c);
-  else finish_any<T, kActNone>(a, lane, m0, n0, c);
+  else if (a.act == kActSwiglu) finish_any<T, kActSwiglu>(a, any[wave], lane, m0, n0, c);
+  else if (a.act == kActSilu) finish_any<T, kActSilu>(a, any[wave], lane, m0, n0, c);
+  else if (a.act == kActGelu) finish_any<T, kActGelu>(a, any[wave], lane, m0, n0, c);
+  else finish_any<T, kActNone>(a, any[wave], lane, m0, n0, c);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -752,44 +692,87 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t ld, int
   }
 }
 
-// The gradient of z: dz = dout * act'(z) (swiglu: both halves), rounded to T as the
-// products' operand, into rows of `ldz` (zeros behind the last column); with `part` the
-// column sums of the unrounded values over each chunk of rows, for the bias.  A workgroup
-// takes 512 columns (64 lanes of 8) of a chunk, a wave every fourth row.
-template <typename T>
+// The gradient of z: dz = dout * act'(z) (swiglu: both halves), rounded to T as the products'
+// operand, into rows of `ldz` with zeros behind the last column; with `part` the column sums
+// of the unrounded values over each chunk of rows, for the bias.  A workgroup takes 512
+// columns of a chunk, a wave every fourth row, kDactRows of them in flight; a lane holds eight
+// consecutive columns (VEC), or every 64th where rows take no 16-byte accesses.  Reads past a
+// row's end give zeros and writes are dropped there, so nothing is behind a branch.
+constexpr int kDactRows = 4;
+
+__device__ __forceinline__ uint16_t load_2(__amdgpu_buffer_rsrc_t rs, int off) {
+  return __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0);
+}
+__device__ __forceinline__ void store_2(uint16_t v, __amdgpu_buffer_rsrc_t rs, int off) {
+  __builtin_amdgcn_raw_buffer_store_b16(v, rs, off, 0, 0);
+}
+
+template <typename T, bool VEC>
+struct Eight {
+  typename Vec8<T>::type v;
+  static __device__ __forceinline__ int col(int lane, int j) { return VEC ? lane * 8 + j : j * 64 + lane; }
+  __device__ __forceinline__ void load(const T* row, int n, int cols, int lane) {
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(row, (uint32_t)cols * 2);
+    if constexpr (VEC) {
+      v = __builtin_bit_cast(typename Vec8<T>::type, load_16(rs, (n + lane * 8) * 2));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __builtin_bit_cast(T, load_2(rs, (n + j * 64 + lane) * 2));
+    }
+  }
+  __device__ __forceinline__ void store(T* row, int n, int cols, int lane) const {
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(row, (uint32_t)cols * 2);
+    if constexpr (VEC) {
+      store_16(__builtin_bit_cast(u32x4, v), rs, (n + lane * 8) * 2);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) store_2(__builtin_bit_cast(uint16_t, (T)v[j]), rs, (n + j * 64 + lane) * 2);
+    }
+  }
+};
+
+template <typename T, int ACT, bool VEC>
 __global__ __launch_bounds__(256) void dact_kernel(DactArgs a) {
-  __shared__ float sum[2][4][512];
+  constexpr bool kGlu = ACT == kActSwiglu;
+  __shared__ float sum[kGlu ? 2 : 1][4][512];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const bool glu = a.act == kActSwiglu;
-  const int n = blockIdx.x * 512 + lane * 8;
+  const int n = blockIdx.x * 512, wide = kGlu ? 2 * a.n : a.n;
   const int64_t r0 = (int64_t)blockIdx.y * a.chunk, r1 = r0 + a.chunk < a.m ? r0 + a.chunk : a.m;
   float s1[8] = {}, s2[8] = {};
-  if (n < a.n) {
-#pragma unroll 2
-    for (int64_t m = r0 + wave; m < r1; m += 4) {
-      float d[8], z[8], z2[8];
-      load8<T>(static_cast<const T*>(a.dout) + m * a.ldd, n, a.n, a.vec_d, d);
-      if (a.act != kActNone) {
-        const T* zr = static_cast<const T*>(a.z) + m * (glu ? 2 * a.n : a.n);
-        load8<T>(zr, n, a.n, a.vec_z, z);
-        if (glu) load8<T>(zr + a.n, n, a.n, a.vec_z, z2);
+  for (int64_t m0 = r0 + wave; m0 < r1; m0 += 4 * kDactRows) {
+    Eight<T, VEC> d[kDactRows], z[kDactRows], z2[kDactRows];
+#pragma unroll
+    for (int u = 0; u < kDactRows; ++u) {
+      const int64_t m = m0 + 4 * u;
+      const int cols = m < r1 ? a.n : 0;  // rows past the chunk: nothing is read, zeros are added
+      d[u].load(static_cast<const T*>(a.dout) + m * a.ldd, n, cols, lane);
+      if constexpr (ACT != kActNone) {
+        z[u].load(static_cast<const T*>(a.z) + m * wide, n, cols, lane);
+        if constexpr (kGlu) z2[u].load(static_cast<const T*>(a.z) + m * wide + a.n, n, cols, lane);
       }
+    }
+#pragma unroll
+    for (int u = 0; u < kDactRows; ++u) {
+      const int64_t m = m0 + 4 * u;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (glu) {
-          const float up = d[j] * act_fwd(a.act, z[j]);
-          d[j] = d[j] * z2[j] * act_grad(a.act, z[j]);
-          z2[j] = up;
+        float g = (float)d[u].v[j];
+        if constexpr (kGlu) {
+          const float zz = (float)z[u].v[j], up = g * act_fwd(ACT, zz);
+          g = g * (float)z2[u].v[j] * act_grad(ACT, zz);
+          z2[u].v[j] = (T)up;
           s2[j] += up;
-        } else if (a.act != kActNone) {
-          d[j] *= act_grad(a.act, z[j]);
+        } else if constexpr (ACT != kActNone) {
+          g *= act_grad(ACT, (float)z[u].v[j]);
         }
-        s1[j] += d[j];
+        d[u].v[j] = (T)g;
+        s1[j] += g;
       }
-      if (a.dz) {
+      if (a.dz && m < r1) {
         T* row = static_cast<T*>(a.dz) + m * a.ldz;
-        store8<T>(row, n, a.n, a.vec_o, d);
-        if (glu) store8<T>(row + a.n, n, a.n, a.vec_o, z2);
+        // the last columns of a row go up to its end
+        d[u].store(row, n, kGlu ? a.n : (int)a.ldz, lane);
+        if constexpr (kGlu) z2[u].store(row + a.n, n, (int)a.ldz - a.n, lane);
       }
     }
   }
@@ -797,26 +780,15 @@ __global__ __launch_bounds__(256) void dact_kernel(DactArgs a) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     sum[0][wave][j * 64 + lane] = s1[j];
-    if (glu) sum[1][wave][j * 64 + lane] = s2[j];
+    if constexpr (kGlu) sum[1][wave][j * 64 + lane] = s2[j];
   }
   __syncthreads();
-  for (int u = threadIdx.x; u < (glu ? 1024 : 512); u += 256) {
-    const int half = u >> 9, at = u & 511, col = blockIdx.x * 512 + at;
-    const int v = (at & 7) * 64 + (at >> 3);
+  for (int u = threadIdx.x; u < (kGlu ? 1024 : 512); u += 256) {
+    const int half = u >> 9, at = u & 511, col = n + at;
+    const int v = VEC ? (at & 7) * 64 + (at >> 3) : at;
     if (col < a.n)
-      a.part[(int64_t)blockIdx.y * (glu ? 2 * a.n : a.n) + half * a.n + col] =
+      a.part[(int64_t)blockIdx.y * wide + half * a.n + col] =
           sum[half][0][v] + sum[half][1][v] + sum[half][2][v] + sum[half][3][v];
-  }
-}
-
-// Zeros behind the last column of packed gradient rows.
-template <typename T>
-__global__ __launch_bounds__(256) void clear_tail_kernel(T* p, int64_t rows, int64_t ld, int cols) {
-  const int w = (int)(ld - cols);
-  const int64_t total = rows * w;
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
-    const int64_t r = u / w;
-    p[r * ld + cols + (u - r * w)] = (T)0.0f;
   }
 }
 
@@ -939,19 +911,25 @@ hipError_t launch_pack(int f16, const void* src, int64_t ld, int64_t rows, int64
   return hipGetLastError();
 }
 
+namespace {
+
+template <typename T, bool VEC>
+void run_dact(const DactArgs& a, dim3 grid, hipStream_t st) {
+  if (a.act == kActSwiglu) dact_kernel<T, kActSwiglu, VEC><<<grid, 256, 0, st>>>(a);
+  else if (a.act == kActSilu) dact_kernel<T, kActSilu, VEC><<<grid, 256, 0, st>>>(a);
+  else if (a.act == kActGelu) dact_kernel<T, kActGelu, VEC><<<grid, 256, 0, st>>>(a);
+  else dact_kernel<T, kActNone, VEC><<<grid, 256, 0, st>>>(a);
+}
+
+}  // namespace
+
 hipError_t launch_dact(int f16, const DactArgs& a, hipStream_t st) {
-  const dim3 grid((uint32_t)((a.n + 511) / 512), (uint32_t)a.chunks);
   const int64_t rows = a.act == kActSwiglu ? 2 * a.n : a.n;
-  if (a.dz && a.ldz > rows) {
-    const int64_t blocks = (a.m * (a.ldz - rows) + 255) / 256;
-    clear_tail_kernel<__bf16><<<(uint32_t)(blocks < 1024 ? blocks : 1024), 256, 0, st>>>(
-        static_cast<__bf16*>(a.dz), a.m, a.ldz, (int)rows);
-  }
-  if (f16)
-    dact_kernel<_Float16><<<grid, 256, 0, st>>>(a);
-  else
-    dact_kernel<__bf16><<<grid, 256, 0, st>>>(a);
-  hipError_t e = hipGetLastError();
+  const int64_t cols = a.dz ? a.ldz - (rows - a.n) : a.n;  // of the (last) half, with the zeros behind it
+  const dim3 grid((uint32_t)((cols + 511) / 512), (uint32_t)a.chunks);
+  if (f16) a.vec ? run_dact<_Float16, true>(a, grid, st) : run_dact<_Float16, false>(a, grid, st);
+  else a.vec ? run_dact<__bf16, true>(a, grid, st) : run_dact<__bf16, false>(a, grid, st);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.part) return e;
   if (f16)
     dbias_kernel<_Float16><<<(uint32_t)((rows + 15) / 16), 256, 0, st>>>(a.part, (int)a.chunks, (int)rows, a.dbias, a.bias_f32);
