@@ -386,7 +386,7 @@ struct GemmArgs {
   void* out;  // T [m][n]
   int vec;    // rows of res, z and out, and the bias, take 16-byte accesses
   // the plan (gemm_plan)
-  int big, skinny, kt, tm, tn;
+  int big, skinny, thin, kt, tm, tn;
   int whole, parts;     // tiles past `whole` run as `parts` pieces of the contraction
   int64_t part_floats;  // fp32 sums of the pieces
   float* part;

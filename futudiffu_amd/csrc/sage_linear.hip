@@ -547,6 +547,50 @@ __global__ __launch_bounds__(TL::NT, TL::SIMD) void gemm_kernel(GemmArgs a) {
     finish_wave<T, kActNone, true>(a, lane, mw, nw, acc);
 }
 
+// The products of at most one stage's contraction (an adapter's second product): bound by
+// the output and the residual, so one stage of LDS, several workgroups a CU, and no steps
+// past the last 16 that exist.
+template <typename T, typename TL>
+__global__ __launch_bounds__(TL::NT, 3) void thin_kernel(GemmArgs a) {
+  __shared__ __align__(1024) uint8_t lds[TL::A_BYTES + TL::B_BYTES];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const bool glu = a.act == kActSwiglu;
+  int tm, tn;
+  tile_at(a, xcd_share(blockIdx.x, a.whole), tm, tn);
+  const int64_t m0 = (int64_t)tm * TL::BM;
+  const int n0 = tn * (glu ? TL::BN / 2 : TL::BN);
+  Operand<TL::BM, true, TL::WAVES> A;
+  Operand<TL::BN, true, TL::WAVES> B;
+  A.init(a.a, a.lda, m0, a.m, wave, lane, false, 0);
+  B.init(a.b, a.ldb, n0, a.n, wave, lane, glu, a.n);
+  A.template issue<0, decltype(A)::LOADS>(lds, 0, a.k, wave);
+  B.template issue<0, decltype(B)::LOADS>(lds + TL::A_BYTES, 0, a.k, wave);
+  const int wm = wave / TL::WN, wn = wave % TL::WN;
+  FragAddr<TL::BM, true> fa[TL::MI];
+  FragAddr<TL::BN, true> fb[TL::NI];
+#pragma unroll
+  for (int i = 0; i < TL::MI; ++i) fa[i].init((wm * TL::MI + i) * 32, lane);
+#pragma unroll
+  for (int i = 0; i < TL::NI; ++i) fb[i].init((wn * TL::NI + i) * 32, lane);
+  f32x16 acc[TL::MI][TL::NI] = {};
+  wait_vmem();
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < kBK / 16; ++s) {
+    if (s * 16 >= a.k) break;
+    typename Vec8<T>::type va[TL::MI], vb[TL::NI];
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i) va[i] = frag<T>(lds, fa[i], s);
+#pragma unroll
+    for (int i = 0; i < TL::NI; ++i) vb[i] = frag<T>(lds + TL::A_BYTES, fb[i], s);
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::NI; ++j) acc[i][j] = mfma32(vb[j], va[i], acc[i][j]);
+  }
+  finish<T>(a, lane, m0 + wm * TL::MI * 32, n0 + wn * TL::NI * (glu ? 16 : 32), acc);
+}
+
 // Adds the pieces of the cut tiles in order and finishes them: a wave takes one 32 x 64
 // block of a tile.  Outputs whose rows take no 16-byte accesses all come through here.
 template <typename T, typename TL>
@@ -847,6 +891,10 @@ hipError_t run_skinny(const GemmArgs& a, hipStream_t st) {
 template <typename T>
 hipError_t run(const GemmArgs& a, hipStream_t st) {
   if (a.skinny) return run_skinny<T>(a, st);
+  if (a.thin) {
+    thin_kernel<T, Small><<<a.whole, Small::NT, 0, st>>>(a);
+    return hipGetLastError();
+  }
   if (a.a_kc && a.b_kc) return run_shape<T, true, true>(a, st);
   if (a.a_kc) return run_shape<T, true, false>(a, st);
   return run_shape<T, false, false>(a, st);
@@ -857,7 +905,7 @@ hipError_t run(const GemmArgs& a, hipStream_t st) {
 void gemm_plan(GemmArgs& a) {
   const bool glu = a.act == kActSwiglu;
   a.kt = (int)((a.k + kBK - 1) / kBK);
-  a.skinny = 0;
+  a.skinny = a.thin = 0;
   if (a.a_kc && a.b_kc) {
     const int64_t most = glu ? 32 : 64;
     if (a.m <= most) a.skinny = 1;
@@ -867,22 +915,36 @@ void gemm_plan(GemmArgs& a) {
   a.parts = 1;
   a.tm = a.tn = a.whole = 0;
   if (a.skinny) return;
-  // the tile shape and the split of the last round's tiles with the least estimated time,
-  // in stages of a 256 x 256 tile (about 1 us); see the measurements there
+  a.thin = a.a_kc && a.b_kc && a.k <= kBK && a.vec;
+  if (a.thin) {
+    a.tm = (int)((a.m + Small::BM - 1) / Small::BM);
+    a.tn = (int)((a.n + (glu ? Small::BN / 2 : Small::BN) - 1) / (glu ? Small::BN / 2 : Small::BN));
+    a.whole = a.tm * a.tn;
+    return;
+  }
+  // The tile shape and the split of the last round's tiles with the least estimated time, in
+  // stages of the large tile on every CU.  Measured at 8192 x 8192 x K: large tiles 1.48 us a
+  // stage and 11 us for a round's start and epilogue; small ones 0.94 us and 5 us for a round
+  // of two a CU, 0.55 us a stage for one a CU; joining 4 us and the sums' way out and back at
+  // 4 TB/s.  1280 x 3840 x 10240: 75 large tiles, whole 254 us, in 3 pieces 109; 300 small
+  // ones 136.
   double best = 1e30;
   for (int big = 1; big >= 0; --big) {
     const int bm = big ? Big::BM : Small::BM, bn = (big ? Big::BN : Small::BN) / (glu ? 2 : 1);
     const int64_t tm = (a.m + bm - 1) / bm, tn = (a.n + bn - 1) / bn, tiles = tm * tn;
     const int slots = big ? 256 : 512;
-    const double stage = big ? 1.0 : 0.75, start = 4.0;  // two small tiles share a CU
+    const double start = big ? 7.5 : 3.6;
     for (int p = 1; p <= 16; ++p) {
+      // rows that take no 16-byte accesses are all finished by the join
       const int64_t rest = !a.vec ? tiles : p == 1 ? 0 : tiles % slots;
       if (p > 1 && (rest == 0 || a.kt / p < 4)) continue;
       const int64_t whole = tiles - rest;
+      const double stage = big ? 1.0 : tiles <= 256 && rest * p <= 256 ? 0.37 : 0.63;
       double cost = (double)((whole + slots - 1) / slots) * (a.kt * stage + start);
       if (rest) {
         const double bytes = (double)rest * p * bm * (big ? Big::BN : Small::BN) * 4;
-        cost += (double)((rest * p + slots - 1) / slots) * ((a.kt + p - 1) / p * stage + start) + 6.0 + bytes * 2 / 4e6;
+        cost += (double)((rest * p + slots - 1) / slots) * ((a.kt + p - 1) / p * stage + start) + 2.7 +
+                bytes * 2 / 4e6 / 1.48;
       }
       if (cost < best) {
         best = cost;
