@@ -1,7 +1,8 @@
 """Build recipe for libsage_mi355x.so (gfx950 only).
 
 Compiles the HIP sources under ``csrc/`` with ``hipcc`` into one in-tree
-shared library.  Packed fp32 VALU instructions are disabled
+shared library, and the host side of the block operators (``block_ops.cpp``) into a
+Python extension beside it.  Packed fp32 VALU instructions are disabled
 (``-packed-fp32-ops``); no fast-math flags are used, so fp32 division stays
 correctly rounded, which the quantization codes depend on.
 """
@@ -13,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -25,6 +27,10 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 PHASE_LIB_PATH = os.path.join(HERE, "libsage_mi355x_phase.so")
 SOURCES = ["sage_quant.hip", "sage_attn.hip", "sage_mask.hip", "sage_bwd.hip", "sage_capi.hip",
            "sage_norm.hip", "sage_linear.hip"]
+# the host side of the block operators: a Python extension over torch's C++ API, which takes
+# the library's entry points from the loaded library
+EXT_SOURCE = "block_ops.cpp"
+EXT_PATH = os.path.join(HERE, "_block_ops.so")
 ARCH = "gfx950"
 
 
@@ -53,6 +59,18 @@ def _link(cc: str, objs: list[str], tmp: str, path: str) -> None:
     os.replace(path + ".tmp", path)
 
 
+def ext_command(out: str) -> list[str]:
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
+    return [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            "-DTORCH_EXTENSION_NAME=_block_ops", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", "-I/opt/rocm/include",
+            f"-I{sysconfig.get_paths()['include']}", os.path.join(CSRC, EXT_SOURCE), f"-L{root}/lib", "-lc10",
+            "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-o", out]
+
+
 def build(verbose: bool = False, phase_timing: bool = False) -> str:
     """Compile every source and link LIB_PATH atomically; returns LIB_PATH.
     With phase_timing, builds PHASE_LIB_PATH (-DSAGE_PHASE_TIMING) instead."""
@@ -71,11 +89,27 @@ def build(verbose: bool = False, phase_timing: bool = False) -> str:
             if res.returncode != 0:
                 raise RuntimeError(f"hipcc failed on {srcs[i]}:\n{res.stderr}")
 
-        # one hipcc process per source file, at most four at a time
+        ext = os.path.join(tmp, os.path.basename(EXT_PATH))
+
+        def compile_ext() -> None:
+            cmd = ext_command(ext)
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            res = subprocess.run(cmd, capture_output=True, text=True)
+            if res.returncode != 0:
+                raise RuntimeError(f"the compiler failed on {EXT_SOURCE}:\n{res.stderr}")
+
+        # one compiler process per source file, at most four at a time
         with concurrent.futures.ThreadPoolExecutor(max_workers=min(4, len(srcs))) as pool:
-            for f in [pool.submit(compile_one, i) for i in range(len(srcs))]:
+            jobs = [pool.submit(compile_one, i) for i in range(len(srcs))]
+            if not phase_timing:
+                jobs.append(pool.submit(compile_ext))
+            for f in jobs:
                 f.result()
         _link(cc, objs, tmp, out_path)
+        if not phase_timing:
+            shutil.copyfile(ext, EXT_PATH + ".tmp")
+            os.replace(EXT_PATH + ".tmp", EXT_PATH)
     return out_path
 
 

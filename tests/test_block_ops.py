@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import futudiffu_amd as F
-from futudiffu_amd import _lib, block_ops
+from futudiffu_amd import _lib
 from oracle import block_oracle as O
 
 fake_addresses = pytest.mark.skipif(torch.cuda.device_count() > 0,
@@ -31,24 +31,60 @@ def test_norm_argument_checks():
         F.rms_norm_modulate(x[0, 0])
     with pytest.raises(ValueError, match="bfloat16 or float16"):
         F.rms_norm_modulate(x.float())
-    check_w, check_c, docs = block_ops._check_weight, block_ops._check_cond, block_ops._check_docs
     for w in (torch.zeros(7), torch.zeros(1, 8), torch.zeros(8, dtype=torch.float16), torch.zeros(8, dtype=torch.float64)):
         with pytest.raises(ValueError, match="weight must be"):
-            check_w("weight", w, x, 8)
+            F.rms_norm_modulate(x, w)
+        with pytest.raises(ValueError, match="next_weight must be"):
+            F.rms_norm_gate_residual_modulate(x, x, None, None, w)
+    ids = torch.zeros(2, 4, dtype=torch.int32)
     for k, d in ((torch.zeros(8), False), (torch.zeros(1, 8), False), (torch.zeros(2, 3, 8), False),
                  (torch.zeros(2, 8), True), (torch.zeros(1, 3, 8), True), (torch.zeros(2, 0, 8), True),
                  (torch.zeros(2, 8, dtype=torch.float16), False)):
         with pytest.raises(ValueError, match="gate must be"):
-            check_c("gate", k, x, 2, 8, d)
-    for ids in (torch.zeros(2, 3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)):
+            F.rms_norm_gate_residual(x, x, None, k, doc_ids=ids if d else None)
+        with pytest.raises(ValueError, match="next_scale must be"):
+            F.rms_norm_gate_residual_modulate(x, x, None, None, None, k, doc_ids=ids if d else None)
+    with pytest.raises(ValueError, match="same documents"):
+        F.rms_norm_gate_residual_modulate(x, x, None, torch.zeros(2, 3, 8), None, torch.zeros(2, 2, 8), doc_ids=ids)
+    for bad in (torch.zeros(2, 3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)):
         with pytest.raises(ValueError, match="doc_ids must be"):
-            docs(ids, x, 2, 4)
+            F.rms_norm_modulate(x, doc_ids=bad)
     for t in (torch.zeros(2, 4), torch.zeros(2, 4, dtype=torch.bool)):
         with pytest.raises(ValueError, match="integers"):
-            docs(t, x, 2, 4)
+            F.rms_norm_modulate(x, doc_ids=t)
     for r in (x[:1], x.half(), x[..., :4]):
         with pytest.raises(ValueError, match="residual must be"):
-            block_ops._tokens("residual", r, x)
+            F.rms_norm_gate_residual(r, x)
+    for eps in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="eps must be"):
+            F.rms_norm_modulate(x, eps=eps)
+    with pytest.raises(ValueError, match="at least one channel"):
+        F.rms_norm_modulate(x[..., :0])
+
+
+def test_linear_argument_checks():
+    x, w = torch.zeros(3, 4, 8, dtype=torch.bfloat16), torch.zeros(6, 8, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="must be a GPU tensor"):
+        F.fused_linear(x, w)
+    with pytest.raises(ValueError, match="activation must be one of"):
+        F.fused_linear(x, w, activation="relu")
+    with pytest.raises(ValueError, match="bfloat16 or float16"):
+        F.fused_linear(x.float(), w.float())
+    for bad in (w[:, :7], w[0], w.half(), w[:0], w.float()):
+        with pytest.raises(ValueError, match="weight must be"):
+            F.fused_linear(x, bad)
+    with pytest.raises(ValueError, match="even number of rows"):
+        F.fused_linear(x, w[:5], activation="swiglu")
+    for bad in (torch.zeros(5), torch.zeros(1, 6), torch.zeros(6, dtype=torch.float16)):
+        with pytest.raises(ValueError, match="bias must be"):
+            F.fused_linear(x, w, bad)
+    for bad in (x, torch.zeros(3, 4, 6), torch.zeros(12, 6, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="residual must be"):
+            F.fused_linear(x, w, None, bad)
+    out = torch.ops.futudiffu_ii.fused_linear_backward
+    d = torch.zeros(3, 4, 6, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="must be a GPU tensor"):
+        out(d, x, w, None, None, "silu", [True, True, False])
 
 
 def _modulate(lib, **over):
@@ -130,6 +166,106 @@ def test_norm_workspace_sizes():
             assert slots <= chunks * min(g + 1, -(-n // (chunks // b)))
     for bad in ((0, 1, 8, 1), (1, 0, 8, 1), (1, 1, 0, 1), (1, 1, 8193, 1), (1, 1 << 23, 8, 1), (2, 8, 8, 20000)):
         assert size(*bad, 1, 0) == 0
+
+
+def _linear(lib, **over):
+    a = dict(x=16, xs=72, w=32, ws=72, b=None, bf=0, r=None, rs=0, m=100, n=40, k=72, dt=0, act=0, ws_=None, wsb=0,
+             z=None, out=None, st=None)
+    a.update(over)
+    return lib.sage_linear(*a.values())
+
+
+@pytest.mark.parametrize("over,status,msg", [
+    (dict(m=0), 1, "positive"),
+    (dict(n=0), 1, "positive"),
+    (dict(k=-1), 1, "positive"),
+    (dict(act=4), 1, "activation"),
+    (dict(dt=2), 1, "dtype"),
+    (dict(m=1 << 24), 1, "exceeds"),
+    (dict(k=1 << 22), 1, "exceeds"),
+    (dict(n=1 << 20, k=1 << 11, ws=1 << 11), 1, "2^31 bytes"),
+    (dict(n=1 << 19, k=1 << 11, ws=1 << 11, act=3), 1, "2^31 bytes"),
+    (dict(n=1 << 12, ws=1 << 20), 1, "2^31 bytes"),
+    (dict(), 1, "null"),
+    (dict(xs=71, out=64), 1, "x rows are"),
+    (dict(ws=71, out=64), 1, "weight rows are"),
+    (dict(r=48, rs=39, out=64), 1, "residual rows are"),
+    (dict(xs=1 << 22, out=64), 1, "2^22 or more"),
+    (dict(x=17, out=64), 2, "aligned"),
+    (dict(b=34, bf=1, out=64), 2, "bias must be aligned"),
+    (dict(x=18, out=64), 3, "workspace of"),             # a copy of x
+    (dict(n=65, out=64), 3, "workspace of"),             # rows that the join finishes
+    (dict(x=18, out=64, ws_=72, wsb=1 << 30), 2, "workspace must be"),
+])
+@fake_addresses
+def test_linear_entry_refuses(over, status, msg):
+    lib = _lib.load()
+    assert _linear(lib, **over) == status
+    assert msg in lib.sage_last_error().decode()
+
+
+@fake_addresses
+def test_linear_backward_entry_refuses():
+    lib = _lib.load()
+
+    def call(**over):
+        a = dict(d=16, ds=40, x=32, xs=72, w=48, ws=72, z=None, m=100, n=40, k=72, dt=0, act=0, bf=0, work=None, wsb=0,
+                 dx=64, dw=None, db=None, st=None)
+        a.update(over)
+        return lib.sage_linear_bwd(*a.values()), lib.sage_last_error().decode()
+
+    for over, status, msg in ((dict(d=None), 1, "null"), (dict(w=None), 1, "null"), (dict(dw=80, x=None), 1, "null"),
+                              (dict(act=1), 1, "null"), (dict(ds=39), 1, "dout rows"), (dict(ws=71), 1, "weight rows"),
+                              (dict(dw=80, xs=71), 1, "x rows"), (dict(d=17), 2, "aligned"),
+                              (dict(db=82, bf=1), 2, "dbias"), (dict(dx=72), 2, "16-byte"),
+                              (dict(d=18), 3, "workspace of"), (dict(act=1, z=96), 3, "workspace of"),
+                              (dict(db=80), 3, "workspace of"),
+                              (dict(d=18, work=72, wsb=1 << 30), 2, "workspace must be")):
+        got = call(**over)
+        assert got[0] == status and msg in got[1], (over, got)
+    assert call(dx=None)[0] == 0  # nothing wanted
+
+
+def test_linear_workspace_sizes():
+    """Copies of operands that cannot be read in place, and the sums of cut tiles."""
+    lib = _lib.load()
+    size, bwd = lib.sage_linear_workspace_bytes, lib.sage_linear_bwd_workspace_bytes
+    assert size(16, 72, 32, 72, 3, 40, 72, 0, 0) == 0
+    up = lambda b: (b + 255) // 256 * 256  # noqa: E731
+    assert size(18, 72, 32, 72, 3, 40, 72, 0, 0) == up(3 * 72 * 2)
+    assert size(16, 73, 32, 73, 3, 40, 73, 0, 0) == up(3 * 80 * 2) + up(40 * 80 * 2)
+    # one tile of 128 x 128 finished by the join: its fp32 sums
+    assert size(16, 72, 32, 72, 100, 65, 72, 0, 0) == 128 * 128 * 4
+    assert size(16, 128, 32, 128, 100, 72, 128, 0, 0) == 0 < size(16, 128, 32, 128, 100, 72, 128, 0, 1)
+    for bad in ((0, 8, 8), (8, 0, 8), (8, 8, 0), (1 << 24, 8, 8), (8, 1 << 22, 8)):
+        assert size(16, 8, 32, 8, *bad, 0, 0) == bwd(16, 8, 32, 8, 48, 8, *bad, 0, 7) == 0
+    assert bwd(16, 40, 32, 72, 48, 72, 100, 40, 72, 0, 0) == 0
+    # the bias's column sums: chunks of 32 rows
+    assert bwd(16, 40, 32, 72, 48, 72, 100, 40, 72, 0, 4) == up(4 * 40 * 4)
+
+
+@pytest.mark.parametrize("act", ["none", "silu", "gelu", "swiglu"])
+def test_linear_oracle_against_differentiation(act):
+    """The oracle's gradients are the derivatives of its output (in 64 bits throughout: the
+    roundings are in its bounds alone)."""
+    g = torch.Generator().manual_seed(0)
+
+    def normal(*s):
+        return torch.randn(*s, generator=g, dtype=torch.float64)
+
+    rows = 12 if act == "swiglu" else 6
+    v = dict(x=normal(5, 7), weight=normal(rows, 7), bias=normal(rows), residual=normal(5, 6))
+    d = normal(5, 6)
+    want = O.linear(*v.values(), act, d)
+    leaves = {k: t.clone().requires_grad_() for k, t in v.items()}
+    out = O.linear(*leaves.values(), act)["out"][0]
+    for k, t in zip(leaves, torch.autograd.grad(out, list(leaves.values()), d)):
+        assert torch.allclose(want["d" + k][0], t, rtol=1e-10, atol=1e-12), k
+    z = v["x"] @ v["weight"].T + v["bias"]
+    plain = {"none": lambda: z, "silu": lambda: torch.nn.functional.silu(z),
+             "gelu": lambda: torch.nn.functional.gelu(z, approximate="tanh"),
+             "swiglu": lambda: torch.nn.functional.silu(z[:, :6]) * z[:, 6:]}[act]()
+    assert torch.allclose(out.detach(), plain + v["residual"], rtol=1e-10)
 
 
 @pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
