@@ -165,7 +165,7 @@ _define("fused_linear(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, s
             _load().linear_forward(x, weight, bias, residual, activation, keep_z), x),
         lambda x, weight, bias, residual, activation, keep_z: (
             x.new_empty(*x.shape[:-1], weight.shape[0] // (2 if activation == "swiglu" else 1)),
-            x.new_empty(x.numel() // x.shape[-1], weight.shape[0]) if keep_z and activation != "none"
+            x.new_empty(x.numel() // x.shape[-1], weight.shape[0], dtype=torch.float32) if keep_z and activation != "none"
             else x.new_empty(0)))
 _define("fused_linear_backward(Tensor dout, Tensor x, Tensor weight, Tensor? bias, Tensor? z, str activation, "
         "bool[] wanted) -> (Tensor, Tensor, Tensor)",
@@ -238,9 +238,10 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
     of the gate and then those it multiplies: ``silu(z[..., :N/2]) * z[..., N/2:]``, and the
     output ``N/2`` columns.  Sums are fp32, the output is rounded once.
 
-    For the gradient of an activation the forward keeps ``z = x weight^T + bias`` rounded to
-    ``x``'s type, and ``dout * act'(z)`` is rounded to it as an operand of the products, each
-    as a 16-bit framework does it; the bias's gradient adds it unrounded.
+    For the gradient of an activation the forward keeps ``z = x weight^T + bias`` in fp32 (in
+    16 bits its rounding, beside that of ``dout * act'(z)``, would nearly double the error of a
+    swiglu's gradients); ``dout * act'(z)`` is rounded to ``x``'s type as an operand of the
+    products, and the bias's gradient adds it unrounded.
     """
     if torch.compiler.is_compiling():
         keep = activation != "none" and torch.is_grad_enabled() and any(

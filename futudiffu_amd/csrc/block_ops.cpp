@@ -348,7 +348,7 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight,
   const Linear a(x, weight, bias, residual, activation);
   const auto options = x.options().requires_grad(false);
   Tensor out = at::empty(a.shape, options), z;
-  if (keep_z && a.act != SAGE_ACT_NONE) z = at::empty({a.M, a.rows}, options);
+  if (keep_z && a.act != SAGE_ACT_NONE) z = at::empty({a.M, a.rows}, options.dtype(at::kFloat));
   if (a.M == 0) return {out, z};
   const Matrix xm(x), wm(weight);
   std::optional<Matrix> rm;
@@ -360,7 +360,7 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight,
   const Tensor ws = workspace(x, bytes);
   const Launch on(x);
   check_status(lib.sage_linear(xm.p(), xm.rs, wm.p(), wm.rs, ptr(a.bias), a.f32, rp, rs, a.M, a.N, a.K, a.dtype, a.act,
-                               ptr(ws), bytes, ptr(z), out.data_ptr(), on.stream));
+                               ptr(ws), bytes, static_cast<float*>(ptr(z)), out.data_ptr(), on.stream));
   return {out, z};
 }
 
@@ -371,7 +371,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dout, const Ten
   a.check_out("dout", dout, x);
   const bool act = a.act != SAGE_ACT_NONE;
   TORCH_CHECK_VALUE(!act || (z && z->defined() && z->dim() == 2 && z->size(0) == a.M && z->size(1) == a.rows &&
-                             z->scalar_type() == x.scalar_type() && z->device() == x.device() && z->is_contiguous()),
+                             z->scalar_type() == at::kFloat && z->device() == x.device() && z->is_contiguous()),
                     "the gradient of an activation needs the z that the forward kept (keep_z)");
   Tensor dx = grad_of(x, wanted[0]), dw = grad_of(weight, wanted[1]), db = grad_of(some(bias), wanted[2]);
   const int want = (dx.defined() ? 1 : 0) | (dw.defined() ? 2 : 0) | (db.defined() ? 4 : 0);
@@ -383,7 +383,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dout, const Ten
                                                              a.K, a.act, want);
     const Tensor ws = workspace(x, bytes);
     const Launch on(x);
-    check_status(lib.sage_linear_bwd(dm.p(), dm.rs, xm.p(), xm.rs, wm.p(), wm.rs, act ? z->data_ptr() : nullptr, a.M,
+    check_status(lib.sage_linear_bwd(dm.p(), dm.rs, xm.p(), xm.rs, wm.p(), wm.rs, act ? z->data_ptr<float>() : nullptr, a.M,
                                      a.N, a.K, a.dtype, a.act, a.f32, ptr(ws), bytes, ptr(dx), ptr(dw), ptr(db),
                                      on.stream));
   }

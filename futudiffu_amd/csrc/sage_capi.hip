@@ -895,6 +895,8 @@ int check_linear(int64_t m, int64_t n, int64_t k, int64_t w_rs, int dtype, int a
   if (m >= (int64_t)1 << 24 || n >= (int64_t)1 << 22 || k >= (int64_t)1 << 22)
     return fail(SAGE_ERR_ARG, "m=%lld, n=%lld or k=%lld exceeds 2^24, 2^22, 2^22", (long long)m, (long long)n,
                 (long long)k);
+  if (rows >= (int64_t)1 << 22)
+    return fail(SAGE_ERR_ARG, "a weight of %lld rows, 2^22 or more", (long long)rows);
   if (rows * up8(k) * 2 >= (int64_t)1 << 31 || (rows - 1) * w_rs * 2 + k * 2 >= (int64_t)1 << 31)
     return fail(SAGE_ERR_ARG, "a weight of %lld x %lld has 2^31 bytes or more", (long long)rows, (long long)k);
   return SAGE_OK;
@@ -1021,7 +1023,7 @@ size_t sage_linear_workspace_bytes(const void* x, int64_t x_rs, const void* weig
 
 int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, const void* bias, int bias_fp32,
                 const void* residual, int64_t r_rs, int64_t m, int64_t n, int64_t k, int dtype, int activation,
-                void* workspace, size_t workspace_bytes, void* z, void* out, hipStream_t stream) {
+                void* workspace, size_t workspace_bytes, float* z, void* out, hipStream_t stream) {
   if (const int e = check_linear(m, n, k, w_rs, dtype, activation)) return e;
   const int64_t rows = activation == SAGE_ACT_SWIGLU ? 2 * n : n;
   if (!x || !weight || !out) return fail(SAGE_ERR_ARG, "null tensor pointer");
@@ -1029,10 +1031,10 @@ int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, c
   if (const int e = check_rows(w_rs, rows, k, "weight")) return e;
   if (residual)
     if (const int e = check_rows(r_rs, m, n, "residual")) return e;
-  for (const void* p : {x, weight, residual, (const void*)z, (const void*)out})
+  for (const void* p : {x, weight, residual, (const void*)out})
     if (reinterpret_cast<uintptr_t>(p) & 1u) return fail(SAGE_ERR_ALIGN, "tensor pointers must be aligned to their elements");
-  if (reinterpret_cast<uintptr_t>(bias) & (bias_fp32 ? 3u : 1u))
-    return fail(SAGE_ERR_ALIGN, "bias must be aligned to its elements");
+  if (reinterpret_cast<uintptr_t>(z) & 3u || reinterpret_cast<uintptr_t>(bias) & (bias_fp32 ? 3u : 1u))
+    return fail(SAGE_ERR_ALIGN, "bias must be aligned to its elements, z to 4 bytes");
   size_t at = 0;
   const LinearOperand xo(x, x_rs, m, k, at);
   const LinearOperand wo(weight, w_rs, rows, k, at);
@@ -1068,7 +1070,7 @@ size_t sage_linear_bwd_workspace_bytes(const void* dout, int64_t d_rs, const voi
 }
 
 int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs, const void* weight, int64_t w_rs,
-                    const void* z, int64_t m, int64_t n, int64_t k, int dtype, int activation, int bias_fp32,
+                    const float* z, int64_t m, int64_t n, int64_t k, int dtype, int activation, int bias_fp32,
                     void* workspace, size_t workspace_bytes, void* dx, void* dweight, void* dbias,
                     hipStream_t stream) {
   if (const int e = check_linear(m, n, k, dx ? w_rs : 0, dtype, activation)) return e;
@@ -1082,7 +1084,8 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
     if (const int e = check_rows(x_rs, m, k, "x")) return e;
   if (dx)
     if (const int e = check_rows(w_rs, rows, k, "weight")) return e;
-  for (const void* p : {dout, x, weight, z, (const void*)dx, (const void*)dweight})
+  if (reinterpret_cast<uintptr_t>(z) & 3u) return fail(SAGE_ERR_ALIGN, "z must be aligned to 4 bytes");
+  for (const void* p : {dout, x, weight, (const void*)dx, (const void*)dweight})
     if (reinterpret_cast<uintptr_t>(p) & 1u) return fail(SAGE_ERR_ALIGN, "tensor pointers must be aligned to their elements");
   if (reinterpret_cast<uintptr_t>(dbias) & (bias_fp32 ? 3u : 1u))
     return fail(SAGE_ERR_ALIGN, "dbias must be aligned to its elements");

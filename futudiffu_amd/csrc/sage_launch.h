@@ -382,7 +382,7 @@ struct GemmArgs {
   int bias_f32;
   const void* res;  // T rows ldr apart; null: none
   int64_t ldr;
-  void* z;    // T [m][rows of B]: acc + bias, for the backward; null: not kept
+  float* z;   // fp32 [m][rows of B]: acc + bias, for the backward; null: not kept
   void* out;  // T [m][n]
   int vec;    // rows of res, z and out, and the bias, take 16-byte accesses
   // the plan (gemm_plan)
@@ -396,7 +396,8 @@ hipError_t launch_gemm(const GemmArgs& a, int f16, hipStream_t st);
 hipError_t launch_pack(int f16, const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t pc,
                        hipStream_t st);
 struct DactArgs {
-  const void *dout, *z;  // z: act != none
+  const void* dout;
+  const float* z;  // act != none
   int64_t ldd, m;
   int n, act;
   void* dz;  // rows ldz apart; null: not formed

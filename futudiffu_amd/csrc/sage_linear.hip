@@ -130,7 +130,7 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int lane, int64_t
   const __amdgpu_buffer_rsrc_t out = raw_rsrc(static_cast<T*>(a.out) + m0 * a.n, (uint32_t)rows * a.n * 2);
   const __amdgpu_buffer_rsrc_t res = raw_rsrc(static_cast<const T*>(a.res) + m0 * a.ldr,
                                               a.res ? (uint32_t)(((rows - 1) * a.ldr + a.n) * 2) : 0u);
-  const __amdgpu_buffer_rsrc_t zs = raw_rsrc(static_cast<T*>(a.z) + m0 * wide, a.z ? (uint32_t)rows * wide * 2 : 0u);
+  const __amdgpu_buffer_rsrc_t zs = raw_rsrc(a.z + m0 * wide, a.z ? (uint32_t)rows * wide * 4 : 0u);
   const __amdgpu_buffer_rsrc_t b16 = raw_rsrc(a.bias, a.bias && !a.bias_f32 ? (uint32_t)wide * 2 : 0u);
   const __amdgpu_buffer_rsrc_t b32 = raw_rsrc(a.bias, a.bias && a.bias_f32 ? (uint32_t)wide * 4 : 0u);
   auto bias_at = [&](int n, float (&b)[8]) {  // one of the two reads zeros
@@ -153,11 +153,16 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int lane, int64_t
 #pragma unroll
       for (int q = 0; q < 2; ++q) ahead[to][i][q] = load_16(res, (int)((32 * i + 16 * q + row) * a.ldr + n) * 2 | none);
   };
-  auto store = [&](__amdgpu_buffer_rsrc_t rs, int i, int width, int n, int none, V v0, V v1) {
+  auto store = [&](int i, int n, int none, V v0, V v1) {
     u32x4 x = __builtin_bit_cast(u32x4, v0), y = __builtin_bit_cast(u32x4, v1);
     halves_to_rows(x, y);
-    store_16(x, rs, ((32 * i + row) * width + n) * 2 | none);
-    store_16(y, rs, ((32 * i + 16 + row) * width + n) * 2 | none);
+    store_16(x, out, ((32 * i + row) * a.n + n) * 2 | none);
+    store_16(y, out, ((32 * i + 16 + row) * a.n + n) * 2 | none);
+  };
+  auto keep = [&](int i, int n, int none, const float (&z)[8]) {
+    const int at = ((32 * i + (lane & 31)) * wide + n) * 4 | none;
+    store_16(__builtin_bit_cast(u32x4, f32x4{z[0], z[1], z[2], z[3]}), zs, at);
+    store_16(__builtin_bit_cast(u32x4, f32x4{z[4], z[5], z[6], z[7]}), zs, at + 16);
   };
   if constexpr (!PLAIN) residual(0, 0);
 #pragma unroll
@@ -175,7 +180,7 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int lane, int64_t
     }
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      V o[2], zv[2], zv2[2];
+      V o[2];
       if constexpr (!PLAIN) halves_to_rows(ahead[j / kStep & 1][i][0], ahead[j / kStep & 1][i][1]);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
@@ -187,11 +192,15 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int lane, int64_t
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             z[e] += b[p][e];
-            zv[p][e] = (T)z[e];
-            if constexpr (kGlu) {
-              z2[e] += b2[p][e];
-              zv2[p][e] = (T)z2[e];
-            }
+            if constexpr (kGlu) z2[e] += b2[p][e];
+          }
+          if constexpr (ACT != kActNone) {
+            const int nz = n0 + (32 / kStep) * j + 16 * p + 8 * h, noz = beyond(nz);
+            keep(i, nz, noz, z);
+            if constexpr (kGlu) keep(i, nz + a.n, noz, z2);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
             z[e] = act_fwd(ACT, z[e]);
             if constexpr (kGlu) z[e] *= z2[e];
             z[e] += (float)rv[e];
@@ -200,11 +209,7 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int lane, int64_t
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[p][e] = (T)z[e];
       }
-      if constexpr (!PLAIN && ACT != kActNone) {
-        store(zs, i, wide, n, none, zv[0], zv[1]);
-        if constexpr (kGlu) store(zs, i, wide, n + a.n, none, zv2[0], zv2[1]);
-      }
-      store(out, i, a.n, n, none, o[0], o[1]);
+      store(i, n, none, o[0], o[1]);
     }
     keep_order();
   }
@@ -249,8 +254,8 @@ __device__ __forceinline__ void finish_any(const GemmArgs& a, float* lds, int la
     const float r = a.res ? (float)static_cast<const T*>(a.res)[m * a.ldr + n] : 0.0f;
     const float z = lds[row * kAnyPitch + col] + b, z2 = kGlu ? lds[row * kAnyPitch + 32 + col] + b2 : 1.0f;
     if (ACT != kActNone && a.z) {
-      static_cast<T*>(a.z)[m * wide + n] = (T)z;
-      if constexpr (kGlu) static_cast<T*>(a.z)[m * wide + a.n + n] = (T)z2;
+      a.z[m * wide + n] = z;
+      if constexpr (kGlu) a.z[m * wide + a.n + n] = z2;
     }
     static_cast<T*>(a.out)[m * a.n + n] = (T)(act_fwd(ACT, z) * z2 + r);
   }
@@ -706,9 +711,9 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(GemmArgs a, i
         if (GLU) v2 += param_at(a.bias, a.bias_f32, std::is_same<T, _Float16>::value, a.n + n);
       }
       if (a.z) {
-        T* row = static_cast<T*>(a.z) + m * a.n * H;
-        row[n] = (T)v;
-        if (GLU) row[a.n + n] = (T)v2;
+        float* row = a.z + m * a.n * H;
+        row[n] = v;
+        if (GLU) row[a.n + n] = v2;
       }
       float y = act_fwd(a.act, v);
       if (GLU) y *= v2;
@@ -751,6 +756,10 @@ __device__ __forceinline__ void store_2(uint16_t v, __amdgpu_buffer_rsrc_t rs, i
   __builtin_amdgcn_raw_buffer_store_b16(v, rs, off, 0, 0);
 }
 
+__device__ __forceinline__ uint32_t load_4(__amdgpu_buffer_rsrc_t rs, int off) {
+  return __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
+}
+
 template <typename T, bool VEC>
 struct Eight {
   typename Vec8<T>::type v;
@@ -775,6 +784,26 @@ struct Eight {
   }
 };
 
+// The same columns of a row of fp32 values.
+template <bool VEC>
+struct EightF32 {
+  float v[8];
+  __device__ __forceinline__ void load(const float* row, int n, int cols, int lane) {
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(row, (uint32_t)cols * 4);
+    if constexpr (VEC) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const f32x4 x = __builtin_bit_cast(f32x4, load_16(rs, (n + lane * 8 + q * 4) * 4));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[q * 4 + j] = x[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(load_4(rs, (n + j * 64 + lane) * 4));
+    }
+  }
+};
+
 template <typename T, int ACT, bool VEC>
 __global__ __launch_bounds__(256) void dact_kernel(DactArgs a) {
   constexpr bool kGlu = ACT == kActSwiglu;
@@ -784,15 +813,16 @@ __global__ __launch_bounds__(256) void dact_kernel(DactArgs a) {
   const int64_t r0 = (int64_t)blockIdx.y * a.chunk, r1 = r0 + a.chunk < a.m ? r0 + a.chunk : a.m;
   float s1[8] = {}, s2[8] = {};
   for (int64_t m0 = r0 + wave; m0 < r1; m0 += 4 * kDactRows) {
-    Eight<T, VEC> d[kDactRows], z[kDactRows], z2[kDactRows];
+    Eight<T, VEC> d[kDactRows], up[kDactRows];
+    EightF32<VEC> z[kDactRows], z2[kDactRows];
 #pragma unroll
     for (int u = 0; u < kDactRows; ++u) {
       const int64_t m = m0 + 4 * u;
       const int cols = m < r1 ? a.n : 0;  // rows past the chunk: nothing is read, zeros are added
       d[u].load(static_cast<const T*>(a.dout) + m * a.ldd, n, cols, lane);
       if constexpr (ACT != kActNone) {
-        z[u].load(static_cast<const T*>(a.z) + m * wide, n, cols, lane);
-        if constexpr (kGlu) z2[u].load(static_cast<const T*>(a.z) + m * wide + a.n, n, cols, lane);
+        z[u].load(a.z + m * wide, n, cols, lane);
+        if constexpr (kGlu) z2[u].load(a.z + m * wide + a.n, n, cols, lane);
       }
     }
 #pragma unroll
@@ -802,12 +832,12 @@ __global__ __launch_bounds__(256) void dact_kernel(DactArgs a) {
       for (int j = 0; j < 8; ++j) {
         float g = (float)d[u].v[j];
         if constexpr (kGlu) {
-          const float zz = (float)z[u].v[j], up = g * act_fwd(ACT, zz);
-          g = g * (float)z2[u].v[j] * act_grad(ACT, zz);
-          z2[u].v[j] = (T)up;
-          s2[j] += up;
+          const float zz = z[u].v[j], h = g * act_fwd(ACT, zz);
+          g = g * z2[u].v[j] * act_grad(ACT, zz);
+          up[u].v[j] = (T)h;
+          s2[j] += h;
         } else if constexpr (ACT != kActNone) {
-          g *= act_grad(ACT, (float)z[u].v[j]);
+          g *= act_grad(ACT, z[u].v[j]);
         }
         d[u].v[j] = (T)g;
         s1[j] += g;
@@ -816,7 +846,7 @@ __global__ __launch_bounds__(256) void dact_kernel(DactArgs a) {
         T* row = static_cast<T*>(a.dz) + m * a.ldz;
         // the last columns of a row go up to its end
         d[u].store(row, n, kGlu ? a.n : (int)a.ldz, lane);
-        if constexpr (kGlu) z2[u].store(row + a.n, n, (int)a.ldz - a.n, lane);
+        if constexpr (kGlu) up[u].store(row + a.n, n, (int)a.ldz - a.n, lane);
       }
     }
   }

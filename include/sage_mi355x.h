@@ -480,13 +480,14 @@ int sage_rms_norm_gate_residual_modulate_bwd(
  *   bias         [rows] of dtype, or fp32 (bias_fp32), or null.
  *   residual     [m][n] rows r_rs apart, or null.
  *   activation   SAGE_ACT_*; gelu is the tanh form.
- *   z            [m][rows] contiguous or null: x weight^T + bias rounded to dtype, which
- *                the gradient of an activation needs.
+ *   z            fp32 [m][rows] contiguous or null: x weight^T + bias, which the gradient
+ *                of an activation needs.
  *   out          [m][n] contiguous.
  *   workspace    sage_linear_workspace_bytes(...) bytes, 16-byte aligned; needs no clearing.
  *                other_rows: whether the residual, bias, z or out may start off 16-byte
  *                boundaries, or the residual's rows (r_rs no multiple of 8).
- * m, n, k at least 1; a weight or a row panel of 256 rows has under 2^31 bytes.  Rows of x
+ * m, n, k at least 1; a weight has under 2^22 rows; a weight or a row panel of 256 rows has
+ * under 2^31 bytes.  Rows of x
  * and weight that do not start on 16-byte boundaries, or a k that is no multiple of 8, are
  * copied into the workspace first. */
 #define SAGE_ACT_NONE 0
@@ -498,7 +499,7 @@ size_t sage_linear_workspace_bytes(const void* x, int64_t x_rs, const void* weig
                                    int64_t n, int64_t k, int activation, int other_rows);
 int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, const void* bias, int bias_fp32,
                 const void* residual, int64_t r_rs, int64_t m, int64_t n, int64_t k, int dtype, int activation,
-                void* workspace, size_t workspace_bytes, void* z, void* out, hipStream_t stream);
+                void* workspace, size_t workspace_bytes, float* z, void* out, hipStream_t stream);
 
 /* Gradients of sage_linear: dx [m][k], dweight [rows][k] (both from 16-byte boundaries), dbias
  * [rows] (dtype or fp32), each null if not wanted; the residual's is dout itself.  dz = dout * act'(z) is rounded to dtype
@@ -512,7 +513,7 @@ size_t sage_linear_bwd_workspace_bytes(const void* dout, int64_t d_rs, const voi
                                        const void* weight, int64_t w_rs, int64_t m, int64_t n, int64_t k,
                                        int activation, int want);
 int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs, const void* weight, int64_t w_rs,
-                    const void* z, int64_t m, int64_t n, int64_t k, int dtype, int activation, int bias_fp32,
+                    const float* z, int64_t m, int64_t n, int64_t k, int dtype, int activation, int bias_fp32,
                     void* workspace, size_t workspace_bytes, void* dx, void* dweight, void* dbias,
                     hipStream_t stream);
 

@@ -160,8 +160,8 @@ def linear(x: Tensor, weight: Tensor, bias, residual, activation: str, dout=None
     """``{name: (exact, bound)}`` of fused_linear's output, and with ``dout`` its gradients.
 
     A product of K terms is summed in any order: K roundings of at most the sum of the
-    terms' sizes.  The gradient of an activation takes the rounded z, and its own rounding
-    as the products' operand: half a step of the type each.
+    terms' sizes.  The gradient of z is rounded as the products' operand: half a step of the
+    type.
     """
     eps = torch.finfo(x.dtype).eps
     xd, wd = x.double().reshape(-1, x.shape[-1]), weight.double()
@@ -189,8 +189,8 @@ def linear(x: Tensor, weight: Tensor, bias, residual, activation: str, dout=None
         return r
     g = dout.double().reshape(M, -1)
 
-    def kept(zz, ee):  # z as the backward has it: half a step off
-        return ee + eps / 2 * (zz.abs() + ee).clamp_min(torch.finfo(x.dtype).tiny)
+    def kept(zz, ee):  # z as the backward has it: fp32
+        return ee + U32 * zz.abs()
 
     if activation == "none":
         dz, unrounded, rounded = g, torch.zeros_like(g), torch.zeros_like(g)

@@ -1,6 +1,6 @@
 """GPU: fused_linear (futudiffu_amd/block_ops.py) against its 64-bit definition
 (oracle/block_oracle.py), output and every gradient, in units of what is allowed: the bound
-on 32-bit sums in any order and on the 16-bit z and dz, then one rounding."""
+on 32-bit sums in any order and on the 16-bit dz, then one rounding."""
 
 import pytest
 import torch
@@ -198,7 +198,7 @@ def test_gradient_against_differences(cuda):
 
             (num, hi), (half, _) = diff(1.0), diff(0.5)
             noise = 4 * ((hi * 2.0 ** -11 * u["dout"].double()) ** 2).sum().sqrt()
-            # z, dz and the gradient itself in fp16: 2^-11 each of terms added in quadrature
+            # dz and the gradient itself in fp16: 2^-11 each of terms added in quadrature
             own = 4 * 2.0 ** -11 * ((got["d" + leaf].double().abs() + 1) * step.double()).pow(2).sum().sqrt() * 8
             cubic = abs(float(num - half)) * 4 / 3 + 2 * float(noise)
             assert abs(float(num - ana)) <= float(noise + own) + cubic, (act, leaf, float(num), float(ana))
