@@ -927,8 +927,8 @@ struct LinearOperand {
   }
   const void* ptr(void* ws) const { return copy ? static_cast<uint8_t*>(ws) + off : src; }
   int64_t ld() const { return copy ? pc : rows == 1 ? up8(cols) : rs; }
-  hipError_t pack(int dtype, void* ws, hipStream_t st) const {
-    return copy ? sage::launch_pack(dtype, src, rs, rows, cols, static_cast<uint8_t*>(ws) + off, pc, st) : hipSuccess;
+  sage::PackArgs pack(void* ws) const {
+    return {copy ? src : nullptr, rs, rows, cols, static_cast<uint8_t*>(ws) + off, pc};
   }
 };
 
@@ -1045,8 +1045,7 @@ int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, c
   if (need && (!workspace || workspace_bytes < need))
     return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu", need, workspace_bytes);
   if (need && !aligned16(workspace)) return fail(SAGE_ERR_ALIGN, "workspace must be 16-byte aligned");
-  hipError_t e = xo.pack(dtype, workspace, stream);
-  if (e == hipSuccess) e = wo.pack(dtype, workspace, stream);
+  const hipError_t e = sage::launch_pack(xo.pack(workspace), wo.pack(workspace), stream);
   if (e != hipSuccess) return launch_status(e, "sage_linear (copy)");
   g.a = xo.ptr(workspace);
   g.lda = xo.ld();
@@ -1115,12 +1114,9 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
     if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (activation)");
   }
   const void* dz = p.form_dz ? ws + p.dz_off : dout;
-  if (p.copy_x) {
-    const hipError_t e = sage::launch_pack(dtype, x, x_rs, m, k, ws + p.x_off, up8(k), stream);
-    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (copy)");
-  }
-  if (p.copy_w) {
-    const hipError_t e = sage::launch_pack(dtype, weight, w_rs, rows, k, ws + p.w_off, up8(k), stream);
+  if (p.copy_x || p.copy_w) {
+    const hipError_t e = sage::launch_pack({p.copy_x ? x : nullptr, x_rs, m, k, ws + p.x_off, up8(k)},
+                                           {p.copy_w ? weight : nullptr, w_rs, rows, k, ws + p.w_off, up8(k)}, stream);
     if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (copy)");
   }
   if (dx) {

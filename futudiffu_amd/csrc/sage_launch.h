@@ -393,8 +393,13 @@ struct GemmArgs {
 };
 void gemm_plan(GemmArgs& a);
 hipError_t launch_gemm(const GemmArgs& a, int f16, hipStream_t st);
-hipError_t launch_pack(int f16, const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t pc,
-                       hipStream_t st);
+struct PackArgs {  // src null: nothing to copy
+  const void* src;
+  int64_t ld, rows, cols;
+  void* dst;
+  int64_t pc;
+};
+hipError_t launch_pack(const PackArgs& a, const PackArgs& b, hipStream_t st);
 struct DactArgs {
   const void* dout;
   const float* z;  // act != none

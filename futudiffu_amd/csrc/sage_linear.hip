@@ -242,15 +242,14 @@ __device__ __forceinline__ void finish_any(const GemmArgs& a, float* lds, int la
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
   const int col = lane % kCols, n = n0 + col;
-  if (n >= a.n) return;
-  const bool f16 = std::is_same<T, _Float16>::value;
-  const float b = a.bias ? param_at(a.bias, a.bias_f32, f16, n) : 0.0f;
-  const float b2 = kGlu && a.bias ? param_at(a.bias, a.bias_f32, f16, a.n + n) : 0.0f;
+  const bool f16 = std::is_same<T, _Float16>::value, in = n < a.n;
+  const float b = in && a.bias ? param_at(a.bias, a.bias_f32, f16, n) : 0.0f;
+  const float b2 = kGlu && in && a.bias ? param_at(a.bias, a.bias_f32, f16, a.n + n) : 0.0f;
   const int64_t wide = kGlu ? 2 * (int64_t)a.n : a.n;
 #pragma unroll 4
   for (int row = lane / kCols; row < 32; row += 64 / kCols) {
     const int64_t m = m0 + row;
-    if (m >= a.m) break;
+    if (m >= a.m || !in) break;
     const float r = a.res ? (float)static_cast<const T*>(a.res)[m * a.ldr + n] : 0.0f;
     const float z = lds[row * kAnyPitch + col] + b, z2 = kGlu ? lds[row * kAnyPitch + 32 + col] + b2 : 1.0f;
     if (ACT != kActNone && a.z) {
@@ -259,6 +258,18 @@ __device__ __forceinline__ void finish_any(const GemmArgs& a, float* lds, int la
     }
     static_cast<T*>(a.out)[m * a.n + n] = (T)(act_fwd(ACT, z) * z2 + r);
   }
+  // the next block's sums are written behind these reads
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <typename T, bool ACTS>
+__device__ __forceinline__ void finish_any_act(const GemmArgs& a, float* lds, int lane, int64_t m0, int n0,
+                                               f32x16 (&c)[1][2]) {
+  if (ACTS && a.act == kActSwiglu) finish_any<T, kActSwiglu>(a, lds, lane, m0, n0, c);
+  else if (ACTS && a.act == kActSilu) finish_any<T, kActSilu>(a, lds, lane, m0, n0, c);
+  else if (ACTS && a.act == kActGelu) finish_any<T, kActGelu>(a, lds, lane, m0, n0, c);
+  else finish_any<T, kActNone>(a, lds, lane, m0, n0, c);
 }
 
 // ---------------------------------------------------------------- tiles
@@ -546,6 +557,20 @@ __global__ __launch_bounds__(TL::NT, TL::SIMD) void gemm_kernel(GemmArgs a) {
   }
   const int64_t mw = m0 + wm * TL::MI * 32;
   const int nw = n0 + wn * TL::NI * (glu ? 16 : 32);
+  if constexpr (TL::SIMD > 1) {
+    if (!a.vec) {
+      barrier();  // every wave has read its last fragments: the stages' LDS is free
+      float* const mine = reinterpret_cast<float*>(lds) + wave * 32 * kAnyPitch;
+#pragma unroll
+      for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < TL::NI; j += 2) {
+          f32x16 c[1][2] = {{acc[i][j], acc[i][j + 1]}};
+          finish_any_act<T, AK && BKC>(a, mine, lane, mw + 32 * i, nw + j * (glu ? 16 : 32), c);
+        }
+      return;
+    }
+  }
   if constexpr (AK && BKC)
     finish<T>(a, lane, mw, nw, acc);
   else
@@ -597,7 +622,7 @@ __global__ __launch_bounds__(TL::NT, 3) void thin_kernel(GemmArgs a) {
 }
 
 // Adds the pieces of the cut tiles in order and finishes them: a wave takes one 32 x 64
-// block of a tile.  Outputs whose rows take no 16-byte accesses all come through here.
+// block of a tile.  Large tiles whose rows take no 16-byte accesses all come through here.
 template <typename T, typename TL>
 __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -626,10 +651,7 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
   const int n0 = tn * (glu ? TL::BN / 2 : TL::BN) + (wn * TL::NI + j) * (glu ? 16 : 32);
   __shared__ float any[4][32 * kAnyPitch];
   if (a.vec) finish<T>(a, lane, m0, n0, c);
-  else if (a.act == kActSwiglu) finish_any<T, kActSwiglu>(a, any[wave], lane, m0, n0, c);
-  else if (a.act == kActSilu) finish_any<T, kActSilu>(a, any[wave], lane, m0, n0, c);
-  else if (a.act == kActGelu) finish_any<T, kActGelu>(a, any[wave], lane, m0, n0, c);
-  else finish_any<T, kActNone>(a, any[wave], lane, m0, n0, c);
+  else finish_any_act<T, true>(a, any[wave], lane, m0, n0, c);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -725,19 +747,22 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(GemmArgs a, i
 
 // ---------------------------------------------------------------- operands and gradients beside the products
 
-// Rows [rows][cols] at any alignment into 16-byte aligned rows of `pc` columns (a multiple
-// of 8), zeros behind the last column: what the products read.
-template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t ld, int64_t rows, int64_t cols, T* dst,
-                                                   int64_t pc) {
-  const int64_t chunks = pc / 8, total = rows * chunks;
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
-    const int64_t r = u / chunks;
-    const int c = (int)(u - r * chunks) * 8;
-    typename Vec8<T>::type v;
+// Rows [rows][cols] of 16-bit elements at any alignment into 16-byte aligned rows of `pc`
+// columns (a multiple of 8), zeros behind the last column: what the products read.  Two
+// operands in one launch.
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs a0, PackArgs a1, int64_t units0, int64_t units) {
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += (int64_t)gridDim.x * 256) {
+    const PackArgs& a = u < units0 ? a0 : a1;
+    const int64_t v = u < units0 ? u : u - units0, chunks = a.pc / 8, r = v / chunks;
+    const int c = (int)(v - r * chunks) * 8;
+    const uint16_t* const src = static_cast<const uint16_t*>(a.src) + r * a.ld + c;
+    uint16_t e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? src[r * ld + c + j] : (T)0.0f;
-    *reinterpret_cast<typename Vec8<T>::type*>(dst + r * pc + c) = v;
+    for (int j = 0; j < 8; ++j) e[j] = c + j < a.cols ? src[j] : (uint16_t)0;
+    u32x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = e[2 * j] | (uint32_t)e[2 * j + 1] << 16;
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.dst) + r * a.pc + c) = o;
   }
 }
 
@@ -965,8 +990,9 @@ void gemm_plan(GemmArgs& a) {
     const int slots = big ? 256 : 512;
     const double start = big ? 7.5 : 3.6;
     for (int p = 1; p <= 16; ++p) {
-      // rows that take no 16-byte accesses are all finished by the join
-      const int64_t rest = !a.vec ? tiles : p == 1 ? 0 : tiles % slots;
+      // rows that take no 16-byte accesses are finished by the small tiles themselves, and
+      // with large ones by the join
+      const int64_t rest = !a.vec && (big || p > 1) ? tiles : p == 1 ? 0 : tiles % slots;
       if (p > 1 && (rest == 0 || a.kt / p < 4)) continue;
       const int64_t whole = tiles - rest;
       const double stage = big ? 1.0 : tiles <= 256 && rest * p <= 256 ? 0.37 : 0.63;
@@ -993,13 +1019,11 @@ hipError_t launch_gemm(const GemmArgs& a, int f16, hipStream_t st) {
   return f16 ? run<_Float16>(a, st) : run<__bf16>(a, st);
 }
 
-hipError_t launch_pack(int f16, const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t pc,
-                       hipStream_t st) {
-  const int64_t units = rows * (pc / 8), blocks = (units + 255) / 256;
-  const uint32_t grid = (uint32_t)(blocks < 4096 ? blocks : 4096);
-  // both types are 16 bits wide and copied as they are
-  (void)f16;
-  pack_kernel<__bf16><<<grid, 256, 0, st>>>(static_cast<const __bf16*>(src), ld, rows, cols, static_cast<__bf16*>(dst), pc);
+hipError_t launch_pack(const PackArgs& a, const PackArgs& b, hipStream_t st) {
+  const int64_t units0 = a.src ? a.rows * (a.pc / 8) : 0, units = units0 + (b.src ? b.rows * (b.pc / 8) : 0);
+  if (units == 0) return hipSuccess;
+  const int64_t blocks = (units + 255) / 256;
+  pack_kernel<<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(a, b, units0, units);
   return hipGetLastError();
 }
 

@@ -194,7 +194,7 @@ def _linear(lib, **over):
     (dict(x=17, out=64), 2, "aligned"),
     (dict(b=34, bf=1, out=64), 2, "bias must be aligned"),
     (dict(x=18, out=64), 3, "workspace of"),             # a copy of x
-    (dict(n=65, out=64), 3, "workspace of"),             # rows that the join finishes
+    (dict(m=1280, n=3840, k=10240, xs=10240, ws=10240, out=64), 3, "workspace of"),  # tiles in pieces
     (dict(x=18, out=64, ws_=72, wsb=1 << 30), 2, "workspace must be"),
 ])
 @fake_addresses
@@ -234,9 +234,9 @@ def test_linear_workspace_sizes():
     up = lambda b: (b + 255) // 256 * 256  # noqa: E731
     assert size(18, 72, 32, 72, 3, 40, 72, 0, 0) == up(3 * 72 * 2)
     assert size(16, 73, 32, 73, 3, 40, 73, 0, 0) == up(3 * 80 * 2) + up(40 * 80 * 2)
-    # one tile of 128 x 128 finished by the join: its fp32 sums
-    assert size(16, 72, 32, 72, 100, 65, 72, 0, 0) == 128 * 128 * 4
-    assert size(16, 128, 32, 128, 100, 72, 128, 0, 0) == 0 < size(16, 128, 32, 128, 100, 72, 128, 0, 1)
+    assert size(16, 72, 32, 72, 100, 65, 72, 0, 0) == size(16, 128, 32, 128, 100, 72, 128, 0, 1) == 0
+    # 75 tiles of 256 x 256 in 3 pieces: their fp32 sums
+    assert size(16, 10240, 32, 10240, 1280, 3840, 10240, 0, 0) == 75 * 3 * 256 * 256 * 4
     for bad in ((0, 8, 8), (8, 0, 8), (8, 8, 0), (1 << 24, 8, 8), (8, 1 << 22, 8)):
         assert size(16, 8, 32, 8, *bad, 0, 0) == bwd(16, 8, 32, 8, 48, 8, *bad, 0, 7) == 0
     assert bwd(16, 40, 32, 72, 48, 72, 100, 40, 72, 0, 0) == 0
