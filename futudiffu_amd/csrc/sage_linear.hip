@@ -223,53 +223,74 @@ __device__ __forceinline__ void finish(const GemmArgs& a, int lane, int64_t m0, 
   else finish_wave<T, kActNone, false>(a, lane, m0, n0, c);
 }
 
-// The same for one row of blocks (a 32 x 64 part of a tile) whose rows have any alignment: by
-// way of LDS, so that a wave's lanes take consecutive elements of a row (of two rows for a
-// swiglu, which has 32 columns here).  `lds`: 32 x kAnyPitch floats of this wave.
-constexpr int kAnyPitch = 65;
+// The same for 32 R x 64 parts of a tile whose rows have any alignment: by way of LDS, so that
+// a wave's lanes take consecutive elements of a row (of two rows for a swiglu, which has 32
+// columns here), kAnyRows rows in flight.  `lds`: 32 R x kAnyPitch floats of this wave.
+constexpr int kAnyPitch = 65, kAnyRows = 16;
 
-template <typename T, int ACT>
-__device__ __forceinline__ void finish_any(const GemmArgs& a, float* lds, int lane, int64_t m0, int n0,
-                                           f32x16 (&c)[1][2]) {
-  constexpr bool kGlu = ACT == kActSwiglu;
-  constexpr int kCols = kGlu ? 32 : 64;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int col = 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-    lds[(lane & 31) * kAnyPitch + col] = c[0][0][i];
-    lds[(lane & 31) * kAnyPitch + 32 + col] = c[0][1][i];
-  }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  const int col = lane % kCols, n = n0 + col;
-  const bool f16 = std::is_same<T, _Float16>::value, in = n < a.n;
-  const float b = in && a.bias ? param_at(a.bias, a.bias_f32, f16, n) : 0.0f;
-  const float b2 = kGlu && in && a.bias ? param_at(a.bias, a.bias_f32, f16, a.n + n) : 0.0f;
-  const int64_t wide = kGlu ? 2 * (int64_t)a.n : a.n;
-#pragma unroll 4
-  for (int row = lane / kCols; row < 32; row += 64 / kCols) {
-    const int64_t m = m0 + row;
-    if (m >= a.m || !in) break;
-    const float r = a.res ? (float)static_cast<const T*>(a.res)[m * a.ldr + n] : 0.0f;
-    const float z = lds[row * kAnyPitch + col] + b, z2 = kGlu ? lds[row * kAnyPitch + 32 + col] + b2 : 1.0f;
-    if (ACT != kActNone && a.z) {
-      a.z[m * wide + n] = z;
-      if constexpr (kGlu) a.z[m * wide + a.n + n] = z2;
-    }
-    static_cast<T*>(a.out)[m * a.n + n] = (T)(act_fwd(ACT, z) * z2 + r);
-  }
-  // the next block's sums are written behind these reads
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
+__device__ __forceinline__ uint16_t load_2(__amdgpu_buffer_rsrc_t rs, int off) {
+  return __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0);
+}
+__device__ __forceinline__ void store_2(uint16_t v, __amdgpu_buffer_rsrc_t rs, int off) {
+  __builtin_amdgcn_raw_buffer_store_b16(v, rs, off, 0, 0);
+}
+__device__ __forceinline__ void store_4(uint32_t v, __amdgpu_buffer_rsrc_t rs, int off) {
+  __builtin_amdgcn_raw_buffer_store_b32(v, rs, off, 0, 0);
 }
 
-template <typename T, bool ACTS>
-__device__ __forceinline__ void finish_any_act(const GemmArgs& a, float* lds, int lane, int64_t m0, int n0,
-                                               f32x16 (&c)[1][2]) {
-  if (ACTS && a.act == kActSwiglu) finish_any<T, kActSwiglu>(a, lds, lane, m0, n0, c);
-  else if (ACTS && a.act == kActSilu) finish_any<T, kActSilu>(a, lds, lane, m0, n0, c);
-  else if (ACTS && a.act == kActGelu) finish_any<T, kActGelu>(a, lds, lane, m0, n0, c);
-  else finish_any<T, kActNone>(a, lds, lane, m0, n0, c);
+// Puts a pair of accumulators at row block i of the wave's LDS.
+__device__ __forceinline__ void stage_any(float* lds, int lane, int i, const f32x16& c0, const f32x16& c1) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int col = 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+    lds[(32 * i + (lane & 31)) * kAnyPitch + col] = c0[e];
+    lds[(32 * i + (lane & 31)) * kAnyPitch + 32 + col] = c1[e];
+  }
+}
+
+template <typename T, int ACT, int R>
+__device__ __forceinline__ void finish_any(const GemmArgs& a, const float* lds, int lane, int64_t m0, int n0) {
+  constexpr bool kGlu = ACT == kActSwiglu;
+  constexpr int kCols = kGlu ? 32 : 64, kPer = 64 / kCols;  // rows a wave takes at a time
+  const int64_t left = a.m - m0;
+  if (left <= 0) return;
+  const int rows = left < 32 * R ? (int)left : 32 * R, wide = kGlu ? 2 * a.n : a.n;
+  const int col = lane % kCols, n = n0 + col, none = n < a.n ? 0 : (int)0x80000000;
+  const __amdgpu_buffer_rsrc_t out = raw_rsrc(static_cast<T*>(a.out) + m0 * a.n, (uint32_t)rows * a.n * 2);
+  const __amdgpu_buffer_rsrc_t res = raw_rsrc(static_cast<const T*>(a.res) + m0 * a.ldr,
+                                              a.res ? (uint32_t)(((rows - 1) * a.ldr + a.n) * 2) : 0u);
+  const __amdgpu_buffer_rsrc_t zs = raw_rsrc(a.z + m0 * wide, a.z ? (uint32_t)rows * wide * 4 : 0u);
+  const bool f16 = std::is_same<T, _Float16>::value, bias = a.bias && !none;
+  const float b = bias ? param_at(a.bias, a.bias_f32, f16, n) : 0.0f;
+  const float b2 = kGlu && bias ? param_at(a.bias, a.bias_f32, f16, a.n + n) : 0.0f;
+#pragma unroll 1
+  for (int r0 = lane / kCols; r0 < 32 * R; r0 += kAnyRows * kPer) {
+    float r[kAnyRows];
+#pragma unroll
+    for (int u = 0; u < kAnyRows; ++u)
+      r[u] = (float)__builtin_bit_cast(T, load_2(res, (int)((r0 + u * kPer) * a.ldr + n) * 2 | none));
+#pragma unroll
+    for (int u = 0; u < kAnyRows; ++u) {
+      const int row = r0 + u * kPer;
+      const float z = lds[row * kAnyPitch + col] + b, z2 = kGlu ? lds[row * kAnyPitch + 32 + col] + b2 : 1.0f;
+      if constexpr (ACT != kActNone) {
+        store_4(__float_as_uint(z), zs, (row * wide + n) * 4 | none);
+        if constexpr (kGlu) store_4(__float_as_uint(z2), zs, (row * wide + a.n + n) * 4 | none);
+      }
+      store_2(__builtin_bit_cast(uint16_t, (T)(act_fwd(ACT, z) * z2 + r[u])), out, (row * a.n + n) * 2 | none);
+    }
+  }
+}
+
+template <typename T, bool ACTS, int R>
+__device__ __forceinline__ void finish_any_act(const GemmArgs& a, float* lds, int lane, int64_t m0, int n0) {
+  // the wave's sums are written before they are read
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (ACTS && a.act == kActSwiglu) finish_any<T, kActSwiglu, R>(a, lds, lane, m0, n0);
+  else if (ACTS && a.act == kActSilu) finish_any<T, kActSilu, R>(a, lds, lane, m0, n0);
+  else if (ACTS && a.act == kActGelu) finish_any<T, kActGelu, R>(a, lds, lane, m0, n0);
+  else finish_any<T, kActNone, R>(a, lds, lane, m0, n0);
 }
 
 // ---------------------------------------------------------------- tiles
@@ -560,14 +581,11 @@ __global__ __launch_bounds__(TL::NT, TL::SIMD) void gemm_kernel(GemmArgs a) {
   if constexpr (TL::SIMD > 1) {
     if (!a.vec) {
       barrier();  // every wave has read its last fragments: the stages' LDS is free
-      float* const mine = reinterpret_cast<float*>(lds) + wave * 32 * kAnyPitch;
+      static_assert(TL::NI == 2 && TL::WAVES * TL::MI * 32 * kAnyPitch * 4 <= TL::LDS, "the sums fit");
+      float* const mine = reinterpret_cast<float*>(lds) + wave * TL::MI * 32 * kAnyPitch;
 #pragma unroll
-      for (int i = 0; i < TL::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < TL::NI; j += 2) {
-          f32x16 c[1][2] = {{acc[i][j], acc[i][j + 1]}};
-          finish_any_act<T, AK && BKC>(a, mine, lane, mw + 32 * i, nw + j * (glu ? 16 : 32), c);
-        }
+      for (int i = 0; i < TL::MI; ++i) stage_any(mine, lane, i, acc[i][0], acc[i][1]);
+      finish_any_act<T, AK && BKC, TL::MI>(a, mine, lane, mw, nw);
       return;
     }
   }
@@ -650,8 +668,12 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
   const int64_t m0 = (int64_t)tm * TL::BM + (wm * TL::MI + i) * 32;
   const int n0 = tn * (glu ? TL::BN / 2 : TL::BN) + (wn * TL::NI + j) * (glu ? 16 : 32);
   __shared__ float any[4][32 * kAnyPitch];
-  if (a.vec) finish<T>(a, lane, m0, n0, c);
-  else finish_any_act<T, true>(a, any[wave], lane, m0, n0, c);
+  if (a.vec) {
+    finish<T>(a, lane, m0, n0, c);
+  } else {
+    stage_any(any[wave], lane, 0, c[0][0], c[0][1]);
+    finish_any_act<T, true, 1>(a, any[wave], lane, m0, n0);
+  }
 }
 
 // ---------------------------------------------------------------- few rows
@@ -773,13 +795,6 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a0, PackArgs a1, int
 // consecutive columns (VEC), or every 64th where rows take no 16-byte accesses.  Reads past a
 // row's end give zeros and writes are dropped there, so nothing is behind a branch.
 constexpr int kDactRows = 4;
-
-__device__ __forceinline__ uint16_t load_2(__amdgpu_buffer_rsrc_t rs, int off) {
-  return __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0);
-}
-__device__ __forceinline__ void store_2(uint16_t v, __amdgpu_buffer_rsrc_t rs, int off) {
-  __builtin_amdgcn_raw_buffer_store_b16(v, rs, off, 0, 0);
-}
 
 __device__ __forceinline__ uint32_t load_4(__amdgpu_buffer_rsrc_t rs, int off) {
   return __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
