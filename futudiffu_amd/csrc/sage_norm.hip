@@ -21,6 +21,7 @@
 //
 // Every kernel is bound by memory: a token's channels are held in registers between
 // the reads and the writes, so each tensor is touched once.
+#include <algorithm>
 #include <type_traits>
 
 #include "sage_common.h"
@@ -428,102 +429,185 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
     for (int s = slot + (int)threadIdx.x; s < a.slots; s += kBwdNT) a.part_id[(int64_t)blockIdx.x * a.slots + s] = -1;
 }
 
-// The parameters' gradients from the partial rows.  blockIdx.y: set * (B * groups + 1) + job;
-// job < B * groups: dcond[b][g] = w * (sum of the partials of its id); the last job: dw =
-// sum over all partials of m * S.  A workgroup takes 64 channels (16 threads of 4), its 32
-// thread rows every 32nd chunk, added in order at the end.  The loads of kBatch chunks are
-// in flight together: with one chunk at a time and 16 thread rows the kernel took 22 us
-// at 256 chunks of 3840 channels, all of it latency.
-constexpr int kParamRows = 32, kBatch = 8;
+// The parameters' gradients from the partial rows, in jobs of one workgroup: first dw = sum
+// over all partials of m * S, 64 channels a job; then dcond[b][g] = w * (sum of the partials
+// of its id), `cond_blocks` jobs a row, each every cond_blocks-th 64 channels.
+// 16 threads of 4 channels; the workgroup's 32 thread rows take every 32nd partial and are
+// added in order at the end.  The loads of kBatch partials are in flight together: with one
+// at a time and 16 thread rows the kernel took 22 us at 256 chunks of 3840 channels, all of
+// it latency.
+//
+// A chunk's ids ascend and end in -1, so a row's partials are found by a search in each
+// chunk, one thread a chunk, once a job: 4000 documents in 16384 tokens of 2304 channels
+// took 5.5 ms with a scan of every chunk's ids.
+constexpr int kParamRows = 32, kBatch = 8, kParamNT = 16 * kParamRows;
 
 template <typename T>
-__global__ __launch_bounds__(16 * kParamRows) void norm_param_kernel(NormArgs a, int sets, int modulate) {
-  __shared__ f32x4 sum[kParamRows][16];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int jobs = a.b * a.groups + 1;
-  const int set = blockIdx.y / jobs, job = blockIdx.y - set * jobs;
-  const int col = blockIdx.x * 64 + tx * 4;
-  const bool dw = job == jobs - 1;
-  const int b = dw ? 0 : job / a.groups, g = dw ? 0 : job - b * a.groups;
-  const NormParam w = set ? a.w2 : a.w;
-  const NormCond k = set ? a.cond2 : a.cond;
-  void* dst = set ? (dw ? a.dw2 : a.dcond2) : (dw ? a.dw : a.dcond);
-  if (!dst) return;  // uniform over the workgroup
-  const bool scale = set || modulate;
-  auto param = [&](const void* p, bool f32, int64_t at) {
-    return f32 ? static_cast<const float*>(p)[at] : (float)static_cast<const T*>(p)[at];
-  };
-  // what a partial of id at chunk q counts for: its m (dw), or 1 or nothing
-  auto factor = [&](int q, int id) {
-    f32x4 m = {};
-    if (!dw) {
-      m += id == g ? 1.0f : 0.0f;
-    } else {
-      const bool live = k.p && id < k.groups;
-      const int64_t off = live ? (q / a.chunks) * k.bs + id * k.gs : 0;
+__device__ __forceinline__ float param_value(const void* p, bool f32, int64_t at) {
+  return f32 ? static_cast<const float*>(p)[at] : (float)static_cast<const T*>(p)[at];
+}
+
+// Stores acc * w (null: acc) at row `row` of dst.
+template <typename T>
+__device__ __forceinline__ void store_param(const f32x4& acc, int col, int c, NormParam w, void* dst, bool f32,
+                                            int64_t row) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[j] = live && col + j < a.c ? param(k.p, k.f32, off + col + j) : scale || k.p ? 0.0f : 1.0f;
-        if (scale) m[j] += 1.0f;
-      }
-    }
-    return m;
-  };
-  auto partial = [&](int64_t q, int s) {
+  for (int j = 0; j < 4; ++j) {
+    const int at = col + j;
+    if (at >= c) continue;
+    const float v = w.p ? acc[j] * param_value<T>(w.p, w.f32, at) : acc[j];
+    if (f32)
+      static_cast<float*>(dst)[row * c + at] = v;
+    else
+      static_cast<T*>(dst)[row * c + at] = (T)v;
+  }
+}
+
+// The thread rows' sums added in order, in the first of them; true there.
+__device__ __forceinline__ bool add_rows(f32x4& acc, f32x4 (*sum)[16]) {
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  __syncthreads();  // an earlier block of channels has been read
+  sum[ty][tx] = acc;
+  __syncthreads();
+  if (ty != 0) return false;
+#pragma unroll
+  for (int i = 1; i < kParamRows; ++i) acc += sum[i][tx];
+  return true;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kParamNT) void norm_param_kernel(NormArgs a, int sets, int modulate, int cond_blocks) {
+  __shared__ f32x4 sum[kParamRows][16];
+  __shared__ int list[kParamNT], counts[kParamNT / 64];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, blocks = (a.c + 63) / 64;
+  const int dws = sets * blocks;
+  auto partial = [&](int set, int64_t q, int s, int col) {
     return *reinterpret_cast<const f32x4*>(a.part + ((q * a.slots + s) * sets + set) * a.cp + col);
   };
-  f32x4 acc = {};
-  if (col < a.cp) {
-    const int first = dw ? 0 : b * a.chunks, last = dw ? a.b * a.chunks : first + a.chunks;
-    for (int q0 = first + ty; q0 < last; q0 += kParamRows * kBatch) {
-      int id[kBatch], id1[kBatch];
+  if ((int)blockIdx.x < dws) {
+    const int set = blockIdx.x / blocks, col = (blockIdx.x - set * blocks) * 64 + tx * 4;
+    const NormParam w = set ? a.w2 : a.w;
+    const NormCond k = set ? a.cond2 : a.cond;
+    void* dst = set ? a.dw2 : a.dw;
+    if (!dst) return;  // uniform over the workgroup
+    const bool scale = set || modulate;
+    f32x4 acc = {};
+    const int last = col < a.cp ? a.b * a.chunks : 0;
+    for (int q0 = ty; q0 < last; q0 += kParamRows * kBatch) {
+      int id[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int q = q0 + i * kParamRows;
         id[i] = q >= last ? -1 : a.doc ? a.part_id[(int64_t)q * a.slots] : 0;
-        id1[i] = q < last && a.slots > 1 ? a.part_id[(int64_t)q * a.slots + 1] : -1;
       }
-      f32x4 v[kBatch], m[kBatch];
+      // a chunk's first document, then its others
+      for (int s = 0; s < a.slots; ++s) {
+        f32x4 v[kBatch], m[kBatch];
+        int more[kBatch], any = -1;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int q = q0 + i * kParamRows;
-        v[i] = q < last ? partial(q, 0) : f32x4{};  // the loads do not wait for the ids
-      }
+        for (int i = 0; i < kBatch; ++i) {
+          const int q = q0 + i * kParamRows;
+          more[i] = id[i] >= 0 && s + 1 < a.slots ? a.part_id[(int64_t)q * a.slots + s + 1] : -1;
+          v[i] = id[i] >= 0 ? partial(set, q, s, col) : f32x4{};
+          const bool live = k.p && id[i] >= 0 && id[i] < k.groups;
+          const int64_t off = live ? (q / a.chunks) * k.bs + id[i] * k.gs + col : 0;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const bool use = id[i] >= 0 && (dw || id[i] == g);
-        m[i] = use ? factor(q0 + i * kParamRows, id[i]) : f32x4{};
-        if (!use) v[i] = f32x4{};
-      }
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int q = q0 + i * kParamRows;
-        acc += m[i] * v[i];
-        // the other documents of a chunk that holds several
-        for (int s = 1, d = id1[i]; d >= 0;) {
-          if (dw || d == g) acc += factor(q, d) * partial(q, s);
-          ++s;
-          d = s < a.slots ? a.part_id[(int64_t)q * a.slots + s] : -1;
+          for (int j = 0; j < 4; ++j) {
+            m[i][j] = live && col + j < a.c ? param_value<T>(k.p, k.f32, off + j) : scale || k.p ? 0.0f : 1.0f;
+            if (scale) m[i][j] += 1.0f;
+          }
         }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          acc += m[i] * v[i];
+          id[i] = more[i];
+          any = max(any, id[i]);
+        }
+        if (any < 0) break;
       }
     }
+    if (add_rows(acc, sum)) store_param<T>(acc, col, a.c, NormParam{}, dst, w.f32, 0);
+    return;
   }
-  sum[ty][tx] = acc;
-  __syncthreads();
-  if (ty != 0) return;
+  const int job = blockIdx.x - dws, row = job / cond_blocks, set = row / (a.b * a.groups);
+  const int at = row - set * a.b * a.groups, b = at / a.groups, g = at - b * a.groups;
+  void* dst = set ? a.dcond2 : a.dcond;
+  if (!dst) return;
+  const int first = b * a.chunks, window = a.doc ? kParamNT : a.chunks;
+  const bool f32 = set ? a.cond2.f32 : a.cond.f32;
+  int count = 0;
+  for (int block = job - row * cond_blocks; block < blocks; block += cond_blocks) {
+    const int col = block * 64 + tx * 4;
+    f32x4 acc = {};
+    for (int w0 = 0; w0 < a.chunks; w0 += window) {
+      // the partials of id g in this window of chunks, listed once where one window is all
+      if (!a.doc) {
+        count = a.chunks;
+      } else if (a.chunks > window || block < cond_blocks) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, q = w0 + (int)threadIdx.x;
+        int lo = 0;
+        bool found = false;
+        if (q < a.chunks) {
+          const int* ids = a.part_id + (int64_t)(first + q) * a.slots;
+          if (a.slots <= kBatch) {  // all of them at once: one latency
 #pragma unroll
-  for (int i = 1; i < kParamRows; ++i) acc += sum[i][tx];
-  const bool f32 = dw ? w.f32 : k.f32;
+            for (int s = 0; s < kBatch; ++s)
+              if (s < a.slots && ids[s] == g) {
+                lo = s;
+                found = true;
+              }
+          } else {
+            int hi = a.slots;  // the first id that is not below g (-1 is above all)
+            while (lo < hi) {
+              const int mid = (lo + hi) / 2;
+              if ((uint32_t)ids[mid] < (uint32_t)g) lo = mid + 1;
+              else hi = mid;
+            }
+            found = lo < a.slots && ids[lo] == g;
+          }
+        }
+        const uint64_t mine = __ballot(found);
+        __syncthreads();  // the last window's list has been read
+        if (lane == 0) counts[wave] = __popcll(mine);
+        __syncthreads();
+        int before = 0;
+        count = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int at = col + j;
-    if (at >= a.c) continue;
-    const float v = dw || !w.p ? acc[j] : acc[j] * param(w.p, w.f32, at);
-    const int64_t o = dw ? at : ((int64_t)b * a.groups + g) * a.c + at;
-    if (f32)
-      static_cast<float*>(dst)[o] = v;
-    else
-      static_cast<T*>(dst)[o] = (T)v;
+        for (int i = 0; i < kParamNT / 64; ++i) {
+          before += i < wave ? counts[i] : 0;
+          count += counts[i];
+        }
+        if (found) list[before + __popcll(mine & ((1ull << lane) - 1))] = q * a.slots + lo;
+        __syncthreads();
+      }
+      if (a.doc && a.chunks <= window && count <= kBatch) {
+        // few partials: a thread row adds them all, the rows take blocks of channels in turn
+        for (int k = block + ty * cond_blocks; k < blocks; k += kParamRows * cond_blocks) {
+          const int at_col = k * 64 + tx * 4;
+          if (at_col >= a.cp) continue;
+          f32x4 v[kBatch], s = {};
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) v[i] = i < count ? partial(set, first, list[i], at_col) : f32x4{};
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) s += v[i];
+          store_param<T>(s, at_col, a.c, set ? a.w2 : a.w, dst, f32, at);
+        }
+        return;
+      }
+      if (col >= a.cp) continue;
+      for (int e0 = ty; e0 < count; e0 += kParamRows * kBatch) {
+        f32x4 v[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int e = e0 + i * kParamRows;
+          v[i] = f32x4{};
+          if (e < count) v[i] = partial(set, first, a.doc ? list[e] : e, col);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) acc += v[i];
+      }
+    }
+    if (add_rows(acc, sum)) store_param<T>(acc, col, a.c, set ? a.w2 : a.w, dst, f32, at);
   }
 }
 
@@ -606,11 +690,15 @@ hipError_t launch_norm_bwd(int op, int f16, const NormArgs& a, hipStream_t st) {
   hipError_t e = f16 ? pick_op<true, _Float16>(op, a, st) : pick_op<true, __bf16>(op, a, st);
   if (e != hipSuccess || !a.part) return e;
   const int sets = op == kNormGateModulate ? 2 : 1;
-  const dim3 grid((uint32_t)((a.c + 63) / 64), (uint32_t)(sets * (a.b * a.groups + 1)));
+  // workgroups a conditioning row: one for each 64 channels while that fills the card about
+  // twice, fewer (which look for the row's partials less often) with more rows
+  const int64_t blocks = (a.c + 63) / 64, rows = (int64_t)sets * a.b * a.groups;
+  const int64_t most = std::max<int64_t>(1, 2048 / rows), cond_blocks = std::min(blocks, most);
+  const uint32_t grid = (uint32_t)(sets * blocks + rows * cond_blocks);
   if (f16)
-    norm_param_kernel<_Float16><<<grid, 16 * kParamRows, 0, st>>>(a, sets, op == kNormModulate);
+    norm_param_kernel<_Float16><<<grid, kParamNT, 0, st>>>(a, sets, op == kNormModulate, (int)cond_blocks);
   else
-    norm_param_kernel<__bf16><<<grid, 16 * kParamRows, 0, st>>>(a, sets, op == kNormModulate);
+    norm_param_kernel<__bf16><<<grid, kParamNT, 0, st>>>(a, sets, op == kNormModulate, (int)cond_blocks);
   return hipGetLastError();
 }
 

@@ -329,3 +329,61 @@ def test_ops_check_and_compile(cuda, op):
                              backend="aot_eager", fullgraph=True)
     got = compiled(*(v[k].detach().requires_grad_() for k in ORDER[op]))
     assert all(torch.equal(a, b) for a, b in zip(got, (want[k] for k in (["hidden", "out"] if op == "gate_modulate" else ["out"]))))
+
+
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_ids_past_32_bits_are_of_no_document(cuda, op):
+    v = _to(_inputs(op, 1, 40, 72, BF, F32, None, seed=2), cuda)
+    ids = torch.arange(40, device=cuda).view(1, 40) % 3
+    for k in ("cond", "next_scale"):
+        if v.get(k) is not None:
+            v[k] = torch.stack([v[k] * f for f in (1.0, -0.5)], 1)
+    v["doc_ids"] = ids.int().masked_fill(ids == 2, -1)
+    want = _with_grads(op, v)
+    for far in ((1 << 32) + 1, -(1 << 32), 1 << 62):
+        v["doc_ids"] = ids.masked_fill(ids == 2, far)
+        got = _with_grads(op, v)
+        assert all(torch.equal(got[k], want[k]) for k in want), far
+
+
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_gradients_are_not_differentiated(cuda, op):
+    v = _to(_inputs(op, 1, 5, 64, BF, BF, None), cuda)
+    v["x"] = v["x"].requires_grad_()
+    out = _call(op, v)["out"]
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(out, v["x"], v["dout"], create_graph=True)
+
+
+def test_offsets_past_32_bits(cuda):
+    """Rows of an x and of a gradient beyond 2^32 bytes: all zeros but a few."""
+    import futudiffu_amd as F
+    C, N = 2048, (1 << 20) + 4100
+    at = torch.tensor([0, (1 << 19) - 1, 1 << 19, (1 << 20) - 1, 1 << 20, N - 1])
+    v = _inputs("modulate", 1, len(at), C, BF, F32, None, seed=4)
+    x, dout = (torch.zeros(1, N, C, dtype=BF, device=cuda) for _ in range(2))
+    x[:, at.to(cuda)], dout[:, at.to(cuda)] = v["x"].to(cuda), v["dout"].to(cuda)
+    few = _with_grads("modulate", _to(v, cuda))
+    v = _to(v, cuda)
+    v["x"], v["dout"] = x, dout
+    got = _with_grads("modulate", v)
+    for k in ("out", "dx"):
+        assert torch.equal(got[k][:, at.to(cuda)], few[k]), k
+        got[k][:, at.to(cuda)] = 0
+        assert got[k].abs().amax().item() == 0, k
+    _check({k: got[k] for k in ("dweight", "dcond")}, {k: t for k, t in _want("modulate", _to(_inputs(
+        "modulate", 1, len(at), C, BF, F32, None, seed=4), "cpu")).items()})
+
+
+@pytest.mark.parametrize("B,N,C,lengths", [
+    (1, 1500, 200, (3,) * 480),             # documents shorter than a chunk, a few partials each
+    (2, 900, 1032, (500, 1, 399)),          # many partials a document, and one
+    (1, 270000, 8, (140000, 7, 129000)),    # more chunks than one search takes
+    (1, 270000, 8, (900,) * 290),
+])
+@pytest.mark.parametrize("op", ["modulate", "gate_modulate"])
+def test_documents_and_chunks(cuda, op, B, N, C, lengths):
+    """The sums of a document over its chunks: every form of the search for them."""
+    print(op, B, N, C, len(lengths), flush=True)
+    v = _inputs(op, B, N, C, BF, F32, (len(lengths), _ids(lengths, N, B)), seed=N)
+    _check(_with_grads(op, _to(v, cuda)), _want(op, v))
