@@ -245,6 +245,6 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
     """
     if torch.compiler.is_compiling():
         keep = activation != "none" and torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias, residual))
+            t is not None and t.requires_grad for t in (x, weight, bias))
         return torch.ops.futudiffu_ii.fused_linear(x, weight, bias, residual, activation, keep)[0]
     return (_native or _load()).fused_linear(x, weight, bias, residual, activation)

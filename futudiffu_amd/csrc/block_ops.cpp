@@ -144,7 +144,11 @@ struct Norm {
                       next_scale.rows);
     if (cond.rows || next_scale.rows) groups = cond.rows ? cond.rows : next_scale.rows;
     need_gpu(x);
-    if (docs) doc = ids->to(x.device(), at::kInt).contiguous();
+    if (docs) {
+      // ids past 32 bits stay ids of no document
+      const Tensor i = ids->scalar_type() == at::kLong ? ids->clamp(-1, groups) : *ids;
+      doc = i.to(x.device(), at::kInt).contiguous();
+    }
   }
   Tensor param(const char* name, const OptTensor& p, const Tensor& x, int bit) {
     if (!p) return Tensor();
@@ -370,7 +374,8 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dout, const Ten
   const Linear a(x, weight, bias, std::nullopt, activation);
   a.check_out("dout", dout, x);
   const bool act = a.act != SAGE_ACT_NONE;
-  TORCH_CHECK_VALUE(!act || (z && z->defined() && z->dim() == 2 && z->size(0) == a.M && z->size(1) == a.rows &&
+  const bool none = !act || !(wanted[0] || wanted[1] || wanted[2]);
+  TORCH_CHECK_VALUE(none || (z && z->defined() && z->dim() == 2 && z->size(0) == a.M && z->size(1) == a.rows &&
                              z->scalar_type() == at::kFloat && z->device() == x.device() && z->is_contiguous()),
                     "the gradient of an activation needs the z that the forward kept (keep_z)");
   Tensor dx = grad_of(x, wanted[0]), dw = grad_of(weight, wanted[1]), db = grad_of(some(bias), wanted[2]);
@@ -409,6 +414,15 @@ void once(const variable_list& args) {
   for (const Tensor& t : args)
     TORCH_CHECK(!t.defined() || !t.requires_grad(),
                 "the gradients of the block operators cannot be differentiated (create_graph=True)");
+}
+
+bool any_requires(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+  return at::GradMode::is_enabled() && any_requires(tensors);
 }
 
 struct ModulateFn : torch::autograd::Function<ModulateFn> {
@@ -467,7 +481,9 @@ struct GateModulateFn : torch::autograd::Function<GateModulateFn> {
 struct LinearFn : torch::autograd::Function<LinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias,
                         const OptTensor& residual, const std::string& activation) {
-    const auto [out, z] = linear_forward(x, weight, bias, residual, activation, true);
+    // a residual's gradient alone needs no z
+    const auto [out, z] =
+        linear_forward(x, weight, bias, residual, activation, any_requires({&x, &weight, &some(bias)}));
     ctx->save_for_backward({x, weight, held(bias), z});
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["residual"] = residual.has_value();
@@ -483,13 +499,6 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     return {dx, dw, db, w[3] ? d[0] : Tensor(), Tensor()};
   }
 };
-
-bool wants_grad(std::initializer_list<const Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : tensors)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
-}
 
 Tensor rms_norm_modulate(const Tensor& x, const OptTensor& weight, const OptTensor& scale, const OptTensor& doc_ids,
                          double eps) {

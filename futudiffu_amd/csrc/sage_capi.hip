@@ -902,9 +902,10 @@ int check_linear(int64_t m, int64_t n, int64_t k, int64_t w_rs, int dtype, int a
   return SAGE_OK;
 }
 
-// Row strides: at least the columns (one row: anything), and panels of 256 rows under 2^31 bytes.
+// Row strides: at least the columns, and panels of 256 rows under 2^31 bytes (one row: any).
 int check_rows(int64_t rs, int64_t rows, int64_t cols, const char* what) {
-  if (rows > 1 && rs < cols) return fail(SAGE_ERR_ARG, "%s rows are %lld apart, under %lld", what, (long long)rs, (long long)cols);
+  if (rows == 1) return SAGE_OK;
+  if (rs < cols) return fail(SAGE_ERR_ARG, "%s rows are %lld apart, under %lld", what, (long long)rs, (long long)cols);
   if (rs >= (int64_t)1 << 22) return fail(SAGE_ERR_ARG, "%s rows are %lld apart, 2^22 or more", what, (long long)rs);
   return SAGE_OK;
 }
@@ -1054,7 +1055,7 @@ int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, c
   g.bias = bias;
   g.bias_f32 = bias_fp32 != 0;
   g.res = residual;
-  g.ldr = r_rs;
+  g.ldr = m == 1 ? n : r_rs;
   g.z = z;
   g.out = out;
   g.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at);
@@ -1098,7 +1099,7 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
     sage::DactArgs d{};
     d.dout = dout;
     d.z = z;
-    d.ldd = d_rs;
+    d.ldd = m == 1 ? n : d_rs;
     d.m = m;
     d.n = (int)n;
     d.act = activation;

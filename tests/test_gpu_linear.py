@@ -249,3 +249,59 @@ def test_op_check_and_compile(cuda):
         want = _run(v, act)
         assert torch.equal(out, want["out"])
         assert all(torch.equal(t, want["d" + k]) for k, t in zip(LEAVES, grads))
+
+
+def test_one_row_of_any_stride(cuda):
+    """One row has no stride to speak of: a view whose row stride is beyond the limit."""
+    g = torch.Generator().manual_seed(3)
+    wide = torch.randn(1, (1 << 22) + 40, generator=g).to(BF).to(cuda)
+    v = _inputs(1, 40, 24, "silu", BF, None, True, device=cuda)
+    v["x"] = wide[:, 8:48]
+    v["residual"] = wide[:, 64:88]
+    v["dout"] = wide[:, 128:152]
+    assert v["x"].stride(0) > 1 << 22
+    _check(_run(v, "silu"), _want(v, "silu"))
+
+
+def test_offsets_past_32_bits(cuda):
+    """An x of more than 2^32 bytes, all zeros but a few rows: first, last and beyond 2^31 and
+    2^32 bytes.  Small integers, so every sum is exact."""
+    import futudiffu_amd as F
+    K, M = 2048, (1 << 20) + 4100
+    at = torch.tensor([0, 1, (1 << 19) - 1, 1 << 19, (1 << 20) - 1, 1 << 20, (1 << 20) + 5, M - 2, M - 1])
+    g = torch.Generator().manual_seed(11)
+    rows = torch.randint(-3, 4, (len(at), K), generator=g).to(BF)
+    x = torch.zeros(M, K, dtype=BF, device=cuda)
+    x[at.to(cuda)] = rows.to(cuda)
+    for N in (24, 136):  # few columns, and tiles
+        w = torch.randint(-2, 3, (N, K), generator=g).to(BF)
+        d = torch.randint(-3, 4, (len(at), N), generator=g).to(BF)
+        dout = torch.zeros(M, N, dtype=BF, device=cuda)
+        dout[at.to(cuda)] = d.to(cuda)
+        xg, wg = x.requires_grad_(), w.to(cuda).requires_grad_()
+        out = F.fused_linear(xg, wg)
+        want = torch.zeros(M, N, dtype=BF)
+        want[at] = (rows.double() @ w.double().T).to(BF)
+        assert torch.equal(out.detach().cpu(), want)
+        dx, dw = torch.autograd.grad(out, (xg, wg), dout)
+        assert torch.equal(dw.cpu(), (d.double().T @ rows.double()).to(BF))
+        assert torch.equal(dx[at.to(cuda)].cpu(), (d.double() @ w.double()).to(BF))
+        dx[at.to(cuda)] = 0
+        assert dx.abs().amax().item() == 0
+        del dx, out
+
+
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+def test_gradients_are_not_differentiated(cuda, act):
+    v = _inputs(5, 24, 16, act, BF, BF, True, device=cuda)
+    import futudiffu_amd as F
+    x = v["x"].requires_grad_()
+    out = F.fused_linear(x, v["weight"], v["bias"], v["residual"], activation=act)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(out, x, v["dout"], create_graph=True)
+
+
+def test_residual_gradient_alone(cuda):
+    v = _inputs(70, 24, 16, "gelu", BF, BF, True, device=cuda)
+    got = _run(v, "gelu", leaves=("residual",))
+    assert torch.equal(got["dresidual"], v["dout"])
