@@ -5,8 +5,10 @@
 //   forward  A = x  [M][K],  B = W [N][K]          (both with the contraction contiguous)
 //   dx       A = dz [M][N'], B = W as [N'][K]      (B: the output's columns contiguous)
 //   dW       A = dz as [M][N'], B = x as [M][K]    (both: the contraction strided)
-// and three kernels: tiles through LDS (gemm_kernel), few rows on one side
-// (skinny_kernel), and the sum of a tile's pieces (join_kernel).
+// and four kernels: tiles through LDS (gemm_kernel) and the sum of their pieces (join_kernel),
+// few rows on one side (skinny_kernel), a contraction of one stage (thin_kernel).  Beside the
+// products: copies of operands whose rows take no 16-byte accesses (pack_kernel), and the
+// gradient through the activation with the bias's (dact_kernel, dbias_kernel).
 #include <type_traits>
 
 #include "sage_common.h"
@@ -231,6 +233,9 @@ constexpr int kAnyPitch = 65, kAnyRows = 16;
 __device__ __forceinline__ uint16_t load_2(__amdgpu_buffer_rsrc_t rs, int off) {
   return __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0);
 }
+__device__ __forceinline__ uint32_t load_4(__amdgpu_buffer_rsrc_t rs, int off) {
+  return __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
+}
 __device__ __forceinline__ void store_2(uint16_t v, __amdgpu_buffer_rsrc_t rs, int off) {
   __builtin_amdgcn_raw_buffer_store_b16(v, rs, off, 0, 0);
 }
@@ -430,6 +435,8 @@ __device__ __forceinline__ int xcd_share(int b, int total) {
 template <int LEFT>
 __device__ __forceinline__ void wait_loads();
 template <>
+__device__ __forceinline__ void wait_loads<0>() { __builtin_amdgcn_s_waitcnt(0x0070); }
+template <>
 __device__ __forceinline__ void wait_loads<4>() { __builtin_amdgcn_s_waitcnt(0x0074); }
 template <>
 __device__ __forceinline__ void wait_loads<6>() { __builtin_amdgcn_s_waitcnt(0x0076); }
@@ -437,6 +444,14 @@ template <>
 __device__ __forceinline__ void wait_loads<8>() { __builtin_amdgcn_s_waitcnt(0x0078); }
 template <>
 __device__ __forceinline__ void wait_loads<12>() { __builtin_amdgcn_s_waitcnt(0x007c); }
+
+// No memory access moves across it.
+__device__ __forceinline__ void hold_memory() { asm volatile("" ::: "memory"); }
+
+template <typename V>
+__device__ __forceinline__ V operand_at(const uint8_t* __restrict__ p) {
+  return *reinterpret_cast<const V*>(p);
+}
 
 // A workgroup barrier that waits for no load (__syncthreads waits for all of them); no
 // memory access moves across it.
@@ -452,6 +467,15 @@ __device__ __forceinline__ void order_read() { __builtin_amdgcn_sched_group_barr
 
 __device__ __forceinline__ void order_load() { __builtin_amdgcn_sched_group_barrier(0x020, 1, 0); }
 
+// The product by tiles.  A wave of 128 x 128 reads 256 rows of fragments for 16 products of 32
+// x 32: LDS gives 128 bytes a cycle to a CU, and four such waves need 64 of them where four
+// of 64 x 64 need all 128.  The large tile therefore runs at one wave a SIMD with 256
+// accumulators; the small one, two workgroups a CU, is for what has too few large tiles.
+// Measured, bf16: 4416 x 11520 x 3840 with the bias 346 us = 1130 TFLOP/s, its dx 332 us =
+// 1177, its dW 356 us = 1097 (transposing reads on both sides); the swiglu of 4416 x 20480 x
+// 3840 570 us = 1220.  The matrix cores bound it at the clock that the power limit leaves: a
+// stage takes the same time with the loads in bursts, with LDS slots a wave and with the
+// next tile's first stages loaded under the epilogue.
 template <typename T, bool AK, bool BKC, typename TL>
 __global__ __launch_bounds__(TL::NT, TL::SIMD) void gemm_kernel(GemmArgs a) {
   __shared__ __align__(1024) uint8_t lds[TL::LDS];
@@ -493,9 +517,8 @@ __global__ __launch_bounds__(TL::NT, TL::SIMD) void gemm_kernel(GemmArgs a) {
   // products run beside the next stage's first reads.  LDS holds three stages of A and two
   // of B.  A wave's eight loads of a stage are spread over the four steps (B's, which the
   // next barrier waits for, first): issued together behind the barrier they hold the
-  // waves up, 64 loads at 16 cycles of the address unit each, and the matrix cores were
-  // busy 65 % of the time.  Loads past the last stage, and the
-  // reads of it in the last round, give nothing that is used.
+  // waves up, 64 loads at 16 cycles of the address unit each.  Loads past the last stage,
+  // and the reads of it in the last round, give nothing that is used.
   using V = typename Vec8<T>::type;
   f32x16 acc[TL::MI][TL::NI] = {};
   V va[2][TL::MI], vb[2][TL::NI];
@@ -597,7 +620,7 @@ __global__ __launch_bounds__(TL::NT, TL::SIMD) void gemm_kernel(GemmArgs a) {
 
 // The products of at most one stage's contraction (an adapter's second product): bound by
 // the output and the residual, so one stage of LDS, several workgroups a CU, and no steps
-// past the last 16 that exist.
+// past the last 16 that exist.  4416 x 3840 x 16 onto a residual: 68 MB in 18.5 us.
 template <typename T, typename TL>
 __global__ __launch_bounds__(TL::NT, 3) void thin_kernel(GemmArgs a) {
   __shared__ __align__(1024) uint8_t lds[TL::A_BYTES + TL::B_BYTES];
@@ -641,6 +664,8 @@ __global__ __launch_bounds__(TL::NT, 3) void thin_kernel(GemmArgs a) {
 
 // Adds the pieces of the cut tiles in order and finishes them: a wave takes one 32 x 64
 // block of a tile.  Large tiles whose rows take no 16-byte accesses all come through here.
+// Bound by the sums' way back: 75 tiles of 256 x 256 in three pieces, 79 MB with the residual
+// and the output, in 16 us = 4.9 TB/s.
 template <typename T, typename TL>
 __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -678,92 +703,149 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
 
 // ---------------------------------------------------------------- few rows
 
-constexpr int kSkinnyWaves = 8;
+constexpr int kSkinnyWaves = 4;
 
 // out for at most 16 * MT rows on the short side: a workgroup takes 16 rows of the long
-// side and reads them once, straight into the matrix operand's registers (lane (q, r): row
-// r, contraction 8 q .. 8 q + 7 of a step of 32); its waves share the contraction, 64 at a
-// time in turn, and their sums are added in order.  swap: the long side is x (m), not W (n).
+// side and reads them once; its waves share the contraction, chunks of 64 in turn, and their
+// sums are added in order.  swap: the long side is x (m), not W (n).
+//
+// A wave has its own ring of D stages in LDS (a chunk of its H x 16 long rows and of the
+// short ones) and waits for nobody.  Direct global -> LDS loads, eight rows of 128 bytes
+// each: loaded straight to the matrix operand's registers, neighbouring lanes lie on
+// different rows, and the address unit takes 64 cycles a load (16 rows by 3840 x 11520 in 22.6
+// us, 32 in 32.8).  Measured so: 14.8 and 17.0 us, 88 MB at the rate of memory and the cache
+// above it; 2 x 256 by 15360 x 256 4.3 us, a launch and two trips to memory.
 template <typename T, int MT, bool GLU>
-__global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(GemmArgs a, int swap) {
+__global__ __launch_bounds__(64 * kSkinnyWaves, 2) void skinny_kernel(GemmArgs a, int swap) {
   using V = typename Vec8<T>::type;
-  constexpr int H = GLU ? 2 : 1;
-  __shared__ f32x4 part[kSkinnyWaves][H][MT][64];
+  constexpr int H = GLU ? 2 : 1, TILES = H + MT, STAGE = TILES * 2048;
+  constexpr int D = TILES == 2 ? 4 : TILES == 3 ? 3 : 2;  // two workgroups a CU
+  __shared__ __align__(1024) uint8_t lds[kSkinnyWaves * D * STAGE];
+  static_assert(sizeof(lds) <= 80 * 1024 && H * MT * 1024 <= D * STAGE, "two workgroups a CU, and the sums fit");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int q = lane >> 4, r = lane & 15;
+  uint8_t* const mine = lds + wave * D * STAGE;
   const uint8_t* lp = static_cast<const uint8_t*>(swap ? a.a : a.b);
-  const uint8_t* sp = static_cast<const uint8_t*>(swap ? a.b : a.a);
   const int64_t lld = (swap ? a.lda : a.ldb) * 2, sld = (swap ? a.ldb : a.lda) * 2;
   const int64_t llen = swap ? a.m : a.n, slen = swap ? a.n : a.m;
   const int64_t l0 = (int64_t)blockIdx.x * 16;
-  // rows past the last read the last one again; what they give is not stored
-  const uint8_t* lrow[H];
+  const __amdgpu_buffer_rsrc_t srs = raw_rsrc(swap ? a.b : a.a, 0x7fffffff);
+  __amdgpu_buffer_rsrc_t lrs[H];
 #pragma unroll
-  for (int h = 0; h < H; ++h) lrow[h] = lp + (min(l0 + r, llen - 1) + h * llen) * lld;
-  const uint8_t* srow[MT];
+  for (int h = 0; h < H; ++h) lrs[h] = raw_rsrc(lp + (l0 + h * llen) * lld, 0x7fffffff);
+  // of a load's eight rows, lane l takes row l / 8 and, as in a stage of the tiles, the
+  // chunk of 16 bytes that lies at l % 8; rows past the last read the last one again (what
+  // they give is not stored), the contraction past its end zeros
+  int kpos[2], loff[2], soff[MT][2];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) srow[i] = sp + min((int64_t)(i * 16 + r), slen - 1) * sld;
-  f32x4 acc[H][MT] = {};
-  auto step = [&](int64_t k, bool tail) {
-    // two steps of 32; a tail's lanes past the end take zeros
-    V l[2][H], s[2][MT];
+  for (int i = 0; i < 2; ++i) {
+    const int row = 8 * i + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+    kpos[i] = c * 8;
+    loff[i] = (int)((min(l0 + row, llen - 1) - l0) * lld) + c * 16;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int64_t at = k + 32 * u + 8 * q;
-      const bool in = !tail || at < a.k;
+    for (int j = 0; j < MT; ++j) soff[j][i] = (int)(min((int64_t)(16 * j + row), slen - 1) * sld) + c * 16;
+  }
+  auto issue = [&](uint8_t* stage, int chunk) {
+    const int k0 = chunk * 64, left = (int)a.k - k0;
 #pragma unroll
-      for (int h = 0; h < H; ++h) l[u][h] = in ? *reinterpret_cast<const V*>(lrow[h] + at * 2) : V{};
+    for (int i = 0; i < 2; ++i) {
+      const int none = kpos[i] < left ? 0 : (int)0x80000000;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) s[u][i] = in ? *reinterpret_cast<const V*>(srow[i] + at * 2) : V{};
+      for (int h = 0; h < H; ++h) dma_16(stage + h * 2048 + i * 1024, lrs[h], (loff[i] + k0 * 2) | none);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) dma_16(stage + (H + j) * 2048 + i * 1024, srs, (soff[j][i] + k0 * 2) | none);
     }
+  };
+  const int q = lane >> 4, r = lane & 15;
+  int at[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+  for (int s = 0; s < 2; ++s) at[s] = r * 128 + (((4 * s + q) ^ ((r >> 1) & 7)) << 4);
+  f32x4 acc[H][MT] = {};
+  const int chunks = (int)((a.k + 63) / 64);
+  // wave i finishes short rows 16 i ..: lane (q, r) long rows 4 q .. + 3 of short row r.  Bias and
+  // residual are asked for first (zeros where there are none) and waited for last.
+  const int64_t mr = 16 * wave + r;
+  uint32_t bias[H][4];
+  uint16_t res[4];
+  if (wave < MT) {
+    const __amdgpu_buffer_rsrc_t brs = raw_rsrc(a.bias, a.bias ? (uint32_t)(a.n * H) * (a.bias_f32 ? 4 : 2) : 0u);
+    const __amdgpu_buffer_rsrc_t rrs =
+        raw_rsrc(static_cast<const T*>(a.res) + (swap ? l0 * a.ldr : 0), a.res ? 0x7fffffffu : 0u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int l = 4 * q + e, n = swap ? (int)mr : (int)l0 + l;
+      const int none = l0 + l < llen && mr < slen ? 0 : (int)0x80000000;
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+        bias[h][e] = a.bias_f32 ? load_4(brs, (n + h * a.n) * 4 | none) : load_2(brs, (n + h * a.n) * 2 | none);
+      res[e] = load_2(rrs, (int)((swap ? l * a.ldr + mr : mr * a.ldr + n) * 2) | none);
+    }
+    keep_order();
+  }
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d)
+    if (wave + d * kSkinnyWaves < chunks) issue(mine + d * STAGE, wave + d * kSkinnyWaves);
+  int now = 0, free = (D - 1) * STAGE;
+#pragma unroll 1
+  for (int c = wave; c < chunks; c += kSkinnyWaves) {
+    // this stage has arrived, and the last one's reads are done: its place takes the next loads
+    if (c + (D - 1) * kSkinnyWaves < chunks) {
+      wait_loads<2 * TILES * (D - 2)>();
+      hold_memory();
+      issue(mine + free, c + (D - 1) * kSkinnyWaves);
+    } else {
+      wait_loads<0>();
+      hold_memory();
+    }
+    const uint8_t* stage = mine + now;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      V l[H], x[MT];
+#pragma unroll
+      for (int h = 0; h < H; ++h) l[h] = operand_at<V>(stage + h * 2048 + at[s]);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) x[j] = operand_at<V>(stage + (H + j) * 2048 + at[s]);
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[h][i] = mfma16(l[u][h], s[u][i], acc[h][i]);
-  };
-  const int64_t whole = a.k / 64;
-  int64_t k = wave;
-#pragma unroll 4
-  for (; k < whole; k += kSkinnyWaves) step(k * 64, false);
-  if (k == whole && whole * 64 < a.k) step(k * 64, true);
+        for (int j = 0; j < MT; ++j) acc[h][j] = mfma16(l[h], x[j], acc[h][j]);
+    }
+    free = now;
+    now = now == (D - 1) * STAGE ? 0 : now + STAGE;
+  }
+  wait_vmem();  // the loads in flight write this wave's LDS
+  hold_memory();
+  // the waves' sums, in the place of the stages
+  f32x4* const part = reinterpret_cast<f32x4*>(mine);
 #pragma unroll
   for (int h = 0; h < H; ++h)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) part[wave][h][i][lane] = acc[h][i];
+    for (int i = 0; i < MT; ++i) part[(h * MT + i) * 64 + lane] = acc[h][i];
   __syncthreads();
-  // lane (q, r) of tile i holds long rows 4 q .. + 3 of short row r
-  for (int u = threadIdx.x; u < MT * 64; u += 64 * kSkinnyWaves) {
-    const int i = u >> 6, ln = u & 63;
-    f32x4 z = {}, z2 = {};
+  if (wave >= MT) return;
+  f32x4 z = {}, z2 = {};
 #pragma unroll
-    for (int w = 0; w < kSkinnyWaves; ++w) {
-      z += part[w][0][i][ln];
-      if (GLU) z2 += part[w][H - 1][i][ln];
-    }
-    const int64_t srow_i = i * 16 + (ln & 15);
-    if (srow_i >= slen) continue;
+  for (int w = 0; w < kSkinnyWaves; ++w) {
+    const f32x4* const p = reinterpret_cast<const f32x4*>(lds + w * D * STAGE) + threadIdx.x;
+    z += p[0];
+    if (GLU) z2 += p[(H - 1) * MT * 64];
+  }
+  if (mr >= slen) return;
+  auto bias_of = [&](uint32_t v) {
+    return a.bias_f32 ? __uint_as_float(v) : (float)__builtin_bit_cast(T, (uint16_t)v);
+  };
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t lrow_j = l0 + 4 * (ln >> 4) + j;
-      if (lrow_j >= llen) continue;
-      const int64_t m = swap ? lrow_j : srow_i, n = swap ? srow_i : lrow_j;
-      float v = z[j], v2 = z2[j];
-      if (a.bias) {
-        v += param_at(a.bias, a.bias_f32, std::is_same<T, _Float16>::value, n);
-        if (GLU) v2 += param_at(a.bias, a.bias_f32, std::is_same<T, _Float16>::value, a.n + n);
-      }
-      if (a.z) {
-        float* row = a.z + m * a.n * H;
-        row[n] = v;
-        if (GLU) row[a.n + n] = v2;
-      }
-      float y = act_fwd(a.act, v);
-      if (GLU) y *= v2;
-      if (a.res) y += (float)static_cast<const T*>(a.res)[m * a.ldr + n];
-      static_cast<T*>(a.out)[m * a.n + n] = (T)y;
+  for (int e = 0; e < 4; ++e) {
+    const int64_t l = l0 + 4 * q + e;
+    if (l >= llen) continue;
+    const int64_t m = swap ? l : mr, n = swap ? mr : l;
+    const float v = z[e] + bias_of(bias[0][e]), v2 = GLU ? z2[e] + bias_of(bias[H - 1][e]) : 1.0f;
+    if (a.z) {
+      float* row = a.z + m * a.n * H;
+      row[n] = v;
+      if (GLU) row[a.n + n] = v2;
     }
+    const float y = act_fwd(a.act, v) * v2 + (float)__builtin_bit_cast(T, res[e]);
+    static_cast<T*>(a.out)[m * a.n + n] = (T)y;
   }
 }
 
@@ -793,12 +875,9 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a0, PackArgs a1, int
 // of the unrounded values over each chunk of rows, for the bias.  A workgroup takes 512
 // columns of a chunk, a wave every fourth row, kDactRows of them in flight; a lane holds eight
 // consecutive columns (VEC), or every 64th where rows take no 16-byte accesses.  Reads past a
-// row's end give zeros and writes are dropped there, so nothing is behind a branch.
+// row's end give zeros and writes are dropped there, so nothing is behind a branch.  The sums
+// of 4416 x 11520 alone: 102 MB in 28.7 us.
 constexpr int kDactRows = 4;
-
-__device__ __forceinline__ uint32_t load_4(__amdgpu_buffer_rsrc_t rs, int off) {
-  return __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
-}
 
 template <typename T, bool VEC>
 struct Eight {
@@ -954,6 +1033,7 @@ hipError_t run_skinny(const GemmArgs& a, hipStream_t st) {
     else skinny_kernel<T, 2, true><<<grid, NT, 0, st>>>(a, swap);
   } else if (s <= 16) skinny_kernel<T, 1, false><<<grid, NT, 0, st>>>(a, swap);
   else if (s <= 32) skinny_kernel<T, 2, false><<<grid, NT, 0, st>>>(a, swap);
+  else if (s <= 48) skinny_kernel<T, 3, false><<<grid, NT, 0, st>>>(a, swap);
   else skinny_kernel<T, 4, false><<<grid, NT, 0, st>>>(a, swap);
   return hipGetLastError();
 }
@@ -977,9 +1057,13 @@ void gemm_plan(GemmArgs& a) {
   a.kt = (int)((a.k + kBK - 1) / kBK);
   a.skinny = a.thin = 0;
   if (a.a_kc && a.b_kc) {
-    const int64_t most = glu ? 32 : 64;
-    if (a.m <= most) a.skinny = 1;
-    else if (a.n <= 64 && !glu) a.skinny = 2;
+    // 49 to 64 rows only while the long side is one round of two workgroups a CU (64 by 3840 x
+    // 3840: 11.4 us, tiles 16.3; by 3840 x 11520: 30.3, tiles 27.0); 48 by 3840 x 11520 25.5,
+    // by 10240 x 3840 22.0, tiles 27.0 and 23.8; 32 by a swiglu of 3840 x 2 x 5760 17.2, tiles
+    // 26.7, by 10240 x 2 x 1920 22.5, tiles 23.3.
+    auto few = [&](int64_t rows, int64_t len) { return rows <= (glu ? 32 : len <= 512 * 16 ? 64 : 48); };
+    if (few(a.m, a.n)) a.skinny = 1;
+    else if (few(a.n, a.m) && !glu) a.skinny = 2;
   }
   a.part_floats = 0;
   a.parts = 1;

@@ -305,3 +305,16 @@ def test_residual_gradient_alone(cuda):
     v = _inputs(70, 24, 16, "gelu", BF, BF, True, device=cuda)
     got = _run(v, "gelu", leaves=("residual",))
     assert torch.equal(got["dresidual"], v["dout"])
+
+
+@pytest.mark.parametrize("M,K,N", [(49, 72, 8200), (64, 136, 8184), (48, 1000, 9000), (33, 264, 40), (8300, 264, 50),
+                                   (8100, 72, 64), (40, 4200, 17), (16, 5000, 300), (3, 328, 2000)])
+def test_few_rows(cuda, M, K, N):
+    """The few-row form's rings of stages (contractions that end in each of them, and one that
+    every wave's first stage holds), its row counts and where tiles take over."""
+    for i, (act, dtype, bias, res) in enumerate((("none", BF, BF, True), ("gelu", FP, F32, False),
+                                                 ("swiglu", BF, BF, True))):
+        print(M, K, N, act, flush=True)
+        v = _inputs(M, K, N, act, dtype, bias, res, seed=M + K + i, device=cuda)
+        got = _run(v, act, grads=False)
+        _check(got, {"out": _want(v, act)["out"]}, act)
