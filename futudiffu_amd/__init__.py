@@ -6,7 +6,9 @@ Importing this package registers the ``futudiffu_ii::sage_attn_masked``,
 ``futudiffu_ii::sage_attn_qkv_masked`` custom ops, and the backward ops
 ``futudiffu_ii::sage_bwd_masked``, ``futudiffu_ii::sage_bwd`` and
 ``futudiffu_ii::sage_bwd_ext`` their autograd formulas call.  ``futudiffu_amd.fused_kernels``
-(imported separately) registers ``futudiffu::fused_qkv_postprocess``.
+(imported separately) registers ``futudiffu::fused_qkv_postprocess``.  ``block_ops`` holds
+what surrounds the attention in a transformer block: RMS norms with modulation, gate and
+residual, and linear layers with bias, activation and residual.
 The compute lives in ``libsage_mi355x.so`` (HIP, built by ``build.py``).
 """
 

@@ -860,9 +860,12 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a0, PackArgs a1, int
     const int64_t v = u < units0 ? u : u - units0, chunks = a.pc / 8, r = v / chunks;
     const int c = (int)(v - r * chunks) * 8;
     const uint16_t* const src = static_cast<const uint16_t*>(a.src) + r * a.ld + c;
+    const int last = (int)a.cols - 1 - c;
     uint16_t e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = c + j < a.cols ? src[j] : (uint16_t)0;
+    for (int j = 0; j < 8; ++j) e[j] = src[min(j, last)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = j <= last ? e[j] : (uint16_t)0;
     u32x4 o;
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = e[2 * j] | (uint32_t)e[2 * j + 1] << 16;
