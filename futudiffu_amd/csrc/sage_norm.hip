@@ -299,7 +299,9 @@ __device__ __forceinline__ void store_partial(float* dst, float* sum, int grp, i
 // chunk has as many as it has documents), and the order is fixed by the ids alone.  One
 // workgroup a CU, so that the partial rows are few.  Measured: modulate of 6912 x 3840 bf16
 // in three documents, 159 MB in 33 us = 4.8 TB/s; gate + modulate of 3071 x 3840, 141 MB in
-// 38.5 us = 3.7 TB/s, bound by its three sums a token, each waiting for the one before.
+// 38.5 us = 3.7 TB/s: six steps a workgroup, two tokens in flight and two behind them, and the
+// start and the two sets of partial rows around them (its second and third sum as one, with
+// the parts of the third in which the gradient of h is linear: 39.6).
 template <typename T, int OP, int TPR, bool VEC>
 __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
   constexpr int G = kBwdNT / TPR, W = kBwdNT / 64;
