@@ -441,14 +441,15 @@ __global__ __launch_bounds__(kBwdNT, 2) void norm_bwd_kernel(NormArgs a) {
 // over all partials of m * S, 64 channels a job; then dcond[b][g] = w * (sum of the partials
 // of its id), `cond_blocks` jobs a row, each every cond_blocks-th 64 channels.
 // 16 threads of 4 channels; the workgroup's 32 thread rows take every 32nd partial and are
-// added in order at the end.  The loads of kBatch partials are in flight together: with one
-// at a time and 16 thread rows the kernel took 22 us at 256 chunks of 3840 channels, all of
-// it latency.
+// added in order at the end.  All of it is latency, so the loads of kBatch partials are in
+// flight together, and two workgroups a CU: with eight partials a batch (160 registers, one
+// workgroup a CU) three documents of 6912 x 3840 took 8.0 us for 7.0, both sets of 3071 x 3840
+// 9.8 for 7.4; with the conditioning loaded value by value 9.2 and 12.6.
 //
 // A chunk's ids ascend and end in -1, so a row's partials are found by a search in each
 // chunk, one thread a chunk, once a job: 4000 documents in 16384 tokens of 2304 channels
-// took 5.5 ms with a scan of every chunk's ids.
-constexpr int kParamRows = 32, kBatch = 8, kParamNT = 16 * kParamRows;
+// took 5.5 ms with a scan of every chunk's ids, and take 58 us.
+constexpr int kParamRows = 32, kBatch = 4, kParamNT = 16 * kParamRows;
 
 template <typename T>
 __device__ __forceinline__ float param_value(const void* p, bool f32, int64_t at) {
@@ -483,8 +484,22 @@ __device__ __forceinline__ bool add_rows(f32x4& acc, f32x4 (*sum)[16]) {
   return true;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kParamNT) void norm_param_kernel(NormArgs a, int sets, int modulate, int cond_blocks) {
+// Four consecutive values as they lie in memory, in one load (WHOLE) or up to the row's last.
+template <bool WHOLE, typename U>
+__device__ __forceinline__ void load_four(const U* p, int last, uint32_t (&v)[4]) {
+  U u[4];
+  if constexpr (WHOLE) {
+    __builtin_memcpy(u, p, sizeof(u));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = p[min(j, last)];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = u[j];
+}
+
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(kParamNT, 4) void norm_param_kernel(NormArgs a, int sets, int modulate, int cond_blocks) {
   __shared__ f32x4 sum[kParamRows][16];
   __shared__ int list[kParamNT], counts[kParamNT / 64];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, blocks = (a.c + 63) / 64;
@@ -510,24 +525,37 @@ __global__ __launch_bounds__(kParamNT) void norm_param_kernel(NormArgs a, int se
       }
       // a chunk's first document, then its others
       for (int s = 0; s < a.slots; ++s) {
-        f32x4 v[kBatch], m[kBatch];
+        // every load of the batch before the first use, none behind a branch of its own: a
+        // partial of no document takes row 0 of the conditioning and a factor of its own
+        f32x4 v[kBatch];
+        uint32_t raw[kBatch][4] = {};
         int more[kBatch], any = -1;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
           const int q = q0 + i * kParamRows;
           more[i] = id[i] >= 0 && s + 1 < a.slots ? a.part_id[(int64_t)q * a.slots + s + 1] : -1;
           v[i] = id[i] >= 0 ? partial(set, q, s, col) : f32x4{};
-          const bool live = k.p && id[i] >= 0 && id[i] < k.groups;
-          const int64_t off = live ? (q / a.chunks) * k.bs + id[i] * k.gs + col : 0;
+        }
+        auto row = [&](int i) {
+          const bool live = id[i] >= 0 && id[i] < k.groups;
+          return live ? ((q0 + i * kParamRows) / a.chunks) * k.bs + id[i] * k.gs + col : (int64_t)col;
+        };
+        if (k.p && k.f32) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            m[i][j] = live && col + j < a.c ? param_value<T>(k.p, k.f32, off + j) : scale || k.p ? 0.0f : 1.0f;
-            if (scale) m[i][j] += 1.0f;
-          }
+          for (int i = 0; i < kBatch; ++i) load_four<WHOLE>(static_cast<const uint32_t*>(k.p) + row(i), a.c - 1 - col, raw[i]);
+        } else if (k.p) {
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) load_four<WHOLE>(static_cast<const uint16_t*>(k.p) + row(i), a.c - 1 - col, raw[i]);
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-          acc += m[i] * v[i];
+          const bool live = k.p && id[i] >= 0 && id[i] < k.groups;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float given = k.f32 ? __uint_as_float(raw[i][j]) : (float)__builtin_bit_cast(T, (uint16_t)raw[i][j]);
+            const float m = live ? given : scale || k.p ? 0.0f : 1.0f;
+            acc[j] += (scale ? m + 1.0f : m) * v[i][j];
+          }
           id[i] = more[i];
           any = max(any, id[i]);
         }
@@ -703,10 +731,12 @@ hipError_t launch_norm_bwd(int op, int f16, const NormArgs& a, hipStream_t st) {
   const int64_t blocks = (a.c + 63) / 64, rows = (int64_t)sets * a.b * a.groups;
   const int64_t most = std::max<int64_t>(1, 2048 / rows), cond_blocks = std::min(blocks, most);
   const uint32_t grid = (uint32_t)(sets * blocks + rows * cond_blocks);
-  if (f16)
-    norm_param_kernel<_Float16><<<grid, kParamNT, 0, st>>>(a, sets, op == kNormModulate, (int)cond_blocks);
-  else
-    norm_param_kernel<__bf16><<<grid, kParamNT, 0, st>>>(a, sets, op == kNormModulate, (int)cond_blocks);
+  auto run = [&](auto kernel) {
+    kernel<<<grid, kParamNT, 0, st>>>(a, sets, op == kNormModulate, (int)cond_blocks);
+  };
+  const bool whole = a.c % 4 == 0;
+  if (f16) whole ? run(norm_param_kernel<_Float16, true>) : run(norm_param_kernel<_Float16, false>);
+  else whole ? run(norm_param_kernel<__bf16, true>) : run(norm_param_kernel<__bf16, false>);
   return hipGetLastError();
 }
 
