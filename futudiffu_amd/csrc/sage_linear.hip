@@ -876,12 +876,10 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a0, PackArgs a1, int
 // The gradient of z: dz = dout * act'(z) (swiglu: both halves), rounded to T as the products'
 // operand, into rows of `ldz` with zeros behind the last column; with `part` the column sums
 // of the unrounded values over each chunk of rows, for the bias.  A workgroup takes 512
-// columns of a chunk, a wave every fourth row, kDactRows of them in flight; a lane holds eight
+// columns of a chunk, a wave every fourth row, kRows of them in flight; a lane holds eight
 // consecutive columns (VEC), or every 64th where rows take no 16-byte accesses.  Reads past a
 // row's end give zeros and writes are dropped there, so nothing is behind a branch.  The sums
-// of 4416 x 11520 alone: 102 MB in 28.7 us.
-constexpr int kDactRows = 4;
-
+// of 4416 x 11520 alone: 102 MB in 27.2 us (four rows in flight: 28.7).
 template <typename T, bool VEC>
 struct Eight {
   typename Vec8<T>::type v;
@@ -929,16 +927,17 @@ struct EightF32 {
 template <typename T, int ACT, bool VEC>
 __global__ __launch_bounds__(256) void dact_kernel(DactArgs a) {
   constexpr bool kGlu = ACT == kActSwiglu;
+  constexpr int kRows = ACT == kActNone ? 8 : 4;
   __shared__ float sum[kGlu ? 2 : 1][4][512];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = blockIdx.x * 512, wide = kGlu ? 2 * a.n : a.n;
   const int64_t r0 = (int64_t)blockIdx.y * a.chunk, r1 = r0 + a.chunk < a.m ? r0 + a.chunk : a.m;
   float s1[8] = {}, s2[8] = {};
-  for (int64_t m0 = r0 + wave; m0 < r1; m0 += 4 * kDactRows) {
-    Eight<T, VEC> d[kDactRows], up[kDactRows];
-    EightF32<VEC> z[kDactRows], z2[kDactRows];
+  for (int64_t m0 = r0 + wave; m0 < r1; m0 += 4 * kRows) {
+    Eight<T, VEC> d[kRows], up[kRows];
+    EightF32<VEC> z[kRows], z2[kRows];
 #pragma unroll
-    for (int u = 0; u < kDactRows; ++u) {
+    for (int u = 0; u < kRows; ++u) {
       const int64_t m = m0 + 4 * u;
       const int cols = m < r1 ? a.n : 0;  // rows past the chunk: nothing is read, zeros are added
       d[u].load(static_cast<const T*>(a.dout) + m * a.ldd, n, cols, lane);
@@ -948,7 +947,7 @@ __global__ __launch_bounds__(256) void dact_kernel(DactArgs a) {
       }
     }
 #pragma unroll
-    for (int u = 0; u < kDactRows; ++u) {
+    for (int u = 0; u < kRows; ++u) {
       const int64_t m = m0 + 4 * u;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
