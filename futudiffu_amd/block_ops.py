@@ -12,13 +12,15 @@ per output.  ``x`` is ``[B, N, C]`` (or ``[N, C]``), bfloat16 or float16, with a
 and ``gate`` have a row per batch item, ``[B, C]``, or with ``doc_ids`` (int32 ``[B, N]``,
 as :func:`futudiffu_amd.build_doc_ids` makes them) a row per document of a packed
 sequence, ``[B, G, C]``: a token whose id is not in ``0 .. G-1`` (padding) has scale 0 and
-gate 0, and behind a gate its ``x`` is not read.  Parameters are of ``x``'s type or float32; chunks of one projection's output are
-read in place.
+gate 0, and behind a gate its ``x`` is not read.  Parameters are of ``x``'s type or
+float32; chunks of one projection's output are read in place.
 
-The functions differentiate (once: not the gradients themselves).  Under ``torch.compile`` they go through the custom ops
+The functions differentiate (once: not the gradients themselves).  Under
+``torch.compile`` they go through the custom ops
 ``futudiffu_ii::rms_norm_modulate``, ``::rms_norm_gate_residual``,
 ``::rms_norm_gate_residual_modulate`` and ``::fused_linear``, which carry the same
-gradients.  Sums are added in a fixed order, so results and gradients repeat bit for bit.  An empty batch gives empty outputs and zero parameter gradients.
+gradients.  Sums are added in a fixed order, so results and gradients repeat bit for
+bit.  An empty batch gives empty outputs and zero parameter gradients.
 """
 
 from __future__ import annotations

@@ -486,10 +486,10 @@ int sage_rms_norm_gate_residual_modulate_bwd(
  *   workspace    sage_linear_workspace_bytes(...) bytes, 16-byte aligned; needs no clearing.
  *                other_rows: whether the residual, bias, z or out may start off 16-byte
  *                boundaries, or the residual's rows (r_rs no multiple of 8).
- * m, n, k at least 1; a weight has under 2^22 rows; a weight or a row panel of 256 rows has
- * under 2^31 bytes.  Rows of x
- * and weight that do not start on 16-byte boundaries, or a k that is no multiple of 8, are
- * copied into the workspace first. */
+ * m at least 1 and below 2^24, n and k at least 1 and below 2^22; a weight has under 2^22 rows
+ * and under 2^31 bytes; rows are at least their columns and less than 2^22 elements apart (one
+ * row: any stride).  Rows of x and weight that do not start on 16-byte boundaries, or a k that
+ * is no multiple of 8, are copied into the workspace first. */
 #define SAGE_ACT_NONE 0
 #define SAGE_ACT_SILU 1
 #define SAGE_ACT_GELU 2
@@ -502,8 +502,9 @@ int sage_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, c
                 void* workspace, size_t workspace_bytes, float* z, void* out, hipStream_t stream);
 
 /* Gradients of sage_linear: dx [m][k], dweight [rows][k] (both from 16-byte boundaries), dbias
- * [rows] (dtype or fp32), each null if not wanted; the residual's is dout itself.  dz = dout * act'(z) is rounded to dtype
- * as the products' operand (the bias's gradient adds it unrounded); sums are in a fixed order.
+ * [rows] (dtype or fp32), each null if not wanted; the residual's is dout itself.
+ * dz = dout * act'(z) is rounded to dtype as the products' operand (the bias's gradient adds it
+ * unrounded); sums are in a fixed order.
  *   dout         [m][n] rows d_rs apart.
  *   z            what sage_linear kept; null with SAGE_ACT_NONE.
  *   x            null if dweight is; weight null if dx is.
