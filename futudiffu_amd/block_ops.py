@@ -15,7 +15,8 @@ sequence, ``[B, G, C]``: a token whose id is not in ``0 .. G-1`` (padding) has s
 gate 0, and behind a gate its ``x`` is not read.  Parameters are of ``x``'s type or
 float32; chunks of one projection's output are read in place.
 
-The functions differentiate (once: not the gradients themselves).  Under
+The functions differentiate in reverse mode, once (not the gradients themselves); a
+forward-mode tangent is refused.  Under
 ``torch.compile`` they go through the custom ops
 ``futudiffu_ii::rms_norm_modulate``, ``::rms_norm_gate_residual``,
 ``::rms_norm_gate_residual_modulate`` and ``::fused_linear``, which carry the same

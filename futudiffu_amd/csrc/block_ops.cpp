@@ -67,6 +67,19 @@ int dtype_of(const Tensor& x) {
   return t == at::kHalf ? SAGE_DTYPE_FP16 : SAGE_DTYPE_BF16;
 }
 
+// Forward-mode differentiation is refused: the operators have no formula for tangents, and a
+// result without one would count as constant.
+void refuse_tangents(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
+                                "the block operators have no forward-mode derivative (a tangent was given)");
+}
+
+const Tensor& some(const OptTensor& t) {
+  static const Tensor none;
+  return t ? *t : none;
+}
+
 bool is_param(const Tensor& p, const Tensor& x) {
   return p.device() == x.device() && (p.scalar_type() == at::kFloat || p.scalar_type() == x.scalar_type());
 }
@@ -185,6 +198,7 @@ struct Norm {
 
 Tensor modulate_forward(const Tensor& x, const OptTensor& weight, const OptTensor& scale, const OptTensor& doc_ids,
                         double eps) {
+  refuse_tangents({&x, &some(weight), &some(scale)});
   const Norm a(x, weight, "scale", scale, doc_ids, eps);
   Tensor out = at::empty(x.sizes(), x.options().requires_grad(false));
   if (a.empty()) return out;
@@ -197,6 +211,7 @@ Tensor modulate_forward(const Tensor& x, const OptTensor& weight, const OptTenso
 
 Tensor gate_forward(const Tensor& residual, const Tensor& x, const OptTensor& weight, const OptTensor& gate,
                     const OptTensor& doc_ids, double eps) {
+  refuse_tangents({&residual, &x, &some(weight), &some(gate)});
   check_like("residual", residual, x);
   const Norm a(x, weight, "gate", gate, doc_ids, eps);
   Tensor out = at::empty(x.sizes(), x.options().requires_grad(false));
@@ -211,6 +226,7 @@ Tensor gate_forward(const Tensor& residual, const Tensor& x, const OptTensor& we
 std::tuple<Tensor, Tensor> gate_modulate_forward(const Tensor& residual, const Tensor& x, const OptTensor& weight,
                                                  const OptTensor& gate, const OptTensor& next_weight,
                                                  const OptTensor& next_scale, const OptTensor& doc_ids, double eps) {
+  refuse_tangents({&residual, &x, &some(weight), &some(gate), &some(next_weight), &some(next_scale)});
   check_like("residual", residual, x);
   const Norm a(x, weight, "gate", gate, doc_ids, eps, next_weight, next_scale);
   Tensor hidden = at::empty(x.sizes(), x.options().requires_grad(false)), out = at::empty_like(hidden);
@@ -225,15 +241,12 @@ std::tuple<Tensor, Tensor> gate_modulate_forward(const Tensor& residual, const T
 }
 
 typedef std::vector<bool> Wanted;
-const Tensor& some(const OptTensor& t) {
-  static const Tensor none;
-  return t ? *t : none;
-}
 
 // Gradients; undefined where not wanted.  gate: the gate_residual form.
 std::tuple<Tensor, Tensor, Tensor> norm_backward(bool gate, const Tensor& dout, const Tensor& x,
                                                  const OptTensor& weight, const OptTensor& cond,
                                                  const OptTensor& doc_ids, double eps, const Wanted& wanted) {
+  refuse_tangents({&dout, &x, &some(weight), &some(cond)});
   check_like("dout", dout, x);
   const Norm a(x, weight, gate ? "gate" : "scale", cond, doc_ids, eps);
   Tensor dx = grad_of(x, wanted[0]), dw = grad_of(some(weight), wanted[1]), dc = grad_of(some(cond), wanted[2]);
@@ -257,6 +270,7 @@ typedef std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> Six;
 Six gate_modulate_backward(const Tensor& dhidden, const Tensor& dout, const Tensor& residual, const Tensor& x,
                            const OptTensor& weight, const OptTensor& gate, const OptTensor& next_weight,
                            const OptTensor& next_scale, const OptTensor& doc_ids, double eps, const Wanted& wanted) {
+  refuse_tangents({&dhidden, &dout, &residual, &x, &some(weight), &some(gate), &some(next_weight), &some(next_scale)});
   check_like("residual", residual, x);
   check_like("dout", dout, x);
   check_like("dhidden", dhidden, x);
@@ -349,6 +363,7 @@ bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15u; }
 // out, and z where it is kept (an activation, keep_z).
 std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias,
                                           const OptTensor& residual, const std::string& activation, bool keep_z) {
+  refuse_tangents({&x, &weight, &some(bias), &some(residual)});
   const Linear a(x, weight, bias, residual, activation);
   const auto options = x.options().requires_grad(false);
   Tensor out = at::empty(a.shape, options), z;
@@ -371,6 +386,7 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight,
 std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dout, const Tensor& x, const Tensor& weight,
                                                    const OptTensor& bias, const OptTensor& z,
                                                    const std::string& activation, const Wanted& wanted) {
+  refuse_tangents({&dout, &x, &weight, &some(bias)});
   const Linear a(x, weight, bias, std::nullopt, activation);
   a.check_out("dout", dout, x);
   const bool act = a.act != SAGE_ACT_NONE;

@@ -310,3 +310,58 @@ def test_allowed_is_half_a_step():
             (y.view(torch.int16) + 1).view(dtype)
         assert O.worst(up, x, torch.zeros_like(x)) > 1.0
     assert O.worst(torch.tensor([float("nan")]), torch.tensor([1.0], dtype=torch.float64), torch.zeros(1)) == float("inf")
+
+
+def _calls():
+    """Every operator on CPU tensors, with all of its arguments: (op, function of its tensors,
+    tensors)."""
+    B, N, C, G = 2, 6, 16, 3
+    ids = torch.zeros(B, N, dtype=torch.int32)
+
+    def t(*shape, dtype=torch.float32):
+        return torch.zeros(*shape, dtype=dtype)
+
+    x, r = t(B, N, C, dtype=torch.bfloat16), t(B, N, C, dtype=torch.bfloat16)
+    rows = t(2 * C, C, dtype=torch.bfloat16)
+    return [("rms_norm_modulate", lambda *a: F.rms_norm_modulate(*a, doc_ids=ids), (x, t(C), t(B, G, C))),
+            ("rms_norm_gate_residual", lambda *a: F.rms_norm_gate_residual(*a, doc_ids=ids),
+             (r, x, t(C), t(B, G, C))),
+            ("rms_norm_gate_residual_modulate", lambda *a: F.rms_norm_gate_residual_modulate(*a, doc_ids=ids),
+             (r, x, t(C), t(B, G, C), t(C), t(B, G, C))),
+            ("fused_linear", lambda *a: F.fused_linear(*a, activation="swiglu"), (x, rows, t(2 * C), r))]
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_tangents_are_refused(i):
+    """Forward-mode differentiation raises instead of returning a result without a tangent,
+    whichever argument carries one; the registered ops too."""
+    from torch.autograd import forward_ad
+    name, fn, args = _calls()[i]
+    for j, a in enumerate(args):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(a, torch.ones_like(a))
+            call = args[:j] + (dual,) + args[j + 1:]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                fn(*call)
+            tail = ("swiglu", False) if name == "fused_linear" else (None, 1e-5)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                getattr(torch.ops.futudiffu_ii, name)(*call, *tail)
+            with pytest.raises((NotImplementedError, RuntimeError)):
+                fn(*args[:j], dual.requires_grad_(), *args[j + 1:])
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.func.jvp(lambda t: fn(*args[:j], t, *args[j + 1:]), (a,), (torch.ones_like(a),))
+
+
+def test_tangents_of_gradients_are_refused():
+    from torch.autograd import forward_ad
+    op = torch.ops.futudiffu_ii
+    x, w = torch.zeros(2, 6, 16, dtype=torch.bfloat16), torch.zeros(16, 16, dtype=torch.bfloat16)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: op.rms_norm_modulate_backward(d, x, None, None, None, 1e-5, [True] * 3),
+                     lambda: op.rms_norm_gate_residual_backward(d, x, None, None, None, 1e-5, [True] * 3),
+                     lambda: op.rms_norm_gate_residual_modulate_backward(x, d, x, x, None, None, None, None, None, 1e-5,
+                                                                         [True] * 6),
+                     lambda: op.fused_linear_backward(d, x, w, None, None, "none", [True] * 3)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
