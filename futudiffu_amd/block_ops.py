@@ -16,8 +16,8 @@ gate 0, and behind a gate its ``x`` is not read.  Parameters are of ``x``'s type
 float32; chunks of one projection's output are read in place.
 
 The functions differentiate in reverse mode, once (not the gradients themselves); a
-forward-mode tangent is refused.  Under
-``torch.compile`` they go through the custom ops
+forward-mode tangent is refused.  Under ``torch.compile``, a tracer, a dispatch mode or
+``vmap`` they go through the custom ops
 ``futudiffu_ii::rms_norm_modulate``, ``::rms_norm_gate_residual``,
 ``::rms_norm_gate_residual_modulate`` and ``::fused_linear``, which carry the same
 gradients.  Sums are added in a fixed order, so results and gradients repeat bit for

@@ -5,6 +5,8 @@
 // backward runs on autograd's own thread, where Python (the interpreter's data lying in the
 // other core's caches) took 50 us of a step's 150 and made the forward's next pass three times
 // as slow; and a call without gradients spends 10 us in Python around a 3 us kernel.
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/extension.h>
@@ -411,6 +413,39 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dout, const Ten
   return {dx, dw, db};
 }
 
+// ---------------------------------------------------------------- tracing
+
+// Whether a call has to go through its registered op: a tracer, a dispatch mode or a functorch
+// transform is active, or an argument is a wrapper or a lazy view (negated, zeros without
+// storage).  The functions below see storage alone: a trace of them would record the allocation
+// of the outputs and nothing that writes them.
+// A tangent is refused here too: behind the dispatcher a transform has taken it off.
+bool through_dispatcher(std::initializer_list<const Tensor*> tensors) {
+  using c10::DispatchKey;
+  static constexpr c10::DispatchKeySet hooks(
+      {DispatchKey::Fake, DispatchKey::Python, DispatchKey::PythonTLSSnapshot, DispatchKey::PythonDispatcher,
+       DispatchKey::Tracer, DispatchKey::Functionalize, DispatchKey::Conjugate, DispatchKey::Negative,
+       DispatchKey::ZeroTensor, DispatchKey::Batched, DispatchKey::VmapMode, DispatchKey::FuncTorchBatched,
+       DispatchKey::FuncTorchBatchedDecomposition, DispatchKey::FuncTorchVmapMode, DispatchKey::FuncTorchGradWrapper,
+       DispatchKey::FuncTorchDynamicLayerBackMode, DispatchKey::FuncTorchDynamicLayerFrontMode});
+  const auto local = c10::impl::tls_local_dispatch_key_set();
+  c10::DispatchKeySet keys = local.included_;
+  for (const Tensor* t : tensors)
+    if (t->defined()) keys = keys | t->key_set();
+  if (((keys - local.excluded_) & hooks).raw_repr() == 0) return false;
+  refuse_tangents(tensors);
+  return true;
+}
+
+// The registered op futudiffu_ii::<name> on these arguments.
+template <typename... Args>
+torch::jit::Stack call_op(const char* name, Args&&... args) {
+  torch::jit::Stack stack;
+  torch::jit::push(stack, std::forward<Args>(args)...);
+  c10::Dispatcher::singleton().findSchemaOrThrow((std::string("futudiffu_ii::") + name).c_str(), "").callBoxed(&stack);
+  return stack;
+}
+
 // ---------------------------------------------------------------- autograd
 
 Tensor held(const OptTensor& t) { return t ? *t : Tensor(); }
@@ -422,6 +457,19 @@ Wanted needs(AutogradContext* ctx, const variable_list& args) {
   size_t edge = 0;
   for (const Tensor& t : args) w.push_back(t.defined() ? ctx->needs_input_grad(edge++) : false);
   return w;
+}
+
+c10::List<bool> list_of(const Wanted& w) {
+  c10::List<bool> l;
+  for (const bool b : w) l.push_back(b);
+  return l;
+}
+
+// What a gradient op returned, undefined in the place of what is not wanted.
+variable_list gradients(const torch::jit::Stack& returned, const Wanted& w) {
+  variable_list g;
+  for (size_t i = 0; i < returned.size(); ++i) g.push_back(w[i] ? returned[i].toTensor() : Tensor());
+  return g;
 }
 
 // The gradients are not themselves differentiable.
@@ -451,8 +499,14 @@ struct ModulateFn : torch::autograd::Function<ModulateFn> {
   static variable_list backward(AutogradContext* ctx, variable_list d) {
     const auto s = ctx->get_saved_variables();
     once({d[0], s[0], s[1], s[2]});
-    const auto [dx, dw, dc] = norm_backward(false, d[0], s[0], given(s[1]), given(s[2]), given(s[3]),
-                                            ctx->saved_data["eps"].toDouble(), needs(ctx, {s[0], s[1], s[2]}));
+    const Wanted w = needs(ctx, {s[0], s[1], s[2]});
+    const double eps = ctx->saved_data["eps"].toDouble();
+    if (through_dispatcher({&d[0], &s[0], &s[1], &s[2], &s[3]})) {
+      const auto g = gradients(
+          call_op("rms_norm_modulate_backward", d[0], s[0], given(s[1]), given(s[2]), given(s[3]), eps, list_of(w)), w);
+      return {g[0], g[1], g[2], Tensor(), Tensor()};
+    }
+    const auto [dx, dw, dc] = norm_backward(false, d[0], s[0], given(s[1]), given(s[2]), given(s[3]), eps, w);
     return {dx, dw, dc, Tensor(), Tensor()};
   }
 };
@@ -467,10 +521,17 @@ struct GateFn : torch::autograd::Function<GateFn> {
   static variable_list backward(AutogradContext* ctx, variable_list d) {
     const auto s = ctx->get_saved_variables();
     once({d[0], s[0], s[1], s[2]});
-    const Wanted w = needs(ctx, {s[0], s[0], s[1], s[2]});  // the residual's edge comes first
-    const auto [dx, dw, dg] = norm_backward(true, d[0], s[0], given(s[1]), given(s[2]), given(s[3]),
-                                            ctx->saved_data["eps"].toDouble(), {w[1], w[2], w[3]});
-    return {w[0] ? d[0] : Tensor(), dx, dw, dg, Tensor(), Tensor()};
+    const Wanted all = needs(ctx, {s[0], s[0], s[1], s[2]});  // the residual's edge comes first
+    const Wanted w = {all[1], all[2], all[3]};
+    const Tensor dr = all[0] ? d[0] : Tensor();
+    const double eps = ctx->saved_data["eps"].toDouble();
+    if (through_dispatcher({&d[0], &s[0], &s[1], &s[2], &s[3]})) {
+      const auto g = gradients(call_op("rms_norm_gate_residual_backward", d[0], s[0], given(s[1]), given(s[2]),
+                                       given(s[3]), eps, list_of(w)), w);
+      return {dr, g[0], g[1], g[2], Tensor(), Tensor()};
+    }
+    const auto [dx, dw, dg] = norm_backward(true, d[0], s[0], given(s[1]), given(s[2]), given(s[3]), eps, w);
+    return {dr, dx, dw, dg, Tensor(), Tensor()};
   }
 };
 
@@ -487,9 +548,14 @@ struct GateModulateFn : torch::autograd::Function<GateModulateFn> {
     const auto s = ctx->get_saved_variables();
     once({d[0], d[1], s[0], s[1], s[2], s[3], s[4], s[5]});
     const Wanted w = needs(ctx, {s[0], s[1], s[2], s[3], s[4], s[5]});
-    auto [dr, dx, dw, dg, dw2, ds] =
-        gate_modulate_backward(d[0], d[1], s[0], s[1], given(s[2]), given(s[3]), given(s[4]), given(s[5]), given(s[6]),
-                               ctx->saved_data["eps"].toDouble(), w);
+    const double eps = ctx->saved_data["eps"].toDouble();
+    if (through_dispatcher({&d[0], &d[1], &s[0], &s[1], &s[2], &s[3], &s[4], &s[5], &s[6]})) {
+      const auto g = gradients(call_op("rms_norm_gate_residual_modulate_backward", d[0], d[1], s[0], s[1], given(s[2]),
+                                       given(s[3]), given(s[4]), given(s[5]), given(s[6]), eps, list_of(w)), w);
+      return {g[0], g[1], g[2], g[3], g[4], g[5], Tensor(), Tensor()};
+    }
+    auto [dr, dx, dw, dg, dw2, ds] = gate_modulate_backward(d[0], d[1], s[0], s[1], given(s[2]), given(s[3]),
+                                                            given(s[4]), given(s[5]), given(s[6]), eps, w);
     return {w[0] ? dr : Tensor(), dx, dw, dg, dw2, ds, Tensor(), Tensor()};
   }
 };
@@ -509,21 +575,32 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     const auto s = ctx->get_saved_variables();
     once({d[0], s[0], s[1], s[2]});
     // x, weight, bias, then the residual's edge
-    const Wanted w = needs(ctx, {s[0], s[1], s[2], ctx->saved_data["residual"].toBool() ? s[0] : Tensor()});
-    const auto [dx, dw, db] = linear_backward(d[0], s[0], s[1], given(s[2]), given(s[3]),
-                                              ctx->saved_data["activation"].toStringRef(), {w[0], w[1], w[2]});
-    return {dx, dw, db, w[3] ? d[0] : Tensor(), Tensor()};
+    const Wanted all = needs(ctx, {s[0], s[1], s[2], ctx->saved_data["residual"].toBool() ? s[0] : Tensor()});
+    const Wanted w = {all[0], all[1], all[2]};
+    const Tensor dr = all[3] ? d[0] : Tensor();
+    const std::string& activation = ctx->saved_data["activation"].toStringRef();
+    if (through_dispatcher({&d[0], &s[0], &s[1], &s[2], &s[3]})) {
+      const auto g = gradients(
+          call_op("fused_linear_backward", d[0], s[0], s[1], given(s[2]), given(s[3]), activation, list_of(w)), w);
+      return {g[0], g[1], g[2], dr, Tensor()};
+    }
+    const auto [dx, dw, db] = linear_backward(d[0], s[0], s[1], given(s[2]), given(s[3]), activation, w);
+    return {dx, dw, db, dr, Tensor()};
   }
 };
 
 Tensor rms_norm_modulate(const Tensor& x, const OptTensor& weight, const OptTensor& scale, const OptTensor& doc_ids,
                          double eps) {
+  if (through_dispatcher({&x, &some(weight), &some(scale), &some(doc_ids)}))
+    return call_op("rms_norm_modulate", x, weight, scale, doc_ids, eps)[0].toTensor();
   if (wants_grad({&x, &some(weight), &some(scale)})) return ModulateFn::apply(x, weight, scale, doc_ids, eps);
   return modulate_forward(x, weight, scale, doc_ids, eps);
 }
 
 Tensor rms_norm_gate_residual(const Tensor& residual, const Tensor& x, const OptTensor& weight, const OptTensor& gate,
                               const OptTensor& doc_ids, double eps) {
+  if (through_dispatcher({&residual, &x, &some(weight), &some(gate), &some(doc_ids)}))
+    return call_op("rms_norm_gate_residual", residual, x, weight, gate, doc_ids, eps)[0].toTensor();
   if (wants_grad({&residual, &x, &some(weight), &some(gate)}))
     return GateFn::apply(residual, x, weight, gate, doc_ids, eps);
   return gate_forward(residual, x, weight, gate, doc_ids, eps);
@@ -533,6 +610,12 @@ std::tuple<Tensor, Tensor> rms_norm_gate_residual_modulate(const Tensor& residua
                                                            const OptTensor& weight, const OptTensor& gate,
                                                            const OptTensor& next_weight, const OptTensor& next_scale,
                                                            const OptTensor& doc_ids, double eps) {
+  if (through_dispatcher({&residual, &x, &some(weight), &some(gate), &some(next_weight), &some(next_scale),
+                          &some(doc_ids)})) {
+    const auto r =
+        call_op("rms_norm_gate_residual_modulate", residual, x, weight, gate, next_weight, next_scale, doc_ids, eps);
+    return {r[0].toTensor(), r[1].toTensor()};
+  }
   if (wants_grad({&residual, &x, &some(weight), &some(gate), &some(next_weight), &some(next_scale)})) {
     const auto r = GateModulateFn::apply(residual, x, weight, gate, next_weight, next_scale, doc_ids, eps);
     return {r[0], r[1]};
@@ -542,6 +625,10 @@ std::tuple<Tensor, Tensor> rms_norm_gate_residual_modulate(const Tensor& residua
 
 Tensor fused_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
                     const std::string& activation) {
+  if (through_dispatcher({&x, &weight, &some(bias), &some(residual)})) {
+    const bool keep_z = activation != "none" && wants_grad({&x, &weight, &some(bias)});
+    return call_op("fused_linear", x, weight, bias, residual, activation, keep_z)[0].toTensor();
+  }
   if (wants_grad({&x, &weight, &some(bias), &some(residual)}))
     return LinearFn::apply(x, weight, bias, residual, activation);
   return std::get<0>(linear_forward(x, weight, bias, residual, activation, false));

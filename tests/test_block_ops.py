@@ -312,13 +312,13 @@ def test_allowed_is_half_a_step():
     assert O.worst(torch.tensor([float("nan")]), torch.tensor([1.0], dtype=torch.float64), torch.zeros(1)) == float("inf")
 
 
-def _calls():
+def _calls(params=torch.float32):
     """Every operator on CPU tensors, with all of its arguments: (op, function of its tensors,
     tensors)."""
     B, N, C, G = 2, 6, 16, 3
     ids = torch.zeros(B, N, dtype=torch.int32)
 
-    def t(*shape, dtype=torch.float32):
+    def t(*shape, dtype=params):
         return torch.zeros(*shape, dtype=dtype)
 
     x, r = t(B, N, C, dtype=torch.bfloat16), t(B, N, C, dtype=torch.bfloat16)
@@ -365,3 +365,52 @@ def test_tangents_of_gradients_are_refused():
                      lambda: op.fused_linear_backward(d, x, w, None, None, "none", [True] * 3)):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+@pytest.mark.parametrize("grads", [False, True])
+def test_a_trace_records_the_operators(grads):
+    """Traced, a call is its op and a gradient the op's gradient, not the allocations of their
+    results."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        for name, fn, args in _calls(torch.bfloat16):
+            if grads:
+                args = tuple(a.requires_grad_() for a in args)
+
+            def traced(*a):
+                out = fn(*a)
+                out = out if isinstance(out, tuple) else (out,)
+                return torch.autograd.grad(out, a, [torch.ones_like(o) for o in out]) if grads else out
+
+            got = {str(n.target) for n in make_fx(traced)(*args).graph.nodes if n.op == "call_function"}
+            want = {f"futudiffu_ii.{name}.default"} | ({f"futudiffu_ii.{name}_backward.default"} if grads else set())
+            assert want <= got and not any("aten.empty" in t for t in got), (name, got)
+
+
+def test_dispatch_modes_see_the_operators():
+    """A dispatch mode (counters, memory tools, checkpoint policies) sees each call and each
+    gradient as its op."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.ops = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.ops.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    with FakeTensorMode():
+        for name, fn, args in _calls():
+            args = tuple(a.requires_grad_() for a in args)
+            with Seen() as seen:
+                out = fn(*args)
+            assert f"futudiffu_ii::{name}" in seen.ops
+            out = out if isinstance(out, tuple) else (out,)
+            with Seen() as seen:
+                grads = torch.autograd.grad(out, args, [torch.ones_like(o) for o in out])
+            assert f"futudiffu_ii::{name}_backward" in seen.ops
+            assert [g.shape for g in grads] == [a.shape for a in args] and [g.dtype for g in grads] == [a.dtype for a in args]
