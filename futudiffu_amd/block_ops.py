@@ -81,6 +81,21 @@ def _only(grads, wanted):
     return [g if w else None for g, w in zip(grads, wanted)]
 
 
+# The gradients are not themselves differentiable: a second derivative through these ops
+# would lack every term that goes through them.
+
+_TWICE = "the gradients of the block operators cannot be differentiated (create_graph=True)"
+
+
+def _once(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(_TWICE)
+
+
+def _refuse_twice(ctx, *grads):
+    raise RuntimeError(_TWICE)
+
+
 _define("rms_norm_modulate(Tensor x, Tensor? weight, Tensor? scale, Tensor? doc_ids, float eps) -> Tensor",
         lambda *args: _load().modulate_forward(*args), lambda x, weight, scale, doc_ids, eps: x.new_empty(x.shape))
 _define("rms_norm_modulate_backward(Tensor dout, Tensor x, Tensor? weight, Tensor? scale, Tensor? doc_ids, "
@@ -119,6 +134,7 @@ def _modulate_setup(ctx, inputs, output):
 
 def _modulate_autograd(ctx, dout):
     x, weight, scale, doc_ids = ctx.saved_tensors
+    _once(dout, x, weight, scale)
     wanted = _wanted(ctx, (0, 1, 2), (x, weight, scale))
     grads = torch.ops.futudiffu_ii.rms_norm_modulate_backward(dout, x, weight, scale, doc_ids, ctx.eps, wanted)
     return *_only(grads, wanted), None, None
@@ -132,6 +148,7 @@ def _gate_setup(ctx, inputs, output):
 
 def _gate_autograd(ctx, dout):
     x, weight, gate, doc_ids = ctx.saved_tensors
+    _once(dout, x, weight, gate)
     wanted = _wanted(ctx, (1, 2, 3), (x, weight, gate))
     grads = (None, None, None)
     if any(wanted):
@@ -148,6 +165,7 @@ def _gate_modulate_setup(ctx, inputs, output):
 
 def _gate_modulate_autograd(ctx, dhidden, dout):
     residual, x, weight, gate, next_weight, next_scale, doc_ids = ctx.saved_tensors
+    _once(dhidden, dout, residual, x, weight, gate, next_weight, next_scale)
     wanted = _wanted(ctx, range(6), (residual, x, weight, gate, next_weight, next_scale))
     grads = torch.ops.futudiffu_ii.rms_norm_gate_residual_modulate_backward(
         dhidden, dout, residual, x, weight, gate, next_weight, next_scale, doc_ids, ctx.eps, wanted)
@@ -186,6 +204,7 @@ def _linear_setup(ctx, inputs, output):
 
 def _linear_autograd(ctx, dout, dz):
     x, weight, bias, z = ctx.saved_tensors
+    _once(dout, x, weight, bias)
     wanted = _wanted(ctx, range(3), (x, weight, bias))
     grads = (None, None, None)
     if any(wanted):
@@ -194,6 +213,8 @@ def _linear_autograd(ctx, dout, dz):
 
 
 torch.library.register_autograd("futudiffu_ii::fused_linear", _linear_autograd, setup_context=_linear_setup, lib=_ops)
+for _name in ("rms_norm_modulate", "rms_norm_gate_residual", "rms_norm_gate_residual_modulate", "fused_linear"):
+    torch.library.register_autograd(f"futudiffu_ii::{_name}_backward", _refuse_twice, lib=_ops)
 
 
 # ---- the functions ---------------------------------------------------------------------

@@ -414,3 +414,48 @@ def test_dispatch_modes_see_the_operators():
                 grads = torch.autograd.grad(out, args, [torch.ones_like(o) for o in out])
             assert f"futudiffu_ii::{name}_backward" in seen.ops
             assert [g.shape for g in grads] == [a.shape for a in args] and [g.dtype for g in grads] == [a.dtype for a in args]
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_gradients_of_the_ops_are_not_differentiated(i):
+    """The registered ops refuse a second derivative as the functions do.  A residual's gradient
+    is the incoming one, which may be differentiated."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        name, _, args = _calls(torch.bfloat16)[i]
+        tail = (None, 1e-5)
+        if name == "fused_linear":
+            tail = ("swiglu", True)
+        else:
+            args = tuple(a[:, 0] if a.shape[1:2] == (3,) else a for a in args)
+        residual = {"rms_norm_gate_residual": 0, "fused_linear": 3}.get(name)
+        for j, a in enumerate(args):
+            leaf = a.detach().requires_grad_()
+
+            def grad(**kw):
+                out = getattr(torch.ops.futudiffu_ii, name)(*args[:j], leaf, *args[j + 1:], *tail)
+                out = out[0] if isinstance(out, (tuple, list)) else out
+                return torch.autograd.grad(out, leaf, torch.ones_like(out), **kw)[0]
+
+            assert grad().shape == a.shape
+            if j == residual:
+                assert grad(create_graph=True).shape == a.shape
+            else:
+                with pytest.raises(RuntimeError, match="create_graph"):
+                    grad(create_graph=True)
+
+
+def test_gradient_ops_are_not_differentiated():
+    """Nor does a gradient op called by itself give a derivative without its own terms."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    op = torch.ops.futudiffu_ii
+    with FakeTensorMode():
+        x, w = torch.zeros(2, 6, 16, dtype=torch.bfloat16), torch.zeros(16, 16, dtype=torch.bfloat16)
+        d = x.clone().requires_grad_()
+        for out in (op.rms_norm_modulate_backward(d, x, None, None, None, 1e-5, [True] * 3),
+                    op.rms_norm_gate_residual_backward(d, x, None, None, None, 1e-5, [True] * 3),
+                    op.rms_norm_gate_residual_modulate_backward(x, d, x, x, None, None, None, None, None, 1e-5,
+                                                                [True] * 6),
+                    op.fused_linear_backward(d, x, w, None, None, "none", [True] * 3)):
+            with pytest.raises(RuntimeError, match="cannot be differentiated"):
+                torch.autograd.grad(out[0], d, torch.ones_like(out[0]))

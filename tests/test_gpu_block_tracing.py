@@ -122,3 +122,22 @@ def test_transforms_without_a_formula_raise(cuda, i):
             torch.func.grad(lambda t: put(t)[0].float().sum())(a)
         with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
             put(forward_ad.make_dual(a, torch.ones_like(a)))
+
+
+@pytest.mark.parametrize("i", OPS)
+def test_gradients_of_the_ops_are_not_differentiated(cuda, i):
+    """The registered ops, called directly, refuse create_graph=True as the functions do; without
+    it their gradients are the functions'."""
+    name, fn, args = _calls(cuda)[i]
+    ids = torch.tensor([[0, 0, 2, 1, -1, 1], [1, 5, 0, 0, 2, 2]], dtype=torch.int32, device=cuda)
+    tail = ("swiglu", True) if name == "fused_linear" else (ids, 1e-5)
+    leaves = tuple(a.detach().requires_grad_() for a in args)
+
+    def outs():
+        out = getattr(torch.ops.futudiffu_ii, name)(*leaves, *tail)
+        return out[:1] if name == "fused_linear" else _outs(out)
+
+    d = [torch.randn_like(o) for o in _outs(fn(*args))]
+    assert _equal(torch.autograd.grad(outs(), leaves, d), _grads(fn, args, d))
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(outs(), leaves, d, create_graph=True)
