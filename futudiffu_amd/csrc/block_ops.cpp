@@ -160,8 +160,12 @@ struct Norm {
     if (cond.rows || next_scale.rows) groups = cond.rows ? cond.rows : next_scale.rows;
     need_gpu(x);
     if (docs) {
-      // ids past 32 bits stay ids of no document
-      const Tensor i = ids->scalar_type() == at::kLong ? ids->clamp(-1, groups) : *ids;
+      // ids past 32 bits stay ids of no document (of 64 bits without a sign: those past 2^63
+      // read as negative ones; of 32 bits without a sign: those past 2^31)
+      Tensor i = *ids;
+      if (i.scalar_type() == at::kUInt64) i = i.view(at::kLong);
+      if (i.scalar_type() == at::kUInt32) i = i.view(at::kInt);
+      if (i.scalar_type() == at::kLong) i = i.clamp(-1, groups);
       doc = i.to(x.device(), at::kInt).contiguous();
     }
   }

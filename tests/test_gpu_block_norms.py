@@ -387,3 +387,28 @@ def test_documents_and_chunks(cuda, op, B, N, C, lengths):
     print(op, B, N, C, len(lengths), flush=True)
     v = _inputs(op, B, N, C, BF, F32, (len(lengths), _ids(lengths, N, B)), seed=N)
     _check(_with_grads(op, _to(v, cuda)), _want(op, v))
+
+
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_ids_of_every_integer_type(cuda, op):
+    """The same documents from ids of any integer type; one beyond 32 bits, with or without a
+    sign, is of no document and does not wrap to one."""
+    v = _to(_inputs(op, 2, 40, 72, BF, F32, None, seed=2), cuda)
+    ids = torch.arange(80, device=cuda).view(2, 40) % 3  # 2: no document
+    for k in ("cond", "next_scale"):
+        if v.get(k) is not None:
+            v[k] = torch.stack([v[k] * f for f in (1.0, -0.5)], 1)
+    v["doc_ids"] = ids.int()
+    want = _with_grads(op, v)
+    far = {torch.uint8: (255,), torch.int8: (-128, 127), torch.int16: (-2 ** 15, 2 ** 15 - 1), torch.uint16: (2 ** 16 - 1,),
+           torch.int32: (-2 ** 31, 2 ** 31 - 1), torch.uint32: (2 ** 31, 2 ** 31 + 1, 2 ** 32 - 1),
+           torch.int64: (2 ** 32, 2 ** 32 + 1, -2 ** 32, -2 ** 63 + 1),
+           torch.uint64: (2 ** 32, 2 ** 32 + 1, 2 ** 63, 2 ** 63 + 1, 2 ** 64 - 1)}
+    for dtype, values in far.items():
+        for value in (2, *values):
+            print(op, dtype, value, flush=True)
+            plain = [[value if i == 2 else i for i in row] for row in ids.tolist()]
+            for device in ("cpu", cuda):
+                v["doc_ids"] = torch.tensor(plain, dtype=dtype).to(device)
+                got = _with_grads(op, v)
+                assert all(torch.equal(got[k], want[k]) for k in want), (dtype, value, device)
