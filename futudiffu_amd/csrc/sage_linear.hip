@@ -69,7 +69,9 @@ __device__ __forceinline__ float act_grad(int act, float z) {
   }
   if (act == kActGelu) {  // with s = sigmoid(2u): s + z s (1 - s) 2 u'
     const float s = sigmoidf(2.0f * kGeluA * (z + 0.044715f * z * z * z));
-    return s + z * s * (1.0f - s) * (2.0f * kGeluA * (1.0f + 3.0f * 0.044715f * z * z));
+    // past |z| = 5e19 u' leaves fp32, where s (1 - s) is long 0: their product stays 0
+    const float up = fminf(2.0f * kGeluA * (1.0f + 3.0f * 0.044715f * z * z), 3e38f);
+    return s + z * s * (1.0f - s) * up;
   }
   return 1.0f;
 }

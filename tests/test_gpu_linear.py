@@ -318,3 +318,21 @@ def test_few_rows(cuda, M, K, N):
         v = _inputs(M, K, N, act, dtype, bias, res, seed=M + K + i, device=cuda)
         got = _run(v, act, grads=False)
         _check(got, {"out": _want(v, act)["out"]}, act)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "swiglu"])
+def test_activations_over_the_whole_range(cuda, act):
+    """To the largest finite value an activation is 0 or the value itself and its gradient 0 or 1,
+    though squares and cubes on the way leave fp32's range."""
+    z = torch.tensor([-3e38, -1e30, -1e20, -1e19, -1e13, 1e13, 1e19, 1e20, 1e30, 3e38])
+    n = len(z)
+    w = torch.eye(n)
+    if act == "swiglu":  # z2 = 1 everywhere, from the bias
+        w = torch.cat([w, torch.zeros(n, n)])
+    bias = torch.cat([torch.zeros(n), torch.ones(n)]) if act == "swiglu" else None
+    v = dict(x=torch.diag(z).to(BF).to(cuda), weight=w.to(BF).to(cuda), bias=None if bias is None else bias.to(cuda),
+             residual=None, dout=torch.eye(n).to(BF).to(cuda))
+    got = _run(v, act)
+    o, d = got["out"].float().cpu(), got["dx"].float().cpu()
+    assert torch.equal(o.diagonal(), z.clamp_min(0).to(BF).float())
+    assert torch.isfinite(d).all() and torch.equal(d.diagonal(), (z > 0).float())
