@@ -177,7 +177,8 @@ __device__ __forceinline__ void finish_wave(const GemmArgs& a, int lane, int64_t
       if (j + kStep < NI) residual(j + kStep, (j / kStep + 1) & 1);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const int nb = n0 + (32 / kStep) * j + 16 * p + 8 * h, nob = beyond(nb);
+        // beyond the last column a column that lies past any bias, in bytes too
+        const int nb = n0 + (32 / kStep) * j + 16 * p + 8 * h, nob = nb < a.n ? 0 : 0x10000000;
         bias_at(nb | nob, b[p]);
         if constexpr (kGlu) bias_at((nb + a.n) | nob, b2[p]);
       }
