@@ -412,3 +412,40 @@ def test_ids_of_every_integer_type(cuda, op):
                 v["doc_ids"] = torch.tensor(plain, dtype=dtype).to(device)
                 got = _with_grads(op, v)
                 assert all(torch.equal(got[k], want[k]) for k in want), (dtype, value, device)
+
+
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_compiled_gradients(cuda, op):
+    """The gradients of the compiled function, whose formulas are the ops' own, are the eager
+    ones bit for bit: all of them, with parameters absent, and where some leaves alone want one."""
+    absent = {"modulate": ("weight", "cond"), "gate": ("weight", "cond"),
+              "gate_modulate": ("weight", "cond", "next_weight", "next_scale")}[op]
+    docs = (2, _ids((8, 9), 20, 2))
+    cases = [((), ORDER[op])] + [((k,), ORDER[op]) for k in absent] + [((), (k,)) for k in ORDER[op]]
+    for gone, leaves in cases:
+        print(op, gone, leaves, flush=True)
+        v = _to(_inputs(op, 2, 20, 136, BF, F32, docs, seed=1), cuda)
+        v.update({k: None for k in gone})
+        leaves = [k for k in leaves if v[k] is not None]
+        want = _with_grads(op, v, leaves=leaves)
+        names = [k for k in ORDER[op] if v[k] is not None]
+
+        def fn(*a):
+            got = _call(op, dict(v, **dict(zip(names, a))))
+            return tuple(got[k] for k in outs)
+
+        outs = ["out", "hidden"] if op == "gate_modulate" else ["out"]
+        torch._dynamo.reset()
+        args = [v[k].detach().requires_grad_(k in leaves) for k in names]
+        out = torch.compile(fn, backend="aot_eager", fullgraph=True)(*args)
+        grads = torch.autograd.grad(out, [args[names.index(k)] for k in leaves], [v["d" + k] for k in outs])
+        assert all(torch.equal(o, want[k]) for o, k in zip(out, outs))
+        for k, g in zip(leaves, grads):
+            assert g.dtype == v[k].dtype and torch.equal(g, want["d" + k]), k
+        for k in outs if len(outs) > 1 else ():  # one of two outputs alone
+            one = [torch.autograd.grad(f(*args)[outs.index(k)], [args[names.index(j)] for j in leaves], v["d" + k],
+                                       allow_unused=True)
+                   for f in (fn, torch.compile(fn, backend="aot_eager", fullgraph=True))]
+            for j, a, b in zip(leaves, *one):
+                # behind hidden alone the second norm's parameters are not reached: zeros, or none
+                assert torch.equal(torch.zeros_like(v[j]) if a is None else a, torch.zeros_like(v[j]) if b is None else b), (k, j)
