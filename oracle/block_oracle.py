@@ -79,7 +79,9 @@ def norms(op: str, x: Tensor, weight, cond, doc_ids, eps: float, residual=None, 
 
     Roundings of one value: a sum of C squares or products in chains of 16 and trees (under
     40 with the scaling around it, twice that where two norms follow each other); a channel
-    sum over tokens in chains of at most 512 tokens, 64 chunks and 16 rows (under 700).
+    sum over tokens in chains of at most 512 tokens of a chunk, a tree of 8, every 32nd chunk's
+    partial and 32 of their sums (under 700 to 10^6 tokens).  Over many tokens that bound is
+    wider than one token's part: sums that are exact in any order are what shows a token lost.
     """
     B, N, C = x.shape
     one = torch.ones(C, dtype=torch.float64, device=x.device)

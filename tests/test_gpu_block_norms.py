@@ -449,3 +449,75 @@ def test_compiled_gradients(cuda, op):
             for j, a, b in zip(leaves, *one):
                 # behind hidden alone the second norm's parameters are not reached: zeros, or none
                 assert torch.equal(torch.zeros_like(v[j]) if a is None else a, torch.zeros_like(v[j]) if b is None else b), (k, j)
+
+
+@pytest.mark.parametrize("B,N,C,lengths", [
+    (1, 270000, 8, None),                   # no documents: every chunk's partial
+    (1, 270000, 8, (140000, 7, 129000)),    # more chunks than one search takes, and padding
+    (1, 270000, 8, (900,) * 290),
+    (2, 30011, 65, 5),                      # 5 documents in turn: every chunk holds them all
+    (3, 700, 1032, (500, 1, 150)),
+    (2, 333, 4104, (100, 200)),
+])
+@pytest.mark.parametrize("op", ["modulate", "gate", "gate_modulate"])
+def test_parameter_sums_are_exact(cuda, op, B, N, C, lengths):
+    """Sums that are exact whatever their order, so that a token lost or taken twice shows at any
+    size: x of +-1 and eps 0 (xhat is x), small integers and halves elsewhere, every sum under
+    2^24 of its unit.  gate + modulate: r = 0 and a gate of +-1 (hidden is +-1, its norm too), and
+    dout in pairs of channels whose products with hidden cancel (its mean with hidden is 0)."""
+    print(op, B, N, C, lengths, flush=True)
+    g = torch.Generator().manual_seed(N)
+
+    def pick(*shape, of):
+        return torch.tensor(of, dtype=torch.float64)[torch.randint(len(of), shape, generator=g)]
+
+    docs = None
+    if isinstance(lengths, int):
+        docs = (lengths, (torch.arange(N, dtype=torch.int32) % lengths).expand(B, N).contiguous())
+    elif lengths:
+        docs = (len(lengths), _ids(lengths, N, B))
+    rows = (B, C) if docs is None else (B, docs[0], C)
+    ids = torch.zeros(B, N, dtype=torch.int64) if docs is None else docs[1].long()
+    G = 1 if docs is None else docs[0]
+    live = (ids >= 0)[..., None]
+    x = pick(B, N, C, of=(-1, 1))
+    d, dh = pick(B, N, C, of=(-3, -2, -1, 1, 2, 3)), pick(B, N, C, of=(-2, -1, 0, 1, 2))
+    cond = pick(*rows, of=(-1, 1) if op == "gate_modulate" else (-1, -0.5, 0, 1, 2))
+    v = dict(x=x, weight=torch.ones(C), cond=cond)
+    m = torch.zeros(B, N, C, dtype=torch.float64)  # of each token; 0 behind the last document
+    at = ids.clamp_min(0)
+    for b in range(B):
+        m[b] = cond[b].view(G, C)[at[b]] * live[b]
+    h_grad, xhat = d, x if op == "modulate" else x * live
+    if op == "gate_modulate":
+        r = x * ~live  # padding: hidden is the residual
+        h = r + m * x
+        scale2 = pick(*rows[:-1], (C + 1) // 2, of=(-2, -1, 0, 1)).repeat_interleave(2, -1)[..., :C]
+        m2 = torch.stack([1 + scale2[b].view(G, C)[at[b]] * live[b] for b in range(B)])
+        d[..., 1:C - C % 2:2] = -(d * h)[..., 0:C - C % 2:2] * h[..., 1:C - C % 2:2]
+        if C % 2:
+            d[..., -1] = 0
+        v.update(residual=r, next_weight=torch.ones(C), next_scale=scale2, dhidden=dh)
+        h_grad = dh + d * m2
+        want2 = d * h
+    elif op == "gate":
+        v["residual"] = pick(B, N, C, of=(-1, 0, 1))
+    v["dout"] = d
+    params = ("weight", "cond", "next_weight", "next_scale")
+    v = {k: t.to(F32 if k in params else BF).to(cuda) for k, t in v.items()}
+    v["doc_ids"] = None if docs is None else docs[1].to(cuda)
+    got = _with_grads(op, v, eps=0.0)
+
+    def by_row(t):  # sums over the tokens of each conditioning row
+        out = torch.zeros(B, G + 1, C, dtype=torch.float64)
+        for b in range(B):
+            out[b].index_add_(0, torch.where(ids[b] < 0, G, ids[b]), t[b])
+        return out[:, :G].reshape(rows)
+
+    one = 1 if op == "modulate" else 0
+    want = {"dweight": (h_grad * xhat * (one + m)).sum((0, 1)), "dcond": by_row(h_grad * xhat)}
+    if op == "gate_modulate":
+        want.update(dnext_weight=(want2 * m2).sum((0, 1)), dnext_scale=by_row(want2))
+    for k, t in want.items():
+        bad = (got[k].cpu().double() != t).nonzero()
+        assert not len(bad), (k, len(bad), bad[:3].tolist(), got[k].cpu()[tuple(bad[0])], t[tuple(bad[0])])
