@@ -9,11 +9,12 @@
 ``xhat = x / sqrt(mean(x^2) + eps)`` over the channels; arithmetic in fp32, one rounding
 per output.  ``x`` is ``[B, N, C]`` (or ``[N, C]``), bfloat16 or float16, with any strides
 (channels that are not contiguous are copied).  ``weight`` is ``[C]`` or None; ``scale``
-and ``gate`` have a row per batch item, ``[B, C]``, or with ``doc_ids`` (int32 ``[B, N]``,
+and ``gate`` have a row per batch item, ``[B, C]``, or with ``doc_ids`` (integers ``[B, N]``,
 as :func:`futudiffu_amd.build_doc_ids` makes them) a row per document of a packed
 sequence, ``[B, G, C]``: a token whose id is not in ``0 .. G-1`` (padding) has scale 0 and
-gate 0, and behind a gate its ``x`` is not read.  Parameters are of ``x``'s type or
-float32; chunks of one projection's output are read in place.
+gate 0, and behind a gate its ``x`` is not read (no gate given: 1 for every token).
+Parameters are of ``x``'s type or float32; chunks of one projection's output are read in
+place.
 
 The functions differentiate in reverse mode, once (not the gradients themselves); a
 forward-mode tangent is refused.  Under ``torch.compile``, a tracer, a dispatch mode or
@@ -265,7 +266,7 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
     For the gradient of an activation the forward keeps ``z = x weight^T + bias`` in fp32 (in
     16 bits its rounding, beside that of ``dout * act'(z)``, would nearly double the error of a
     swiglu's gradients); ``dout * act'(z)`` is rounded to ``x``'s type as an operand of the
-    products, and the bias's gradient adds it unrounded.
+    products (in float16 it has to be at most 65504), and the bias's gradient adds it unrounded.
     """
     if torch.compiler.is_compiling():
         keep = activation != "none" and torch.is_grad_enabled() and any(

@@ -476,9 +476,13 @@ __device__ __forceinline__ void order_load() { __builtin_amdgcn_sched_group_barr
 // accumulators; the small one, two workgroups a CU, is for what has too few large tiles.
 // Measured, bf16: 4416 x 11520 x 3840 with the bias 346 us = 1130 TFLOP/s, its dx 332 us =
 // 1177, its dW 356 us = 1097 (transposing reads on both sides); the swiglu of 4416 x 20480 x
-// 3840 570 us = 1220.  The matrix cores bound it at the clock that the power limit leaves: a
-// stage takes the same time with the loads in bursts, with LDS slots a wave and with the
-// next tile's first stages loaded under the epilogue.
+// 3840 570 us = 1220.  Two things bound it.  The clock, which falls with the data's power: the
+// forward's 549 k cycles take 343 us at 1.6 GHz, those of zeros 267 us at 2.1.  And the 27 to 34 %
+// of the cycles in which the matrix cores are idle (busy: 70 %, dx 73, dW 66, swiglu 68): the
+// last, partly filled round, each round's start and epilogue, and the barriers; no LDS bank
+// conflict, 4 to 5 % of the waves' time waits for LDS, memory moves 1.4 to 1.5 TB/s.  A stage
+// takes the same time with the loads in bursts, with LDS slots a wave and with the next tile's
+// first stages loaded under the epilogue.
 template <typename T, bool AK, bool BKC, typename TL>
 __global__ __launch_bounds__(TL::NT, TL::SIMD) void gemm_kernel(GemmArgs a) {
   __shared__ __align__(1024) uint8_t lds[TL::LDS];
@@ -878,11 +882,15 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a0, PackArgs a1, int
 
 // The gradient of z: dz = dout * act'(z) (swiglu: both halves), rounded to T as the products'
 // operand, into rows of `ldz` with zeros behind the last column; with `part` the column sums
-// of the unrounded values over each chunk of rows, for the bias.  A workgroup takes 512
-// columns of a chunk, a wave every fourth row, kRows of them in flight; a lane holds eight
-// consecutive columns (VEC), or every 64th where rows take no 16-byte accesses.  Reads past a
-// row's end give zeros and writes are dropped there, so nothing is behind a branch.  The sums
-// of 4416 x 11520 alone: 102 MB in 27.2 us (four rows in flight: 28.7).
+// of the unrounded values over each chunk of rows, for the bias.  The rounding is the matrix
+// cores' operand type: its remainder as a second operand would double both products.  With it dx
+// and dW are 1.4 times as far from the exact gradients as their own rounding alone puts them
+// (bf16 2.35e-3 for 1.66e-3 of their norm, fp16 2.9e-4 for 2.1e-4); db has its own alone.
+// A workgroup takes 512 columns of a chunk, a wave every fourth row, kRows of them in flight; a
+// lane holds eight consecutive columns (VEC), or every 64th where rows take no 16-byte accesses.
+// Reads past a row's end give zeros and writes are dropped there, so nothing is behind a branch.
+// Memory bounds it: the swiglu of 4416 x 10240 reads dout and z and writes dz, 633 MB in 130 us
+// = 4.9 TB/s; the sums of 4416 x 11520 alone take 102 MB in 27.2 us (four rows in flight: 28.7).
 template <typename T, bool VEC>
 struct Eight {
   typename Vec8<T>::type v;
