@@ -336,3 +336,32 @@ def test_activations_over_the_whole_range(cuda, act):
     o, d = got["out"].float().cpu(), got["dx"].float().cpu()
     assert torch.equal(o.diagonal(), z.clamp_min(0).to(BF).float())
     assert torch.isfinite(d).all() and torch.equal(d.diagonal(), (z > 0).float())
+
+
+@pytest.mark.parametrize("M,K,N,act,dtype", [(333, 501, 389, "silu", FP), (331, 520, 777, "gelu", BF),
+                                             (700, 264, 300, "swiglu", BF), (40, 72, 65, "swiglu", FP),
+                                             (331, 520, 777, "none", BF)])
+def test_gradients_have_one_rounding_more(cuda, M, K, N, act, dtype):
+    """How far dx and dW are from the exact gradients, over all elements: their own rounding and
+    that of dz = dout * act'(z) to the type, nothing else.  Both are computed in 64 bits.  32-bit
+    sums add 2^-24 times the root of their terms (under 1600), under 2^-18 of a value, where a
+    rounding is 2^-12 (fp16) or more, rms: under 2^-12 of it in quadrature.  A dz within that of a
+    tie may round the other way, by as much.  1 % is allowed.  The bias's gradient adds dz
+    unrounded: its own rounding alone."""
+    v = _inputs(M, K, N, act, dtype, dtype, False, seed=M, device=cuda)
+    got = _run(v, act)
+    exact = {k: t[0] for k, t in _want(v, act).items()}
+    x, w, d = (v[k].double() for k in ("x", "weight", "dout"))
+    z = (x @ w.T + v["bias"].double()).requires_grad_()
+    if act == "swiglu":
+        y = torch.nn.functional.silu(z[:, :N]) * z[:, N:]
+    else:
+        y = {"none": lambda t: t, "silu": torch.nn.functional.silu,
+             "gelu": lambda t: torch.nn.functional.gelu(t, approximate="tanh")}[act](z)
+    dz, = torch.autograd.grad(y, z, d)
+    rounded = dz.to(dtype).double()
+    for k, t in (("dx", rounded @ w), ("dweight", rounded.T @ x), ("dbias", dz.sum(0))):
+        want = float((t.to(dtype).double() - exact[k]).norm() / exact[k].norm())
+        off = float((got[k].double() - exact[k]).norm() / exact[k].norm())
+        print(act, dtype, k, f"{off:.4g} expected {want:.4g}", flush=True)
+        assert off <= 1.01 * want, (k, off, want)
