@@ -630,7 +630,12 @@ std::tuple<Tensor, Tensor> rms_norm_gate_residual_modulate(const Tensor& residua
 Tensor fused_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
                     const std::string& activation) {
   if (through_dispatcher({&x, &weight, &some(bias), &some(residual)})) {
-    const bool keep_z = activation != "none" && wants_grad({&x, &weight, &some(bias)});
+    // what vmap batches does not say whether what lies under it wants a gradient: z is kept
+    const bool hidden = x.key_set().has(c10::DispatchKey::FuncTorchBatched) ||
+                        weight.key_set().has(c10::DispatchKey::FuncTorchBatched) ||
+                        some(bias).key_set().has(c10::DispatchKey::FuncTorchBatched);
+    const bool keep_z = activation != "none" && at::GradMode::is_enabled() &&
+                        (hidden || any_requires({&x, &weight, &some(bias)}));
     return call_op("fused_linear", x, weight, bias, residual, activation, keep_z)[0].toTensor();
   }
   if (wants_grad({&x, &weight, &some(bias), &some(residual)}))

@@ -141,3 +141,16 @@ def test_gradients_of_the_ops_are_not_differentiated(cuda, i):
     assert _equal(torch.autograd.grad(outs(), leaves, d), _grads(fn, args, d))
     with pytest.raises(RuntimeError, match="create_graph"):
         torch.autograd.grad(outs(), leaves, d, create_graph=True)
+
+
+@pytest.mark.parametrize("i", OPS)
+def test_gradients_through_vmap(cuda, i):
+    """A gradient that is taken outside of vmap: the samples' own."""
+    name, fn, args = _calls(cuda)[i]
+    for at in range(len(args)):
+        put = lambda t: _outs(fn(*args[:at], t, *args[at + 1:]))  # noqa: E731
+        xs = torch.stack([args[at], 2 * args[at], -args[at]]).requires_grad_()
+        out = torch.vmap(put)(xs)
+        got, = torch.autograd.grad(out, xs, [torch.ones_like(o) for o in out])
+        for s in range(3):
+            assert _equal([got[s]], _grads(put, (xs[s],))), (name, at)
