@@ -8,7 +8,8 @@ Importing this package registers the ``futudiffu_ii::sage_attn_masked``,
 ``futudiffu_ii::sage_bwd_ext`` their autograd formulas call.  ``futudiffu_amd.fused_kernels``
 (imported separately) registers ``futudiffu::fused_qkv_postprocess``.  ``block_ops`` holds
 what surrounds the attention in a transformer block: RMS norms with modulation, gate and
-residual, and linear layers with bias, activation and residual.
+residual, and linear layers with bias, activation and residual; ``mxfp4`` the linear layers over
+weights in 4-bit floating point, and the norms that feed them.
 The compute lives in ``libsage_mi355x.so`` (HIP, built by ``build.py``).
 """
 
@@ -28,6 +29,14 @@ from .block_ops import (  # noqa: F401  (registers the ops around the attention)
     rms_norm_gate_residual,
     rms_norm_gate_residual_modulate,
     rms_norm_modulate,
+)
+from .mxfp4 import (  # noqa: F401  (registers the ops in 4-bit floating point)
+    MXFP4,
+    mxfp4_dequantize,
+    mxfp4_linear,
+    mxfp4_quantize,
+    rms_norm_gate_residual_modulate_mxfp4,
+    rms_norm_modulate_mxfp4,
 )
 from .block_mask import build_block_mask, build_doc_ids  # noqa: F401
 from .sage_attention import (  # noqa: F401

@@ -84,6 +84,20 @@ SIGNATURES = {
     "sage_linear_bwd": (_c.c_int, [
         _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _c.c_int, _c.c_int, _c.c_int, _P, _c.c_size_t, _P, _P,
         _P, _P]),
+    "sage_mxfp4_quantize": (_c.c_int, [_P, _I64, _I64, _I64, _c.c_int, _P, _P, _P]),
+    "sage_mxfp4_dequantize": (_c.c_int, [_P, _P, _I64, _I64, _c.c_int, _P, _P]),
+    "sage_mxfp4_linear_workspace_bytes": (_c.c_size_t, [_I64, _I64, _I64, _c.c_int, _c.c_int, _c.c_int]),
+    "sage_mxfp4_linear": (_c.c_int, [
+        _P, _I64, _P, _P, _P, _P, _P, _c.c_int, _P, _I64, _I64, _I64, _I64, _c.c_int, _c.c_int, _P, _c.c_size_t, _P,
+        _P, _P]),
+    "sage_mxfp4_linear_bwd_workspace_bytes": (_c.c_size_t, [_P, _I64, _I64, _I64, _I64, _c.c_int, _c.c_int]),
+    "sage_mxfp4_linear_bwd": (_c.c_int, [
+        _P, _I64, _P, _P, _P, _I64, _I64, _I64, _c.c_int, _c.c_int, _c.c_int, _P, _c.c_size_t, _P, _P, _P]),
+    "sage_rms_norm_modulate_mxfp4": (_c.c_int, [
+        _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _c.c_int, _c.c_int, _c.c_float, _P, _P, _P]),
+    "sage_rms_norm_gate_residual_modulate_mxfp4": (_c.c_int, [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
+        _c.c_int, _c.c_int, _c.c_float, _P, _P, _P, _P]),
 }
 
 _lock = threading.Lock()

@@ -26,7 +26,7 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 # --phase-timing; never loaded by the product path
 PHASE_LIB_PATH = os.path.join(HERE, "libsage_mi355x_phase.so")
 SOURCES = ["sage_quant.hip", "sage_attn.hip", "sage_mask.hip", "sage_bwd.hip", "sage_capi.hip",
-           "sage_norm.hip", "sage_linear.hip"]
+           "sage_norm.hip", "sage_linear.hip", "sage_mxfp4.hip"]
 # the host side of the block operators: a Python extension over torch's C++ API, which takes
 # the library's entry points from the loaded library
 EXT_SOURCE = "block_ops.cpp"

@@ -26,7 +26,10 @@ typedef std::optional<Tensor> OptTensor;
   X(sage_rms_norm_gate_residual_modulate) X(sage_rms_norm_bwd_workspace_bytes)                              \
   X(sage_rms_norm_modulate_bwd) X(sage_rms_norm_gate_residual_bwd)                                          \
   X(sage_rms_norm_gate_residual_modulate_bwd) X(sage_linear_workspace_bytes) X(sage_linear)                 \
-  X(sage_linear_bwd_workspace_bytes) X(sage_linear_bwd)
+  X(sage_linear_bwd_workspace_bytes) X(sage_linear_bwd)                                                     \
+  X(sage_mxfp4_quantize) X(sage_mxfp4_dequantize) X(sage_mxfp4_linear_workspace_bytes) X(sage_mxfp4_linear) \
+  X(sage_mxfp4_linear_bwd_workspace_bytes) X(sage_mxfp4_linear_bwd) X(sage_rms_norm_modulate_mxfp4)         \
+  X(sage_rms_norm_gate_residual_modulate_mxfp4)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -643,6 +646,8 @@ Tensor fused_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias
   return std::get<0>(linear_forward(x, weight, bias, residual, activation, false));
 }
 
+#include "block_mxfp4.h"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -659,4 +664,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gate_modulate_backward", &gate_modulate_backward);
   m.def("linear_forward", &linear_forward);
   m.def("linear_backward", &linear_backward);
+  m.def("mxfp4_quantize", &mxfp4_quantize);
+  m.def("mxfp4_dequantize", &mxfp4_dequantize);
+  m.def("mxfp4_linear", &mxfp4_linear);
+  m.def("mxfp4_linear_codes", &mxfp4_linear_codes);
+  m.def("rms_norm_modulate_mxfp4", &rms_norm_modulate_mxfp4);
+  m.def("rms_norm_gate_residual_modulate_mxfp4", &rms_norm_gate_residual_modulate_mxfp4);
+  m.def("mx_quantize", &mx_quantize);
+  m.def("mx_dequantize", &mx_dequantize);
+  m.def("mx_linear_forward", &mx_linear_forward);
+  m.def("mx_linear_codes", &mx_linear_codes);
+  m.def("mx_linear_backward", &mx_linear_backward);
+  m.def("mx_modulate", &mx_modulate);
+  m.def("mx_gate_modulate", &mx_gate_modulate);
 }

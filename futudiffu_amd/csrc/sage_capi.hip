@@ -958,8 +958,9 @@ struct LinearBwd {
   // x and weight as rows whose columns the products read 16 bytes at a time
   size_t x_off, w_off;
   bool copy_x, copy_w;
+  // form_w: the weight's rows are formed in the workspace, whatever w is
   LinearBwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs, const void* w, int64_t w_rs, int64_t m,
-            int64_t n, int64_t k, int act, int want) {
+            int64_t n, int64_t k, int act, int want, bool form_w = false) {
     rows = act == SAGE_ACT_SWIGLU ? 2 * n : n;
     const bool products = want & 3;
     form_dz = products && (act != SAGE_ACT_NONE || !in_place(dout, d_rs, m, n));
@@ -974,7 +975,7 @@ struct LinearBwd {
     sum_off = at;
     if (want & 4) at += up256((size_t)(chunks * rows) * 4);
     copy_x = (want & 2) && !in_place(x, x_rs, m, k);
-    copy_w = (want & 1) && !in_place(w, w_rs, rows, k);
+    copy_w = (want & 1) && (form_w || !in_place(w, w_rs, rows, k));
     x_off = at;
     if (copy_x) at += up256((size_t)(m * up8(k)) * 2);
     w_off = at;
@@ -1006,6 +1007,66 @@ struct LinearBwd {
     bytes = at + up256(part);
   }
 };
+
+// The backward's launches.  w_codes (with w_scales): the weight is MXFP4, and its rows are formed
+// in the workspace; else `weight` is read or copied.
+int run_linear_bwd(const LinearBwd& plan, const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
+                   const void* weight, int64_t w_rs, const uint8_t* w_codes, const uint8_t* w_scales, const float* z,
+                   int64_t m, int64_t n, int64_t k, int dtype, int activation, int bias_fp32, void* workspace,
+                   size_t workspace_bytes, void* dx, void* dweight, void* dbias, hipStream_t stream) {
+  LinearBwd p = plan;
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes))
+    return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu", p.bytes, workspace_bytes);
+  if (p.bytes && !aligned16(workspace)) return fail(SAGE_ERR_ALIGN, "workspace must be 16-byte aligned");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (p.form_dz || dbias) {
+    sage::DactArgs d{};
+    d.dout = dout;
+    d.z = z;
+    d.ldd = m == 1 ? n : d_rs;
+    d.m = m;
+    d.n = (int)n;
+    d.act = activation;
+    d.dz = p.form_dz ? ws + p.dz_off : nullptr;
+    d.ldz = p.ldz;
+    d.vec = in_place(dout, d_rs, m, n) && aligned16(z);
+    d.part = dbias ? reinterpret_cast<float*>(ws + p.sum_off) : nullptr;
+    d.chunks = p.chunks;
+    d.chunk = p.chunk;
+    d.dbias = dbias;
+    d.bias_f32 = bias_fp32 != 0;
+    const hipError_t e = sage::launch_dact(dtype, d, stream);
+    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (activation)");
+  }
+  const void* dz = p.form_dz ? ws + p.dz_off : dout;
+  if (dx && w_codes) {
+    const sage::MxDequantArgs q{w_codes, w_scales,      p.rows, (int)up8(k), (int)sage::mx_cols(k),
+                                ws + p.w_off, up8(k), 1};
+    const hipError_t e = sage::launch_mx_dequantize(q, dtype, stream);
+    if (e != hipSuccess) return launch_status(e, "sage_mxfp4_linear_bwd (weight)");
+  } else if (p.copy_x || p.copy_w) {
+    const hipError_t e = sage::launch_pack({p.copy_x ? x : nullptr, x_rs, m, k, ws + p.x_off, up8(k)},
+                                           {p.copy_w ? weight : nullptr, w_rs, p.rows, k, ws + p.w_off, up8(k)}, stream);
+    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (copy)");
+  }
+  if (dx) {
+    p.gx.a = dz;
+    p.gx.b = p.copy_w ? ws + p.w_off : weight;
+    p.gx.out = dx;
+    p.gx.part = reinterpret_cast<float*>(ws + p.part_off);
+    const hipError_t e = sage::launch_gemm(p.gx, dtype, stream);
+    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (dx)");
+  }
+  if (dweight) {
+    p.gw.a = dz;
+    p.gw.b = p.copy_x ? ws + p.x_off : x;
+    p.gw.out = dweight;
+    p.gw.part = reinterpret_cast<float*>(ws + p.part_off);
+    const hipError_t e = sage::launch_gemm(p.gw, dtype, stream);
+    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (dweight)");
+  }
+  return launch_status(hipSuccess, "sage_linear_bwd");
+}
 
 }  // namespace
 
@@ -1090,53 +1151,199 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
   if (reinterpret_cast<uintptr_t>(dbias) & (bias_fp32 ? 3u : 1u))
     return fail(SAGE_ERR_ALIGN, "dbias must be aligned to its elements");
   if (!aligned16(dx) || !aligned16(dweight)) return fail(SAGE_ERR_ALIGN, "dx and dweight must be 16-byte aligned");
-  LinearBwd p(dout, d_rs, x, x_rs, weight, w_rs, m, n, k, activation, want);
-  if (p.bytes && (!workspace || workspace_bytes < p.bytes))
-    return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu", p.bytes, workspace_bytes);
-  if (p.bytes && !aligned16(workspace)) return fail(SAGE_ERR_ALIGN, "workspace must be 16-byte aligned");
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if (p.form_dz || dbias) {
-    sage::DactArgs d{};
-    d.dout = dout;
-    d.z = z;
-    d.ldd = m == 1 ? n : d_rs;
-    d.m = m;
-    d.n = (int)n;
-    d.act = activation;
-    d.dz = p.form_dz ? ws + p.dz_off : nullptr;
-    d.ldz = p.ldz;
-    d.vec = in_place(dout, d_rs, m, n) && aligned16(z);
-    d.part = dbias ? reinterpret_cast<float*>(ws + p.sum_off) : nullptr;
-    d.chunks = p.chunks;
-    d.chunk = p.chunk;
-    d.dbias = dbias;
-    d.bias_f32 = bias_fp32 != 0;
-    const hipError_t e = sage::launch_dact(dtype, d, stream);
-    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (activation)");
+  const LinearBwd p(dout, d_rs, x, x_rs, weight, w_rs, m, n, k, activation, want);
+  return run_linear_bwd(p, dout, d_rs, x, x_rs, weight, w_rs, nullptr, nullptr, z, m, n, k, dtype, activation, bias_fp32,
+                        workspace, workspace_bytes, dx, dweight, dbias, stream);
+}
+
+}  // extern "C"
+
+namespace {
+
+// ---- MXFP4
+
+int check_mx_rows(int64_t m, int64_t k, int dtype, const void* codes, const void* scales) {
+  if (m <= 0 || k <= 0) return fail(SAGE_ERR_ARG, "m=%lld and k=%lld must be positive", (long long)m, (long long)k);
+  if (m >= (int64_t)1 << 24 || k >= (int64_t)1 << 22)
+    return fail(SAGE_ERR_ARG, "m=%lld or k=%lld exceeds 2^24, 2^22", (long long)m, (long long)k);
+  if (dtype != SAGE_DTYPE_BF16 && dtype != SAGE_DTYPE_FP16) return fail(SAGE_ERR_ARG, "unknown dtype %d", dtype);
+  if (!codes || !scales) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  if (!aligned16(codes) || reinterpret_cast<uintptr_t>(scales) & 7u)
+    return fail(SAGE_ERR_ALIGN, "codes must be 16-byte and scales 8-byte aligned");
+  return SAGE_OK;
+}
+
+int check_mx_linear(int64_t m, int64_t n, int64_t k, int dtype, int activation) {
+  if (m <= 0 || n <= 0 || k <= 0)
+    return fail(SAGE_ERR_ARG, "m=%lld, n=%lld and k=%lld must be positive", (long long)m, (long long)n, (long long)k);
+  if (activation < SAGE_ACT_NONE || activation > SAGE_ACT_SWIGLU)
+    return fail(SAGE_ERR_ARG, "unknown activation %d", activation);
+  if (dtype != SAGE_DTYPE_BF16 && dtype != SAGE_DTYPE_FP16) return fail(SAGE_ERR_ARG, "unknown dtype %d", dtype);
+  if (m >= (int64_t)1 << 24 || n >= (int64_t)1 << 22 || k >= (int64_t)1 << 22)
+    return fail(SAGE_ERR_ARG, "m=%lld, n=%lld or k=%lld exceeds 2^24, 2^22, 2^22", (long long)m, (long long)n,
+                (long long)k);
+  const int64_t rows = activation == SAGE_ACT_SWIGLU ? 2 * n : n;
+  if (rows >= (int64_t)1 << 22)
+    return fail(SAGE_ERR_ARG, "a weight of %lld rows, 2^22 or more", (long long)rows);
+  if (rows * (sage::mx_cols(k) / 2) >= (int64_t)1 << 31)
+    return fail(SAGE_ERR_ARG, "a weight of %lld x %lld has 2^31 bytes of codes or more", (long long)rows, (long long)k);
+  return SAGE_OK;
+}
+
+// Codes and scales of x in the workspace, and what follows them.
+struct MxLinear {
+  size_t scales, part;
+  sage::GemmArgs g{};
+  MxLinear(int64_t m, int64_t n, int64_t k, int act, bool quantize, bool vec) {
+    const int64_t kp = sage::mx_cols(k);
+    scales = quantize ? up256((size_t)m * (kp / 2)) : 0;
+    part = quantize ? scales + up256((size_t)m * (kp / 32)) : 0;
+    g.vec = vec;
+    g.m = m;
+    g.n = (int)n;
+    g.k = g.kv = g.lda = g.ldb = kp / 4;
+    g.a_kc = g.b_kc = 1;
+    g.act = act;
+    sage::mx_gemm_plan(g);
   }
-  const void* dz = p.form_dz ? ws + p.dz_off : dout;
-  if (p.copy_x || p.copy_w) {
-    const hipError_t e = sage::launch_pack({p.copy_x ? x : nullptr, x_rs, m, k, ws + p.x_off, up8(k)},
-                                           {p.copy_w ? weight : nullptr, w_rs, rows, k, ws + p.w_off, up8(k)}, stream);
-    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (copy)");
+  size_t bytes() const { return part + (size_t)g.part_floats * 4; }
+};
+
+}  // namespace
+
+extern "C" {
+
+int sage_mxfp4_quantize(const void* x, int64_t x_rs, int64_t m, int64_t k, int dtype, void* codes, void* scales,
+                        hipStream_t stream) {
+  if (const int e = check_mx_rows(m, k, dtype, codes, scales)) return e;
+  if (!x) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  if (reinterpret_cast<uintptr_t>(x) & 1u) return fail(SAGE_ERR_ALIGN, "x must be aligned to its elements");
+  const sage::MxQuantArgs a{x, m == 1 ? k : x_rs, m, (int)k, (int)sage::mx_cols(k), in_place(x, x_rs, m, k),
+                            static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales)};
+  return launch_status(sage::launch_mx_quantize(a, dtype, stream), "sage_mxfp4_quantize");
+}
+
+int sage_mxfp4_dequantize(const void* codes, const void* scales, int64_t m, int64_t k, int dtype, void* out,
+                          hipStream_t stream) {
+  if (const int e = check_mx_rows(m, k, dtype, codes, scales)) return e;
+  if (!out) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  if (reinterpret_cast<uintptr_t>(out) & 1u) return fail(SAGE_ERR_ALIGN, "out must be aligned to its elements");
+  const sage::MxDequantArgs a{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), m, (int)k,
+                              (int)sage::mx_cols(k), out, k, aligned16(out) && k % 8 == 0};
+  return launch_status(sage::launch_mx_dequantize(a, dtype, stream), "sage_mxfp4_dequantize");
+}
+
+size_t sage_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int activation, int quantize_x,
+                                         int other_rows) {
+  if (check_mx_linear(m, n, k, SAGE_DTYPE_BF16, activation)) return 0;
+  // outputs, residual and bias on 16-byte boundaries or not: room for either
+  return std::max(MxLinear(m, n, k, activation, quantize_x, n % 8 == 0).bytes(),
+                  other_rows ? MxLinear(m, n, k, activation, quantize_x, false).bytes() : 0);
+}
+
+int sage_mxfp4_linear(const void* x, int64_t x_rs, const void* x_codes, const void* x_scales, const void* w_codes,
+                      const void* w_scales, const void* bias, int bias_fp32, const void* residual, int64_t r_rs,
+                      int64_t m, int64_t n, int64_t k, int dtype, int activation, void* workspace,
+                      size_t workspace_bytes, float* z, void* out, hipStream_t stream) {
+  if (const int e = check_mx_linear(m, n, k, dtype, activation)) return e;
+  if (!out || !w_codes || !w_scales || (!x && (!x_codes || !x_scales)))
+    return fail(SAGE_ERR_ARG, "null tensor pointer");
+  if (residual)
+    if (const int e = check_rows(r_rs, m, n, "residual")) return e;
+  for (const void* p : {x, residual, (const void*)out})
+    if (reinterpret_cast<uintptr_t>(p) & 1u) return fail(SAGE_ERR_ALIGN, "tensor pointers must be aligned to their elements");
+  if (reinterpret_cast<uintptr_t>(z) & 3u || reinterpret_cast<uintptr_t>(bias) & (bias_fp32 ? 3u : 1u))
+    return fail(SAGE_ERR_ALIGN, "bias must be aligned to its elements, z to 4 bytes");
+  if (!aligned16(w_codes) || reinterpret_cast<uintptr_t>(w_scales) & 7u ||
+      (!x && (!aligned16(x_codes) || reinterpret_cast<uintptr_t>(x_scales) & 7u)))
+    return fail(SAGE_ERR_ALIGN, "codes must be 16-byte and scales 8-byte aligned");
+  const bool vec = n % 8 == 0 && aligned16(out) && aligned16(z) && aligned16(bias) && aligned16(residual) &&
+                   (!residual || m == 1 || r_rs % 8 == 0);
+  MxLinear p(m, n, k, activation, x != nullptr, vec);
+  if (p.bytes() && (!workspace || workspace_bytes < p.bytes()))
+    return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu", p.bytes(), workspace_bytes);
+  if (p.bytes() && !aligned16(workspace)) return fail(SAGE_ERR_ALIGN, "workspace must be 16-byte aligned");
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  if (x) {
+    const int e = sage_mxfp4_quantize(x, x_rs, m, k, dtype, ws, ws + p.scales, stream);
+    if (e) return e;
   }
-  if (dx) {
-    p.gx.a = dz;
-    p.gx.b = p.copy_w ? ws + p.w_off : weight;
-    p.gx.out = dx;
-    p.gx.part = reinterpret_cast<float*>(ws + p.part_off);
-    const hipError_t e = sage::launch_gemm(p.gx, dtype, stream);
-    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (dx)");
-  }
-  if (dweight) {
-    p.gw.a = dz;
-    p.gw.b = p.copy_x ? ws + p.x_off : x;
-    p.gw.out = dweight;
-    p.gw.part = reinterpret_cast<float*>(ws + p.part_off);
-    const hipError_t e = sage::launch_gemm(p.gw, dtype, stream);
-    if (e != hipSuccess) return launch_status(e, "sage_linear_bwd (dweight)");
-  }
-  return launch_status(hipSuccess, "sage_linear_bwd");
+  sage::MxGemmArgs a{};
+  a.g = p.g;
+  a.g.a = x ? ws : x_codes;
+  a.g.b = w_codes;
+  a.sa = x ? ws + p.scales : static_cast<const uint8_t*>(x_scales);
+  a.sb = static_cast<const uint8_t*>(w_scales);
+  a.g.bias = bias;
+  a.g.bias_f32 = bias_fp32 != 0;
+  a.g.res = residual;
+  a.g.ldr = m == 1 ? n : r_rs;
+  a.g.z = z;
+  a.g.out = out;
+  a.g.part = reinterpret_cast<float*>(ws + p.part);
+  return launch_status(sage::launch_mx_gemm(a, dtype, stream), "sage_mxfp4_linear");
+}
+
+size_t sage_mxfp4_linear_bwd_workspace_bytes(const void* dout, int64_t d_rs, int64_t m, int64_t n, int64_t k,
+                                             int activation, int want) {
+  if (check_mx_linear(m, n, k, SAGE_DTYPE_BF16, activation)) return 0;
+  return LinearBwd(dout, d_rs, nullptr, 0, nullptr, 0, m, n, k, activation, want & 5, true).bytes;
+}
+
+int sage_mxfp4_linear_bwd(const void* dout, int64_t d_rs, const void* w_codes, const void* w_scales, const float* z,
+                          int64_t m, int64_t n, int64_t k, int dtype, int activation, int bias_fp32, void* workspace,
+                          size_t workspace_bytes, void* dx, void* dbias, hipStream_t stream) {
+  if (const int e = check_mx_linear(m, n, k, dtype, activation)) return e;
+  if (const int e = check_linear(m, n, k, 0, dtype, activation)) return e;  // the weight's 16-bit rows
+  const int want = (dx ? 1 : 0) | (dbias ? 4 : 0);
+  if (!dout || (dx && (!w_codes || !w_scales)) || (activation != SAGE_ACT_NONE && !z))
+    return fail(SAGE_ERR_ARG, "null tensor pointer");
+  if (!want) return SAGE_OK;
+  if (const int e = check_rows(d_rs, m, n, "dout")) return e;
+  if (reinterpret_cast<uintptr_t>(z) & 3u) return fail(SAGE_ERR_ALIGN, "z must be aligned to 4 bytes");
+  if (reinterpret_cast<uintptr_t>(dout) & 1u || reinterpret_cast<uintptr_t>(dbias) & (bias_fp32 ? 3u : 1u))
+    return fail(SAGE_ERR_ALIGN, "tensor pointers must be aligned to their elements");
+  if (!aligned16(dx) || !aligned16(w_codes) || reinterpret_cast<uintptr_t>(w_scales) & 7u)
+    return fail(SAGE_ERR_ALIGN, "dx and codes must be 16-byte and scales 8-byte aligned");
+  const LinearBwd p(dout, d_rs, nullptr, 0, nullptr, 0, m, n, k, activation, want, true);
+  return run_linear_bwd(p, dout, d_rs, nullptr, 0, nullptr, 0, static_cast<const uint8_t*>(w_codes),
+                        static_cast<const uint8_t*>(w_scales), z, m, n, k, dtype, activation, bias_fp32, workspace,
+                        workspace_bytes, dx, nullptr, dbias, stream);
+}
+
+int sage_rms_norm_modulate_mxfp4(const void* x, int64_t x_bs, int64_t x_rs, const void* weight, const void* scale,
+                                 int64_t scale_bs, int64_t scale_gs, int64_t groups, const int32_t* doc_ids, int64_t b,
+                                 int64_t n, int64_t c, int dtype, int fp32_params, float eps, void* codes,
+                                 void* scales, hipStream_t stream) {
+  sage::NormArgs a = norm_args(x, x_bs, x_rs, weight, scale, scale_bs, scale_gs, groups, doc_ids, b, n, c,
+                               fp32_params, eps);
+  if (const int e = check_norm(a, b, n, c, groups, dtype, fp32_params)) return e;
+  if (!x) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  if (const int e = check_norm_align(a)) return e;
+  if (const int e = check_mx_rows(b * n, c, dtype, codes, scales)) return e;
+  return launch_status(sage::launch_norm_mx(sage::kNormModulate, dtype, a, static_cast<uint8_t*>(codes),
+                                            static_cast<uint8_t*>(scales), stream),
+                       "sage_rms_norm_modulate_mxfp4");
+}
+
+int sage_rms_norm_gate_residual_modulate_mxfp4(
+    const void* residual, int64_t r_bs, int64_t r_rs, const void* x, int64_t x_bs, int64_t x_rs, const void* weight,
+    const void* gate, int64_t gate_bs, int64_t gate_gs, const void* next_weight, const void* next_scale,
+    int64_t scale_bs, int64_t scale_gs, int64_t groups, const int32_t* doc_ids, int64_t b, int64_t n, int64_t c,
+    int dtype, int fp32_params, float eps, void* hidden, void* codes, void* scales, hipStream_t stream) {
+  sage::NormArgs a = norm_args(x, x_bs, x_rs, weight, gate, gate_bs, gate_gs, groups, doc_ids, b, n, c, fp32_params,
+                               eps);
+  if (const int e = check_norm(a, b, n, c, groups, dtype, fp32_params)) return e;
+  if (!residual || !x || !hidden) return fail(SAGE_ERR_ARG, "null tensor pointer");
+  a.res = {residual, r_bs, r_rs};
+  a.w2 = {next_weight, fp32_params & SAGE_FP32_NEXT_WEIGHT ? 1 : 0};
+  a.cond2 = {next_scale, fp32_params & SAGE_FP32_NEXT_SCALE ? 1 : 0, (int)groups, scale_bs, scale_gs};
+  a.hidden = hidden;
+  if (const int e = check_norm_align(a)) return e;
+  if (const int e = check_mx_rows(b * n, c, dtype, codes, scales)) return e;
+  return launch_status(sage::launch_norm_mx(sage::kNormGateModulate, dtype, a, static_cast<uint8_t*>(codes),
+                                            static_cast<uint8_t*>(scales), stream),
+                       "sage_rms_norm_gate_residual_modulate_mxfp4");
 }
 
 }  // extern "C"

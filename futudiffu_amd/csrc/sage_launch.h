@@ -362,6 +362,8 @@ struct NormChunks {
 };
 NormChunks norm_chunks(int64_t b, int64_t n, int64_t c, int64_t groups, bool doc);
 hipError_t launch_norm_fwd(int op, int f16, const NormArgs& a, hipStream_t st);
+// kNormModulate or kNormGateModulate with the modulated output in MXFP4 in the place of `out`
+hipError_t launch_norm_mx(int op, int f16, const NormArgs& a, uint8_t* codes, uint8_t* scales, hipStream_t st);
 hipError_t launch_norm_bwd(int op, int f16, const NormArgs& a, hipStream_t st);
 
 // Linear layers (sage_linear.hip).
@@ -414,5 +416,33 @@ struct DactArgs {
   int bias_f32;
 };
 hipError_t launch_dact(int f16, const DactArgs& a, hipStream_t st);
+
+// MXFP4 (sage_mxfp4.hip): codes [m][kp / 2] with the scales [kp / 256][m][8], kp = mx_cols(k).
+inline int64_t mx_cols(int64_t k) { return (k + 255) / 256 * 256; }
+struct MxQuantArgs {
+  const void* x;  // rows of 16-bit elements, ldx apart
+  int64_t ldx, m;
+  int k, kp;
+  int vec;  // rows take 16-byte accesses
+  uint8_t *codes, *scales;
+};
+struct MxDequantArgs {
+  const uint8_t *codes, *scales;
+  int64_t m;
+  int k, kp;
+  void* out;  // rows of 16-bit elements, ldo apart
+  int64_t ldo;
+  int vec;
+};
+// The product of two MXFP4 operands: g.a, g.b, g.lda, g.ldb and g.k count 16-bit units of four
+// codes; scales of A (g.m rows) and of B (g.n, or 2 g.n rows for a swiglu).
+struct MxGemmArgs {
+  GemmArgs g;
+  const uint8_t *sa, *sb;
+};
+void mx_gemm_plan(GemmArgs& a);
+hipError_t launch_mx_gemm(const MxGemmArgs& a, int f16, hipStream_t st);
+hipError_t launch_mx_quantize(const MxQuantArgs& a, int f16, hipStream_t st);
+hipError_t launch_mx_dequantize(const MxDequantArgs& a, int f16, hipStream_t st);
 
 }  // namespace sage

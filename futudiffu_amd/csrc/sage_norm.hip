@@ -26,6 +26,7 @@
 
 #include "sage_common.h"
 #include "sage_launch.h"
+#include "sage_mx.h"
 
 namespace sage {
 
@@ -246,6 +247,204 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(NormArg
     for (int j = 0; j < kPer; ++j) y[j] = y[j] * r2 * wm2[j];
   }
   if (live) store_row<T, TPR, VEC>(static_cast<T*>(a.out) + row * a.c, t, c, y);
+}
+
+// ---------------------------------------------------------------- norms into MXFP4
+
+// A thread's channels of a row of E for the quantization: two runs of eight whatever the access, so
+// that a block of 32 is four neighbouring lanes'.
+template <typename E, int TPR, bool VEC>
+__device__ __forceinline__ void load_runs(const E* row, int t, int c, float (&f)[kPer]) {
+  const __amdgpu_buffer_rsrc_t rs = raw_rsrc(row, (uint32_t)c * (uint32_t)sizeof(E));
+#pragma unroll
+  for (int i = 0; i < kPer / kVec; ++i) {
+    const int at = (i * TPR + t) * kVec;
+    if constexpr (VEC && sizeof(E) == 2) {
+      const auto v = __builtin_bit_cast(typename Vec8<E>::type, __builtin_amdgcn_raw_buffer_load_b128(rs, at * 2, 0, 0));
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) f[i * kVec + j] = (float)v[j];
+    } else if constexpr (VEC) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at * 4 + q * 16, 0, 0));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[i * kVec + q * 4 + j] = v[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        if constexpr (sizeof(E) == 2)
+          f[i * kVec + j] = (float)__builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b16(rs, (at + j) * 2, 0, 0));
+        else
+          f[i * kVec + j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, (at + j) * 4, 0, 0));
+      }
+    }
+  }
+}
+
+template <typename T, int TPR, bool VEC>
+__device__ __forceinline__ void param_runs(const void* p, bool f32, int64_t off, int t, int c, float fill,
+                                           float (&f)[kPer]) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) f[j] = fill;
+  } else if (f32) {
+    load_runs<float, TPR, VEC>(static_cast<const float*>(p) + off, t, c, f);
+  } else {
+    load_runs<T, TPR, VEC>(static_cast<const T*>(p) + off, t, c, f);
+  }
+}
+
+// scale or gate of conditioning row `id` (weight_row's rule).
+template <typename T, int TPR, bool VEC>
+__device__ __forceinline__ void cond_runs(const NormCond& k, bool scale, int b, int id, int t, int c, float (&f)[kPer]) {
+  const bool live = k.p && id >= 0 && id < k.groups;
+  param_runs<T, TPR, VEC>(live ? k.p : nullptr, k.f32, b * k.bs + id * k.gs, t, c, scale || k.p ? 0.0f : 1.0f, f);
+}
+
+// wave_sum of fp64 values.
+__device__ __forceinline__ double wave_sum64(double v) {
+  auto moved = [](double x, auto move) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(double, (uint64_t)move((uint32_t)(u >> 32)) << 32 | move((uint32_t)u));
+  };
+  auto dpp = [&](double x, auto ctrl) {
+    return moved(x, [](uint32_t w) {
+      return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, decltype(ctrl)::value, 0xf, 0xf, true);
+    });
+  };
+  v += dpp(v, std::integral_constant<int, 0xb1>{});
+  v += dpp(v, std::integral_constant<int, 0x4e>{});
+  v += dpp(v, std::integral_constant<int, 0x141>{});
+  v += dpp(v, std::integral_constant<int, 0x140>{});
+  const bool up16 = threadIdx.x & 16, up32 = threadIdx.x & 32;
+  v += moved(v, [&](uint32_t w) {
+    const auto s = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    return up16 ? s[0] : s[1];
+  });
+  v += moved(v, [&](uint32_t w) {
+    const auto s = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return up32 ? s[0] : s[1];
+  });
+  return v;
+}
+
+// token_sum of one fp64 value.
+template <int TPR>
+__device__ __forceinline__ double token_sum64(double v, double* red, int wave) {
+  v = wave_sum64(v);
+  if constexpr (TPR > 64) {
+    constexpr int W = TPR / 64;
+    if ((threadIdx.x & 63) == 0) red[wave] = v;
+    __syncthreads();
+    const int w0 = wave / W * W;
+    v = red[w0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) v += red[w0 + w];
+  }
+  return v;
+}
+
+__device__ __forceinline__ double rrms64(double sum_sq, int c, float eps) {
+  return 1.0 / sqrt(sum_sq / (double)c + (double)eps);
+}
+
+// fp64 to fp32 by rounding to odd: what lies beside a border between two codes stays on its
+// side when the codes are taken from the fp32 value.
+__device__ __forceinline__ float to_odd(double y) {
+  const float f = (float)y;
+  const double d = y - (double)f;
+  const bool past = (d < 0.0) == (f > 0.0);  // the rounding went away from zero
+  uint32_t u = __float_as_uint(f);
+  if (d != 0.0 && d == d) u = (u - (past ? 1u : 0u)) | 1u;  // d is NaN where y is, or infinite
+  return __uint_as_float(u);
+}
+
+// Forward of the modulated norms with y in MXFP4: norm_fwd_kernel's shares.  Sums, and all
+// that lies between them and the codes, are fp64: fp32 would put one value in 10^6 on the other side
+// of a border between two codes, a whole step away.
+template <typename T, int OP, int TPR, bool VEC>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_mx_kernel(NormArgs a, uint8_t* codes, uint8_t* scales) {
+  constexpr int NT = TPR > 256 ? TPR : 256;
+  constexpr int TOK = NT / TPR;
+  __shared__ double red[NT / 64], red2[NT / 64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * TOK + wave / (TPR / 64), rows = (int64_t)a.b * a.n;
+  const bool live = row < rows;  // a thread group past the last token takes part in the barriers alone
+  const int b = live ? (int)(row / a.n) : 0;
+  const int64_t n = live ? row - (int64_t)b * a.n : 0;
+  const int c = live ? a.c : 0;
+  const int id = a.doc && live ? load_uniform(a.doc, row) : 0;
+  const bool gated = OP == kNormModulate || !no_document(a, id);
+  float x[kPer], r[kPer], w[kPer], k[kPer], w2[kPer], k2[kPer];
+  load_runs<T, TPR, VEC>(row_of<T>(a.x, b, n), t, gated ? c : 0, x);
+  if constexpr (OP == kNormGateModulate) load_runs<T, TPR, VEC>(row_of<T>(a.res, b, n), t, c, r);
+  param_runs<T, TPR, VEC>(a.w.p, a.w.f32, 0, t, c, 1.0f, w);
+  cond_runs<T, TPR, VEC>(a.cond, OP == kNormModulate, b, id, t, c, k);
+  if constexpr (OP == kNormGateModulate) {
+    param_runs<T, TPR, VEC>(a.w2.p, a.w2.f32, 0, t, c, 1.0f, w2);
+    cond_runs<T, TPR, VEC>(a.cond2, true, b, id, t, c, k2);
+  }
+  double s = 0.0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) s = fma((double)x[j], (double)x[j], s);
+  s = token_sum64<TPR>(s, red, wave);
+  const double rr = gated ? rrms64(s, a.c, a.eps) : 0.0;
+  double y[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const double m = OP == kNormModulate ? 1.0 + (double)k[j] : (double)k[j];
+    y[j] = (double)x[j] * rr * (double)w[j] * m;
+  }
+  if constexpr (OP == kNormGateModulate) {
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(static_cast<T*>(a.hidden) + row * a.c, (uint32_t)c * 2);
+    s = 0.0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      y[j] += (double)r[j];
+      s = fma(y[j], y[j], s);
+    }
+#pragma unroll
+    for (int i = 0; i < kPer / kVec; ++i) {
+      typename Vec8<T>::type o;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) o[j] = (T)to_odd(y[i * kVec + j]);
+      const int at = (i * TPR + t) * kVec;
+      if constexpr (VEC) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rs, at * 2, 0, 0);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (T)o[j]), rs, (at + j) * 2, 0, 0);
+      }
+    }
+    s = token_sum64<TPR>(s, red2, wave);
+    const double r2 = rrms64(s, a.c, a.eps);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) y[j] = y[j] * r2 * (double)w2[j] * (1.0 + (double)k2[j]);
+  }
+  const int kp = (a.c + 255) / 256 * 256;
+#pragma unroll
+  for (int i = 0; i < kPer / kVec; ++i) {
+    const int at = (i * TPR + t) * kVec;
+    float f[kVec];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      f[j] = at + j < a.c ? to_odd(y[i * kVec + j]) : 0.0f;
+      top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+    }
+    const int e = block_exponent(quad_max(top));
+    const float sc = scale_of(e);
+    uint32_t q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0], f[1], sc, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[2], f[3], sc, 1);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[4], f[5], sc, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[6], f[7], sc, 3);
+    if (live && at < kp) {
+      *reinterpret_cast<uint32_t*>(codes + row * (kp / 2) + at / 2) = e == 255 ? 0u : q;
+      if ((t & 3) == 0) scales[((int64_t)(at >> 8) * rows + row) * 8 + (at >> 5 & 7)] = (uint8_t)e;
+    }
+  }
 }
 
 constexpr int kBwdNT = 512;  // threads of a backward workgroup; also the most tokens of its chunk
@@ -682,6 +881,22 @@ hipError_t bwd(const NormArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <typename T, int OP, int TPR>
+hipError_t fwd_mx(const NormArgs& a, uint8_t* codes, uint8_t* scales, hipStream_t st) {
+  constexpr int NT = TPR > 256 ? TPR : 256, TOK = NT / TPR;
+  const uint32_t grid = (uint32_t)(((int64_t)a.b * a.n + TOK - 1) / TOK);
+  if (all_vec(a)) norm_mx_kernel<T, OP, TPR, true><<<grid, NT, 0, st>>>(a, codes, scales);
+  else norm_mx_kernel<T, OP, TPR, false><<<grid, NT, 0, st>>>(a, codes, scales);
+  return hipGetLastError();
+}
+
+template <typename T, int OP>
+hipError_t mx_width(const NormArgs& a, uint8_t* codes, uint8_t* scales, hipStream_t st) {
+  if (a.c <= 64 * kPer) return fwd_mx<T, OP, 64>(a, codes, scales, st);
+  if (a.c <= 256 * kPer) return fwd_mx<T, OP, 256>(a, codes, scales, st);
+  return fwd_mx<T, OP, 512>(a, codes, scales, st);
+}
+
 template <bool BWD, typename T, int OP, int TPR>
 hipError_t pick_vec(const NormArgs& a, hipStream_t st) {
   if (all_vec(a)) return BWD ? bwd<T, OP, TPR, true>(a, st) : fwd<T, OP, TPR, true>(a, st);
@@ -720,6 +935,14 @@ NormChunks norm_chunks(int64_t b, int64_t n, int64_t c, int64_t groups, bool doc
 
 hipError_t launch_norm_fwd(int op, int f16, const NormArgs& a, hipStream_t st) {
   return f16 ? pick_op<false, _Float16>(op, a, st) : pick_op<false, __bf16>(op, a, st);
+}
+
+hipError_t launch_norm_mx(int op, int f16, const NormArgs& a, uint8_t* codes, uint8_t* scales, hipStream_t st) {
+  if (op == kNormModulate)
+    return f16 ? mx_width<_Float16, kNormModulate>(a, codes, scales, st)
+               : mx_width<__bf16, kNormModulate>(a, codes, scales, st);
+  return f16 ? mx_width<_Float16, kNormGateModulate>(a, codes, scales, st)
+             : mx_width<__bf16, kNormGateModulate>(a, codes, scales, st);
 }
 
 hipError_t launch_norm_bwd(int op, int f16, const NormArgs& a, hipStream_t st) {

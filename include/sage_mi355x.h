@@ -518,6 +518,71 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
                     void* workspace, size_t workspace_bytes, void* dx, void* dweight, void* dbias,
                     hipStream_t stream);
 
+/* ---- Microscaled 4-bit floating point (MXFP4) -----------------------------------
+ *
+ * Rows [m][k] in blocks of 32 columns: a block has a scale 2^e, a column a 4-bit code (e2m1,
+ * sign first: +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}) times it.
+ *   codes        [m][kp / 2] bytes, kp = k rounded up to 256: the even column in the low half
+ *                of its byte, zeros behind column k.  16-byte aligned.
+ *   scales       [kp / 256][m][8] bytes e + 127: scales[g][r][i] of row r's columns
+ *                256 g + 32 i .. + 31; 255: the block is NaN.  8-byte aligned.
+ * Quantizing takes e = max(floor(log2 amax) - 2, -127) of a block's largest magnitude amax and
+ * the nearest code of x / 2^e, ties to the even code, past 6 the code of 6; a block that holds NaN
+ * or an infinity becomes NaN.  Exact in every step but the rounding.
+ * m at least 1 and below 2^24, k at least 1 and below 2^22. */
+
+/* x: 16-bit rows x_rs elements apart, columns contiguous. */
+int sage_mxfp4_quantize(const void* x, int64_t x_rs, int64_t m, int64_t k, int dtype, void* codes, void* scales,
+                        hipStream_t stream);
+
+/* out: [m][k] contiguous; what the codes stand for, in fp16 rounded where it is subnormal there
+ * and infinite past 65504. */
+int sage_mxfp4_dequantize(const void* codes, const void* scales, int64_t m, int64_t k, int dtype, void* out,
+                          hipStream_t stream);
+
+/* out = act(q(x) weight^T + bias) + residual as sage_linear, both operands MXFP4, fp32
+ * accumulation, one rounding to dtype.
+ *   x            16-bit rows, quantized in the workspace first; or null, and x_codes,
+ *                x_scales hold it.
+ *   w_codes, w_scales  the weight's rows: n, or 2 n for SAGE_ACT_SWIGLU; under 2^22 rows and
+ *                under 2^31 bytes of codes.
+ *   others       as in sage_linear (dtype: of x, residual, out and a bias that is not fp32).
+ *   workspace    sage_mxfp4_linear_workspace_bytes(...) bytes, 16-byte aligned; needs no
+ *                clearing.  quantize_x: whether x is given; other_rows as in sage_linear. */
+size_t sage_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int activation, int quantize_x,
+                                         int other_rows);
+int sage_mxfp4_linear(const void* x, int64_t x_rs, const void* x_codes, const void* x_scales, const void* w_codes,
+                      const void* w_scales, const void* bias, int bias_fp32, const void* residual, int64_t r_rs,
+                      int64_t m, int64_t n, int64_t k, int dtype, int activation, void* workspace,
+                      size_t workspace_bytes, float* z, void* out, hipStream_t stream);
+
+/* Gradients, the rounding of x taken as the identity: dz = dout * act'(z) rounded to dtype as
+ * the product's operand, dx = dz weight over the weight's values in dtype, dbias = the unrounded
+ * dz's column sums; each null if not wanted.  Arguments as in sage_linear_bwd; the weight's 16-bit
+ * rows (formed in the workspace) have under 2^31 bytes. */
+size_t sage_mxfp4_linear_bwd_workspace_bytes(const void* dout, int64_t d_rs, int64_t m, int64_t n, int64_t k,
+                                             int activation, int want);
+int sage_mxfp4_linear_bwd(const void* dout, int64_t d_rs, const void* w_codes, const void* w_scales, const float* z,
+                          int64_t m, int64_t n, int64_t k, int dtype, int activation, int bias_fp32, void* workspace,
+                          size_t workspace_bytes, void* dx, void* dbias, hipStream_t stream);
+
+/* sage_rms_norm_modulate with its output in MXFP4, quantized from the unrounded values (sums
+ * and products in fp64, so that a value next to a border between two codes falls on its own
+ * side).  codes, scales: b * n rows of c columns. */
+int sage_rms_norm_modulate_mxfp4(const void* x, int64_t x_bs, int64_t x_rs, const void* weight,
+                                 const void* scale, int64_t scale_bs, int64_t scale_gs, int64_t groups,
+                                 const int32_t* doc_ids, int64_t b, int64_t n, int64_t c, int dtype,
+                                 int fp32_params, float eps, void* codes, void* scales, hipStream_t stream);
+
+/* sage_rms_norm_gate_residual_modulate with the second norm's output in MXFP4; hidden is
+ * rounded once from fp64. */
+int sage_rms_norm_gate_residual_modulate_mxfp4(
+    const void* residual, int64_t r_bs, int64_t r_rs, const void* x, int64_t x_bs, int64_t x_rs,
+    const void* weight, const void* gate, int64_t gate_bs, int64_t gate_gs, const void* next_weight,
+    const void* next_scale, int64_t scale_bs, int64_t scale_gs, int64_t groups, const int32_t* doc_ids,
+    int64_t b, int64_t n, int64_t c, int dtype, int fp32_params, float eps, void* hidden, void* codes,
+    void* scales, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
