@@ -390,6 +390,7 @@ struct GemmArgs {
   // the plan (gemm_plan)
   int big, skinny, thin, kt, tm, tn;
   int whole, parts;     // tiles past `whole` run as `parts` pieces of the contraction
+  int tails;            // MXFP4 with one piece: small tiles that cover what the whole ones leave
   int64_t part_floats;  // fp32 sums of the pieces
   float* part;
 };

@@ -138,7 +138,7 @@ __global__ __launch_bounds__(TL::NT, TL::SIMD) void gemm_kernel(GemmArgs a) {
   }
   wait_vmem();  // the loads in flight write this workgroup's LDS
   if (cut) {
-    store_piece<TL>(a, t, piece, wave, lane, acc);
+    store_piece(a.part + ((int64_t)(t - a.whole) * a.parts + piece) * (TL::BM * TL::BN), wave, lane, acc);
     return;
   }
   const int64_t mw = m0 + wm * TL::MI * 32;

@@ -161,182 +161,361 @@ __device__ __forceinline__ f32x4 mx16(i32x4 a, int sa, i32x4 b, int sb, f32x4 c)
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a), wide(b), c, 4, 4, S, sa, S, sb);
 }
 
-// The scales of MI blocks of 32 rows in one stage: lane (h, r) gets the four bytes of row r that
-// belong to the 16-byte chunks 4 h .. 4 h + 3 of its codes; in step s of the stage it multiplies
-// chunk 4 h + s with byte s.  Rows past the last read the last one's.
-template <int N>
-struct Scales {
-  int off[N];
+constexpr int kMxGroup = 8;  // tile rows that the schedule takes together
+
+// A tile shape: WM x WN waves, each with MI x NI blocks of 32 x 32, two waves a SIMD, and D stages
+// of LDS.  A stage is 128 columns: 64 bytes a row.
+template <int WM_, int WN_, int MI_, int NI_, int D_>
+struct MxTile {
+  static constexpr int WM = WM_, WN = WN_, MI = MI_, NI = NI_, D = D_;
+  static constexpr int WAVES = WM * WN, NT = 64 * WAVES;
+  static constexpr int BM = WM * MI * 32, BN = WN * NI * 32;
+  static constexpr int A_BYTES = BM * 64, STAGE = (BM + BN) * 64;
+  // of the epilogue: what a wave finishes together, 32 rows
+  static constexpr int OUT_PITCH = NI * 64 + 16, OUT = 32 * (OUT_PITCH > kAnyPitch * 4 ? OUT_PITCH : kAnyPitch * 4);
+  static constexpr int LDS = D * STAGE > WAVES * OUT ? D * STAGE : WAVES * OUT;
+};
+
+// One operand's part of an LDS stage: ROWS rows of 64 bytes, row r's 16-byte chunk c at
+// c ^ ((r >> 2) & 3): the 16 rows that a fragment read touches at a time lie on 16 different
+// 16-byte columns of the 256 bytes of banks.  A load moves 16 rows, four lanes a row.
+template <int ROWS, int WAVES>
+struct MxOperand {
+  static constexpr int LOADS = ROWS * 64 / 1024 / WAVES;  // of one wave
   const uint8_t* base;
-  int64_t step;  // bytes of a stage's scales
-  __device__ __forceinline__ void issue(int (&v)[N], int kt) const {
-    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(base + kt * step, 0x7fffffff);
+  int off[LOADS];
+  // glu: tile row j is row (j / 64) * 32 + j % 32 of half (j / 32) % 2, the halves `half` rows apart
+  __device__ __forceinline__ void init(const void* p, int64_t pitch, int64_t row0, int64_t rows, int wave, int lane,
+                                       bool glu, int64_t half) {
+    base = static_cast<const uint8_t*>(p) + row0 * pitch;
+    const int64_t left = rows - row0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = (int)load_4(rs, off[i]);
+    for (int i = 0; i < LOADS; ++i) {
+      int r = (i * WAVES + wave) * 16 + (lane >> 2);
+      const int c = (lane & 3) ^ ((r >> 2) & 3);
+      const bool up = glu && ((r >> 5) & 1);
+      if (glu) r = (r >> 6) * 32 + (r & 31);
+      off[i] = r < left ? (int)(r * pitch + (up ? half * pitch : 0)) + c * 16 : (int)0x80000000;
+    }
+  }
+  // Issues the loads of stage t into `lds`; past `end` they give zeros.
+  __device__ __forceinline__ void issue(uint8_t* lds, int t, int end, int wave) const {
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(base + (int64_t)t * 64, t < end ? 0x7fffffffu : 0u);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) dma_16(lds + (i * WAVES + wave) * 1024, rs, off[i]);
   }
 };
 
-// The product by tiles, as the linear layers' gemm_kernel: three LDS stages of A and two of B,
-// the next step's fragments read under this one's products.  A stage is 256 columns.  Scales go
-// straight to registers, a stage ahead.
-template <typename T, typename TL>
-__global__ __launch_bounds__(TL::NT, TL::SIMD) void mx_gemm_kernel(MxGemmArgs x) {
-  const GemmArgs& a = x.g;
-  __shared__ __align__(1024) uint8_t lds[TL::LDS];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const bool glu = a.act == kActSwiglu;
-  const int bid = blockIdx.x;
-  int t, piece = 0;
-  int kt0 = 0, kt1 = a.kt;
-  const bool cut = bid >= a.whole;
-  if (!cut) {
-    t = xcd_share(bid, a.whole);
-  } else {
-    const int u = xcd_share(bid - a.whole, ((int)gridDim.x - a.whole));
-    t = a.whole + u / a.parts;
-    piece = u - (t - a.whole) * a.parts;
-    kt0 = (int)((int64_t)a.kt * piece / a.parts);
-    kt1 = (int)((int64_t)a.kt * (piece + 1) / a.parts);
+// The scales of N blocks of 32 rows in 256 columns (two stages): lane (h, r) loads its row's eight
+// bytes and keeps the four that it needs, of chunks 2 h and 2 h + 1 of either stage, in the order of
+// the four steps.  Rows past the last read the last one's.
+template <int N>
+struct MxScales {
+  int off[N];
+  const uint8_t* base;
+  int64_t step;  // bytes of 256 columns' scales
+  __device__ __forceinline__ void issue(uint2 (&v)[N], int g) const {
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(base + g * step, 0x7fffffff);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, off[i], 0, 0));
   }
-  int tm, tn;
-  tile_at(a, t, tm, tn);
-  const int64_t m0 = (int64_t)tm * TL::BM;
-  const int n0 = tn * (glu ? TL::BN / 2 : TL::BN);
-
-  Operand<TL::BM, true, TL::WAVES> A;
-  Operand<TL::BN, true, TL::WAVES> B;
-  A.init(a.a, a.lda, m0, a.m, wave, lane, false, 0);
-  B.init(a.b, a.ldb, n0, a.n, wave, lane, glu, a.n);
-  const int wm = wave / TL::WN, wn = wave % TL::WN;
-  const int h = lane >> 5, r = lane & 31;
-  Scales<TL::MI> SA;
-  Scales<TL::NI> SB;
-  const int rows = glu ? 2 * a.n : a.n;
-  SA.base = x.sa + m0 * 8;
-  SA.step = a.m * 8;
-  SB.base = x.sb;
-  SB.step = (int64_t)rows * 8;
-  // fragment addresses: chunk 4 h + s of row r in step s
-  int fa[TL::MI][4], fb[TL::NI][4];
-  auto frag_at = [&](int row, int s) { return row * 128 + (((4 * h + s) ^ ((row >> 1) & 7)) << 4); };
-#pragma unroll
-  for (int i = 0; i < TL::MI; ++i) {
-    const int row = (wm * TL::MI + i) * 32 + r;
-    SA.off[i] = (int)min((int64_t)row, a.m - 1 - m0) * 8 + 4 * h;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) fa[i][s] = frag_at(row, s);
-  }
-#pragma unroll
-  for (int i = 0; i < TL::NI; ++i) {
-    const int row = (wn * TL::NI + i) * 32 + r;
-    const int n = n0 + (glu ? (row >> 6) * 32 + r : row);
-    SB.off[i] = (min(n, a.n - 1) + (glu && (row >> 5 & 1) ? a.n : 0)) * 8 + 4 * h;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) fb[i][s] = frag_at(row, s);
-  }
-
-  f32x16 acc[TL::MI][TL::NI] = {};
-  i32x4 va[2][TL::MI], vb[2][TL::NI];
-  int sa[2][TL::MI], sb[2][TL::NI];
-  const int64_t end = (int64_t)kt1 * kBK, ka = min(a.k, end);
-  auto read = [&](const uint8_t* pa, const uint8_t* pb, int s, int to) {
-#pragma unroll
-    for (int i = 0; i < TL::NI; ++i) vb[to][i] = operand_at<i32x4>(pb + fb[i][s]);
-#pragma unroll
-    for (int i = 0; i < TL::MI; ++i) va[to][i] = operand_at<i32x4>(pa + fa[i][s]);
-  };
-  auto products = [&](int from, auto step) {
-#pragma unroll
-    for (int i = 0; i < TL::MI; ++i)
-#pragma unroll
-      for (int j = 0; j < TL::NI; ++j)
-        acc[i][j] = mx32<decltype(step)::value>(vb[from][j], sb[0][j], va[from][i], sa[0][i], acc[i][j]);
-  };
-  constexpr int H = decltype(A)::LOADS / 2;
-  static_assert(H * 2 == decltype(B)::LOADS, "as many loads of A as of B");
-  auto order = [&]() {
-    constexpr int M = TL::MI * TL::NI, R = TL::MI + TL::NI;
-#pragma unroll
-    for (int i = 0; i < M; ++i) {
-      order_mfma();
-      if (i < R) order_read();
-      if (i % (M / H) == M / H / 2) order_load();
-    }
-  };
-  uint8_t* const lb = lds + TL::B_AT;
-  SA.issue(sa[0], kt0);
-  SB.issue(sb[0], kt0);
-  A.template issue<0, 2 * H>(lds, (int64_t)kt0 * kBK, ka, wave);
-  B.template issue<0, 2 * H>(lb, (int64_t)kt0 * kBK, ka, wave);
-  A.template issue<0, 2 * H>(lds + TL::A_BYTES, (int64_t)(kt0 + 1) * kBK, ka, wave);
-  B.template issue<0, H>(lb + TL::B_BYTES, (int64_t)(kt0 + 1) * kBK, ka, wave);
-  wait_loads<3 * H>();
-  barrier();
-  read(lds, lb, 0, 0);
-  int a0 = 0, b0 = 0;        // the present stage's place
-  int a2 = 2 * TL::A_BYTES;  // the place of the stage after next
-  for (int kt = kt0; kt < kt1; ++kt) {
-    uint8_t* const pa = lds + a0;
-    uint8_t* const pb = lb + b0;
-    const int next = min(kt + 1, kt1 - 1);
-    SA.issue(sa[1], next);
-    SB.issue(sb[1], next);
-    read(pa, pb, 1, 1);
-    products(0, std::integral_constant<int, 0>{});
-    B.template issue<H, H>(lb + (b0 ^ TL::B_BYTES), (int64_t)(kt + 1) * kBK, ka, wave);
-    order();
-    read(pa, pb, 2, 0);
-    products(1, std::integral_constant<int, 1>{});
-    A.template issue<0, H>(lds + a2, (int64_t)(kt + 2) * kBK, ka, wave);
-    order();
-    read(pa, pb, 3, 1);
-    products(0, std::integral_constant<int, 2>{});
-    A.template issue<H, H>(lds + a2, (int64_t)(kt + 2) * kBK, ka, wave);
-    order();
-    wait_loads<2 * H>();
-    barrier();
-    a2 = a0;
-    a0 = a0 == 2 * TL::A_BYTES ? 0 : a0 + TL::A_BYTES;
-    b0 ^= TL::B_BYTES;
-    read(lds + a0, lb + b0, 0, 0);
-    products(1, std::integral_constant<int, 3>{});
-    B.template issue<0, H>(pb, (int64_t)(kt + 2) * kBK, ka, wave);
-    order();
-#pragma unroll
-    for (int i = 0; i < TL::MI; ++i) sa[0][i] = sa[1][i];
-#pragma unroll
-    for (int i = 0; i < TL::NI; ++i) sb[0][i] = sb[1][i];
-  }
-  wait_vmem();  // the loads in flight write this workgroup's LDS
-  if (cut) {
-    store_piece<TL>(a, t, piece, wave, lane, acc);
-    return;
-  }
-  const int64_t mw = m0 + wm * TL::MI * 32;
-  const int nw = n0 + wn * TL::NI * (glu ? 16 : 32);
-  if constexpr (TL::SIMD > 1) {
-    if (!a.vec) {
-      barrier();  // every wave has read its last fragments: the stages' LDS is free
-      static_assert(TL::NI == 2 && TL::WAVES * TL::MI * 32 * kAnyPitch * 4 <= TL::LDS, "the sums fit");
-      float* const mine = reinterpret_cast<float*>(lds) + wave * TL::MI * 32 * kAnyPitch;
-#pragma unroll
-      for (int i = 0; i < TL::MI; ++i) stage_any(mine, lane, i, acc[i][0], acc[i][1]);
-      finish_any_act<T, true, TL::MI>(a, mine, lane, mw, nw);
-      return;
-    }
-  }
-  finish<T>(a, lane, mw, nw, acc);
-}
-
-// ---------------------------------------------------------------- few rows
-
-constexpr int kMxSkinnyWaves = 4;
+};
 
 // Waits for every LDS read and for all but the last N loads.
 template <int N>
 __device__ __forceinline__ void wait_all_but() {
   __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
 }
+
+// The epilogue of a wave's MI x NI blocks from row m0 and column n0 on: z = acc + bias, kept when the
+// backward wants it, out = act(z) + residual, rounded once.  A lane's accumulators are four
+// consecutive columns of its row, again and again: 32 rows at a time go through LDS (`lds`: this
+// wave's, rows of PITCH bytes: no bank conflicts), so that the stores are whole rows of the wave.
+// What a call does not have (residual, z) has a resource of no bytes.  PLAIN: out alone.
+template <typename T, int ACT, bool PLAIN, int PITCH, int MI, int NI>
+__device__ __forceinline__ void mx_finish(const GemmArgs& a, uint8_t* lds, int lane, int64_t m0, int n0,
+                                          f32x16 (&c)[MI][NI]) {
+  constexpr bool kGlu = ACT == kActSwiglu;
+  constexpr int kStep = kGlu ? 2 : 1, kCols = NI * 32 / kStep, kLanes = kCols / 8, kRows = 64 / kLanes;
+  const int64_t left = a.m - m0;
+  if (left <= 0) return;
+  const int rows = left < 32 * MI ? (int)left : 32 * MI, h = lane >> 5, r = lane & 31;
+  const int wide = kGlu ? 2 * a.n : a.n;
+  const __amdgpu_buffer_rsrc_t out = raw_rsrc(static_cast<T*>(a.out) + m0 * a.n, (uint32_t)rows * a.n * 2);
+  const __amdgpu_buffer_rsrc_t res = raw_rsrc(static_cast<const T*>(a.res) + m0 * a.ldr,
+                                              a.res ? (uint32_t)(((rows - 1) * a.ldr + a.n) * 2) : 0u);
+  const __amdgpu_buffer_rsrc_t zs = raw_rsrc(a.z + m0 * wide, a.z ? (uint32_t)rows * wide * 4 : 0u);
+  const __amdgpu_buffer_rsrc_t bs = raw_rsrc(a.bias, a.bias ? (uint32_t)wide * (a.bias_f32 ? 4 : 2) : 0u);
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  auto load_8 = [](__amdgpu_buffer_rsrc_t rs, int off) {
+    return __builtin_bit_cast(V4, __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, 0));
+  };
+  auto bias_at = [&](int n) {
+    if (a.bias_f32) return __builtin_bit_cast(f32x4, load_16(bs, n * 4));
+    const V4 v = load_8(bs, n * 2);
+    return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+  };
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+#pragma unroll
+    for (int j = 0; j < NI; j += kStep) {
+      V4 rv[4];
+      f32x4 b[4], b2[4];
+      if constexpr (!PLAIN) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = n0 + j / kStep * 32 + 8 * q + 4 * h, none = n < a.n ? 0 : (int)0x80000000;
+          rv[q] = load_8(res, (int)((32 * i + r) * a.ldr + n) * 2 | none);
+          // past the last column a column that lies past any bias, in bytes too
+          const int nb = n | (n < a.n ? 0 : 0x10000000);
+          b[q] = bias_at(nb);
+          if constexpr (kGlu) b2[q] = bias_at(nb + a.n);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = n0 + j / kStep * 32 + 8 * q + 4 * h, none = n < a.n ? 0 : (int)0x80000000;
+        f32x4 z = {c[i][j][4 * q], c[i][j][4 * q + 1], c[i][j][4 * q + 2], c[i][j][4 * q + 3]};
+        if constexpr (!PLAIN) {
+          f32x4 z2;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            z[e] += b[q][e];
+            if constexpr (kGlu) z2[e] = c[i][j + 1][4 * q + e] + b2[q][e];
+          }
+          if constexpr (ACT != kActNone) {
+            const int at = ((32 * i + r) * wide + n) * 4 | none;
+            store_16(__builtin_bit_cast(u32x4, z), zs, at);
+            if constexpr (kGlu) store_16(__builtin_bit_cast(u32x4, z2), zs, at + a.n * 4);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            z[e] = act_fwd(ACT, z[e]);
+            if constexpr (kGlu) z[e] *= z2[e];
+            z[e] += (float)rv[q][e];
+          }
+        }
+        V4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (T)z[e];
+        *reinterpret_cast<V4*>(lds + r * PITCH + (j / kStep * 32 + 8 * q + 4 * h) * 2) = o;
+      }
+      if constexpr (!PLAIN) keep_order();
+    }
+    // the wave's values are written before they are read, and read before the next are written
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int n = n0 + lane % kLanes * 8, none = n < a.n ? 0 : (int)0x80000000;
+#pragma unroll
+    for (int u = 0; u < 32 / kRows; ++u) {
+      const int row = u * kRows + lane / kLanes;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(lds + row * PITCH + lane % kLanes * 16);
+      store_16(v, out, ((32 * i + row) * a.n + n) * 2 | none);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// One tile: rows from m0 and columns from n0 on, columns 256 g0 .. 256 g1 of the contraction; its sums to
+// `part` where that is given, else finished.  LDS holds D stages; a stage is two steps of 64 columns,
+// the next step's fragments read under this one's products.  Before a stage's last step the next
+// stage has arrived and every wave has read this one's last fragments: behind that barrier the loads of
+// the stage D further on go into its place.  Scales go straight to registers, 256 columns ahead.
+template <typename T, typename TL>
+__device__ __forceinline__ void mx_tile(const MxGemmArgs& x, uint8_t* lds, int wave, int lane, int64_t m0, int n0, int g0,
+                                        int g1, float* part) {
+  const GemmArgs& a = x.g;
+  const bool glu = a.act == kActSwiglu;
+  MxOperand<TL::BM, TL::WAVES> A;
+  MxOperand<TL::BN, TL::WAVES> B;
+  constexpr int LOADS = decltype(A)::LOADS + decltype(B)::LOADS;
+  A.init(a.a, a.lda * 2, m0, a.m, wave, lane, false, 0);
+  B.init(a.b, a.ldb * 2, n0, a.n, wave, lane, glu, a.n);
+  const int wm = wave / TL::WN, wn = wave % TL::WN;
+  const int h = lane >> 5, r = lane & 31;
+  MxScales<TL::MI> SA;
+  MxScales<TL::NI> SB;
+  SA.base = x.sa + m0 * 8;
+  SA.step = a.m * 8;
+  SB.base = x.sb;
+  SB.step = (int64_t)(glu ? 2 * a.n : a.n) * 8;
+#pragma unroll
+  for (int i = 0; i < TL::MI; ++i) SA.off[i] = (int)min((int64_t)(wm * TL::MI + i) * 32 + r, a.m - 1 - m0) * 8;
+#pragma unroll
+  for (int i = 0; i < TL::NI; ++i) {
+    const int row = (wn * TL::NI + i) * 32 + r, n = n0 + (glu ? (row >> 6) * 32 + r : row);
+    SB.off[i] = (min(n, a.n - 1) + (glu && (row >> 5 & 1) ? a.n : 0)) * 8;
+  }
+  // the fragment of block i in step s: chunk 2 h + s of row r; blocks are 2 KiB apart
+  int fa[2], fb[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int in = r * 64 + (((2 * h + s) ^ ((r >> 2) & 3)) << 4);
+    fa[s] = wm * TL::MI * 2048 + in;
+    fb[s] = TL::A_BYTES + wn * TL::NI * 2048 + in;
+  }
+
+  f32x16 acc[TL::MI][TL::NI] = {};
+  i32x4 va[2][TL::MI], vb[2][TL::NI];
+  uint2 na[TL::MI], nb[TL::NI];
+  int sa[TL::MI], sb[TL::NI];
+  auto read = [&](const uint8_t* p, int s) {
+#pragma unroll
+    for (int i = 0; i < TL::NI; ++i) vb[s][i] = operand_at<i32x4>(p + fb[s] + i * 2048);
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i) va[s][i] = operand_at<i32x4>(p + fa[s] + i * 2048);
+  };
+  auto products = [&](auto step) {  // step of the 256 columns
+    constexpr int S = decltype(step)::value;
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::NI; ++j)
+        acc[i][j] = mx32<S>(vb[S & 1][j], sb[j], va[S & 1][i], sa[i], acc[i][j]);
+  };
+  const uint32_t pick = h ? 0x07060302u : 0x05040100u;
+  auto keep_scales = [&]() {
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i) sa[i] = (int)__builtin_amdgcn_perm(na[i].y, na[i].x, pick);
+#pragma unroll
+    for (int i = 0; i < TL::NI; ++i) sb[i] = (int)__builtin_amdgcn_perm(nb[i].y, nb[i].x, pick);
+  };
+  auto issue = [&](uint8_t* to, int stage) {
+    A.issue(to, stage, 2 * g1, wave);
+    B.issue(to + TL::A_BYTES, stage, 2 * g1, wave);
+  };
+  // the order of one step: the next step's reads first, two a product, then the loads (direct ones
+  // stay behind the reads)
+  auto order = [&](auto loads) {
+    constexpr int M = TL::MI * TL::NI, R = TL::MI + TL::NI, E = (R + 1) / 2, L = M - E, N = decltype(loads)::value;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      order_mfma();
+      if (i < E) order_read(), order_read();
+      if (i >= E) {
+#pragma unroll
+        for (int l = (i - E) * N / L; l < (i - E + 1) * N / L; ++l) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+      }
+    }
+    keep_order();
+  };
+  SA.issue(na, g0);
+  SB.issue(nb, g0);
+  int t0 = 2 * g0;
+#pragma unroll
+  for (int d = 0; d < TL::D; ++d) issue(lds + d * TL::STAGE, t0 + d);
+  keep_scales();
+  wait_all_but<(TL::D - 1) * LOADS>();
+  barrier();
+  read(lds, 0);
+  int now = 0;  // the present stage's place
+  for (int g = g0; g < g1; ++g) {
+    auto stage = [&](auto half) {
+      constexpr int J = decltype(half)::value;
+      uint8_t* const p = lds + now;
+      read(p, 1);
+      products(std::integral_constant<int, 2 * J>{});
+      if constexpr (J == 0) {
+        const int next = min(g + 1, g1 - 1);
+        SA.issue(na, next);
+        SB.issue(nb, next);
+      }
+      order(std::integral_constant<int, J == 0 ? TL::MI + TL::NI : 0>{});
+      // all but the stages after next, and the scales
+      wait_all_but<(TL::D - 2) * LOADS + (J == 0 ? TL::MI + TL::NI : 0)>();
+      barrier();
+      now = now == (TL::D - 1) * TL::STAGE ? 0 : now + TL::STAGE;
+      read(lds + now, 0);
+      products(std::integral_constant<int, 2 * J + 1>{});
+      issue(p, t0 + TL::D);
+      order(std::integral_constant<int, LOADS>{});
+      ++t0;
+    };
+    stage(std::integral_constant<int, 0>{});
+    stage(std::integral_constant<int, 1>{});
+    keep_scales();
+  }
+  wait_vmem();  // the loads in flight write this workgroup's LDS
+  if (part) {
+    store_piece(part, wave, lane, acc);
+    return;
+  }
+  const int64_t mw = m0 + wm * TL::MI * 32;
+  const int nw = n0 + wn * TL::NI * (glu ? 16 : 32);
+  barrier();  // every wave has read its last fragments: the stages' LDS is free
+  uint8_t* const mine = lds + wave * TL::OUT;
+  if (!a.vec) {
+    float* const sums = reinterpret_cast<float*>(mine);
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i) {
+#pragma unroll
+      for (int j = 0; j < TL::NI; j += 2) {
+        stage_any(sums, lane, 0, acc[i][j], acc[i][j + 1]);
+        finish_any_act<T, true, 1>(a, sums, lane, mw + 32 * i, nw + j * (glu ? 16 : 32));
+        // the next columns' sums are written behind these reads
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    return;
+  }
+  constexpr int P = TL::OUT_PITCH;
+  if (a.act == kActSwiglu) mx_finish<T, kActSwiglu, false, P>(a, mine, lane, mw, nw, acc);
+  else if (a.act == kActSilu) mx_finish<T, kActSilu, false, P>(a, mine, lane, mw, nw, acc);
+  else if (a.act == kActGelu) mx_finish<T, kActGelu, false, P>(a, mine, lane, mw, nw, acc);
+  else if (a.bias || a.res) mx_finish<T, kActNone, false, P>(a, mine, lane, mw, nw, acc);
+  else mx_finish<T, kActNone, true, P>(a, mine, lane, mw, nw, acc);
+}
+
+// The product by tiles TL, and behind them by tiles TAIL that cover what is left: the rows past the
+// last whole tile row, and the whole tiles of a last round that would leave most of the card idle.
+template <typename T, typename TL, typename TAIL>
+__global__ __launch_bounds__(TL::NT, 2) void mx_gemm_kernel(MxGemmArgs x) {
+  const GemmArgs& a = x.g;
+  static_assert(TL::NT == TAIL::NT, "one workgroup size");
+  __shared__ __align__(1024) uint8_t lds[TL::LDS > TAIL::LDS ? TL::LDS : TAIL::LDS];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int cols = a.act == kActSwiglu ? 2 : 1;  // columns of the product for one of the output
+  const int bid = blockIdx.x;
+  int tm, tn;
+  if (bid < a.whole) {
+    tile_at<kMxGroup>(a, xcd_share(bid, a.whole), tm, tn);
+    mx_tile<T, TL>(x, lds, wave, lane, (int64_t)tm * TL::BM, tn * (TL::BN / cols), 0, a.kt, nullptr);
+    return;
+  }
+  int u = xcd_share(bid - a.whole, (int)gridDim.x - a.whole);
+  if (a.parts > 1) {  // pieces of the contraction
+    const int t = u / a.parts, piece = u - t * a.parts;
+    tile_at<kMxGroup>(a, a.whole + t, tm, tn);
+    mx_tile<T, TL>(x, lds, wave, lane, (int64_t)tm * TL::BM, tn * (TL::BN / cols),
+                   (int)((int64_t)a.kt * piece / a.parts), (int)((int64_t)a.kt * (piece + 1) / a.parts),
+                   a.part + (int64_t)u * (TL::BM * TL::BN));
+    return;
+  }
+  constexpr int KM = TL::BM / TAIL::BM, KN = TL::BN / TAIL::BN;
+  int64_t m0;
+  int n0;
+  const int cut = (a.tm * a.tn - a.whole) * (KM * KN);
+  if (u < cut) {
+    const int t = u / (KM * KN), in = u - t * (KM * KN);
+    tile_at<kMxGroup>(a, a.whole + t, tm, tn);
+    m0 = (int64_t)tm * TL::BM + in / KN * TAIL::BM;
+    n0 = tn * (TL::BN / cols) + in % KN * (TAIL::BN / cols);
+    if (m0 >= a.m || n0 >= a.n) return;
+  } else {
+    u -= cut;
+    const int strip = (int)((a.m - (int64_t)a.tm * TL::BM + TAIL::BM - 1) / TAIL::BM);
+    m0 = (int64_t)a.tm * TL::BM + u % strip * TAIL::BM;
+    n0 = u / strip * (TAIL::BN / cols);
+  }
+  mx_tile<T, TAIL>(x, lds, wave, lane, m0, n0, 0, a.kt, nullptr);
+}
+
+// ---------------------------------------------------------------- few rows
+
+constexpr int kMxSkinnyWaves = 4;
 
 // out for at most 16 * MT rows of x, as the linear layers' skinny_kernel: a workgroup reads 16
 // rows of W (of both halves for a swiglu) once, its waves take 256-column stages in turn through
@@ -493,24 +672,25 @@ __global__ __launch_bounds__(64 * kMxSkinnyWaves, MT < 4 ? 2 : 1) void mx_skinny
   }
 }
 
-using MxBig = Tile<2, 2, 4, 4, 1>;    // 256 x 256, 4 waves of 128 x 128, one workgroup a CU
-using MxSmall = Tile<2, 2, 2, 2, 2>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
+using MxBig = MxTile<2, 4, 4, 2, 4>;    // 256 x 256, 8 waves of 128 x 64, one workgroup a CU
+using MxTail = MxTile<4, 2, 1, 2, 4>;   // 128 x 128, 8 waves of 32 x 64, behind them
+using MxSmall = MxTile<2, 2, 2, 2, 3>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
 
-template <typename T, typename TL>
+template <typename T, typename TL, typename TAIL>
 hipError_t run_mx_tiles(const MxGemmArgs& x, hipStream_t st) {
   const GemmArgs& a = x.g;
-  const int tiles = a.tm * a.tn, rest = tiles - a.whole;
-  mx_gemm_kernel<T, TL><<<a.whole + rest * a.parts, TL::NT, 0, st>>>(x);
+  const int rest = a.parts > 1 ? (a.tm * a.tn - a.whole) * a.parts : a.tails;
+  mx_gemm_kernel<T, TL, TAIL><<<a.whole + rest, TL::NT, 0, st>>>(x);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || rest == 0) return e;
-  join_kernel<T, TL><<<rest * (TL::WAVES * TL::MI * TL::NI / 2) / 4, 256, 0, st>>>(a);
+  if (e != hipSuccess || a.parts == 1) return e;
+  join_kernel<T, TL, kMxGroup><<<(a.tm * a.tn - a.whole) * (TL::WAVES * TL::MI * TL::NI / 2) / 4, 256, 0, st>>>(a);
   return hipGetLastError();
 }
 
 template <typename T>
 hipError_t run_mx(const MxGemmArgs& x, hipStream_t st) {
   const GemmArgs& a = x.g;
-  if (!a.skinny) return a.big ? run_mx_tiles<T, MxBig>(x, st) : run_mx_tiles<T, MxSmall>(x, st);
+  if (!a.skinny) return a.big ? run_mx_tiles<T, MxBig, MxTail>(x, st) : run_mx_tiles<T, MxSmall, MxSmall>(x, st);
   const uint32_t grid = (uint32_t)((a.n + 15) / 16);
   constexpr int NT = 64 * kMxSkinnyWaves;
   if (a.act == kActSwiglu) {
@@ -550,37 +730,51 @@ void mx_gemm_plan(GemmArgs& a) {
   a.parts = 1;
   a.tm = a.tn = a.whole = 0;
   if (a.skinny) return;
-  // The tile shape and the split of the last round's tiles with the least estimated time, in
-  // stages of the large tile on every CU.
+  // The least estimated time, in 256 columns of the large tile on every CU (1.85 us), where a round of
+  // large tiles costs 1.45 more for its start and epilogue.  Measured at 4096 x 4096 x K and its like: small
+  // tiles 0.83 us alone on a CU, 1.35 two a CU, the small ones behind large ones 0.68; the sums of
+  // pieces move at 8 TB/s and their join costs 4 us.
+  const int64_t rows = glu ? 2 * (int64_t)a.n : a.n;
+  auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
   double best = 1e30;
+  auto take = [&](double cost, int big, int64_t tm, int64_t tn, int64_t whole, int parts, int64_t tails, int64_t sums) {
+    if (cost >= best) return;
+    best = cost;
+    a.big = big;
+    a.tm = (int)tm;
+    a.tn = (int)tn;
+    a.whole = (int)whole;
+    a.parts = parts;
+    a.tails = (int)tails;
+    a.part_floats = sums;
+  };
   for (int big = 1; big >= 0; --big) {
-    const int bm = big ? MxBig::BM : MxSmall::BM, bn = (big ? MxBig::BN : MxSmall::BN) / (glu ? 2 : 1);
-    const int64_t tm = (a.m + bm - 1) / bm, tn = (a.n + bn - 1) / bn, tiles = tm * tn;
-    const int slots = big ? 256 : 512;
-    const double start = big ? 7.5 : 3.6;
-    for (int p = 1; p <= 16; ++p) {
-      // rows that take no 16-byte accesses are finished by the small tiles themselves, and
-      // with large ones by the join
-      const int64_t rest = !a.vec && (big || p > 1) ? tiles : p == 1 ? 0 : tiles % slots;
-      if (p > 1 && (rest == 0 || a.kt / p < 2)) continue;
-      const int64_t whole = tiles - rest;
-      const double stage = big ? 1.0 : tiles <= 256 && rest * p <= 256 ? 0.37 : 0.63;
-      double cost = (double)((whole + slots - 1) / slots) * (a.kt * stage + start);
-      if (rest) {
-        const double bytes = (double)rest * p * bm * (big ? MxBig::BN : MxSmall::BN) * 4;
-        cost += (double)((rest * p + slots - 1) / slots) * ((a.kt + p - 1) / p * stage + start) + 2.7 +
-                bytes * 2 / 4e6 / 1.48;
-      }
-      if (cost < best) {
-        best = cost;
-        a.big = big;
-        a.tm = (int)tm;
-        a.tn = (int)tn;
-        a.whole = (int)whole;
-        a.parts = p;
-        a.part_floats = rest * p * bm * (big ? MxBig::BN : MxSmall::BN);
-      }
+    const int bm = big ? MxBig::BM : MxSmall::BM, bn = big ? MxBig::BN : MxSmall::BN, slots = big ? 256 : 512;
+    const int64_t tm = up(a.m, bm), tn = up(rows, bn), tiles = tm * tn;
+    const double stage = big ? 1.0 : tiles <= 256 ? 0.45 : 0.73, start = big ? 1.45 : 0.5;
+    // whole tiles alone
+    take((double)up(tiles, slots) * (a.kt * stage + start), big, tm, tn, tiles, 1, 0, 0);
+    // the last round's tiles in pieces of the contraction, joined by a second kernel
+    for (int p = 2; p <= 16 && a.kt / p >= 2; ++p) {
+      const int64_t rest = tiles % slots, whole = tiles - rest;
+      if (rest == 0) continue;
+      const double bytes = (double)rest * p * bm * bn * 4;
+      take((double)(whole / slots) * (a.kt * stage + start) + (double)up(rest * p, slots) * (up(a.kt, p) * stage + start) +
+               2.0 + bytes * 2 / 8e6 / 1.85,
+           big, tm, tn, whole, p, 0, rest * p * bm * bn);
     }
+    if (!big) continue;
+    // the rows past the last whole tile row, with or without the last round's tiles, as small ones
+    const int64_t fm = a.m / bm, full = fm * tn, strip = up(a.m - fm * bm, MxTail::BM) * up(rows, MxTail::BN);
+    const double tail = a.kt * 0.37 + 0.5;
+    const int64_t left = full % slots;
+    // after the whole rounds `left` CUs take a tile each and the others small ones beside them
+    const double one = a.kt * stage + start;
+    const int64_t beside = (slots - left) * (int64_t)(one / tail);
+    if (left) take((double)(full / slots + 1) * one + (double)up(strip > beside ? strip - beside : 0, slots) * tail, 1, fm,
+                   tn, full, 1, strip, 0);
+    take((double)(full / slots) * one + (double)up(strip + left * 4, slots) * tail, 1, fm, tn, full - left, 1,
+         strip + left * 4, 0);
   }
 }
 

@@ -410,10 +410,10 @@ __device__ __forceinline__ typename Vec8<T>::type frag(const uint8_t* __restrict
   }
 }
 
-// Tile t of the schedule: groups of 4 tile rows, column by column inside, so that the 32
-// tiles an XCD runs together share 4 row panels and 8 column panels.
+// Tile t of the schedule: groups of G tile rows, column by column inside, so that the 32
+// tiles an XCD runs together share G row panels and 32 / G column panels.
+template <int G = 4>
 __device__ __forceinline__ void tile_at(const GemmArgs& a, int t, int& tm, int& tn) {
-  constexpr int G = 4;
   const int g = t / (G * a.tn), in = t - g * G * a.tn;
   const int rows = min(G, a.tm - g * G);
   tn = in / rows;
@@ -463,19 +463,17 @@ __device__ __forceinline__ void order_read() { __builtin_amdgcn_sched_group_barr
 
 __device__ __forceinline__ void order_load() { __builtin_amdgcn_sched_group_barrier(0x020, 1, 0); }
 
-// A cut tile's sums of one piece, in the order the lanes hold them.
-template <typename TL>
-__device__ __forceinline__ void store_piece(const GemmArgs& a, int t, int piece, int wave, int lane,
-                                            const f32x16 (&acc)[TL::MI][TL::NI]) {
-  float* dst = a.part + ((int64_t)(t - a.whole) * a.parts + piece) * (TL::BM * TL::BN) +
-               wave * (TL::MI * TL::NI * 1024);
+// A tile's sums of one piece of the contraction, in the order the lanes hold them.
+template <int MI, int NI>
+__device__ __forceinline__ void store_piece(float* part, int wave, int lane, const f32x16 (&acc)[MI][NI]) {
+  float* const dst = part + wave * (MI * NI * 1024) + lane * 4;
 #pragma unroll
-  for (int i = 0; i < TL::MI; ++i)
+  for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < TL::NI; ++j)
+    for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f32x4*>(dst + ((i * TL::NI + j) * 4 + q) * 256 + lane * 4) =
+        *reinterpret_cast<f32x4*>(dst + ((i * NI + j) * 4 + q) * 256) =
             f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
 }
 
@@ -483,7 +481,7 @@ __device__ __forceinline__ void store_piece(const GemmArgs& a, int t, int piece,
 // block of a tile.  Large tiles whose rows take no 16-byte accesses all come through here.
 // Bound by the sums' way back: 75 tiles of 256 x 256 in three pieces, 79 MB with the residual
 // and the output, in 16 us = 4.9 TB/s.
-template <typename T, typename TL>
+template <typename T, typename TL, int G = 4>
 __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   constexpr int PAIRS = TL::NI / 2, BLOCKS = TL::WAVES * TL::MI * PAIRS;
@@ -503,7 +501,7 @@ __global__ __launch_bounds__(256) void join_kernel(GemmArgs a) {
     src += TL::BM * TL::BN;
   }
   int tm, tn;
-  tile_at(a, a.whole + t, tm, tn);
+  tile_at<G>(a, a.whole + t, tm, tn);
   const int w = blk / (TL::MI * PAIRS), wm = w / TL::WN, wn = w % TL::WN;
   const int i = blk / PAIRS % TL::MI, j = blk % PAIRS * 2;
   const bool glu = a.act == kActSwiglu;
