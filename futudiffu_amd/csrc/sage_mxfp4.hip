@@ -161,7 +161,7 @@ __device__ __forceinline__ f32x4 mx16(i32x4 a, int sa, i32x4 b, int sb, f32x4 c)
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a), wide(b), c, 4, 4, S, sa, S, sb);
 }
 
-constexpr int kMxGroup = 8;  // tile rows that the schedule takes together
+constexpr int kMxGroup = 8;   // tile rows that the schedule takes together
 
 // A tile shape: WM x WN waves, each with MI x NI blocks of 32 x 32, two waves a SIMD, and D stages
 // of LDS.  A stage is 128 columns: 64 bytes a row.
@@ -170,11 +170,13 @@ struct MxTile {
   static constexpr int WM = WM_, WN = WN_, MI = MI_, NI = NI_, D = D_;
   static constexpr int WAVES = WM * WN, NT = 64 * WAVES;
   static constexpr int BM = WM * MI * 32, BN = WN * NI * 32;
-  static constexpr int A_BYTES = BM * 64, STAGE = (BM + BN) * 64;
-  // of the epilogue: what a wave finishes together, 32 rows
-  static constexpr int OUT_PITCH = NI * 64 + 16, OUT = 32 * (OUT_PITCH > kAnyPitch * 4 ? OUT_PITCH : kAnyPitch * 4);
-  static constexpr int LDS = D * STAGE > WAVES * OUT ? D * STAGE : WAVES * OUT;
+  static constexpr int A_BYTES = BM * 64, STAGE = (BM + BN) * 64, RING = D * STAGE;
+  static constexpr int OUT = 32 * NI * 64;  // of the epilogue: 32 rows of a wave's columns
 };
+
+using MxBig = MxTile<2, 4, 4, 2, 4>;    // 256 x 256, 8 waves of 128 x 64, one workgroup a CU
+using MxTail = MxTile<4, 2, 1, 2, 4>;   // 128 x 128, 8 waves of 32 x 64, behind them
+using MxSmall = MxTile<2, 2, 2, 2, 4>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
 
 // One operand's part of an LDS stage: ROWS rows of 64 bytes, row r's 16-byte chunk c at
 // c ^ ((r >> 2) & 3): the 16 rows that a fragment read touches at a time lie on 16 different
@@ -182,45 +184,39 @@ struct MxTile {
 template <int ROWS, int WAVES>
 struct MxOperand {
   static constexpr int LOADS = ROWS * 64 / 1024 / WAVES;  // of one wave
-  const uint8_t* base;
   int off[LOADS];
   // glu: tile row j is row (j / 64) * 32 + j % 32 of half (j / 32) % 2, the halves `half` rows apart
-  __device__ __forceinline__ void init(const void* p, int64_t pitch, int64_t row0, int64_t rows, int wave, int lane,
-                                       bool glu, int64_t half) {
-    base = static_cast<const uint8_t*>(p) + row0 * pitch;
-    const int64_t left = rows - row0;
+  __device__ __forceinline__ void init(int64_t pitch, int wave, int lane, bool glu, int64_t half) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       int r = (i * WAVES + wave) * 16 + (lane >> 2);
       const int c = (lane & 3) ^ ((r >> 2) & 3);
       const bool up = glu && ((r >> 5) & 1);
       if (glu) r = (r >> 6) * 32 + (r & 31);
-      off[i] = r < left ? (int)(r * pitch + (up ? half * pitch : 0)) + c * 16 : (int)0x80000000;
+      off[i] = (int)(r * pitch + (up ? half * pitch : 0)) + c * 16;
     }
   }
-  // Issues the loads of stage t into `lds`; past `end` they give zeros.
-  __device__ __forceinline__ void issue(uint8_t* lds, int t, int end, int wave) const {
-    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(base + (int64_t)t * 64, t < end ? 0x7fffffffu : 0u);
+  // Issues the loads of a stage that starts at `p`, `left` bytes before the operand's end: rows past
+  // the last read zeros.
+  __device__ __forceinline__ void issue(uint8_t* lds, const uint8_t* p, uint32_t left, int wave) const {
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(p, left);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) dma_16(lds + (i * WAVES + wave) * 1024, rs, off[i]);
   }
 };
 
-// The scales of N blocks of 32 rows in 256 columns (two stages): lane (h, r) loads its row's eight
-// bytes and keeps the four that it needs, of chunks 2 h and 2 h + 1 of either stage, in the order of
-// the four steps.  Rows past the last read the last one's.
-template <int N>
-struct MxScales {
-  int off[N];
-  const uint8_t* base;
-  int64_t step;  // bytes of 256 columns' scales
-  __device__ __forceinline__ void issue(uint2 (&v)[N], int g) const {
-    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(base + g * step, 0x7fffffff);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      v[i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, off[i], 0, 0));
-  }
+// A tile's place: rows from m0 and columns from n0 on, columns 256 g0 .. 256 g1 of the contraction, and where
+// its sums go if they are a piece's.
+struct MxPlace {
+  int64_t m0;
+  int n0, g0, g1;
+  float* part;
 };
+
+// The bytes from row row0 to the end of `rows` rows, as a resource takes them.
+__device__ __forceinline__ uint32_t bytes_left(int64_t rows, int64_t row0, int64_t pitch) {
+  return (uint32_t)min((rows - row0) * pitch, (int64_t)0x7fffffff);
+}
 
 // Waits for every LDS read and for all but the last N loads.
 template <int N>
@@ -231,13 +227,18 @@ __device__ __forceinline__ void wait_all_but() {
 // The epilogue of a wave's MI x NI blocks from row m0 and column n0 on: z = acc + bias, kept when the
 // backward wants it, out = act(z) + residual, rounded once.  A lane's accumulators are four
 // consecutive columns of its row, again and again: 32 rows at a time go through LDS (`lds`: this
-// wave's, rows of PITCH bytes: no bank conflicts), so that the stores are whole rows of the wave.
+// wave's; a row's 16-byte chunks permuted so that rows lie on different banks), so that the stores
+// are whole rows of the wave.
 // What a call does not have (residual, z) has a resource of no bytes.  PLAIN: out alone.
-template <typename T, int ACT, bool PLAIN, int PITCH, int MI, int NI>
+template <typename T, int ACT, bool PLAIN, int MI, int NI>
 __device__ __forceinline__ void mx_finish(const GemmArgs& a, uint8_t* lds, int lane, int64_t m0, int n0,
                                           f32x16 (&c)[MI][NI]) {
   constexpr bool kGlu = ACT == kActSwiglu;
   constexpr int kStep = kGlu ? 2 : 1, kCols = NI * 32 / kStep, kLanes = kCols / 8, kRows = 64 / kLanes;
+  // byte offset of 16-byte chunk v of row r: 256 bytes hold 128 / kCols rows, which the permutation keeps
+  auto at_of = [](int r, int v) {
+    return r * (kCols * 2) + ((v ^ (kLanes == 4 ? (r >> 2) & 3 : r & (kLanes - 1))) << 4);
+  };
   const int64_t left = a.m - m0;
   if (left <= 0) return;
   const int rows = left < 32 * MI ? (int)left : 32 * MI, h = lane >> 5, r = lane & 31;
@@ -251,57 +252,74 @@ __device__ __forceinline__ void mx_finish(const GemmArgs& a, uint8_t* lds, int l
   auto load_8 = [](__amdgpu_buffer_rsrc_t rs, int off) {
     return __builtin_bit_cast(V4, __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, 0));
   };
-  auto bias_at = [&](int n) {
-    if (a.bias_f32) return __builtin_bit_cast(f32x4, load_16(bs, n * 4));
-    const V4 v = load_8(bs, n * 2);
-    return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
-  };
+  // the column of this lane's first accumulator of block j (its half for a swiglu), group q; an offset past any
+  // size for one that does not exist
+  auto column = [&](int j, int q) { return n0 + j / kStep * 32 + 8 * q + 4 * h; };
+  auto beyond = [&](int n) { return n < a.n ? 0 : (int)0x80000000; };
+  // the bias of the lane's columns, and a row block's residual: asked for together
+  f32x4 bias[NI][4] = {};
+  V4 rows_of[NI / kStep][4];
+  auto residual = [&](int i) {
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-#pragma unroll
-    for (int j = 0; j < NI; j += kStep) {
-      V4 rv[4];
-      f32x4 b[4], b2[4];
-      if constexpr (!PLAIN) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = n0 + j / kStep * 32 + 8 * q + 4 * h, none = n < a.n ? 0 : (int)0x80000000;
-          rv[q] = load_8(res, (int)((32 * i + r) * a.ldr + n) * 2 | none);
-          // past the last column a column that lies past any bias, in bytes too
-          const int nb = n | (n < a.n ? 0 : 0x10000000);
-          b[q] = bias_at(nb);
-          if constexpr (kGlu) b2[q] = bias_at(nb + a.n);
-        }
-      }
+    for (int j = 0; j < NI; j += kStep)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int n = n0 + j / kStep * 32 + 8 * q + 4 * h, none = n < a.n ? 0 : (int)0x80000000;
+        const int n = column(j, q);
+        rows_of[j / kStep][q] = load_8(res, (int)((32 * i + r) * a.ldr + n) * 2 | beyond(n));
+      }
+  };
+  if constexpr (!PLAIN) {
+    if (a.bias) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          // past the last column a column that lies past any bias, in bytes too
+          const int n = column(j, q), at = (n < a.n ? n : 0x10000000) + (kGlu && (j & 1) ? a.n : 0);
+          if (a.bias_f32) {
+            bias[j][q] = __builtin_bit_cast(f32x4, load_16(bs, at * 4));
+          } else {
+            const V4 v = load_8(bs, at * 2);
+            bias[j][q] = f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    if constexpr (!PLAIN) residual(i);
+#pragma unroll
+    for (int j = 0; j < NI; j += kStep) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
         f32x4 z = {c[i][j][4 * q], c[i][j][4 * q + 1], c[i][j][4 * q + 2], c[i][j][4 * q + 3]};
         if constexpr (!PLAIN) {
+          const V4 rv = rows_of[j / kStep][q];
           f32x4 z2;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            z[e] += b[q][e];
-            if constexpr (kGlu) z2[e] = c[i][j + 1][4 * q + e] + b2[q][e];
+            z[e] += bias[j][q][e];
+            if constexpr (kGlu) z2[e] = c[i][j + 1][4 * q + e] + bias[j + 1][q][e];
           }
           if constexpr (ACT != kActNone) {
-            const int at = ((32 * i + r) * wide + n) * 4 | none;
-            store_16(__builtin_bit_cast(u32x4, z), zs, at);
-            if constexpr (kGlu) store_16(__builtin_bit_cast(u32x4, z2), zs, at + a.n * 4);
+            if (a.z) {
+              const int n = column(j, q), at = ((32 * i + r) * wide + n) * 4 | beyond(n);
+              store_16(__builtin_bit_cast(u32x4, z), zs, at);
+              if constexpr (kGlu) store_16(__builtin_bit_cast(u32x4, z2), zs, at + a.n * 4);
+            }
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             z[e] = act_fwd(ACT, z[e]);
             if constexpr (kGlu) z[e] *= z2[e];
-            z[e] += (float)rv[q][e];
+            z[e] += (float)rv[e];
           }
         }
         V4 o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = (T)z[e];
-        *reinterpret_cast<V4*>(lds + r * PITCH + (j / kStep * 32 + 8 * q + 4 * h) * 2) = o;
+        *reinterpret_cast<V4*>(lds + at_of(r, j / kStep * 4 + q) + 8 * h) = o;
       }
-      if constexpr (!PLAIN) keep_order();
     }
     // the wave's values are written before they are read, and read before the next are written
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -310,7 +328,7 @@ __device__ __forceinline__ void mx_finish(const GemmArgs& a, uint8_t* lds, int l
 #pragma unroll
     for (int u = 0; u < 32 / kRows; ++u) {
       const int row = u * kRows + lane / kLanes;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(lds + row * PITCH + lane % kLanes * 16);
+      const u32x4 v = *reinterpret_cast<const u32x4*>(lds + at_of(row, lane % kLanes));
       store_16(v, out, ((32 * i + row) * a.n + n) * 2 | none);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -318,36 +336,26 @@ __device__ __forceinline__ void mx_finish(const GemmArgs& a, uint8_t* lds, int l
   }
 }
 
-// One tile: rows from m0 and columns from n0 on, columns 256 g0 .. 256 g1 of the contraction; its sums to
-// `part` where that is given, else finished.  LDS holds D stages; a stage is two steps of 64 columns,
-// the next step's fragments read under this one's products.  Before a stage's last step the next
-// stage has arrived and every wave has read this one's last fragments: behind that barrier the loads of
-// the stage D further on go into its place.  Scales go straight to registers, 256 columns ahead.
-template <typename T, typename TL>
-__device__ __forceinline__ void mx_tile(const MxGemmArgs& x, uint8_t* lds, int wave, int lane, int64_t m0, int n0, int g0,
-                                        int g1, float* part) {
+constexpr int kPlain = 8, kAny = 9;
+
+// One tile.  LDS holds D stages; a stage is two steps of 64 columns, the next step's fragments read under
+// this one's products.  Before a stage's last step the next stage has arrived and every wave has read
+// this one's last fragments: behind that barrier the loads of the stage D further on go into its place.
+// Scales go straight to registers, 256 columns ahead.  FIN: the activation (kPlain: no bias and no
+// residual either), a kernel each, so that none carries the others' registers; or kAny for rows that
+// take no 16-byte accesses.
+template <typename T, typename TL, int FIN>
+__device__ __forceinline__ void mx_tile(const MxGemmArgs& x, uint8_t* lds, int wave, int lane, const MxPlace p) {
   const GemmArgs& a = x.g;
-  const bool glu = a.act == kActSwiglu;
+  const bool glu = FIN == kAny ? a.act == kActSwiglu : FIN == kActSwiglu;
+  const int64_t pitch = a.lda * 2, rows = glu ? 2 * (int64_t)a.n : a.n;
   MxOperand<TL::BM, TL::WAVES> A;
   MxOperand<TL::BN, TL::WAVES> B;
   constexpr int LOADS = decltype(A)::LOADS + decltype(B)::LOADS;
-  A.init(a.a, a.lda * 2, m0, a.m, wave, lane, false, 0);
-  B.init(a.b, a.ldb * 2, n0, a.n, wave, lane, glu, a.n);
+  A.init(pitch, wave, lane, false, 0);
+  B.init(pitch, wave, lane, glu, a.n);
   const int wm = wave / TL::WN, wn = wave % TL::WN;
   const int h = lane >> 5, r = lane & 31;
-  MxScales<TL::MI> SA;
-  MxScales<TL::NI> SB;
-  SA.base = x.sa + m0 * 8;
-  SA.step = a.m * 8;
-  SB.base = x.sb;
-  SB.step = (int64_t)(glu ? 2 * a.n : a.n) * 8;
-#pragma unroll
-  for (int i = 0; i < TL::MI; ++i) SA.off[i] = (int)min((int64_t)(wm * TL::MI + i) * 32 + r, a.m - 1 - m0) * 8;
-#pragma unroll
-  for (int i = 0; i < TL::NI; ++i) {
-    const int row = (wn * TL::NI + i) * 32 + r, n = n0 + (glu ? (row >> 6) * 32 + r : row);
-    SB.off[i] = (min(n, a.n - 1) + (glu && (row >> 5 & 1) ? a.n : 0)) * 8;
-  }
   // the fragment of block i in step s: chunk 2 h + s of row r; blocks are 2 KiB apart
   int fa[2], fb[2];
 #pragma unroll
@@ -356,24 +364,27 @@ __device__ __forceinline__ void mx_tile(const MxGemmArgs& x, uint8_t* lds, int w
     fa[s] = wm * TL::MI * 2048 + in;
     fb[s] = TL::A_BYTES + wn * TL::NI * 2048 + in;
   }
-
-  f32x16 acc[TL::MI][TL::NI] = {};
-  i32x4 va[2][TL::MI], vb[2][TL::NI];
+  // the scales of 32 rows in 256 columns (two stages): lane (h, r) loads its row's eight bytes and keeps
+  // the four that it needs, of chunks 2 h and 2 h + 1 of either stage, in the order of the four steps
+  int soa[TL::MI], sob[TL::NI];
+#pragma unroll
+  for (int i = 0; i < TL::MI; ++i) soa[i] = ((wm * TL::MI + i) * 32 + r) * 8;
+#pragma unroll
+  for (int i = 0; i < TL::NI; ++i) {
+    const int row = (wn * TL::NI + i) * 32 + r;
+    sob[i] = glu ? ((row >> 6) * 32 + r + (row >> 5 & 1) * a.n) * 8 : row * 8;
+  }
   uint2 na[TL::MI], nb[TL::NI];
   int sa[TL::MI], sb[TL::NI];
-  auto read = [&](const uint8_t* p, int s) {
-#pragma unroll
-    for (int i = 0; i < TL::NI; ++i) vb[s][i] = operand_at<i32x4>(p + fb[s] + i * 2048);
-#pragma unroll
-    for (int i = 0; i < TL::MI; ++i) va[s][i] = operand_at<i32x4>(p + fa[s] + i * 2048);
-  };
-  auto products = [&](auto step) {  // step of the 256 columns
-    constexpr int S = decltype(step)::value;
+  auto issue_scales = [&](int g) {
+    const __amdgpu_buffer_rsrc_t ra = raw_rsrc(x.sa + ((int64_t)g * a.m + p.m0) * 8, bytes_left(a.m, p.m0, 8));
+    const __amdgpu_buffer_rsrc_t rb = raw_rsrc(x.sb + ((int64_t)g * rows + p.n0) * 8, bytes_left(rows, p.n0, 8));
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i)
+      na[i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(ra, soa[i], 0, 0));
 #pragma unroll
-      for (int j = 0; j < TL::NI; ++j)
-        acc[i][j] = mx32<S>(vb[S & 1][j], sb[j], va[S & 1][i], sa[i], acc[i][j]);
+    for (int i = 0; i < TL::NI; ++i)
+      nb[i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rb, sob[i], 0, 0));
   };
   const uint32_t pick = h ? 0x07060302u : 0x05040100u;
   auto keep_scales = [&]() {
@@ -382,9 +393,31 @@ __device__ __forceinline__ void mx_tile(const MxGemmArgs& x, uint8_t* lds, int w
 #pragma unroll
     for (int i = 0; i < TL::NI; ++i) sb[i] = (int)__builtin_amdgcn_perm(nb[i].y, nb[i].x, pick);
   };
-  auto issue = [&](uint8_t* to, int stage) {
-    A.issue(to, stage, 2 * g1, wave);
-    B.issue(to + TL::A_BYTES, stage, 2 * g1, wave);
+  const uint8_t* const pa = static_cast<const uint8_t*>(a.a) + p.m0 * pitch;
+  const uint8_t* const pb = static_cast<const uint8_t*>(a.b) + p.n0 * pitch;
+  const uint32_t la = bytes_left(a.m, p.m0, pitch), lb = bytes_left(rows, p.n0, pitch);
+  auto issue = [&](uint8_t* to, int t) {  // the loads of stage t: zeros past the last
+    const uint32_t k = (uint32_t)t * 64;
+    const bool none = t >= 2 * p.g1;
+    A.issue(to, pa + k, none ? 0 : la - k, wave);
+    B.issue(to + TL::A_BYTES, pb + k, none ? 0 : lb - k, wave);
+  };
+
+  f32x16 acc[TL::MI][TL::NI] = {};
+  i32x4 va[2][TL::MI], vb[2][TL::NI];
+  auto read = [&](const uint8_t* at, int s) {
+#pragma unroll
+    for (int i = 0; i < TL::NI; ++i) vb[s][i] = operand_at<i32x4>(at + fb[s] + i * 2048);
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i) va[s][i] = operand_at<i32x4>(at + fa[s] + i * 2048);
+  };
+  auto products = [&](auto step) {  // step of the 256 columns
+    constexpr int S = decltype(step)::value;
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::NI; ++j)
+        acc[i][j] = mx32<S>(vb[S & 1][j], sb[j], va[S & 1][i], sa[i], acc[i][j]);
   };
   // the order of one step: the next step's reads first, two a product, then the loads (direct ones
   // stay behind the reads)
@@ -401,53 +434,48 @@ __device__ __forceinline__ void mx_tile(const MxGemmArgs& x, uint8_t* lds, int w
     }
     keep_order();
   };
-  SA.issue(na, g0);
-  SB.issue(nb, g0);
-  int t0 = 2 * g0;
+  issue_scales(p.g0);
 #pragma unroll
-  for (int d = 0; d < TL::D; ++d) issue(lds + d * TL::STAGE, t0 + d);
+  for (int d = 0; d < TL::D; ++d) issue(lds + d * TL::STAGE, 2 * p.g0 + d);
   keep_scales();
   wait_all_but<(TL::D - 1) * LOADS>();
   barrier();
   read(lds, 0);
   int now = 0;  // the present stage's place
-  for (int g = g0; g < g1; ++g) {
+  for (int g = p.g0; g < p.g1; ++g) {
     auto stage = [&](auto half) {
       constexpr int J = decltype(half)::value;
-      uint8_t* const p = lds + now;
-      read(p, 1);
+      uint8_t* const at = lds + now;
+      read(at, 1);
       products(std::integral_constant<int, 2 * J>{});
-      if constexpr (J == 0) {
-        const int next = min(g + 1, g1 - 1);
-        SA.issue(na, next);
-        SB.issue(nb, next);
-      }
+      if constexpr (J == 0) issue_scales(min(g + 1, p.g1 - 1));
       order(std::integral_constant<int, J == 0 ? TL::MI + TL::NI : 0>{});
       // all but the stages after next, and the scales
       wait_all_but<(TL::D - 2) * LOADS + (J == 0 ? TL::MI + TL::NI : 0)>();
       barrier();
-      now = now == (TL::D - 1) * TL::STAGE ? 0 : now + TL::STAGE;
+      now = now == TL::RING - TL::STAGE ? 0 : now + TL::STAGE;
       read(lds + now, 0);
       products(std::integral_constant<int, 2 * J + 1>{});
-      issue(p, t0 + TL::D);
+      issue(at, 2 * g + J + TL::D);
       order(std::integral_constant<int, LOADS>{});
-      ++t0;
     };
     stage(std::integral_constant<int, 0>{});
     stage(std::integral_constant<int, 1>{});
     keep_scales();
   }
   wait_vmem();  // the loads in flight write this workgroup's LDS
-  if (part) {
-    store_piece(part, wave, lane, acc);
+  if (p.part) {
+    store_piece(p.part, wave, lane, acc);
     return;
   }
-  const int64_t mw = m0 + wm * TL::MI * 32;
-  const int nw = n0 + wn * TL::NI * (glu ? 16 : 32);
   barrier();  // every wave has read its last fragments: the stages' LDS is free
-  uint8_t* const mine = lds + wave * TL::OUT;
-  if (!a.vec) {
-    float* const sums = reinterpret_cast<float*>(mine);
+  const int64_t mw = p.m0 + wm * TL::MI * 32;
+  const int nw = p.n0 + wn * TL::NI * (glu ? 16 : 32);
+  if constexpr (FIN != kAny) {
+    mx_finish<T, FIN == kPlain ? kActNone : FIN, FIN == kPlain>(a, lds + wave * TL::OUT, lane, mw, nw, acc);
+  } else {
+    static_assert(TL::WAVES * 32 * kAnyPitch * 4 <= TL::RING, "the sums fit");
+    float* const sums = reinterpret_cast<float*>(lds) + wave * 32 * kAnyPitch;
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i) {
 #pragma unroll
@@ -459,58 +487,71 @@ __device__ __forceinline__ void mx_tile(const MxGemmArgs& x, uint8_t* lds, int w
         __builtin_amdgcn_wave_barrier();
       }
     }
-    return;
   }
-  constexpr int P = TL::OUT_PITCH;
-  if (a.act == kActSwiglu) mx_finish<T, kActSwiglu, false, P>(a, mine, lane, mw, nw, acc);
-  else if (a.act == kActSilu) mx_finish<T, kActSilu, false, P>(a, mine, lane, mw, nw, acc);
-  else if (a.act == kActGelu) mx_finish<T, kActGelu, false, P>(a, mine, lane, mw, nw, acc);
-  else if (a.bias || a.res) mx_finish<T, kActNone, false, P>(a, mine, lane, mw, nw, acc);
-  else mx_finish<T, kActNone, true, P>(a, mine, lane, mw, nw, acc);
 }
 
-// The product by tiles TL, and behind them by tiles TAIL that cover what is left: the rows past the
-// last whole tile row, and the whole tiles of a last round that would leave most of the card idle.
-template <typename T, typename TL, typename TAIL>
-__global__ __launch_bounds__(TL::NT, 2) void mx_gemm_kernel(MxGemmArgs x) {
-  const GemmArgs& a = x.g;
-  static_assert(TL::NT == TAIL::NT, "one workgroup size");
-  __shared__ __align__(1024) uint8_t lds[TL::LDS > TAIL::LDS ? TL::LDS : TAIL::LDS];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int cols = a.act == kActSwiglu ? 2 : 1;  // columns of the product for one of the output
-  const int bid = blockIdx.x;
+// The place of work unit u behind the whole tiles: a piece of a cut tile's contraction.
+template <typename TL>
+__device__ __forceinline__ MxPlace piece_at(const GemmArgs& a, int u) {
+  const int piece = u % a.parts;
   int tm, tn;
+  tile_at<kMxGroup>(a, a.whole + u / a.parts, tm, tn);
+  return {(int64_t)tm * TL::BM, tn * (TL::BN / (a.act == kActSwiglu ? 2 : 1)), (int)((int64_t)a.kt * piece / a.parts),
+          (int)((int64_t)a.kt * (piece + 1) / a.parts), a.part + (int64_t)u * (TL::BM * TL::BN)};
+}
+template <typename TL>
+__device__ __forceinline__ MxPlace whole_at(const GemmArgs& a, int t) {
+  int tm, tn;
+  tile_at<kMxGroup>(a, t, tm, tn);
+  return {(int64_t)tm * TL::BM, tn * (TL::BN / (a.act == kActSwiglu ? 2 : 1)), 0, a.kt, nullptr};
+}
+
+// The product by large tiles, one workgroup a CU, and behind them by small ones that cover what is left: the
+// rows past the last whole tile row, and the whole tiles of a last round that would leave most of the card
+// idle.
+template <typename T, int FIN>
+__global__ __launch_bounds__(MxBig::NT, 2) void mx_gemm_kernel(MxGemmArgs x) {
+  const GemmArgs& a = x.g;
+  static_assert(MxBig::NT == MxTail::NT && MxTail::RING <= MxBig::RING && MxBig::WAVES * MxBig::OUT <= MxBig::RING &&
+                    MxTail::WAVES * MxTail::OUT <= MxTail::RING, "one workgroup size, one LDS");
+  __shared__ __align__(1024) uint8_t lds[MxBig::RING];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, bid = blockIdx.x;
   if (bid < a.whole) {
-    tile_at<kMxGroup>(a, xcd_share(bid, a.whole), tm, tn);
-    mx_tile<T, TL>(x, lds, wave, lane, (int64_t)tm * TL::BM, tn * (TL::BN / cols), 0, a.kt, nullptr);
+    mx_tile<T, MxBig, FIN>(x, lds, wave, lane, whole_at<MxBig>(a, xcd_share(bid, a.whole)));
     return;
   }
-  int u = xcd_share(bid - a.whole, (int)gridDim.x - a.whole);
-  if (a.parts > 1) {  // pieces of the contraction
-    const int t = u / a.parts, piece = u - t * a.parts;
-    tile_at<kMxGroup>(a, a.whole + t, tm, tn);
-    mx_tile<T, TL>(x, lds, wave, lane, (int64_t)tm * TL::BM, tn * (TL::BN / cols),
-                   (int)((int64_t)a.kt * piece / a.parts), (int)((int64_t)a.kt * (piece + 1) / a.parts),
-                   a.part + (int64_t)u * (TL::BM * TL::BN));
+  const int u = xcd_share(bid - a.whole, (int)gridDim.x - a.whole);
+  if (a.parts > 1) {
+    mx_tile<T, MxBig, FIN>(x, lds, wave, lane, piece_at<MxBig>(a, u));
     return;
   }
-  constexpr int KM = TL::BM / TAIL::BM, KN = TL::BN / TAIL::BN;
-  int64_t m0;
-  int n0;
-  const int cut = (a.tm * a.tn - a.whole) * (KM * KN);
+  constexpr int KM = MxBig::BM / MxTail::BM, KN = MxBig::BN / MxTail::BN;
+  const int cut = (a.tm * a.tn - a.whole) * (KM * KN), width = MxTail::BN / (FIN == kActSwiglu ? 2 : 1);
+  MxPlace p;
   if (u < cut) {
-    const int t = u / (KM * KN), in = u - t * (KM * KN);
-    tile_at<kMxGroup>(a, a.whole + t, tm, tn);
-    m0 = (int64_t)tm * TL::BM + in / KN * TAIL::BM;
-    n0 = tn * (TL::BN / cols) + in % KN * (TAIL::BN / cols);
-    if (m0 >= a.m || n0 >= a.n) return;
+    p = whole_at<MxBig>(a, a.whole + u / (KM * KN));
+    p.m0 += u % (KM * KN) / KN * MxTail::BM;
+    p.n0 += u % KN * width;
+    if (p.n0 >= a.n) return;  // a part of the last tile column that lies past the last column
   } else {
-    u -= cut;
-    const int strip = (int)((a.m - (int64_t)a.tm * TL::BM + TAIL::BM - 1) / TAIL::BM);
-    m0 = (int64_t)a.tm * TL::BM + u % strip * TAIL::BM;
-    n0 = u / strip * (TAIL::BN / cols);
+    const int64_t from = (int64_t)a.tm * MxBig::BM;
+    const int v = u - cut, strip = (int)((a.m - from + MxTail::BM - 1) / MxTail::BM);
+    p = {from + v % strip * MxTail::BM, v / strip * width, 0, a.kt, nullptr};
   }
-  mx_tile<T, TAIL>(x, lds, wave, lane, m0, n0, 0, a.kt, nullptr);
+  mx_tile<T, MxTail, FIN>(x, lds, wave, lane, p);
+}
+
+// The product by small tiles, two workgroups a CU.
+template <typename T, int FIN>
+__global__ __launch_bounds__(MxSmall::NT, 2) void mx_small_kernel(MxGemmArgs x) {
+  const GemmArgs& a = x.g;
+  static_assert(MxSmall::RING <= 80 * 1024 && MxSmall::WAVES * MxSmall::OUT <= MxSmall::RING, "two workgroups a CU");
+  __shared__ __align__(1024) uint8_t lds[MxSmall::RING];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, bid = blockIdx.x;
+  if (bid < a.whole)
+    mx_tile<T, MxSmall, FIN>(x, lds, wave, lane, whole_at<MxSmall>(a, xcd_share(bid, a.whole)));
+  else
+    mx_tile<T, MxSmall, FIN>(x, lds, wave, lane, piece_at<MxSmall>(a, xcd_share(bid - a.whole, (int)gridDim.x - a.whole)));
 }
 
 // ---------------------------------------------------------------- few rows
@@ -672,25 +713,39 @@ __global__ __launch_bounds__(64 * kMxSkinnyWaves, MT < 4 ? 2 : 1) void mx_skinny
   }
 }
 
-using MxBig = MxTile<2, 4, 4, 2, 4>;    // 256 x 256, 8 waves of 128 x 64, one workgroup a CU
-using MxTail = MxTile<4, 2, 1, 2, 4>;   // 128 x 128, 8 waves of 32 x 64, behind them
-using MxSmall = MxTile<2, 2, 2, 2, 3>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
 
-template <typename T, typename TL, typename TAIL>
-hipError_t run_mx_tiles(const MxGemmArgs& x, hipStream_t st) {
-  const GemmArgs& a = x.g;
-  const int rest = a.parts > 1 ? (a.tm * a.tn - a.whole) * a.parts : a.tails;
-  mx_gemm_kernel<T, TL, TAIL><<<a.whole + rest, TL::NT, 0, st>>>(x);
+template <typename T, typename TL>
+hipError_t join_mx(const GemmArgs& a, hipStream_t st) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
   join_kernel<T, TL, kMxGroup><<<(a.tm * a.tn - a.whole) * (TL::WAVES * TL::MI * TL::NI / 2) / 4, 256, 0, st>>>(a);
   return hipGetLastError();
 }
 
+template <typename T, int FIN>
+hipError_t run_mx_tiles(const MxGemmArgs& x, hipStream_t st) {
+  const GemmArgs& a = x.g;
+  const int rest = (a.tm * a.tn - a.whole) * a.parts;
+  if constexpr (FIN != kAny) {
+    if (a.big) {
+      mx_gemm_kernel<T, FIN><<<a.whole + (a.parts > 1 ? rest : a.tails), MxBig::NT, 0, st>>>(x);
+      return join_mx<T, MxBig>(a, st);
+    }
+  }
+  mx_small_kernel<T, FIN><<<a.whole + rest, MxSmall::NT, 0, st>>>(x);
+  return join_mx<T, MxSmall>(a, st);
+}
+
 template <typename T>
 hipError_t run_mx(const MxGemmArgs& x, hipStream_t st) {
   const GemmArgs& a = x.g;
-  if (!a.skinny) return a.big ? run_mx_tiles<T, MxBig, MxTail>(x, st) : run_mx_tiles<T, MxSmall, MxSmall>(x, st);
+  if (!a.skinny) {
+    if (!a.vec) return run_mx_tiles<T, kAny>(x, st);
+    if (a.act == kActSwiglu) return run_mx_tiles<T, kActSwiglu>(x, st);
+    if (a.act == kActSilu) return run_mx_tiles<T, kActSilu>(x, st);
+    if (a.act == kActGelu) return run_mx_tiles<T, kActGelu>(x, st);
+    return a.bias || a.res ? run_mx_tiles<T, kActNone>(x, st) : run_mx_tiles<T, kPlain>(x, st);
+  }
   const uint32_t grid = (uint32_t)((a.n + 15) / 16);
   constexpr int NT = 64 * kMxSkinnyWaves;
   if (a.act == kActSwiglu) {
@@ -748,7 +803,8 @@ void mx_gemm_plan(GemmArgs& a) {
     a.tails = (int)tails;
     a.part_floats = sums;
   };
-  for (int big = 1; big >= 0; --big) {
+  // rows that take no 16-byte accesses are the small tiles'
+  for (int big = a.vec ? 1 : 0; big >= 0; --big) {
     const int bm = big ? MxBig::BM : MxSmall::BM, bn = big ? MxBig::BN : MxSmall::BN, slots = big ? 256 : 512;
     const int64_t tm = up(a.m, bm), tn = up(rows, bn), tiles = tm * tn;
     const double stage = big ? 1.0 : tiles <= 256 ? 0.45 : 0.73, start = big ? 1.45 : 0.5;
@@ -768,13 +824,12 @@ void mx_gemm_plan(GemmArgs& a) {
     const int64_t fm = a.m / bm, full = fm * tn, strip = up(a.m - fm * bm, MxTail::BM) * up(rows, MxTail::BN);
     const double tail = a.kt * 0.37 + 0.5;
     const int64_t left = full % slots;
-    // after the whole rounds `left` CUs take a tile each and the others small ones beside them
-    const double one = a.kt * stage + start;
+    const double one = a.kt * stage + start, rounds = (double)(full / slots) * one;
+    // CUs without a tile in the last round take small ones meanwhile
     const int64_t beside = (slots - left) * (int64_t)(one / tail);
-    if (left) take((double)(full / slots + 1) * one + (double)up(strip > beside ? strip - beside : 0, slots) * tail, 1, fm,
-                   tn, full, 1, strip, 0);
-    take((double)(full / slots) * one + (double)up(strip + left * 4, slots) * tail, 1, fm, tn, full - left, 1,
-         strip + left * 4, 0);
+    if (left)
+      take(rounds + one + (double)up(std::max<int64_t>(strip - beside, 0), slots) * tail, 1, fm, tn, full, 1, strip, 0);
+    take(rounds + (double)up(strip + left * 4, slots) * tail, 1, fm, tn, full - left, 1, strip + left * 4, 0);
   }
 }
 
