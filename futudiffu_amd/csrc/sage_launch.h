@@ -346,6 +346,7 @@ struct NormArgs {
   int b, c;
   int64_t n;
   float eps;
+  double inv_c;  // 1 / c, of the norms into MXFP4
   // contiguous outputs [B, N, C]; dx may be null in the backward
   void *out, *hidden, *dx, *dres;
   // parameter gradients (each may be null), in the parameters' types

@@ -345,8 +345,12 @@ __device__ __forceinline__ double token_sum64(double v, double* red, int wave) {
   return v;
 }
 
-__device__ __forceinline__ double rrms64(double sum_sq, int c, float eps) {
-  return 1.0 / sqrt(sum_sq / (double)c + (double)eps);
+// 1 / sqrt(sum_sq / c + eps) by v_rsq_f64 (2^-23 off or less) and one step of third order: a sixth of the
+// instructions of the library's root and quotient.
+__device__ __forceinline__ double rrms64(double sum_sq, double inv_c, float eps) {
+  const double v = fma(sum_sq, inv_c, (double)eps), r = __builtin_amdgcn_rsq(v);
+  const double e = fma(-v * r, r, 1.0);
+  return e == e ? fma(r * e, fma(e, 0.375, 0.5), r) : r;  // of 0 and infinity
 }
 
 // fp64 to fp32 by rounding to odd: what lies beside a border between two codes stays on its
@@ -360,55 +364,110 @@ __device__ __forceinline__ float to_odd(double y) {
   return __uint_as_float(u);
 }
 
-// Forward of the modulated norms with y in MXFP4: norm_fwd_kernel's shares.  Sums, and all
-// that lies between them and the codes, are fp64: fp32 would put one value in 10^6 on the other side
-// of a border between two codes, a whole step away.
+// A lane's eight channels (from `at` on, of c) to codes and the scale of their block.  y: the values
+// in fp32, off by less than 7 of its roundings (2^-24 each); exact(j): in fp64.  Where y (1 +- 2^-21) have the same
+// codes and scale, so has the exact value; where they have not (one in 10^6 values) the wave takes the
+// codes from the exact ones.  So it does where fp32's range may have cost more than that: `odd`, and a block below
+// 2^-30 or not finite.
+template <typename Exact>
+__device__ __forceinline__ uint32_t mx_codes(const float (&y)[kVec], bool odd, int at, int c, Exact exact, int& e) {
+  constexpr float kLow = 1.0f - 0x1p-21f, kHigh = 1.0f + 0x1p-21f;
+  float top = fabsf(y[0]);  // NaN if one is
+#pragma unroll
+  for (int j = 1; j < kVec; ++j) top = __builtin_elementwise_maximum(top, fabsf(y[j]));
+  const float t = __uint_as_float(quad_max(__float_as_uint(top)));
+  e = block_exponent(__float_as_uint(t * kLow));
+  odd = odd || e == 255 || e != block_exponent(__float_as_uint(t * kHigh)) || t < 0x1p-30f;
+  const float sc = scale_of(e);
+  uint32_t lo = 0, hi = 0;
+  auto two = [&](auto q) {
+    constexpr int Q = decltype(q)::value;
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(lo, y[2 * Q] * kLow, y[2 * Q + 1] * kLow, sc, Q);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(hi, y[2 * Q] * kHigh, y[2 * Q + 1] * kHigh, sc, Q);
+  };
+  two(std::integral_constant<int, 0>{});
+  two(std::integral_constant<int, 1>{});
+  two(std::integral_constant<int, 2>{});
+  two(std::integral_constant<int, 3>{});
+  if (__ballot(odd || lo != hi) == 0) return lo;
+  float f[kVec];
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) {
+    f[j] = at + j < c ? to_odd(exact(j)) : 0.0f;
+    most = max(most, __float_as_uint(f[j]) & 0x7fffffffu);
+  }
+  e = block_exponent(quad_max(most));
+  const float s = scale_of(e);
+  uint32_t q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0], f[1], s, 0);
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[2], f[3], s, 1);
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[4], f[5], s, 2);
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[6], f[7], s, 3);
+  return e == 255 ? 0u : q;
+}
+
+// Forward of the modulated norms with y in MXFP4: norm_fwd_kernel's shares.  fp32 would put one value in
+// 10^6 on the other side of a border between two codes, a whole step away: sums, and the hidden stream, are
+// fp64, and the codes those of the exact values (mx_codes).  The instructions bound it (402 a wave for its 16
+// channels a lane): 24 us for 6912 tokens of 3840 channels modulated, 35 us for 4416 gated and modulated, where
+// the bytes take 13.5 and 22.6.  All of it in fp64 took 30.5 and 39.2; a wave a token with 64 channels a lane,
+// which does the sums over lanes once for four times the channels, 25.7 and, for its registers, 69.
 template <typename T, int OP, int TPR, bool VEC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_mx_kernel(NormArgs a, uint8_t* codes, uint8_t* scales) {
   constexpr int NT = TPR > 256 ? TPR : 256;
   constexpr int TOK = NT / TPR;
+  constexpr bool kGate = OP == kNormGateModulate;
   __shared__ double red[NT / 64], red2[NT / 64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * TOK + wave / (TPR / 64), rows = (int64_t)a.b * a.n;
   const bool live = row < rows;  // a thread group past the last token takes part in the barriers alone
-  const int b = live ? (int)(row / a.n) : 0;
+  const int b = live ? (int)((uint32_t)row / (uint32_t)a.n) : 0;  // rows are fewer than 2^23
   const int64_t n = live ? row - (int64_t)b * a.n : 0;
   const int c = live ? a.c : 0;
   const int id = a.doc && live ? load_uniform(a.doc, row) : 0;
   const bool gated = OP == kNormModulate || !no_document(a, id);
-  float x[kPer], r[kPer], w[kPer], k[kPer], w2[kPer], k2[kPer];
+  // w, k: the parameters behind the last norm; w1, g: the gated one's
+  float x[kPer], r[kPer], w1[kPer], g[kPer], w[kPer], k[kPer];
   load_runs<T, TPR, VEC>(row_of<T>(a.x, b, n), t, gated ? c : 0, x);
-  if constexpr (OP == kNormGateModulate) load_runs<T, TPR, VEC>(row_of<T>(a.res, b, n), t, c, r);
-  param_runs<T, TPR, VEC>(a.w.p, a.w.f32, 0, t, c, 1.0f, w);
-  cond_runs<T, TPR, VEC>(a.cond, OP == kNormModulate, b, id, t, c, k);
-  if constexpr (OP == kNormGateModulate) {
-    param_runs<T, TPR, VEC>(a.w2.p, a.w2.f32, 0, t, c, 1.0f, w2);
-    cond_runs<T, TPR, VEC>(a.cond2, true, b, id, t, c, k2);
+  if constexpr (kGate) {
+    load_runs<T, TPR, VEC>(row_of<T>(a.res, b, n), t, c, r);
+    param_runs<T, TPR, VEC>(a.w.p, a.w.f32, 0, t, c, 1.0f, w1);
+    cond_runs<T, TPR, VEC>(a.cond, false, b, id, t, c, g);
   }
+  param_runs<T, TPR, VEC>(kGate ? a.w2.p : a.w.p, kGate ? a.w2.f32 : a.w.f32, 0, t, c, 1.0f, w);
+  cond_runs<T, TPR, VEC>(kGate ? a.cond2 : a.cond, true, b, id, t, c, k);
   double s = 0.0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) s = fma((double)x[j], (double)x[j], s);
   s = token_sum64<TPR>(s, red, wave);
-  const double rr = gated ? rrms64(s, a.c, a.eps) : 0.0;
-  double y[kPer];
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const double m = OP == kNormModulate ? 1.0 + (double)k[j] : (double)k[j];
-    y[j] = (double)x[j] * rr * (double)w[j] * m;
-  }
-  if constexpr (OP == kNormGateModulate) {
+  double rr = gated ? rrms64(s, a.inv_c, a.eps) : 0.0;
+  double h[kPer];  // what the last norm takes
+  if constexpr (kGate) {
     const __amdgpu_buffer_rsrc_t rs = raw_rsrc(static_cast<T*>(a.hidden) + row * a.c, (uint32_t)c * 2);
     s = 0.0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      y[j] += (double)r[j];
-      s = fma(y[j], y[j], s);
+      h[j] = fma((double)x[j] * rr, (double)w1[j] * (double)g[j], (double)r[j]);
+      s = fma(h[j], h[j], s);
     }
 #pragma unroll
     for (int i = 0; i < kPer / kVec; ++i) {
+      // rounded by way of fp32, but for what lies between two values of T there
+      constexpr uint32_t kTie = std::is_same<T, __bf16>::value ? 0x7fffu : 0xfffu;
+      float f[kVec];
+      bool tie = false;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        f[j] = (float)h[i * kVec + j];
+        tie = tie || (__float_as_uint(f[j]) & kTie) == 0;
+      }
+      if (__ballot(tie)) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) f[j] = to_odd(h[i * kVec + j]);
+      }
       typename Vec8<T>::type o;
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) o[j] = (T)to_odd(y[i * kVec + j]);
+      for (int j = 0; j < kVec; ++j) o[j] = (T)f[j];
       const int at = (i * TPR + t) * kVec;
       if constexpr (VEC) {
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rs, at * 2, 0, 0);
@@ -419,29 +478,29 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_mx_kernel(NormArgs
       }
     }
     s = token_sum64<TPR>(s, red2, wave);
-    const double r2 = rrms64(s, a.c, a.eps);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) y[j] = y[j] * r2 * (double)w2[j] * (1.0 + (double)k2[j]);
+    rr = rrms64(s, a.inv_c, a.eps);
   }
+  // rf * wm can leave fp32's range at the bottom only where |wm| is under 2^-66, so that the value is 0 beside
+  // any block that counts
+  const float rf = (float)rr;
+  const bool odd = !(rf > 0x1p-60f && rf < 0x1p60f);
   const int kp = (a.c + 255) / 256 * 256;
 #pragma unroll
   for (int i = 0; i < kPer / kVec; ++i) {
     const int at = (i * TPR + t) * kVec;
-    float f[kVec];
-    uint32_t top = 0;
+    float y[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      f[j] = at + j < a.c ? to_odd(y[i * kVec + j]) : 0.0f;
-      top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+      const int v = i * kVec + j;
+      y[j] = (kGate ? (float)h[v] : x[v]) * (rf * (w[v] * (1.0f + k[v])));
     }
-    const int e = block_exponent(quad_max(top));
-    const float sc = scale_of(e);
-    uint32_t q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0], f[1], sc, 0);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[2], f[3], sc, 1);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[4], f[5], sc, 2);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[6], f[7], sc, 3);
+    int e;
+    const uint32_t q = mx_codes(y, odd, at, a.c, [&](int j) {
+      const int v = i * kVec + j;
+      return (kGate ? h[v] : (double)x[v]) * rr * (double)w[v] * (1.0 + (double)k[v]);
+    }, e);
     if (live && at < kp) {
-      *reinterpret_cast<uint32_t*>(codes + row * (kp / 2) + at / 2) = e == 255 ? 0u : q;
+      *reinterpret_cast<uint32_t*>(codes + row * (kp / 2) + at / 2) = q;
       if ((t & 3) == 0) scales[((int64_t)(at >> 8) * rows + row) * 8 + (at >> 5 & 7)] = (uint8_t)e;
     }
   }
@@ -937,7 +996,9 @@ hipError_t launch_norm_fwd(int op, int f16, const NormArgs& a, hipStream_t st) {
   return f16 ? pick_op<false, _Float16>(op, a, st) : pick_op<false, __bf16>(op, a, st);
 }
 
-hipError_t launch_norm_mx(int op, int f16, const NormArgs& a, uint8_t* codes, uint8_t* scales, hipStream_t st) {
+hipError_t launch_norm_mx(int op, int f16, const NormArgs& args, uint8_t* codes, uint8_t* scales, hipStream_t st) {
+  NormArgs a = args;
+  a.inv_c = 1.0 / (double)a.c;
   if (op == kNormModulate)
     return f16 ? mx_width<_Float16, kNormModulate>(a, codes, scales, st)
                : mx_width<__bf16, kNormModulate>(a, codes, scales, st);
