@@ -1264,11 +1264,15 @@ int sage_mxfp4_linear(const void* x, int64_t x_rs, const void* x_codes, const vo
     return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu", p.bytes(), workspace_bytes);
   if (p.bytes() && !aligned16(workspace)) return fail(SAGE_ERR_ALIGN, "workspace must be 16-byte aligned");
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
-  if (x) {
+  sage::MxGemmArgs a{};
+  if (x && p.g.skinny && m <= sage::kMxQuantRows && k <= sage::kMxQuantCols && in_place(x, x_rs, m, k) && x_rs < (int64_t)1 << 22) {
+    a.x = x;
+    a.ldx = m == 1 ? k : x_rs;
+    a.kx = (int)k;
+  } else if (x) {
     const int e = sage_mxfp4_quantize(x, x_rs, m, k, dtype, ws, ws + p.scales, stream);
     if (e) return e;
   }
-  sage::MxGemmArgs a{};
   a.g = p.g;
   a.g.a = x ? ws : x_codes;
   a.g.b = w_codes;

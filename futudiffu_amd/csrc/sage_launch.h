@@ -438,9 +438,14 @@ struct MxDequantArgs {
 };
 // The product of two MXFP4 operands: g.a, g.b, g.lda, g.ldb and g.k count 16-bit units of four
 // codes; scales of A (g.m rows) and of B (g.n, or 2 g.n rows for a swiglu).
+constexpr int kMxQuantRows = 4, kMxQuantCols = 4096;
 struct MxGemmArgs {
   GemmArgs g;
   const uint8_t *sa, *sb;
+  // x in 16 bits in place of A and sa: at most kMxQuantRows x kMxQuantCols on 16-byte boundaries
+  const void* x;
+  int64_t ldx;
+  int kx;  // columns
 };
 void mx_gemm_plan(GemmArgs& a);
 hipError_t launch_mx_gemm(const MxGemmArgs& a, int f16, hipStream_t st);

@@ -556,25 +556,31 @@ __global__ __launch_bounds__(MxSmall::NT, 2) void mx_small_kernel(MxGemmArgs x) 
 
 // ---------------------------------------------------------------- few rows
 
-constexpr int kMxSkinnyWaves = 4;
-
-// out for at most 16 * MT rows of x, as the linear layers' skinny_kernel: a workgroup reads 16
-// rows of W (of both halves for a swiglu) once, its waves take 256-column stages in turn through
-// rings of LDS slots of their own, and their sums are added in order.  A slot holds, for each
+// out for groups of 16 * MT rows of x (blockIdx.y), as the linear layers' skinny_kernel: a workgroup
+// reads 16 rows of W (of both halves for a swiglu) once, its W waves take 256-column stages in turn
+// through rings of D LDS slots of their own, and their sums are added in order.  A slot holds, for each
 // group of 16 rows, 2 KiB of codes and 128 bytes of scales.
-template <typename T, int MT, bool GLU>
-__global__ __launch_bounds__(64 * kMxSkinnyWaves, MT < 4 ? 2 : 1) void mx_skinny_kernel(MxGemmArgs args) {
+// QX: x is 16-bit, and its up to kMxQuantRows rows are quantized into LDS first, as mx_quantize_kernel
+// does it; each workgroup does so again, while the first stages of W are under way: one row of 3840 onto 11520
+// 7.1 us, onto 15360 from 256 columns 4.3, where a kernel before it makes that 8.3 and 5.0.  Of four rows onto
+// 11520 it is 8.5 and 8.7, and with more the kernel before is faster.
+// What bounds it are the operands' way into LDS (15 TB/s over the chip) and the start: 22 MB of W onto 11520 take
+// 6.2 us with up to 16 rows, 4.4 at the rate of a copy.  Operands read to registers as the matrix
+// instructions take them, without LDS, were slower from 8 rows on (32 rows 12 us, now 7.6).
+template <typename T, int MT, bool GLU, int W, int D, bool QX>
+__global__ __launch_bounds__(64 * W) void mx_skinny_kernel(MxGemmArgs args) {
   const GemmArgs& a = args.g;
-  constexpr int H = GLU ? 2 : 1, TILES = H + MT, PART = 2048 + 128, STAGE = TILES * PART;
-  constexpr int D = TILES == 2 ? 4 : TILES == 3 ? 3 : 2;
-  __shared__ __align__(1024) uint8_t lds[kMxSkinnyWaves * D * STAGE];
-  static_assert(sizeof(lds) <= (MT < 4 ? 80 : 160) * 1024 && H * MT * 1024 <= D * STAGE,
-                "two workgroups a CU, and the sums fit");
+  constexpr int H = GLU ? 2 : 1, TILES = H + (QX ? 0 : MT), PART = 2048 + 128, STAGE = TILES * PART;
+  constexpr int XPART = kMxQuantRows * 136;
+  __shared__ __align__(1024) uint8_t lds[W * D * STAGE + (QX ? kMxQuantCols / 256 * XPART : 0)];
+  static_assert(H * MT * 1024 <= D * STAGE, "the sums fit");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   uint8_t* const mine = lds + wave * D * STAGE;
-  const int64_t pitch = a.ldb * 2, m = a.m;  // bytes of a row of codes, the same on both sides
+  uint8_t* const xlds = lds + W * D * STAGE;
+  const int64_t pitch = a.ldb * 2, m0 = (int64_t)blockIdx.y * 16 * MT;  // bytes of a row of codes, the same on both sides
+  const int m = (int)(a.m - m0), chunks = a.kt;
   const int n0 = blockIdx.x * 16, rows = GLU ? 2 * a.n : a.n;
-  const __amdgpu_buffer_rsrc_t xrs = raw_rsrc(a.a, 0x7fffffff);
+  const __amdgpu_buffer_rsrc_t xrs = raw_rsrc(static_cast<const uint8_t*>(a.a) + m0 * pitch, 0x7fffffff);
   __amdgpu_buffer_rsrc_t wrs[H];
 #pragma unroll
   for (int h = 0; h < H; ++h)
@@ -587,7 +593,7 @@ __global__ __launch_bounds__(64 * kMxSkinnyWaves, MT < 4 ? 2 : 1) void mx_skinny
     const int row = 8 * i + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
     woff[i] = (int)((min(n0 + row, a.n - 1) - n0) * pitch) + c * 16;
 #pragma unroll
-    for (int j = 0; j < MT; ++j) xoff[j][i] = (int)(min((int64_t)(16 * j + row), m - 1) * pitch) + c * 16;
+    for (int j = 0; j < MT; ++j) xoff[j][i] = (int)(min(16 * j + row, m - 1) * pitch) + c * 16;
   }
   // scales: lane l of the lower ones takes four bytes of row l / 2
   const int srow = lane >> 1;
@@ -595,17 +601,18 @@ __global__ __launch_bounds__(64 * kMxSkinnyWaves, MT < 4 ? 2 : 1) void mx_skinny
 #pragma unroll
   for (int h = 0; h < H; ++h) wsoff[h] = (min(n0 + srow, a.n - 1) + h * a.n) * 8 + 4 * (lane & 1);
 #pragma unroll
-  for (int j = 0; j < MT; ++j) xsoff[j] = (int)min((int64_t)(16 * j + srow), m - 1) * 8 + 4 * (lane & 1);
+  for (int j = 0; j < MT; ++j) xsoff[j] = min(16 * j + srow, m - 1) * 8 + 4 * (lane & 1);
   auto issue = [&](uint8_t* stage, int chunk) {
     const int at = chunk * 128;
     const __amdgpu_buffer_rsrc_t wss = raw_rsrc(args.sb + (int64_t)chunk * rows * 8, (uint32_t)rows * 8);
-    const __amdgpu_buffer_rsrc_t xss = raw_rsrc(args.sa + (int64_t)chunk * m * 8, (uint32_t)m * 8);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) dma_16(stage + h * PART + i * 1024, wrs[h], woff[i] + at);
       if (lane < 32) __builtin_amdgcn_raw_ptr_buffer_load_lds(wss, stage + h * PART + 2048, 4, wsoff[h], 0, 0, 0);
     }
+    if constexpr (QX) return;
+    const __amdgpu_buffer_rsrc_t xss = raw_rsrc(args.sa + ((int64_t)chunk * a.m + m0) * 8, (uint32_t)m * 8);
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
 #pragma unroll
@@ -619,37 +626,81 @@ __global__ __launch_bounds__(64 * kMxSkinnyWaves, MT < 4 ? 2 : 1) void mx_skinny
 #pragma unroll
   for (int s = 0; s < 2; ++s) at[s] = r * 128 + (((2 * q + s) ^ ((r >> 1) & 7)) << 4);
   const int sat = 2048 + r * 8 + 2 * q;
+  const int xrow = r % kMxQuantRows;  // QX: rows past the last are some other's, and not stored
   f32x4 acc[H][MT] = {};
-  const int chunks = a.kt;
-  // wave i finishes rows 16 i .. of x: lane (q, r) columns 4 q .. + 3 of row r.  Bias and residual
-  // are asked for first (zeros where there are none) and waited for last.
-  const int64_t mr = 16 * wave + r;
+  // wave i finishes the rows 16 i .. of x and every W-th 16 after: lane (q, r) columns 4 q .. + 3 of
+  // row r.  Bias and residual are asked for first (zeros where there are none) and used last.
+  constexpr int G = (MT + W - 1) / W;
   uint32_t bias[H][4];
-  uint16_t res[4];
+  uint16_t res[G][4];
   if (wave < MT) {
-    const __amdgpu_buffer_rsrc_t brs = raw_rsrc(a.bias, a.bias ? (uint32_t)(a.n * H) * (a.bias_f32 ? 4 : 2) : 0u);
-    const __amdgpu_buffer_rsrc_t rrs = raw_rsrc(a.res, a.res ? 0x7fffffffu : 0u);
+    const __amdgpu_buffer_rsrc_t brs = raw_rsrc(a.bias, a.bias ? (uint32_t)rows * (a.bias_f32 ? 4 : 2) : 0u);
+    const __amdgpu_buffer_rsrc_t rrs = raw_rsrc(static_cast<const T*>(a.res) + m0 * a.ldr, a.res ? 0x7fffffffu : 0u);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int n = n0 + 4 * q + e, out = n < a.n && mr < m ? 0 : (int)0x80000000;
+      const int n = n0 + 4 * q + e, out = n < a.n ? 0 : (int)0x80000000;
 #pragma unroll
       for (int h = 0; h < H; ++h)
         bias[h][e] = a.bias_f32 ? load_4(brs, (n + h * a.n) * 4 | out) : load_2(brs, (n + h * a.n) * 2 | out);
-      res[e] = load_2(rrs, (int)((mr * a.ldr + n) * 2) | out);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const int mr = 16 * (wave + W * g) + r;
+        res[g][e] = load_2(rrs, mr < m ? (int)((mr * a.ldr + n) * 2) | out : (int)0x80000000);
+      }
     }
+    keep_order();
+  }
+  // half a wave quantizes 256 columns of a row; rows 1, 2 or 4 are taken in turn, kAhead in flight
+  constexpr int kAhead = 8;
+  using V = typename Vec8<T>::type;
+  const int shift = m <= 1 ? 0 : m <= 2 ? 1 : 2, units = chunks << shift, col = (lane & 31) * 8;
+  V ahead[QX ? kAhead : 1];
+  auto ask = [&](int u0) {
+    const __amdgpu_buffer_rsrc_t rs = raw_rsrc(args.x, 0x7fffffffu);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int u = u0 + 2 * W * i, row = u & ((1 << shift) - 1), c = (u >> shift) * 256 + col;
+      ahead[i] = __builtin_bit_cast(V, load_16(rs, (int)(row * args.ldx + c) * 2 | (row < m && c < args.kx ? 0 : (int)0x80000000)));
+    }
+  };
+  auto put = [&](int u0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int u = u0 + 2 * W * i, row = u & ((1 << shift) - 1);
+      const int e = block_exponent(quad_max(top_of(ahead[i])));
+      const uint32_t codes = e == 255 ? 0u : codes_of(ahead[i], scale_of(e));
+      if (u < units) {
+        uint8_t* const to = xlds + (u >> shift) * XPART;
+        *reinterpret_cast<uint32_t*>(to + row * 128 + (lane & 31) * 4) = codes;
+        if ((lane & 3) == 0) to[kMxQuantRows * 128 + row * 8 + (lane & 31) / 4] = (uint8_t)e;
+      }
+    }
+  };
+  const int u0 = 2 * wave + (lane >> 5);
+  if constexpr (QX) {
+    ask(u0);
     keep_order();
   }
 #pragma unroll
   for (int d = 0; d < D - 1; ++d)
-    if (wave + d * kMxSkinnyWaves < chunks) issue(mine + d * STAGE, wave + d * kMxSkinnyWaves);
+    if (wave + d * W < chunks) issue(mine + d * STAGE, wave + d * W);
+  if constexpr (QX) {
+    put(u0);
+#pragma unroll 1
+    for (int u = u0 + 2 * W * kAhead; u - (lane >> 5) < units; u += 2 * W * kAhead) {
+      ask(u);
+      put(u);
+    }
+    __syncthreads();
+  }
   int now = 0, free = (D - 1) * STAGE;
 #pragma unroll 1
-  for (int c = wave; c < chunks; c += kMxSkinnyWaves) {
+  for (int c = wave; c < chunks; c += W) {
     // this stage has arrived, and the last one's reads are done: its place takes the next loads
-    if (c + (D - 1) * kMxSkinnyWaves < chunks) {
+    if (c + (D - 1) * W < chunks) {
       wait_all_but<3 * TILES * (D - 2)>();
       hold_memory();
-      issue(mine + free, c + (D - 1) * kMxSkinnyWaves);
+      issue(mine + free, c + (D - 1) * W);
     } else {
       wait_all_but<0>();
       hold_memory();
@@ -659,14 +710,16 @@ __global__ __launch_bounds__(64 * kMxSkinnyWaves, MT < 4 ? 2 : 1) void mx_skinny
 #pragma unroll
     for (int h = 0; h < H; ++h) ws[h] = *reinterpret_cast<const uint16_t*>(stage + h * PART + sat);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) xs[j] = *reinterpret_cast<const uint16_t*>(stage + (H + j) * PART + sat);
+    for (int j = 0; j < MT; ++j)
+      xs[j] = *reinterpret_cast<const uint16_t*>(QX ? xlds + c * XPART + kMxQuantRows * 128 + xrow * 8 + 2 * q
+                                                    : stage + (H + j) * PART + sat);
     auto step = [&](auto s) {
       constexpr int S = decltype(s)::value;
       i32x4 w[H], x[MT];
 #pragma unroll
       for (int h = 0; h < H; ++h) w[h] = operand_at<i32x4>(stage + h * PART + at[S]);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) x[j] = operand_at<i32x4>(stage + (H + j) * PART + at[S]);
+      for (int j = 0; j < MT; ++j) x[j] = operand_at<i32x4>(QX ? xlds + c * XPART + xrow * 128 + (2 * q + S) * 16 : stage + (H + j) * PART + at[S]);
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -686,33 +739,36 @@ __global__ __launch_bounds__(64 * kMxSkinnyWaves, MT < 4 ? 2 : 1) void mx_skinny
 #pragma unroll
     for (int i = 0; i < MT; ++i) part[(h * MT + i) * 64 + lane] = acc[h][i];
   __syncthreads();
-  if (wave >= MT) return;
-  f32x4 z = {}, z2 = {};
-#pragma unroll
-  for (int w = 0; w < kMxSkinnyWaves; ++w) {
-    const f32x4* const p = reinterpret_cast<const f32x4*>(lds + w * D * STAGE) + threadIdx.x;
-    z += p[0];
-    if (GLU) z2 += p[(H - 1) * MT * 64];
-  }
-  if (mr >= m) return;
   auto bias_of = [&](uint32_t v) {
     return a.bias_f32 ? __uint_as_float(v) : (float)__builtin_bit_cast(T, (uint16_t)v);
   };
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int64_t n = n0 + 4 * q + e;
-    if (n >= a.n) continue;
-    const float v = z[e] + bias_of(bias[0][e]), v2 = GLU ? z2[e] + bias_of(bias[H - 1][e]) : 1.0f;
-    if (a.z) {
-      float* row = a.z + mr * a.n * H;
-      row[n] = v;
-      if (GLU) row[a.n + n] = v2;
+  for (int g = 0; g < G; ++g) {
+    const int group = wave + W * g, mr = 16 * group + r;
+    if (group >= MT) return;
+    f32x4 z = {}, z2 = {};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const f32x4* const p = reinterpret_cast<const f32x4*>(lds + w * D * STAGE) + group * 64 + lane;
+      z += p[0];
+      if (GLU) z2 += p[(H - 1) * MT * 64];
     }
-    const float y = act_fwd(a.act, v) * v2 + (float)__builtin_bit_cast(T, res[e]);
-    static_cast<T*>(a.out)[mr * a.n + n] = (T)y;
+    if (mr >= m) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t n = n0 + 4 * q + e;
+      if (n >= a.n) continue;
+      const float v = z[e] + bias_of(bias[0][e]), v2 = GLU ? z2[e] + bias_of(bias[H - 1][e]) : 1.0f;
+      if (a.z) {
+        float* row = a.z + (m0 + mr) * rows;
+        row[n] = v;
+        if (GLU) row[a.n + n] = v2;
+      }
+      const float y = act_fwd(a.act, v) * v2 + (float)__builtin_bit_cast(T, res[g][e]);
+      static_cast<T*>(a.out)[(m0 + mr) * a.n + n] = (T)y;
+    }
   }
 }
-
 
 template <typename T, typename TL>
 hipError_t join_mx(const GemmArgs& a, hipStream_t st) {
@@ -736,6 +792,31 @@ hipError_t run_mx_tiles(const MxGemmArgs& x, hipStream_t st) {
   return join_mx<T, MxSmall>(a, st);
 }
 
+// Waves and LDS slots of a wave.  Up to as many workgroups as the chip holds of them: four waves with deep rings,
+// more bytes in flight on a CU (3840 columns of 3840, one row: 3.7 us against 4.9 for the other).  Past that: two
+// waves, four and more workgroups a CU, so that all run at once (11520 columns: 6.2 us against 7.7; with 64
+// rows 10.7 against 14.5; 15360 of 256: 2.9 against 4.2).
+template <int MT, bool GLU, bool QX>
+struct SkinnyShape {
+  static constexpr int STAGE = ((GLU ? 2 : 1) + (QX ? 0 : MT)) * 2176, XLDS = QX ? kMxQuantCols / 256 * kMxQuantRows * 136 : 0;
+  static constexpr int fit(int bytes) { return (bytes - XLDS) / STAGE; }
+  static constexpr int bound(int d, int lo, int hi) { return d < lo ? lo : d > hi ? hi : d; }
+  // LDS: 80 KB (64 rows: all of it), or 40 KB
+  static constexpr int FEW = bound(fit(80 * 1024) / 4, MT == 4 ? 3 : 2, 4), MANY = bound(fit(40 * 1024) / 2, 2, 3);
+  // the same with QX: its sums are those of the codes, bit for bit
+  static constexpr int FEW_SLOTS = MT == 4 ? 256 : 512;
+};
+
+template <typename T, int MT, bool GLU, bool QX>
+hipError_t run_skinny(const MxGemmArgs& x, hipStream_t st) {
+  const GemmArgs& a = x.g;
+  using S = SkinnyShape<MT, GLU, QX>;
+  const dim3 grid((uint32_t)((a.n + 15) / 16), (uint32_t)((a.m + 16 * MT - 1) / (16 * MT)));
+  if ((int64_t)grid.x * grid.y > S::FEW_SLOTS) mx_skinny_kernel<T, MT, GLU, 2, S::MANY, QX><<<grid, 128, 0, st>>>(x);
+  else mx_skinny_kernel<T, MT, GLU, 4, S::FEW, QX><<<grid, 256, 0, st>>>(x);
+  return hipGetLastError();
+}
+
 template <typename T>
 hipError_t run_mx(const MxGemmArgs& x, hipStream_t st) {
   const GemmArgs& a = x.g;
@@ -746,16 +827,14 @@ hipError_t run_mx(const MxGemmArgs& x, hipStream_t st) {
     if (a.act == kActGelu) return run_mx_tiles<T, kActGelu>(x, st);
     return a.bias || a.res ? run_mx_tiles<T, kActNone>(x, st) : run_mx_tiles<T, kPlain>(x, st);
   }
-  const uint32_t grid = (uint32_t)((a.n + 15) / 16);
-  constexpr int NT = 64 * kMxSkinnyWaves;
-  if (a.act == kActSwiglu) {
-    if (a.m <= 16) mx_skinny_kernel<T, 1, true><<<grid, NT, 0, st>>>(x);
-    else mx_skinny_kernel<T, 2, true><<<grid, NT, 0, st>>>(x);
-  } else if (a.m <= 16) mx_skinny_kernel<T, 1, false><<<grid, NT, 0, st>>>(x);
-  else if (a.m <= 32) mx_skinny_kernel<T, 2, false><<<grid, NT, 0, st>>>(x);
-  else if (a.m <= 48) mx_skinny_kernel<T, 3, false><<<grid, NT, 0, st>>>(x);
-  else mx_skinny_kernel<T, 4, false><<<grid, NT, 0, st>>>(x);
-  return hipGetLastError();
+  const bool glu = a.act == kActSwiglu;
+  if (x.x && glu) return run_skinny<T, 1, true, true>(x, st);
+  if (x.x) return run_skinny<T, 1, false, true>(x, st);
+  if (glu) return a.skinny == 1 ? run_skinny<T, 1, true, false>(x, st) : run_skinny<T, 2, true, false>(x, st);
+  if (a.skinny == 1) return run_skinny<T, 1, false, false>(x, st);
+  if (a.skinny == 2) return run_skinny<T, 2, false, false>(x, st);
+  if (a.skinny == 3) return run_skinny<T, 3, false, false>(x, st);
+  return run_skinny<T, 4, false, false>(x, st);
 }
 
 template <typename T>
@@ -779,22 +858,37 @@ hipError_t run_dequantize(const MxDequantArgs& a, hipStream_t st) {
 void mx_gemm_plan(GemmArgs& a) {
   const bool glu = a.act == kActSwiglu;
   a.kt = (int)(a.k / kBK);
-  a.skinny = a.m <= (glu ? 32 : 64);
   a.thin = 0;
   a.part_floats = 0;
   a.parts = 1;
   a.tm = a.tn = a.whole = 0;
-  if (a.skinny) return;
   // The least estimated time, in 256 columns of the large tile on every CU (1.85 us), where a round of
   // large tiles costs 1.45 more for its start and epilogue.  Measured at 4096 x 4096 x K and its like: small
   // tiles 0.83 us alone on a CU, 1.35 two a CU, the small ones behind large ones 0.68; the sums of
-  // pieces move at 8 TB/s and their join costs 4 us.
+  // pieces move at 8 TB/s and their join costs 4 us; a launch 1.85.  The kernel for few rows: 1.5 us a round and 0.7 for
+  // each 16 rows of x (and the swiglu's second half), its operands at 15 TB/s.  Where the two meet,
+  // few rows and tiles in us: 3840 columns of 3840, 192 rows 10.6 and 13.6, 256 rows 17.8 and 14.6; 11520
+  // columns, 64 rows 10.7 and 12.8, 65 rows 17.7 and 12.9; 15360 columns of 256, 32 rows 3.8 and 3.5, 64
+  // rows 7.2 and 3.7; swiglu to 10240 columns of 3840, 32 rows 10.3 and 13.2, 48 rows 17.1 and 13.5; 1536 columns of
+  // 1536, 256 rows 5.4 and 6.0, 667 rows 9.8 and 6.3; 256 columns of 3840, 2000 rows 8.9 and 10.1, 4000 rows 19.2 and
+  // 10.4.
   const int64_t rows = glu ? 2 * (int64_t)a.n : a.n;
   auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
   double best = 1e30;
+  a.skinny = 0;
+  if (a.m <= 16384) {
+    a.skinny = (int)std::min<int64_t>(up(a.m, 16), glu ? 2 : 4);
+    const int tiles = a.skinny + glu;
+    const int64_t groups = up(a.n, 16) * up(a.m, 16 * a.skinny);
+    // workgroups that the chip holds, as SkinnyShape has them
+    const int few = a.skinny == 4 ? 256 : 512, many = tiles == 4 ? 768 : tiles > 1 ? 1024 : 1536;
+    best = ((double)up(groups, groups > few ? many : few) * (1.5 + 0.7 * tiles) +
+            (double)groups * (tiles + 1) * a.kt * 2048 / 15e6) / 1.85;
+  }
   auto take = [&](double cost, int big, int64_t tm, int64_t tn, int64_t whole, int parts, int64_t tails, int64_t sums) {
-    if (cost >= best) return;
-    best = cost;
+    if (cost + 1.0 >= best) return;
+    best = cost + 1.0;
+    a.skinny = 0;
     a.big = big;
     a.tm = (int)tm;
     a.tn = (int)tn;
@@ -816,7 +910,7 @@ void mx_gemm_plan(GemmArgs& a) {
       if (rest == 0) continue;
       const double bytes = (double)rest * p * bm * bn * 4;
       take((double)(whole / slots) * (a.kt * stage + start) + (double)up(rest * p, slots) * (up(a.kt, p) * stage + start) +
-               2.0 + bytes * 2 / 8e6 / 1.85,
+               3.0 + bytes * 2 / 8e6 / 1.85,
            big, tm, tn, whole, p, 0, rest * p * bm * bn);
     }
     if (!big) continue;

@@ -398,6 +398,44 @@ def test_few_rows(cuda, M, K, N):
         _check(_run(v, act, grads=False), {"out": _want(v, act, False)["out"]}, act)
 
 
+@pytest.mark.parametrize("K,N", [(8, 5), (264, 40), (1000, 8192), (1000, 8208), (3840, 500), (4096, 48), (4104, 48),
+                                 (333, 48)])
+def test_few_rows_quantize_in_place(cuda, K, N):
+    """Up to four rows are quantized by the product itself, where they are aligned and short: the
+    bits of codes that were made before, whatever the rows hold and however they lie."""
+    import futudiffu_amd as F
+    for M in (1, 2, 3, 4, 5):
+        for act, dtype in (("none", BF), ("swiglu", FP)):
+            print(K, N, M, act, flush=True)
+            v = _inputs(M, K, N, act, dtype, F32, True, seed=K + M, device=cuda)
+            x = v["x"]
+            x[M - 1, K - 1] = float("inf")
+            x[M // 2, : K // 2] = 0.0
+            if M > 1:
+                x[0] *= 2.0 ** -14
+            x[M - 1, : K // 3] *= 2.0 ** 9
+            spread = torch.full((M, K + 16), float("nan"), dtype=dtype, device=cuda)
+            spread[:, 8:K + 8] = x
+            for name, rows in (("rows", x), ("spread", spread[:, 8:K + 8]), ("columns", x.T.contiguous().T),
+                               ("one", x[M - 1:].expand(M, K))):
+                args = (v["weight"], v["bias"], v["residual"])
+                got = F.mxfp4_linear(rows, *args, activation=act)
+                want = F.mxfp4_linear(F.mxfp4_quantize(rows), *args, activation=act, dtype=dtype)
+                assert torch.equal(got.view(torch.int16), want.view(torch.int16)), name
+            _check({"out": F.mxfp4_linear(x, *args, activation=act)}, {"out": _want(v, act, False)["out"]}, act)
+
+
+@pytest.mark.parametrize("M,K,N", [(667, 1001, 779), (2000, 3840, 16), (7000, 264, 24), (192, 1536, 3840), (1025, 72, 8),
+                                   (97, 776, 8300)])
+def test_few_columns(cuda, M, K, N):
+    """The few-row form in several groups of 64 rows (of 32 for a swiglu), the last one partly filled."""
+    for i, (act, dtype, bias, res) in enumerate((("none", FP, F32, True), ("silu", BF, None, False),
+                                                 ("swiglu", BF, BF, True))):
+        print(M, K, N, act, flush=True)
+        v = _inputs(M, K, N, act, dtype, bias, res, seed=M + K + i, device=cuda)
+        _check(_run(v, act), _want(v, act), act)
+
+
 # ---------------------------------------------------------------- norms
 
 def _ids(lengths, n, batch):
