@@ -22,6 +22,7 @@ namespace {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // ---------------------------------------------------------------- codes
 
@@ -164,18 +165,21 @@ __device__ __forceinline__ f32x4 mx16(i32x4 a, int sa, i32x4 b, int sb, f32x4 c)
 constexpr int kMxGroup = 8;   // tile rows that the schedule takes together
 
 // A tile shape: WM x WN waves, each with MI x NI blocks of 32 x 32, two waves a SIMD, and D stages
-// of LDS.  A stage is 128 columns: 64 bytes a row.
+// of LDS.  A stage is 128 columns: 64 bytes a row.  The scales of two stages (8 bytes a row) lie behind the ring, in
+// D / 2 places.
 template <int WM_, int WN_, int MI_, int NI_, int D_>
 struct MxTile {
   static constexpr int WM = WM_, WN = WN_, MI = MI_, NI = NI_, D = D_;
   static constexpr int WAVES = WM * WN, NT = 64 * WAVES;
   static constexpr int BM = WM * MI * 32, BN = WN * NI * 32;
   static constexpr int A_BYTES = BM * 64, STAGE = (BM + BN) * 64, RING = D * STAGE;
+  static constexpr int SCALES = (BM + BN) * 8, LDS = RING + D / 2 * SCALES, SLOADS = (SCALES / 256 + WAVES - 1) / WAVES;
   static constexpr int OUT = 32 * NI * 64;  // of the epilogue: 32 rows of a wave's columns
 };
 
 using MxBig = MxTile<2, 4, 4, 2, 4>;    // 256 x 256, 8 waves of 128 x 64, one workgroup a CU
-using MxTail = MxTile<4, 2, 1, 2, 4>;   // 128 x 128, 8 waves of 32 x 64, behind them
+using MxTail = MxTile<4, 2, 1, 2, 4>;    // 128 x 128, 8 waves of 32 x 64, behind them
+using MxMid = MxTile<4, 2, 2, 2, 4>;    // 256 x 128, 8 waves of 64 x 64, one workgroup a CU
 using MxSmall = MxTile<2, 2, 2, 2, 4>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
 
 // One operand's part of an LDS stage: ROWS rows of 64 bytes, row r's 16-byte chunk c at
@@ -351,7 +355,7 @@ __device__ __forceinline__ void mx_tile(const MxGemmArgs& x, uint8_t* lds, int w
   const int64_t pitch = a.lda * 2, rows = glu ? 2 * (int64_t)a.n : a.n;
   MxOperand<TL::BM, TL::WAVES> A;
   MxOperand<TL::BN, TL::WAVES> B;
-  constexpr int LOADS = decltype(A)::LOADS + decltype(B)::LOADS;
+  constexpr int ALOADS = decltype(A)::LOADS, BLOADS = decltype(B)::LOADS, LOADS = ALOADS + BLOADS;
   A.init(pitch, wave, lane, false, 0);
   B.init(pitch, wave, lane, glu, a.n);
   const int wm = wave / TL::WN, wn = wave % TL::WN;
@@ -364,43 +368,47 @@ __device__ __forceinline__ void mx_tile(const MxGemmArgs& x, uint8_t* lds, int w
     fa[s] = wm * TL::MI * 2048 + in;
     fb[s] = TL::A_BYTES + wn * TL::NI * 2048 + in;
   }
-  // the scales of 32 rows in 256 columns (two stages): lane (h, r) loads its row's eight bytes and keeps
-  // the four that it needs, of chunks 2 h and 2 h + 1 of either stage, in the order of the four steps
-  int soa[TL::MI], sob[TL::NI];
+  // the scales of 32 rows in 256 columns (two stages): a load moves them to LDS; lane (h, r) reads its row's
+  // eight bytes and keeps the four that it needs, of chunks 2 h and 2 h + 1 of either stage, in the order of
+  // the four steps.  (Through registers they would be waited for in order, and the stages asked for before
+  // them too.)
+  auto issue_scales = [&](int g) {  // zeros past the last
+    uint8_t* const to = lds + TL::RING + (uint32_t)(g - p.g0) % (TL::D / 2) * TL::SCALES;
 #pragma unroll
-  for (int i = 0; i < TL::MI; ++i) soa[i] = ((wm * TL::MI + i) * 32 + r) * 8;
-#pragma unroll
-  for (int i = 0; i < TL::NI; ++i) {
-    const int row = (wn * TL::NI + i) * 32 + r;
-    sob[i] = glu ? ((row >> 6) * 32 + r + (row >> 5 & 1) * a.n) * 8 : row * 8;
-  }
-  uint2 na[TL::MI], nb[TL::NI];
+    for (int i = 0; i < TL::SLOADS; ++i) {
+      // (of 12 parts and 8 waves four are loaded twice: every wave waits for the same number)
+      const int u = (i * TL::WAVES + wave) % (TL::SCALES / 256), v = u - TL::BM / 32;
+      const bool left = v < 0;
+      const uint8_t* const from = left ? x.sa + ((int64_t)g * a.m + p.m0) * 8 : x.sb + ((int64_t)g * rows + p.n0) * 8;
+      const uint32_t bytes = left ? bytes_left(a.m, p.m0, 8) : bytes_left(rows, p.n0, 8);
+      const int row = left ? u * 32 : glu ? (v >> 1) * 32 + (v & 1) * a.n : v * 32;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(raw_rsrc(from, g < p.g1 ? bytes : 0u), to + u * 256, 4,
+                                               row * 8 + lane * 4, 0, 0, 0);
+    }
+  };
+  u32x2 na[TL::MI], nb[TL::NI];
   int sa[TL::MI], sb[TL::NI];
-  auto issue_scales = [&](int g) {
-    const __amdgpu_buffer_rsrc_t ra = raw_rsrc(x.sa + ((int64_t)g * a.m + p.m0) * 8, bytes_left(a.m, p.m0, 8));
-    const __amdgpu_buffer_rsrc_t rb = raw_rsrc(x.sb + ((int64_t)g * rows + p.n0) * 8, bytes_left(rows, p.n0, 8));
+  auto read_scales = [&](int g) {
+    const uint8_t* const at = lds + TL::RING + (uint32_t)(g - p.g0) % (TL::D / 2) * TL::SCALES + r * 8;
 #pragma unroll
-    for (int i = 0; i < TL::MI; ++i)
-      na[i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(ra, soa[i], 0, 0));
+    for (int i = 0; i < TL::MI; ++i) na[i] = operand_at<u32x2>(at + (wm * TL::MI + i) * 256);
 #pragma unroll
-    for (int i = 0; i < TL::NI; ++i)
-      nb[i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rb, sob[i], 0, 0));
+    for (int i = 0; i < TL::NI; ++i) nb[i] = operand_at<u32x2>(at + TL::BM * 8 + (wn * TL::NI + i) * 256);
   };
   const uint32_t pick = h ? 0x07060302u : 0x05040100u;
   auto keep_scales = [&]() {
 #pragma unroll
-    for (int i = 0; i < TL::MI; ++i) sa[i] = (int)__builtin_amdgcn_perm(na[i].y, na[i].x, pick);
+    for (int i = 0; i < TL::MI; ++i) sa[i] = (int)__builtin_amdgcn_perm(na[i][1], na[i][0], pick);
 #pragma unroll
-    for (int i = 0; i < TL::NI; ++i) sb[i] = (int)__builtin_amdgcn_perm(nb[i].y, nb[i].x, pick);
+    for (int i = 0; i < TL::NI; ++i) sb[i] = (int)__builtin_amdgcn_perm(nb[i][1], nb[i][0], pick);
   };
   const uint8_t* const pa = static_cast<const uint8_t*>(a.a) + p.m0 * pitch;
   const uint8_t* const pb = static_cast<const uint8_t*>(a.b) + p.n0 * pitch;
   const uint32_t la = bytes_left(a.m, p.m0, pitch), lb = bytes_left(rows, p.n0, pitch);
-  auto issue = [&](uint8_t* to, int t) {  // the loads of stage t: zeros past the last
-    const uint32_t k = (uint32_t)t * 64;
-    const bool none = t >= 2 * p.g1;
-    A.issue(to, pa + k, none ? 0 : la - k, wave);
-    B.issue(to + TL::A_BYTES, pb + k, none ? 0 : lb - k, wave);
+  // the loads of stage t: zeros past the last
+  auto issue_a = [&](uint8_t* to, int t) { A.issue(to, pa + t * 64u, t < 2 * p.g1 ? la - t * 64u : 0, wave); };
+  auto issue_b = [&](uint8_t* to, int t) {
+    B.issue(to + TL::A_BYTES, pb + t * 64u, t < 2 * p.g1 ? lb - t * 64u : 0, wave);
   };
 
   f32x16 acc[TL::MI][TL::NI] = {};
@@ -419,45 +427,57 @@ __device__ __forceinline__ void mx_tile(const MxGemmArgs& x, uint8_t* lds, int w
       for (int j = 0; j < TL::NI; ++j)
         acc[i][j] = mx32<S>(vb[S & 1][j], sb[j], va[S & 1][i], sa[i], acc[i][j]);
   };
-  // the order of one step: the next step's reads first, two a product, then the loads (direct ones
-  // stay behind the reads)
-  auto order = [&](auto loads) {
-    constexpr int M = TL::MI * TL::NI, R = TL::MI + TL::NI, E = (R + 1) / 2, L = M - E, N = decltype(loads)::value;
+  // the order of one step: the reads first, two a product, then the loads (direct ones stay behind the
+  // reads)
+  auto order = [&](auto reads, auto loads) {
+    constexpr int M = TL::MI * TL::NI, R = decltype(reads)::value, N = decltype(loads)::value;
+    constexpr int E = (R + 1) / 2 < M ? (R + 1) / 2 : M, L = M - E;
 #pragma unroll
     for (int i = 0; i < M; ++i) {
       order_mfma();
       if (i < E) order_read(), order_read();
-      if (i >= E) {
+      if constexpr (L > 0) {
+        if (i >= E) {
 #pragma unroll
-        for (int l = (i - E) * N / L; l < (i - E + 1) * N / L; ++l) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+          for (int l = (i - E) * N / L; l < (i - E + 1) * N / L; ++l) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+        }
       }
     }
     keep_order();
   };
-  issue_scales(p.g0);
+  constexpr int R = TL::MI + TL::NI, AHEAD = (TL::D / 2 - 1) * (2 * LOADS + TL::SLOADS);
 #pragma unroll
-  for (int d = 0; d < TL::D; ++d) issue(lds + d * TL::STAGE, 2 * p.g0 + d);
-  keep_scales();
-  wait_all_but<(TL::D - 1) * LOADS>();
+  for (int d = 0; d < TL::D; ++d) {
+    issue_a(lds + d * TL::STAGE, 2 * p.g0 + d);
+    if (d < TL::D - 1) issue_b(lds + d * TL::STAGE, 2 * p.g0 + d);
+    if (d % 2 == 0) issue_scales(p.g0 + d / 2);
+  }
+  wait_all_but<AHEAD + ALOADS>();
   barrier();
   read(lds, 0);
-  int now = 0;  // the present stage's place
+  read_scales(p.g0);
+  keep_scales();
+  int now = 0, before = TL::RING - TL::STAGE;  // the present stage's place, and the one before
   for (int g = p.g0; g < p.g1; ++g) {
     auto stage = [&](auto half) {
       constexpr int J = decltype(half)::value;
       uint8_t* const at = lds + now;
       read(at, 1);
       products(std::integral_constant<int, 2 * J>{});
-      if constexpr (J == 0) issue_scales(min(g + 1, p.g1 - 1));
-      order(std::integral_constant<int, J == 0 ? TL::MI + TL::NI : 0>{});
-      // all but the stages after next, and the scales
-      wait_all_but<(TL::D - 2) * LOADS + (J == 0 ? TL::MI + TL::NI : 0)>();
+      issue_b(lds + before, 2 * g + J + TL::D - 1);
+      order(std::integral_constant<int, R>{}, std::integral_constant<int, BLOADS>{});
+      // the next stage is there, and with the second of a pair its scales
+      wait_all_but<AHEAD>();
       barrier();
+      before = now;
       now = now == TL::RING - TL::STAGE ? 0 : now + TL::STAGE;
       read(lds + now, 0);
+      if constexpr (J == 1) read_scales(g + 1);
       products(std::integral_constant<int, 2 * J + 1>{});
-      issue(at, 2 * g + J + TL::D);
-      order(std::integral_constant<int, LOADS>{});
+      issue_a(at, 2 * g + J + TL::D);
+      if constexpr (J == 0) issue_scales(g + TL::D / 2);
+      order(std::integral_constant<int, J == 0 ? R : 2 * R>{},
+            std::integral_constant<int, ALOADS + (J == 0 ? TL::SLOADS : 0)>{});
     };
     stage(std::integral_constant<int, 0>{});
     stage(std::integral_constant<int, 1>{});
@@ -512,9 +532,9 @@ __device__ __forceinline__ MxPlace whole_at(const GemmArgs& a, int t) {
 template <typename T, int FIN>
 __global__ __launch_bounds__(MxBig::NT, 2) void mx_gemm_kernel(MxGemmArgs x) {
   const GemmArgs& a = x.g;
-  static_assert(MxBig::NT == MxTail::NT && MxTail::RING <= MxBig::RING && MxBig::WAVES * MxBig::OUT <= MxBig::RING &&
+  static_assert(MxBig::NT == MxTail::NT && MxTail::LDS <= MxBig::LDS && MxBig::WAVES * MxBig::OUT <= MxBig::RING &&
                     MxTail::WAVES * MxTail::OUT <= MxTail::RING, "one workgroup size, one LDS");
-  __shared__ __align__(1024) uint8_t lds[MxBig::RING];
+  __shared__ __align__(1024) uint8_t lds[MxBig::LDS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, bid = blockIdx.x;
   if (bid < a.whole) {
     mx_tile<T, MxBig, FIN>(x, lds, wave, lane, whole_at<MxBig>(a, xcd_share(bid, a.whole)));
@@ -541,12 +561,21 @@ __global__ __launch_bounds__(MxBig::NT, 2) void mx_gemm_kernel(MxGemmArgs x) {
   mx_tile<T, MxTail, FIN>(x, lds, wave, lane, p);
 }
 
+// The product by tiles of half the size.
+template <typename T, int FIN>
+__global__ __launch_bounds__(MxMid::NT, 2) void mx_mid_kernel(MxGemmArgs x) {
+  static_assert(MxMid::WAVES * MxMid::OUT <= MxMid::RING, "the epilogue fits");
+  __shared__ __align__(1024) uint8_t lds[MxMid::LDS];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  mx_tile<T, MxMid, FIN>(x, lds, wave, lane, whole_at<MxMid>(x.g, xcd_share(blockIdx.x, (int)gridDim.x)));
+}
+
 // The product by small tiles, two workgroups a CU.
 template <typename T, int FIN>
 __global__ __launch_bounds__(MxSmall::NT, 2) void mx_small_kernel(MxGemmArgs x) {
   const GemmArgs& a = x.g;
-  static_assert(MxSmall::RING <= 80 * 1024 && MxSmall::WAVES * MxSmall::OUT <= MxSmall::RING, "two workgroups a CU");
-  __shared__ __align__(1024) uint8_t lds[MxSmall::RING];
+  static_assert(MxSmall::LDS <= 80 * 1024 && MxSmall::WAVES * MxSmall::OUT <= MxSmall::RING, "two workgroups a CU");
+  __shared__ __align__(1024) uint8_t lds[MxSmall::LDS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, bid = blockIdx.x;
   if (bid < a.whole)
     mx_tile<T, MxSmall, FIN>(x, lds, wave, lane, whole_at<MxSmall>(a, xcd_share(bid, a.whole)));
@@ -783,6 +812,10 @@ hipError_t run_mx_tiles(const MxGemmArgs& x, hipStream_t st) {
   const GemmArgs& a = x.g;
   const int rest = (a.tm * a.tn - a.whole) * a.parts;
   if constexpr (FIN != kAny) {
+    if (a.big == 2) {
+      mx_mid_kernel<T, FIN><<<a.whole, MxMid::NT, 0, st>>>(x);
+      return hipGetLastError();
+    }
     if (a.big) {
       mx_gemm_kernel<T, FIN><<<a.whole + (a.parts > 1 ? rest : a.tails), MxBig::NT, 0, st>>>(x);
       return join_mx<T, MxBig>(a, st);
@@ -897,6 +930,10 @@ void mx_gemm_plan(GemmArgs& a) {
     a.tails = (int)tails;
     a.part_floats = sums;
   };
+  if (a.vec) {
+    const int64_t tm = up(a.m, MxMid::BM), tn = up(rows, MxMid::BN), tiles = tm * tn;
+    take((double)up(tiles, 256) * (a.kt * (tiles < 190 ? 0.455 : 0.6) + 1.5), 2, tm, tn, tiles, 1, 0, 0);
+  }
   // rows that take no 16-byte accesses are the small tiles'
   for (int big = a.vec ? 1 : 0; big >= 0; --big) {
     const int bm = big ? MxBig::BM : MxSmall::BM, bn = big ? MxBig::BN : MxSmall::BN, slots = big ? 256 : 512;
