@@ -178,7 +178,7 @@ struct MxTile {
 };
 
 using MxBig = MxTile<2, 4, 4, 2, 4>;    // 256 x 256, 8 waves of 128 x 64, one workgroup a CU
-using MxTail = MxTile<4, 2, 1, 2, 4>;    // 128 x 128, 8 waves of 32 x 64, behind them
+using MxTail = MxTile<4, 2, 1, 2, 4>;   // 128 x 128, 8 waves of 32 x 64, behind them
 using MxMid = MxTile<4, 2, 2, 2, 4>;    // 256 x 128, 8 waves of 64 x 64, one workgroup a CU
 using MxSmall = MxTile<2, 2, 2, 2, 4>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
 
@@ -895,16 +895,18 @@ void mx_gemm_plan(GemmArgs& a) {
   a.part_floats = 0;
   a.parts = 1;
   a.tm = a.tn = a.whole = 0;
-  // The least estimated time, in 256 columns of the large tile on every CU (1.85 us), where a round of
-  // large tiles costs 1.45 more for its start and epilogue.  Measured at 4096 x 4096 x K and its like: small
-  // tiles 0.83 us alone on a CU, 1.35 two a CU, the small ones behind large ones 0.68; the sums of
-  // pieces move at 8 TB/s and their join costs 4 us; a launch 1.85.  The kernel for few rows: 1.5 us a round and 0.7 for
-  // each 16 rows of x (and the swiglu's second half), its operands at 15 TB/s.  Where the two meet,
-  // few rows and tiles in us: 3840 columns of 3840, 192 rows 10.6 and 13.6, 256 rows 17.8 and 14.6; 11520
-  // columns, 64 rows 10.7 and 12.8, 65 rows 17.7 and 12.9; 15360 columns of 256, 32 rows 3.8 and 3.5, 64
-  // rows 7.2 and 3.7; swiglu to 10240 columns of 3840, 32 rows 10.3 and 13.2, 48 rows 17.1 and 13.5; 1536 columns of
-  // 1536, 256 rows 5.4 and 6.0, 667 rows 9.8 and 6.3; 256 columns of 3840, 2000 rows 8.9 and 10.1, 4000 rows 19.2 and
-  // 10.4.
+  // The least estimated time, in units of 1.85 us: 256 columns of the contraction for large tiles on every CU.
+  // The sums of pieces move at 8 TB/s, their join and the launch cost 5.5 us.  Measured, the choice against each
+  // shape alone (small, half, large, in us): 512 x 3840 onto 3840 11.7 (11.6, 16.3, 23.7), 1280 x 10240 onto 3840 40.7
+  // (50.7, 41.4, 56.0), 1536 x 3840 onto 3840 19.5 (21.5, 20.0, 26.0), 2048 x 3840 onto 3840 22.5 (24.1, 22.7,
+  // 27.2), 3000 x 3840 onto 3840 29.7 (35.4, 37.4, 29.8), 4416 x 3840 onto 11520 111 (139, 136, 123), 4416 x 10240
+  // onto 3840 105 (131, 132, 135).
+  // The kernel for few rows: 1.5 us a round and 0.7 for each 16 rows of x (and the swiglu's second half), its
+  // operands at 15 TB/s.  Where the two meet, few rows and tiles in us: 3840 columns of 3840, 192 rows 10.6 and 13.6,
+  // 256 rows 17.8 and 14.6; 11520 columns, 64 rows 10.7 and 12.8, 65 rows 17.7 and 12.9; 15360 columns of 256, 32 rows
+  // 3.8 and 3.5, 64 rows 7.2 and 3.7; swiglu to 10240 columns of 3840, 32 rows 10.3 and 13.2, 48 rows 17.1 and 13.5;
+  // 1536 columns of 1536, 256 rows 5.4 and 6.0, 667 rows 9.8 and 6.3; 256 columns of 3840, 2000 rows 8.9 and 10.1,
+  // 4000 rows 19.2 and 10.4.
   const int64_t rows = glu ? 2 * (int64_t)a.n : a.n;
   auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
   double best = 1e30;
@@ -930,32 +932,42 @@ void mx_gemm_plan(GemmArgs& a) {
     a.tails = (int)tails;
     a.part_floats = sums;
   };
+  // a stage of 256 columns of a round of `n` tiles, by shape: what the power allows past 150 busy CUs
+  auto some = [](int64_t n, double few, double all) { return few + (all - few) * (double)std::max<int64_t>(n - 150, 0) / 106; };
+  auto big_stage = [&](int64_t n) { return some(n, 0.68, 1.0); };
+  auto mid_stage = [&](int64_t n) { return some(n, 0.465, 0.63); };
+  auto small_stage = [](int64_t n) { return n <= 256 ? 0.4 : 0.69; };
+  // n tiles in rounds of `slots`
+  auto rounds_of = [&](int64_t n, int64_t slots, int kt, double start, auto stage) {
+    const int64_t rest = n % slots;
+    return (double)(n / slots) * (kt * stage(slots) + start) + (rest ? kt * stage(rest) + start : 0.0);
+  };
+  constexpr double kBig = 1.7, kMid = 1.2, kSmall = 0.7;  // start and epilogue of a round
   if (a.vec) {
     const int64_t tm = up(a.m, MxMid::BM), tn = up(rows, MxMid::BN), tiles = tm * tn;
-    take((double)up(tiles, 256) * (a.kt * (tiles < 190 ? 0.455 : 0.6) + 1.5), 2, tm, tn, tiles, 1, 0, 0);
+    take(rounds_of(tiles, 256, a.kt, kMid, mid_stage), 2, tm, tn, tiles, 1, 0, 0);
   }
   // rows that take no 16-byte accesses are the small tiles'
   for (int big = a.vec ? 1 : 0; big >= 0; --big) {
     const int bm = big ? MxBig::BM : MxSmall::BM, bn = big ? MxBig::BN : MxSmall::BN, slots = big ? 256 : 512;
-    const int64_t tm = up(a.m, bm), tn = up(rows, bn), tiles = tm * tn;
-    const double stage = big ? 1.0 : tiles <= 256 ? 0.45 : 0.73, start = big ? 1.45 : 0.5;
+    const int64_t tm = up(a.m, bm), tn = up(rows, bn), tiles = tm * tn, rest = tiles % slots, whole = tiles - rest;
+    auto cost = [&](int64_t n, int kt) {
+      return big ? rounds_of(n, slots, kt, kBig, big_stage) : rounds_of(n, slots, kt, kSmall, small_stage);
+    };
     // whole tiles alone
-    take((double)up(tiles, slots) * (a.kt * stage + start), big, tm, tn, tiles, 1, 0, 0);
+    take(cost(tiles, a.kt), big, tm, tn, tiles, 1, 0, 0);
     // the last round's tiles in pieces of the contraction, joined by a second kernel
-    for (int p = 2; p <= 16 && a.kt / p >= 2; ++p) {
-      const int64_t rest = tiles % slots, whole = tiles - rest;
-      if (rest == 0) continue;
+    for (int p = 2; p <= 16 && a.kt / p >= 2 && rest; ++p) {
       const double bytes = (double)rest * p * bm * bn * 4;
-      take((double)(whole / slots) * (a.kt * stage + start) + (double)up(rest * p, slots) * (up(a.kt, p) * stage + start) +
-               3.0 + bytes * 2 / 8e6 / 1.85,
-           big, tm, tn, whole, p, 0, rest * p * bm * bn);
+      take(cost(whole, a.kt) + cost(rest * p, (int)up(a.kt, p)) + 3.0 + bytes * 2 / 8e6 / 1.85, big, tm, tn, whole, p, 0,
+           rest * p * bm * bn);
     }
     if (!big) continue;
     // the rows past the last whole tile row, with or without the last round's tiles, as small ones
     const int64_t fm = a.m / bm, full = fm * tn, strip = up(a.m - fm * bm, MxTail::BM) * up(rows, MxTail::BN);
-    const double tail = a.kt * 0.37 + 0.5;
+    const double tail = a.kt * 0.44 + kSmall;
     const int64_t left = full % slots;
-    const double one = a.kt * stage + start, rounds = (double)(full / slots) * one;
+    const double one = cost(slots, a.kt), rounds = (double)(full / slots) * one;
     // CUs without a tile in the last round take small ones meanwhile
     const int64_t beside = (slots - left) * (int64_t)(one / tail);
     if (left)
