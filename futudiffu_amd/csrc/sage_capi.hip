@@ -1265,7 +1265,9 @@ int sage_mxfp4_linear(const void* x, int64_t x_rs, const void* x_codes, const vo
   if (p.bytes() && !aligned16(workspace)) return fail(SAGE_ERR_ALIGN, "workspace must be 16-byte aligned");
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
   sage::MxGemmArgs a{};
-  if (x && p.g.skinny && m <= sage::kMxQuantRows && k <= sage::kMxQuantCols && in_place(x, x_rs, m, k) && x_rs < (int64_t)1 << 22) {
+  // rows that the product quantizes itself: its loads of x have 32-bit offsets
+  if (x && p.g.skinny && m <= sage::kMxQuantRows && k <= sage::kMxQuantCols && in_place(x, x_rs, m, k) &&
+      (m == 1 || x_rs < (int64_t)1 << 22)) {
     a.x = x;
     a.ldx = m == 1 ? k : x_rs;
     a.kx = (int)k;

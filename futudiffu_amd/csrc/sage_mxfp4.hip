@@ -71,7 +71,8 @@ __device__ __forceinline__ typename Vec8<T>::type load_eight(const T* row, int n
 
 constexpr int kQuantRows = 4;  // rows of a wave, in flight together
 
-// A wave takes 512 columns of kQuantRows rows, a lane eight of each row: four lanes a block.
+// A wave takes 512 columns of kQuantRows rows, a lane eight of each row: four lanes a block.  The bytes bound it:
+// 17408 x 3840, 170 MB in 33 us, a large copy's rate; one row, 1.7 us of latency.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -529,6 +530,15 @@ __device__ __forceinline__ MxPlace whole_at(const GemmArgs& a, int t) {
 // The product by large tiles, one workgroup a CU, and behind them by small ones that cover what is left: the
 // rows past the last whole tile row, and the whole tiles of a last round that would leave most of the card
 // idle.
+// A stage of 256 columns takes a CU 1.24 us when few work, 85 % of the matrix instructions' rate, and 1.85 when
+// all do: the power then allows the matrix instructions alone 5600 to 6300 TFLOP/s on random codes (8500 on zeros).
+// 8192 x 8192 x 8192 258 us, 4250 TFLOP/s (the library's product of the same codes 3185); 4416 x 3840 onto 11520 112
+// us, 3470, with a bias 119; with a swiglu onto 2 x 10240 194 us, 3580: a contraction of 15 stages leaves a
+// fifth of the time to starts and epilogues.
+// Kept out: a persistent workgroup that asks for the next tile during the epilogue (3 % for a product alone, and
+// with a bias or an activation its registers spilled); 128 x 256 tiles by two workgroups a CU (their operands' way
+// to LDS bounds them); rings of five and more stages and other orders of the tiles (no difference); each half
+// of the waves on half of the contraction (none either).
 template <typename T, int FIN>
 __global__ __launch_bounds__(MxBig::NT, 2) void mx_gemm_kernel(MxGemmArgs x) {
   const GemmArgs& a = x.g;
@@ -561,7 +571,10 @@ __global__ __launch_bounds__(MxBig::NT, 2) void mx_gemm_kernel(MxGemmArgs x) {
   mx_tile<T, MxTail, FIN>(x, lds, wave, lane, p);
 }
 
-// The product by tiles of half the size.
+// The product by tiles of half the size, where the large ones would be too few for the CUs: a stage of 256
+// columns takes 0.86 us with 150 busy CUs and 1.14 with all, the way of its operands to LDS and its
+// products one after the other (0.4 us each).  1280 x 10240 onto 3840 41 us, where large tiles in three pieces of the
+// contraction and their sums take 50 and whole ones 56.
 template <typename T, int FIN>
 __global__ __launch_bounds__(MxMid::NT, 2) void mx_mid_kernel(MxGemmArgs x) {
   static_assert(MxMid::WAVES * MxMid::OUT <= MxMid::RING, "the epilogue fits");
@@ -570,7 +583,8 @@ __global__ __launch_bounds__(MxMid::NT, 2) void mx_mid_kernel(MxGemmArgs x) {
   mx_tile<T, MxMid, FIN>(x, lds, wave, lane, whole_at<MxMid>(x.g, xcd_share(blockIdx.x, (int)gridDim.x)));
 }
 
-// The product by small tiles, two workgroups a CU.
+// The product by small tiles, two workgroups a CU: 0.75 us a stage of 256 columns alone on a CU, 1.28 for two, their
+// operands' way to LDS (12 to 15 TB/s over the chip).  512 x 3840 onto 3840 11.7 us.
 template <typename T, int FIN>
 __global__ __launch_bounds__(MxSmall::NT, 2) void mx_small_kernel(MxGemmArgs x) {
   const GemmArgs& a = x.g;
@@ -580,7 +594,8 @@ __global__ __launch_bounds__(MxSmall::NT, 2) void mx_small_kernel(MxGemmArgs x) 
   if (bid < a.whole)
     mx_tile<T, MxSmall, FIN>(x, lds, wave, lane, whole_at<MxSmall>(a, xcd_share(bid, a.whole)));
   else
-    mx_tile<T, MxSmall, FIN>(x, lds, wave, lane, piece_at<MxSmall>(a, xcd_share(bid - a.whole, (int)gridDim.x - a.whole)));
+    mx_tile<T, MxSmall, FIN>(x, lds, wave, lane,
+                             piece_at<MxSmall>(a, xcd_share(bid - a.whole, (int)gridDim.x - a.whole)));
 }
 
 // ---------------------------------------------------------------- few rows
@@ -606,7 +621,8 @@ __global__ __launch_bounds__(64 * W) void mx_skinny_kernel(MxGemmArgs args) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   uint8_t* const mine = lds + wave * D * STAGE;
   uint8_t* const xlds = lds + W * D * STAGE;
-  const int64_t pitch = a.ldb * 2, m0 = (int64_t)blockIdx.y * 16 * MT;  // bytes of a row of codes, the same on both sides
+  // pitch: bytes of a row of codes, the same on both sides
+  const int64_t pitch = a.ldb * 2, m0 = (int64_t)blockIdx.y * 16 * MT;
   const int m = (int)(a.m - m0), chunks = a.kt;
   const int n0 = blockIdx.x * 16, rows = GLU ? 2 * a.n : a.n;
   const __amdgpu_buffer_rsrc_t xrs = raw_rsrc(static_cast<const uint8_t*>(a.a) + m0 * pitch, 0x7fffffff);
@@ -689,7 +705,8 @@ __global__ __launch_bounds__(64 * W) void mx_skinny_kernel(MxGemmArgs args) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int u = u0 + 2 * W * i, row = u & ((1 << shift) - 1), c = (u >> shift) * 256 + col;
-      ahead[i] = __builtin_bit_cast(V, load_16(rs, (int)(row * args.ldx + c) * 2 | (row < m && c < args.kx ? 0 : (int)0x80000000)));
+      const int none = row < m && c < args.kx ? 0 : (int)0x80000000;
+      ahead[i] = __builtin_bit_cast(V, load_16(rs, (int)(row * args.ldx + c) * 2 | none));
     }
   };
   auto put = [&](int u0) {
@@ -748,7 +765,9 @@ __global__ __launch_bounds__(64 * W) void mx_skinny_kernel(MxGemmArgs args) {
 #pragma unroll
       for (int h = 0; h < H; ++h) w[h] = operand_at<i32x4>(stage + h * PART + at[S]);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) x[j] = operand_at<i32x4>(QX ? xlds + c * XPART + xrow * 128 + (2 * q + S) * 16 : stage + (H + j) * PART + at[S]);
+      for (int j = 0; j < MT; ++j)
+        x[j] = operand_at<i32x4>(QX ? xlds + c * XPART + xrow * 128 + (2 * q + S) * 16
+                                    : stage + (H + j) * PART + at[S]);
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -831,7 +850,8 @@ hipError_t run_mx_tiles(const MxGemmArgs& x, hipStream_t st) {
 // rows 10.7 against 14.5; 15360 of 256: 2.9 against 4.2).
 template <int MT, bool GLU, bool QX>
 struct SkinnyShape {
-  static constexpr int STAGE = ((GLU ? 2 : 1) + (QX ? 0 : MT)) * 2176, XLDS = QX ? kMxQuantCols / 256 * kMxQuantRows * 136 : 0;
+  static constexpr int STAGE = ((GLU ? 2 : 1) + (QX ? 0 : MT)) * 2176;
+  static constexpr int XLDS = QX ? kMxQuantCols / 256 * kMxQuantRows * 136 : 0;
   static constexpr int fit(int bytes) { return (bytes - XLDS) / STAGE; }
   static constexpr int bound(int d, int lo, int hi) { return d < lo ? lo : d > hi ? hi : d; }
   // LDS: 80 KB (64 rows: all of it), or 40 KB
@@ -902,11 +922,11 @@ void mx_gemm_plan(GemmArgs& a) {
   // 27.2), 3000 x 3840 onto 3840 29.7 (35.4, 37.4, 29.8), 4416 x 3840 onto 11520 111 (139, 136, 123), 4416 x 10240
   // onto 3840 105 (131, 132, 135).
   // The kernel for few rows: 1.5 us a round and 0.7 for each 16 rows of x (and the swiglu's second half), its
-  // operands at 15 TB/s.  Where the two meet, few rows and tiles in us: 3840 columns of 3840, 192 rows 10.6 and 13.6,
-  // 256 rows 17.8 and 14.6; 11520 columns, 64 rows 10.7 and 12.8, 65 rows 17.7 and 12.9; 15360 columns of 256, 32 rows
-  // 3.8 and 3.5, 64 rows 7.2 and 3.7; swiglu to 10240 columns of 3840, 32 rows 10.3 and 13.2, 48 rows 17.1 and 13.5;
-  // 1536 columns of 1536, 256 rows 5.4 and 6.0, 667 rows 9.8 and 6.3; 256 columns of 3840, 2000 rows 8.9 and 10.1,
-  // 4000 rows 19.2 and 10.4.
+  // operands at 15 TB/s.  Where the two meet, few rows and tiles in us: 3840 columns of 3840, 192 rows 10.6 and 10.8,
+  // 256 rows 17.9 and 11.0; 11520 columns, 48 rows 9.0 and 10.6, 65 rows 17.7 and 10.9; 15360 columns of 256, 32 rows
+  // 3.9 and 3.5, 48 rows 4.6 and 3.6; swiglu to 10240 columns of 3840, 32 rows 10.4 and 10.7, 33 rows 17.9 and 10.7;
+  // 1536 columns of 1536, 256 rows 5.4 and 6.0, 667 rows 9.8 and 6.2; 256 columns of 3840, 2000 rows 8.9 and 14.6,
+  // 4000 rows 19.3 and 10.4.
   const int64_t rows = glu ? 2 * (int64_t)a.n : a.n;
   auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
   double best = 1e30;
@@ -933,7 +953,9 @@ void mx_gemm_plan(GemmArgs& a) {
     a.part_floats = sums;
   };
   // a stage of 256 columns of a round of `n` tiles, by shape: what the power allows past 150 busy CUs
-  auto some = [](int64_t n, double few, double all) { return few + (all - few) * (double)std::max<int64_t>(n - 150, 0) / 106; };
+  auto some = [](int64_t n, double few, double all) {
+    return few + (all - few) * (double)std::max<int64_t>(n - 150, 0) / 106;
+  };
   auto big_stage = [&](int64_t n) { return some(n, 0.68, 1.0); };
   auto mid_stage = [&](int64_t n) { return some(n, 0.465, 0.63); };
   auto small_stage = [](int64_t n) { return n <= 256 ? 0.4 : 0.69; };

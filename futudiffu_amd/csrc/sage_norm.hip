@@ -411,7 +411,8 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&y)[kVec], bool odd, i
 // fp64, and the codes those of the exact values (mx_codes).  The instructions bound it (402 a wave for its 16
 // channels a lane): 24 us for 6912 tokens of 3840 channels modulated, 35 us for 4416 gated and modulated, where
 // the bytes take 13.5 and 22.6.  All of it in fp64 took 30.5 and 39.2; a wave a token with 64 channels a lane,
-// which does the sums over lanes once for four times the channels, 25.7 and, for its registers, 69.
+// which does the sums over lanes once for four times the channels, 25.7 and, for its registers, 69; several
+// tokens a workgroup with their parameters kept and the next token's rows on their way, 24.6 and 33.9 at best.
 template <typename T, int OP, int TPR, bool VEC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_mx_kernel(NormArgs a, uint8_t* codes, uint8_t* scales) {
   constexpr int NT = TPR > 256 ? TPR : 256;
@@ -465,16 +466,16 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_mx_kernel(NormArgs
 #pragma unroll
         for (int j = 0; j < kVec; ++j) f[j] = to_odd(h[i * kVec + j]);
       }
-      typename Vec8<T>::type o;
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) o[j] = (T)f[j];
       const int at = (i * TPR + t) * kVec;
       if constexpr (VEC) {
+        typename Vec8<T>::type o;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) o[j] = (T)f[j];
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rs, at * 2, 0, 0);
       } else {
 #pragma unroll
         for (int j = 0; j < kVec; ++j)
-          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (T)o[j]), rs, (at + j) * 2, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (T)f[j]), rs, (at + j) * 2, 0, 0);
       }
     }
     s = token_sum64<TPR>(s, red2, wave);
