@@ -195,6 +195,29 @@ def test_large_products(cuda, M, K, N, act):
     _check(_run(v, act), _want(v, act), act)
 
 
+@pytest.mark.parametrize("M,K,N,acts", [
+    # large tiles: with rows behind the last whole tile row, with the last round's tiles cut, with both
+    (1110, 526, 7280, "swiglu"), (2229, 300, 7176, "none silu gelu"), (1536, 688, 12280, "none"),
+    (6996, 578, 2352, "silu"), (4876, 300, 1728, "swiglu"),
+    # in pieces of the contraction, and behind a whole round; several rounds
+    (1609, 11030, 1216, "none gelu"), (700, 11030, 1400, "swiglu"), (9361, 3510, 1752, "none"),
+    (1302, 300, 8960, "swiglu"), (1030, 300, 9576, "silu"),
+    # tiles of half the size, one round and two
+    (405, 524, 8520, "none silu gelu"), (137, 575, 8600, "swiglu"), (2319, 2091, 3208, "swiglu"),
+    # small ones in pieces, rows of any alignment, two rounds
+    (66, 4530, 6800, "none silu"), (65, 4937, 6667, "none gelu"), (97, 5792, 4371, "swiglu"),
+    (102, 5196, 4416, "swiglu"), (813, 2875, 9571, "none"), (902, 300, 8387, "silu")])
+def test_every_shape_of_tile(cuda, M, K, N, acts):
+    for act in acts.split():
+        for bias, residual in ((None, False), (F32, True)):
+            print(M, K, N, act, bias, flush=True)
+            v = _inputs(M, K, N, act, BF, bias, residual, seed=M + K, device=cuda)
+            grads = act != "none" and residual  # z from every epilogue
+            _check(_run(v, act, grads=grads, leaves=("bias",) if grads else None),
+                   {k: t for k, t in _want(v, act, grads).items() if k in ("out", "dbias")}, act)
+            del v
+
+
 @pytest.mark.parametrize("M,K,N", [(5, 264, 136), (20, 1000, 1000), (40, 1000, 1000), (64, 600, 500), (200, 331, 140),
                                    (700, 520, 600), (2000, 72, 40), (1500, 2048, 1032), (300, 5000, 2000)])
 def test_small_integers_are_exact(cuda, M, K, N):
@@ -416,7 +439,8 @@ def test_few_rows_quantize_in_place(cuda, K, N):
             x[M - 1, : K // 3] *= 2.0 ** 9
             spread = torch.full((M, K + 16), float("nan"), dtype=dtype, device=cuda)
             spread[:, 8:K + 8] = x
-            for name, rows in (("rows", x), ("spread", spread[:, 8:K + 8]), ("columns", x.T.contiguous().T),
+            off = torch.cat([x.new_zeros(1), x.flatten()])[1:].view(M, K)  # two bytes off a boundary of 16
+            for name, rows in (("rows", x), ("spread", spread[:, 8:K + 8]), ("columns", x.T.contiguous().T), ("off", off),
                                ("one", x[M - 1:].expand(M, K))):
                 args = (v["weight"], v["bias"], v["residual"])
                 got = F.mxfp4_linear(rows, *args, activation=act)
