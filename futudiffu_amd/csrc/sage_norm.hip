@@ -358,7 +358,7 @@ __device__ __forceinline__ double rrms64(double sum_sq, double inv_c, float eps)
 __device__ __forceinline__ float to_odd(double y) {
   const float f = (float)y;
   const double d = y - (double)f;
-  const bool past = (d < 0.0) == (f > 0.0);  // the rounding went away from zero
+  const bool past = fabs((double)f) > fabs(y);  // the rounding went away from zero
   uint32_t u = __float_as_uint(f);
   if (d != 0.0 && d == d) u = (u - (past ? 1u : 0u)) | 1u;  // d is NaN where y is, or infinite
   return __uint_as_float(u);

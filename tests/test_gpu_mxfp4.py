@@ -568,6 +568,68 @@ def test_norms_of_rows_that_are_not_finite(cuda):
     assert hidden[0, 3, 7] == float("inf") and torch.isfinite(hidden).sum() == hidden.numel() - 1
 
 
+def test_norms_of_extreme_sizes(cuda):
+    """Parameters and rows where fp32 leaves its range or keeps few bits of a value: codes as ever."""
+    v = {k: None if t is None else t.to(cuda) for k, t in _norm_inputs(2, 9, 520, BF, F32, seed=4).items()}
+    big, small = 2.0 ** 100, 2.0 ** -100
+
+    def like(t, value):
+        return torch.full_like(t, value)
+
+    some = torch.arange(520, device=cuda) % 3 == 0
+    cases = dict(
+        heavy=dict(weight=v["weight"] * big, next_weight=v["next_weight"] * big),
+        light=dict(weight=v["weight"] * small, next_weight=v["next_weight"] * small),
+        faint=dict(weight=v["weight"] * 2.0 ** -140, next_weight=v["next_weight"] * 2.0 ** -140),
+        mixed=dict(weight=torch.where(some, v["weight"] * big, v["weight"] * small),
+                   next_weight=torch.where(some, v["next_weight"] * big, v["next_weight"] * small)),
+        none=dict(cond=like(v["cond"], -1.0), next_scale=like(v["next_scale"], -1.0)),
+        hardly=dict(cond=like(v["cond"], -1.0 + 2.0 ** -20), next_scale=like(v["next_scale"], -1.0 + 2.0 ** -20)),
+        opposed=dict(cond=v["cond"] * big, next_scale=v["next_scale"] * big, weight=v["weight"] * small,
+                     next_weight=v["next_weight"] * small),
+        vanishing=dict(cond=v["cond"] * 2.0 ** -140, weight=v["weight"] * 2.0 ** -40, residual=like(v["residual"], 0.0)),
+        nothing=dict(cond=like(v["cond"], 0.0), residual=like(v["residual"], 0.0)))
+    for name, change in cases.items():
+        for eps in (EPS, 1e-30, 1e20):
+            print(name, eps, flush=True)
+            _norm_check(dict(v, **change), eps=eps, case=f"{name} {eps}")
+    for scale in (2.0 ** 120, 2.0 ** 60, 2.0 ** -60, 2.0 ** -126, 2.0 ** -132):
+        for eps in (EPS, 0.0):
+            print(scale, eps, flush=True)
+            _norm_check(dict(v, x=v["x"] * scale, residual=v["residual"] * scale), eps=eps, case=f"{scale} {eps}")
+    for bad in (float("nan"), float("inf")):
+        for key in ("weight", "next_weight", "cond", "next_scale"):
+            t = v[key].clone()
+            t[..., 77] = bad
+            y = _norm_codes(dict(v, **{key: t}))
+            for q, want in y:
+                _same(q, O.quantize(want), f"{bad} {key}")
+
+
+def _norm_codes(v):
+    import futudiffu_amd as F
+    x, k = v["x"], v["doc_ids"]
+    first = F.rms_norm_modulate_mxfp4(x, v["weight"], v["cond"], doc_ids=k, eps=EPS)
+    _, second = F.rms_norm_gate_residual_modulate_mxfp4(v["residual"], x, v["weight"], v["cond"], v["next_weight"],
+                                                        v["next_scale"], doc_ids=k, eps=EPS)
+    return ((first, O.norm_values(x, v["weight"], v["cond"], k, EPS)),
+            (second, O.norm_values(x, v["weight"], v["cond"], k, EPS, v["residual"], v["next_weight"], v["next_scale"])[1]))
+
+
+def test_norms_decide_next_to_borders(cuda):
+    """So many values that some lie within fp32's roundings of a border between two codes."""
+    for dtype, params in ((BF, BF), (FP, F32)):
+        v = _norm_inputs(1, 3000, 3840, dtype, params, seed=6)
+        v = {k: None if t is None else t.to(cuda) for k, t in v.items()}
+        for q, y in _norm_codes(v):
+            _same(q, O.quantize(y), f"{dtype}")
+            # y over its block's scale, against the borders
+            e = torch.frexp(y.abs().reshape(-1, 32).amax(-1, keepdim=True))[1] - 3
+            t = torch.ldexp(y.reshape(-1, 32).abs(), -e)
+            near = sum(((t - b).abs() < 2.0 ** -22 * b).sum() for b in (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0))
+            assert near > 0
+
+
 # ---------------------------------------------------------------- traced, refused
 
 def _calls(device, seed=0):
