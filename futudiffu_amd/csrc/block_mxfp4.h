@@ -123,7 +123,8 @@ std::tuple<Tensor, Tensor> mx_product(const MxLinear& a, const Tensor* x, const 
   if (residual) rm.emplace(*residual);
   const void* rp = rm ? rm->p() : nullptr;
   const int64_t rs = rm ? rm->rs : 0;
-  const size_t bytes = lib.sage_mxfp4_linear_workspace_bytes(a.M, a.N, a.w.k, a.act, x != nullptr,
+  const bool near = x && !off16(xm->p()) && a.w.k % 8 == 0 && (a.M == 1 || (xm->rs % 8 == 0 && xm->rs < 1 << 22));
+  const size_t bytes = lib.sage_mxfp4_linear_workspace_bytes(a.M, a.N, a.w.k, a.act, near ? 2 : x ? 1 : 0,
                                                              off16(rp) || off16(ptr(a.bias)) || rs % 8 != 0);
   const Tensor ws = workspace(a.w.codes, bytes);
   const Launch on(a.w.codes);

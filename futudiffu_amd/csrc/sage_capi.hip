@@ -1190,14 +1190,20 @@ int check_mx_linear(int64_t m, int64_t n, int64_t k, int dtype, int activation) 
   return SAGE_OK;
 }
 
+// What a product's x is: codes, 16-bit rows, or such rows on 16-byte boundaries and near enough for 32-bit
+// offsets, which it quantizes itself where they are few and short.
+enum { kMxCodes = 0, kMxRows = 1, kMxNearRows = 2 };
+int mx_rows(const void* x, int64_t rs, int64_t m, int64_t k) {
+  return !x ? kMxCodes : in_place(x, rs, m, k) && (m == 1 || rs < (int64_t)1 << 22) ? kMxNearRows : kMxRows;
+}
+
 // Codes and scales of x in the workspace, and what follows them.
 struct MxLinear {
   size_t scales, part;
+  bool quantizes;  // the product itself
   sage::GemmArgs g{};
-  MxLinear(int64_t m, int64_t n, int64_t k, int act, bool quantize, bool vec) {
+  MxLinear(int64_t m, int64_t n, int64_t k, int act, int x, bool vec) {
     const int64_t kp = sage::mx_cols(k);
-    scales = quantize ? up256((size_t)m * (kp / 2)) : 0;
-    part = quantize ? scales + up256((size_t)m * (kp / 32)) : 0;
     g.vec = vec;
     g.m = m;
     g.n = (int)n;
@@ -1205,6 +1211,10 @@ struct MxLinear {
     g.a_kc = g.b_kc = 1;
     g.act = act;
     sage::mx_gemm_plan(g);
+    quantizes = x == kMxNearRows && g.skinny && m <= sage::kMxQuantRows && k <= sage::kMxQuantCols;
+    const bool quantize = x != kMxCodes && !quantizes;
+    scales = quantize ? up256((size_t)m * (kp / 2)) : 0;
+    part = quantize ? scales + up256((size_t)m * (kp / 32)) : 0;
   }
   size_t bytes() const { return part + (size_t)g.part_floats * 4; }
 };
@@ -1237,8 +1247,8 @@ size_t sage_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int ac
                                          int other_rows) {
   if (check_mx_linear(m, n, k, SAGE_DTYPE_BF16, activation)) return 0;
   // outputs, residual and bias on 16-byte boundaries or not: room for either
-  return std::max(MxLinear(m, n, k, activation, quantize_x, n % 8 == 0).bytes(),
-                  other_rows ? MxLinear(m, n, k, activation, quantize_x, false).bytes() : 0);
+  const size_t bytes = MxLinear(m, n, k, activation, quantize_x, n % 8 == 0).bytes();
+  return other_rows ? std::max(bytes, MxLinear(m, n, k, activation, quantize_x, false).bytes()) : bytes;
 }
 
 int sage_mxfp4_linear(const void* x, int64_t x_rs, const void* x_codes, const void* x_scales, const void* w_codes,
@@ -1259,15 +1269,13 @@ int sage_mxfp4_linear(const void* x, int64_t x_rs, const void* x_codes, const vo
     return fail(SAGE_ERR_ALIGN, "codes must be 16-byte and scales 8-byte aligned");
   const bool vec = n % 8 == 0 && aligned16(out) && aligned16(z) && aligned16(bias) && aligned16(residual) &&
                    (!residual || m == 1 || r_rs % 8 == 0);
-  MxLinear p(m, n, k, activation, x != nullptr, vec);
+  MxLinear p(m, n, k, activation, mx_rows(x, x_rs, m, k), vec);
   if (p.bytes() && (!workspace || workspace_bytes < p.bytes()))
     return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu", p.bytes(), workspace_bytes);
   if (p.bytes() && !aligned16(workspace)) return fail(SAGE_ERR_ALIGN, "workspace must be 16-byte aligned");
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
   sage::MxGemmArgs a{};
-  // rows that the product quantizes itself: its loads of x have 32-bit offsets
-  if (x && p.g.skinny && m <= sage::kMxQuantRows && k <= sage::kMxQuantCols && in_place(x, x_rs, m, k) &&
-      (m == 1 || x_rs < (int64_t)1 << 22)) {
+  if (x && p.quantizes) {
     a.x = x;
     a.ldx = m == 1 ? k : x_rs;
     a.kx = (int)k;

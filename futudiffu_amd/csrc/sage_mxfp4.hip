@@ -939,6 +939,8 @@ void mx_gemm_plan(GemmArgs& a) {
     const int few = a.skinny == 4 ? 256 : 512, many = tiles == 4 ? 768 : tiles > 1 ? 1024 : 1536;
     best = ((double)up(groups, groups > few ? many : few) * (1.5 + 0.7 * tiles) +
             (double)groups * (tiles + 1) * a.kt * 2048 / 15e6) / 1.85;
+    // less than any tiles take, whole or in pieces
+    if (best <= 1.7 + std::min(a.kt * 0.4, 3.0 + a.kt * 0.025)) return;
   }
   auto take = [&](double cost, int big, int64_t tm, int64_t tn, int64_t whole, int parts, int64_t tails, int64_t sums) {
     if (cost + 1.0 >= best) return;

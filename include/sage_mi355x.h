@@ -542,13 +542,15 @@ int sage_mxfp4_dequantize(const void* codes, const void* scales, int64_t m, int6
 
 /* out = act(q(x) weight^T + bias) + residual as sage_linear, both operands MXFP4, fp32
  * accumulation, one rounding to dtype.
- *   x            16-bit rows, quantized in the workspace first; or null, and x_codes,
+ *   x            16-bit rows, quantized in the call; or null, and x_codes,
  *                x_scales hold it.
  *   w_codes, w_scales  the weight's rows: n, or 2 n for SAGE_ACT_SWIGLU; under 2^22 rows and
  *                under 2^31 bytes of codes.
  *   others       as in sage_linear (dtype: of x, residual, out and a bias that is not fp32).
  *   workspace    sage_mxfp4_linear_workspace_bytes(...) bytes, 16-byte aligned; needs no
- *                clearing.  quantize_x: whether x is given; other_rows as in sage_linear. */
+ *                clearing.  quantize_x: 0 where x_codes are given, 1 for an x, 2 for an x whose rows
+ *                are on 16-byte boundaries, k a multiple of 8 and x_rs under 2^22 (never more than
+ *                for 1); other_rows as in sage_linear. */
 size_t sage_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int activation, int quantize_x,
                                          int other_rows);
 int sage_mxfp4_linear(const void* x, int64_t x_rs, const void* x_codes, const void* x_scales, const void* w_codes,

@@ -202,7 +202,7 @@ def test_quantize_entries_refuse(over, status, msg):
 ])
 def test_linear_entry_refuses(over, status, msg):
     lib = _lib.load()
-    a = dict(x=16, xrs=40, xc=None, xs=None, w=64, ws=64, bias=None, bf32=0, r=None, rrs=16, m=4, n=16, k=40, dt=0, act=0,
+    a = dict(x=16, xrs=40, xc=None, xs=None, w=64, ws=64, bias=None, bf32=0, r=None, rrs=16, m=5, n=16, k=40, dt=0, act=0,
              wksp=None, bytes=0, z=None, out=64, st=None)
     a.update(over)
     assert lib.sage_mxfp4_linear(*a.values()) == status
@@ -258,6 +258,8 @@ def test_workspace_sizes():
         for act in range(4):
             with_x, without = size(m, n, k, act, 1, 1), size(m, n, k, act, 0, 1)
             assert held <= with_x - without <= held + 512
+            # rows on 16-byte boundaries: the product quantizes few and short ones itself
+            assert size(m, n, k, act, 2, 1) == (without if m <= 4 and k <= 4096 else with_x)
     for m, n, k, act in ((0, 1, 1, 0), (1, 0, 1, 0), (1, 1, 0, 0), (1 << 24, 1, 1, 0), (1, 1 << 22, 1, 0), (1, 1, 1 << 22, 0),
                          (1, 1, 1, 9), (4, 1 << 20, 4096, 0)):
         assert size(m, n, k, act, 1, 1) == 0
