@@ -535,7 +535,7 @@ __device__ __forceinline__ MxPlace whole_at(const GemmArgs& a, int t) {
 // A stage of 256 columns takes a CU 1.24 us when few work, 85 % of the matrix instructions' rate, and 1.85 when
 // all do: the power then allows the matrix instructions alone 5600 to 6300 TFLOP/s on random codes (8500 on zeros).
 // 8192 x 8192 x 8192 258 us, 4250 TFLOP/s (the library's product of the same codes 3185); 4416 x 3840 onto 11520 112
-// us, 3470, with a bias 119; with a swiglu onto 2 x 10240 194 us, 3580: a contraction of 15 stages leaves a
+// us, 3470, with a bias 118; with a swiglu onto 2 x 10240 194 us, 3580: a contraction of 15 stages leaves a
 // fifth of the time to starts and epilogues.
 // Kept out: a persistent workgroup that asks for the next tile during the epilogue (3 % for a product alone, and
 // with a bias or an activation its registers spilled); 128 x 256 tiles by two workgroups a CU (their operands' way
