@@ -383,6 +383,51 @@ def test_other_stream_overlap_and_graph(cuda):
             assert all(torch.equal(got[k], want[k]) for k in want)
 
 
+def test_graphs_of_one_pool_and_streams(cuda):
+    """Products in pieces, of half tiles and of rows that they quantize themselves: two graphs whose workspaces lie in
+    one pool replayed in turn on changing inputs, and eager calls on two streams at once."""
+    import futudiffu_amd as F
+    sizes = ((1609, 11030, 1216, "none"), (66, 4530, 6800, "silu"), (405, 524, 8520, "gelu"), (2, 264, 8208, "none"),
+             (3, 1000, 48, "swiglu"), (200, 5000, 2000, "none"))
+
+    def inputs(seed):
+        return [_inputs(M, K, N, act, BF, F32, True, seed=seed + i, device=cuda)
+                for i, (M, K, N, act) in enumerate(sizes)]
+
+    def run(vs):
+        return [F.mxfp4_linear(v["x"], v["weight"], v["bias"], v["residual"], activation=s[3]) for v, s in zip(vs, sizes)]
+
+    statics, graphs, outs, pool = [inputs(0), inputs(10)], [], [], None
+    for static in statics:
+        run(static)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(run(static))
+        pool = graph.pool()
+        graphs.append(graph)
+    for turn in range(3):
+        for i in (0, 1):
+            new = inputs(100 * (turn + 1) + 10 * i)
+            for old, v in zip(statics[i], new):
+                for k in ("x", "bias", "residual"):
+                    old[k].copy_(v[k])
+                old["weight"].codes.copy_(v["weight"].codes)
+                old["weight"].scales.copy_(v["weight"].scales)
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert _equal(outs[i], run(new)), (turn, i)
+    want = [run(v) for v in statics]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for v, stream in zip(statics, streams):
+            with torch.cuda.stream(stream):
+                got.append(run(v))
+        assert all(_equal(g, w) for g, w in zip(got, want))
+
+
 def test_offsets_past_32_bits(cuda):
     """An x, and a dequantized tensor, of more than 2^32 bytes, all zeros but a few rows.  Small
     integers, so every sum is exact."""
