@@ -389,7 +389,9 @@ struct GemmArgs {
   void* out;  // T [m][n]
   int vec;    // rows of res, z and out, and the bias, take 16-byte accesses
   // the plan (gemm_plan)
-  int big, skinny, thin, kt, tm, tn;
+  int big;              // large tiles or small ones; MXFP4: 2 for those of half the size
+  int skinny, thin;     // few rows: which side; MXFP4: 16-row blocks of a group
+  int kt, tm, tn;
   int whole, parts;     // tiles past `whole` run as `parts` pieces of the contraction
   int tails;            // MXFP4 with one piece: small tiles that cover what the whole ones leave
   int64_t part_floats;  // fp32 sums of the pieces
@@ -436,9 +438,9 @@ struct MxDequantArgs {
   int64_t ldo;
   int vec;
 };
+constexpr int kMxQuantRows = 4, kMxQuantCols = 4096;  // of an x that the product can quantize itself
 // The product of two MXFP4 operands: g.a, g.b, g.lda, g.ldb and g.k count 16-bit units of four
 // codes; scales of A (g.m rows) and of B (g.n, or 2 g.n rows for a swiglu).
-constexpr int kMxQuantRows = 4, kMxQuantCols = 4096;
 struct MxGemmArgs {
   GemmArgs g;
   const uint8_t *sa, *sb;

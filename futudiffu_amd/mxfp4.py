@@ -191,7 +191,7 @@ def mxfp4_linear(x: Tensor | MXFP4, weight: MXFP4, bias: Tensor | None = None, r
 def rms_norm_modulate_mxfp4(x: Tensor, weight: Tensor | None = None, scale: Tensor | None = None, *,
                             doc_ids: Tensor | None = None, eps: float = 1e-5) -> MXFP4:
     """:func:`futudiffu_amd.rms_norm_modulate` in MXFP4, quantized from the unrounded values
-    (formed in fp64: a value next to a border between two codes falls on its own side)."""
+    (a value next to a border between two codes is decided in fp64 and falls on its own side)."""
     if _traced_without_grad(x, weight, scale):
         return MXFP4(*torch.ops.futudiffu_ii.rms_norm_modulate_mxfp4(x, weight, scale, doc_ids, eps), x.shape[-1])
     return MXFP4(*_native().rms_norm_modulate_mxfp4(x, weight, scale, doc_ids, eps), x.shape[-1])

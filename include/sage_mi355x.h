@@ -569,7 +569,7 @@ int sage_mxfp4_linear_bwd(const void* dout, int64_t d_rs, const void* w_codes, c
                           size_t workspace_bytes, void* dx, void* dbias, hipStream_t stream);
 
 /* sage_rms_norm_modulate with its output in MXFP4, quantized from the unrounded values (sums
- * and products in fp64, so that a value next to a border between two codes falls on its own
+ * in fp64; a value next to a border between two codes is decided there and falls on its own
  * side).  codes, scales: b * n rows of c columns. */
 int sage_rms_norm_modulate_mxfp4(const void* x, int64_t x_bs, int64_t x_rs, const void* weight,
                                  const void* scale, int64_t scale_bs, int64_t scale_gs, int64_t groups,
