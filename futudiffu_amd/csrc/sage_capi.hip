@@ -952,13 +952,15 @@ struct LinearBwd {
   bool form_dz;     // dz is formed (an activation, or rows that no product can read in place)
   bool dz_in_place; // dout itself is the products' operand
   int64_t ldz;
+  int64_t plane;    // elements between dz's two parts; 0: it has one
   size_t dz_off, sum_off, part_off, bytes;
   int64_t chunks, chunk;
   sage::GemmArgs gx{}, gw{};
   // x and weight as rows whose columns the products read 16 bytes at a time
   size_t x_off, w_off;
   bool copy_x, copy_w;
-  // form_w: the weight's rows are formed in the workspace, whatever w is
+  // form_w: the weight's rows are formed in the workspace, whatever w is, and the dz of an
+  // activation is two bf16 matrices
   LinearBwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs, const void* w, int64_t w_rs, int64_t m,
             int64_t n, int64_t k, int act, int want, bool form_w = false) {
     rows = act == SAGE_ACT_SWIGLU ? 2 * n : n;
@@ -968,7 +970,8 @@ struct LinearBwd {
     ldz = form_dz ? up8(rows) : m == 1 ? up8(rows) : d_rs;
     size_t at = 0;
     dz_off = at;
-    if (form_dz) at += up256((size_t)(m * ldz) * 2);
+    plane = form_w && form_dz && act != SAGE_ACT_NONE ? (int64_t)(up256((size_t)(m * ldz) * 2) / 2) : 0;
+    if (form_dz) at += up256((size_t)(m * ldz) * 2) * (plane ? 2 : 1);
     // bias: chunks of at least 32 rows, at most 256 of them
     chunk = (m + 255) / 256 < 32 ? 32 : (m + 255) / 256;
     chunks = (m + chunk - 1) / chunk;
@@ -990,6 +993,8 @@ struct LinearBwd {
       gx.lda = ldz;
       gx.ldb = copy_w ? up8(k) : rows == 1 ? up8(k) : w_rs;
       gx.vec = k % 8 == 0;  // dx and dweight start on 16-byte boundaries
+      gx.half = plane ? (rows + 63) / 64 * 64 : 0;
+      gx.plane = plane;
       sage::gemm_plan(gx);
       part = (size_t)gx.part_floats * 4;
     }
@@ -1029,6 +1034,7 @@ int run_linear_bwd(const LinearBwd& plan, const void* dout, int64_t d_rs, const 
     d.act = activation;
     d.dz = p.form_dz ? ws + p.dz_off : nullptr;
     d.ldz = p.ldz;
+    d.plane = d.dz ? p.plane : 0;
     d.vec = in_place(dout, d_rs, m, n) && aligned16(z);
     d.part = dbias ? reinterpret_cast<float*>(ws + p.sum_off) : nullptr;
     d.chunks = p.chunks;
@@ -1042,7 +1048,7 @@ int run_linear_bwd(const LinearBwd& plan, const void* dout, int64_t d_rs, const 
   if (dx && w_codes) {
     const sage::MxDequantArgs q{w_codes, w_scales,      p.rows, (int)up8(k), (int)sage::mx_cols(k),
                                 ws + p.w_off, up8(k), 1};
-    const hipError_t e = sage::launch_mx_dequantize(q, dtype, stream);
+    const hipError_t e = sage::launch_mx_dequantize(q, p.plane ? SAGE_DTYPE_BF16 : dtype, stream);
     if (e != hipSuccess) return launch_status(e, "sage_mxfp4_linear_bwd (weight)");
   } else if (p.copy_x || p.copy_w) {
     const hipError_t e = sage::launch_pack({p.copy_x ? x : nullptr, x_rs, m, k, ws + p.x_off, up8(k)},

@@ -374,10 +374,15 @@ constexpr int kActNone = 0, kActSilu = 1, kActGelu = 2, kActSwiglu = 3;
 // [k][m]; B likewise.  Rows from 16-byte boundaries, lda and ldb multiples of 8.  An
 // operand with the contraction contiguous has k columns, k a multiple of 8 (zeros behind
 // kv); one without has kv rows.
+// half > 0 (a_kc, not b_kc, act none): A is the sum of two bf16 matrices, the second `plane`
+// elements behind the first, and B is bf16: the contraction runs over the first's stages, from
+// `half` on (the first multiple of a stage) over the second's and B's rows again.  k and kv are
+// those of one of them.
 struct GemmArgs {
   const void *a, *b;
   int64_t lda, ldb;
   int64_t m, k, kv;
+  int64_t half, plane;
   int n;  // columns of the output (swiglu: B has 2 n rows, the gates and then the others)
   int a_kc, b_kc;
   int act;
@@ -413,6 +418,7 @@ struct DactArgs {
   int n, act;
   void* dz;  // rows ldz apart; null: not formed
   int64_t ldz;
+  int64_t plane;  // not 0: dz is two bf16 matrices whose sum it is, the second this many elements on
   int vec;  // every row takes 16-byte accesses (n a multiple of 8)
   float* part;  // column sums [chunks][n or 2n]; null: no bias gradient
   int64_t chunks, chunk;

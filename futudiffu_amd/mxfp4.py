@@ -174,8 +174,9 @@ def mxfp4_linear(x: Tensor | MXFP4, weight: MXFP4, bias: Tensor | None = None, r
     ``weight`` holds rows ``[N, K]``, ``bias``, ``residual`` and ``activation`` are
     :func:`futudiffu_amd.fused_linear`'s.  Sums are fp32, the output is rounded once.
 
-    The gradient of a tensor ``x`` is ``dz weight`` over the weight's values in ``x``'s type, with
-    ``dz = dout * act'(z)`` rounded to that type; for an activation the forward keeps ``z`` in fp32.
+    The gradient of a tensor ``x`` is ``dz weight``, rounded once: for an activation the forward keeps
+    ``z`` in fp32, and ``dz = dout * act'(z)`` enters the product as two bfloat16 parts.  Without
+    one ``dz`` is ``dout``, and the weight's values are taken in ``x``'s type.
     """
     if isinstance(x, MXFP4):
         if _traced_without_grad(bias, residual):

@@ -558,9 +558,10 @@ int sage_mxfp4_linear(const void* x, int64_t x_rs, const void* x_codes, const vo
                       int64_t m, int64_t n, int64_t k, int dtype, int activation, void* workspace,
                       size_t workspace_bytes, float* z, void* out, hipStream_t stream);
 
-/* Gradients, the rounding of x taken as the identity: dz = dout * act'(z) rounded to dtype as
- * the product's operand, dx = dz weight over the weight's values in dtype, dbias = the unrounded
- * dz's column sums; each null if not wanted.  Arguments as in sage_linear_bwd; the weight's 16-bit
+/* Gradients, the rounding of x taken as the identity: dz = dout * act'(z), dx = dz weight, dbias =
+ * dz's column sums; each null if not wanted.  Of an activation dz enters the product as two bf16
+ * matrices (2^-17 of a value is lost) and the weight in bf16; without one it is dout itself and the
+ * weight's values are in dtype.  Arguments as in sage_linear_bwd; the weight's 16-bit
  * rows (formed in the workspace) have under 2^31 bytes. */
 size_t sage_mxfp4_linear_bwd_workspace_bytes(const void* dout, int64_t d_rs, int64_t m, int64_t n, int64_t k,
                                              int activation, int want);

@@ -15,6 +15,7 @@ from oracle import block_oracle as B
 
 VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 MFMA = 2.0 ** -14
+DZ = 2.0 ** -17  # what the two bf16 parts of an activation's dz leave of it: half a step of half a step
 
 
 def columns_held(k: int) -> int:
@@ -67,12 +68,12 @@ def rounded(x: Tensor) -> Tensor:
 
 def linear(x: Tensor, weight: Tensor, bias, residual, activation: str, dout=None) -> dict[str, tuple[Tensor, Tensor]]:
     """``{name: (exact, bound)}`` of mxfp4_linear over a weight of these exact values, and with
-    ``dout`` its gradients: block_oracle's of the rounded ``x``, whose products are off by MFMA
-    times the sum of their sizes on top, and that through the activation (its slope is at most
-    1.13, its curvature too)."""
+    ``dout`` its gradients: block_oracle's of the rounded ``x`` in 64 bits (whose dz it does not
+    round), whose products are off by MFMA times the sum of their sizes on top, and that through
+    the activation (its slope is at most 1.13, its curvature too); the dz of an activation by DZ of it."""
     k = x.shape[-1]
     q = rounded(x).reshape(-1, k)
-    ref = B.linear(q.to(x.dtype), weight, bias, None if residual is None else residual.reshape(q.shape[0], -1),
+    ref = B.linear(q, weight, bias, None if residual is None else residual.reshape(q.shape[0], -1),
                    activation, None if dout is None else dout.reshape(q.shape[0], -1))
     size = q.abs() @ weight.double().abs().T
     more = MFMA * size
@@ -93,14 +94,16 @@ def linear(x: Tensor, weight: Tensor, bias, residual, activation: str, dout=None
         return r
     g = dout.reshape(q.shape[0], -1).double().abs()
     if activation == "none":
-        dz = torch.zeros_like(more)
+        dz = size = torch.zeros_like(more)
     elif activation == "swiglu":
         dz = torch.cat([g * (1.13 * m1 * (z2.abs() + m2) + 1.13 * m2), g * 1.13 * m1], -1)
+        size = torch.cat([g * 1.13 * (z2.abs() + m2), g * (f + 1.13 * m1)], -1)
     else:
         dz = g * 1.13 * more
-    dz = dz * (1 + torch.finfo(x.dtype).eps)
+        size = g * 1.13
     exact, bound = ref["dx"]
-    r["dx"] = (exact.reshape(x.shape), (bound + dz @ weight.double().abs()).reshape(x.shape))
+    off = dz + DZ * (size + dz)  # of the operand
+    r["dx"] = (exact.reshape(x.shape), (bound + off @ weight.double().abs()).reshape(x.shape))
     if bias is not None:
         r["dbias"] = (ref["dbias"][0], ref["dbias"][1] + dz.sum(0))
     if residual is not None:

@@ -350,6 +350,37 @@ def test_gradient_against_differences(cuda):
         assert abs(float(num - ana)) <= float(noise + own + cubic), (act, float(num), float(ana))
 
 
+@pytest.mark.parametrize("M,K,N,act,dtype", [(667, 1001, 779, "silu", FP), (331, 520, 777, "gelu", BF),
+                                             (700, 264, 300, "swiglu", BF), (40, 72, 65, "swiglu", FP),
+                                             (1300, 700, 5000, "silu", BF), (64, 1032, 4100, "swiglu", FP)])
+def test_dx_has_its_own_rounding_alone(cuda, M, K, N, act, dtype):
+    """How far dx is from the exact gradient, over all elements, against the exact values rounded
+    to its type: what enters the product loses 2^-17 of a value or less, beside the 2^-12 (rms, of fp16)
+    of the rounding under 2^-10 of it in quadrature; 32-bit sums of up to 10000 terms, and z's, under
+    2^-16 of a value, 2^-8 of it in quadrature; 1 % is allowed.  A dz rounded to 16 bits would add 40 %."""
+    v = _inputs(M, K, N, act, dtype, dtype, False, seed=M, device=cuda)
+    got, exact = _run(v, act)["dx"].double(), _want(v, act)["dx"][0]
+    want = float((exact.to(dtype).double() - exact).norm() / exact.norm())
+    off = float((got - exact).norm() / exact.norm())
+    print(act, dtype, f"{off:.4g} expected {want:.4g}", flush=True)
+    assert off <= 1.01 * want, (off, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_dz_past_the_types_range(cuda, dtype):
+    """dout * act'(z) past fp16's largest value and under its smallest, beside a weight that brings dx back
+    into the range: dx is the exact gradient's, rounded once."""
+    # dz around 2^20 over a weight around 2^-16, and around 2^-23 over one around 2^8
+    for zoom, up, thin, gate in ((-12, 2.0 ** 9, 1.0, 1000.0), (12, 2.0 ** -20, 2.0 ** -14, 0.0)):
+        v = _inputs(150, 264, 72, "swiglu", dtype, F32, False, seed=3, device=cuda)
+        w = v["weight"]
+        scales = (w.scales.int() + zoom).clamp_min(0).to(torch.uint8)
+        v.update(weight=w._replace(scales=scales), values=O.dequantize(w.codes, scales, w.columns),
+                 x=v["x"] * thin, dout=v["dout"] * up)
+        v["bias"][72:] = v["bias"][72:] * 2.0 ** -6 + gate
+        _check(_run(v, "swiglu"), _want(v, "swiglu"), f"{dtype} {zoom}")
+
+
 def test_other_stream_overlap_and_graph(cuda):
     a = _inputs(700, 1032, 640, "swiglu", BF, BF, True, seed=1, device=cuda)
     b = _inputs(40, 2048, 1000, "silu", FP, None, False, seed=2, device=cuda)
