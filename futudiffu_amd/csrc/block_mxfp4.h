@@ -237,11 +237,14 @@ struct MxLinearFn : torch::autograd::Function<MxLinearFn> {
     ctx->saved_data["columns"] = columns;
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["residual"] = residual.has_value();
+    // x is not saved, but its gradient and the bias's depend on it
+    ctx->saved_data["x_requires"] = x.requires_grad();
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
     const auto s = ctx->get_saved_variables();
     once({d[0], s[2]});
+    TORCH_CHECK(!at::GradMode::is_enabled() || !ctx->saved_data["x_requires"].toBool(), kTwice);
     // x, codes, scales, bias, then the residual's edge
     const Wanted all = needs(ctx, {s[0], s[0], s[1], s[2], ctx->saved_data["residual"].toBool() ? s[0] : Tensor()});
     const Wanted w = {all[0], all[3]};

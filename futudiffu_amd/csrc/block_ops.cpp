@@ -480,11 +480,11 @@ variable_list gradients(const torch::jit::Stack& returned, const Wanted& w) {
 }
 
 // The gradients are not themselves differentiable.
+constexpr const char* kTwice = "the gradients of the block operators cannot be differentiated (create_graph=True)";
 void once(const variable_list& args) {
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor& t : args)
-    TORCH_CHECK(!t.defined() || !t.requires_grad(),
-                "the gradients of the block operators cannot be differentiated (create_graph=True)");
+    TORCH_CHECK(!t.defined() || !t.requires_grad(), kTwice);
 }
 
 bool any_requires(std::initializer_list<const Tensor*> tensors) {

@@ -125,11 +125,14 @@ def _linear_setup(ctx, inputs, output):
     ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(codes, scales, bias, output[1])
     ctx.columns, ctx.activation = columns, activation
+    ctx.x_requires = x.requires_grad  # x is not saved, but its gradient and the bias's depend on it
 
 
 def _linear_autograd(ctx, dout, dz):
     codes, scales, bias, z = ctx.saved_tensors
     _b._once(dout, bias)
+    if ctx.x_requires and torch.is_grad_enabled():
+        raise RuntimeError(_b._TWICE)
     wanted = [ctx.needs_input_grad[0], bias is not None and ctx.needs_input_grad[4]]
     dx = db = None
     if any(wanted):

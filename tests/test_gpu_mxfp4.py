@@ -818,6 +818,31 @@ def test_linear_op_check_and_compile(cuda):
                           test_utils=checks)
 
 
+@pytest.mark.parametrize("act", ["none", "silu", "swiglu"])
+def test_second_derivatives_raise(cuda, act):
+    """The function and the op, with x the only leaf (a frozen bias or none), beside a bias, and by a
+    transform; the residual's gradient alone is the incoming one."""
+    import futudiffu_amd as F
+    v = _inputs(24, 40, 16, act, BF, F32, True, seed=4, device=cuda)
+    w, d = v["weight"], v["dout"]
+    calls = (lambda x, b, r: F.mxfp4_linear(x, w, b, r, activation=act),
+             lambda x, b, r: torch.ops.futudiffu_ii.mxfp4_linear(x, *w, b, r, act, True)[0])
+    for call in calls:
+        for b in (v["bias"], None):
+            x = v["x"].detach().requires_grad_()
+            want = torch.autograd.grad(call(x, b, v["residual"]), x, d)[0]
+            assert torch.equal(want, _run(dict(v, bias=b), act)["dx"])
+            with pytest.raises(RuntimeError, match="create_graph"):
+                torch.autograd.grad(call(x, b, v["residual"]), x, d, create_graph=True)
+            with pytest.raises(RuntimeError):  # torch's own: the ops have no formula for transforms
+                torch.func.grad(lambda t: call(t, b, v["residual"]).float().sum())(v["x"])
+        x, b = v["x"].detach().requires_grad_(), v["bias"].detach().requires_grad_()
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(call(x, b, None), b, d, create_graph=True)
+        r = v["residual"].detach().requires_grad_()
+        assert torch.equal(torch.autograd.grad(call(v["x"], v["bias"], r), r, d, create_graph=True)[0], d)
+
+
 # ---------------------------------------------------------------- together
 
 H, D, C, F_ = 4, 64, 256, 640

@@ -170,6 +170,37 @@ def test_fakes_have_the_outputs_shapes():
         assert h.shape == x.shape and c.shape == codes.shape and s.shape == scales.shape
 
 
+@pytest.mark.parametrize("act", ["none", "silu", "swiglu"])
+def test_gradients_of_the_op_are_not_differentiated(act):
+    """As fused_linear's: whichever of x and the bias wants a gradient, alone or beside the other,
+    create_graph=True raises.  A residual's gradient is the incoming one, which may be differentiated."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x, r = torch.empty(5, 40, dtype=BF), torch.empty(5, 4, dtype=BF)
+        n = 8 if act == "swiglu" else 4
+        w = torch.empty(n, 128, dtype=torch.uint8), torch.empty(1, n, 8, dtype=torch.uint8), 40
+        bias = torch.empty(n)
+        for wants, of, twice in (("x", "x", False), ("b", "b", False), ("xb", "b", False), ("xb", "x", False),
+                                 ("r", "r", True), ("xr", "r", False)):
+            for b in (bias, None):
+                t = dict(x=x.detach(), b=None if b is None else b.detach(), r=r.detach())
+                if any(t[k] is None for k in wants):
+                    continue
+                for k in wants:
+                    t[k].requires_grad_()
+
+                def grad(**kw):
+                    out = torch.ops.futudiffu_ii.mxfp4_linear(t["x"], *w, t["b"], t["r"], act, True)[0]
+                    return torch.autograd.grad(out, t[of], torch.ones_like(out), **kw)[0]
+
+                assert grad().shape == t[of].shape
+                if twice:
+                    assert grad(create_graph=True).shape == r.shape
+                else:
+                    with pytest.raises(RuntimeError, match="create_graph"):
+                        grad(create_graph=True)
+
+
 # ---- the C entries
 
 @fake_addresses
