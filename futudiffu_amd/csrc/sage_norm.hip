@@ -391,14 +391,30 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&y)[kVec], bool odd, i
   two(std::integral_constant<int, 3>{});
   if (__ballot(odd || lo != hi) == 0) return lo;
   float f[kVec];
-  uint32_t most = 0;
+  auto take = [&](double unit) {
+    uint32_t most = 0;
 #pragma unroll
-  for (int j = 0; j < kVec; ++j) {
-    f[j] = at + j < c ? to_odd(exact(j)) : 0.0f;
-    most = max(most, __float_as_uint(f[j]) & 0x7fffffffu);
+    for (int j = 0; j < kVec; ++j) {
+      f[j] = at + j < c ? to_odd(exact(j) * unit) : 0.0f;
+      most = max(most, __float_as_uint(f[j]) & 0x7fffffffu);
+    }
+    return quad_max(most);
+  };
+  uint32_t most = take(1.0);
+  // a finite value past fp32's range became its largest: such a block's are taken 2^-16 times, and past the
+  // largest scale (2^127) the code is that of 6
+  int up = 0;
+  if (__ballot(most == 0x7f7fffffu)) {
+    up = most == 0x7f7fffffu ? 16 : 0;
+    most = take(up ? 0x1p-16 : 1.0);
+    const float six = up ? 6.0f * 0x1p111f : INFINITY;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) f[j] = fminf(fmaxf(f[j], -six), six);
   }
-  e = block_exponent(quad_max(most));
+  e = block_exponent(most);
+  e = e == 255 ? 255 : min(e, 254 - up);
   const float s = scale_of(e);
+  e = e == 255 ? 255 : e + up;
   uint32_t q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0], f[1], s, 0);
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[2], f[3], s, 1);
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[4], f[5], s, 2);

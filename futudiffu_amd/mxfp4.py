@@ -7,7 +7,7 @@
 
 Columns in blocks of 32 share a scale ``2^e``; a column is a 4-bit code (e2m1), one of ``0, 0.5,
 1, 1.5, 2, 3, 4, 6`` with a sign, times the scale.  Of a block whose largest magnitude is
-``amax``, ``e = max(floor(log2 amax) - 2, -127)`` (the OCP microscaling specification's rule); codes are
+``amax``, ``e = floor(log2 amax) - 2`` (the OCP microscaling specification's rule), from -127 to 127; codes are
 the nearest, ties to the even one, and past 6 the code of 6.  A block that holds NaN or an
 infinity is NaN as a whole.
 
@@ -161,8 +161,8 @@ def mxfp4_quantize(x: Tensor) -> MXFP4:
 
 
 def mxfp4_dequantize(q: MXFP4, *, dtype: torch.dtype = torch.bfloat16) -> Tensor:
-    """What ``q`` stands for, as bfloat16 (exactly) or float16 (rounded where that is subnormal,
-    infinite past 65504)."""
+    """What ``q`` stands for, as bfloat16 (exactly; infinite from ``2^128`` on, which only a norm's output
+    reaches) or float16 (rounded where that is subnormal, infinite past 65504)."""
     if torch.compiler.is_compiling():
         return torch.ops.futudiffu_ii.mxfp4_dequantize(q.codes, q.scales, q.columns, dtype)
     return _native().mxfp4_dequantize(q.codes, q.scales, q.columns, dtype)

@@ -526,7 +526,7 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
  *                of its byte, zeros behind column k.  16-byte aligned.
  *   scales       [kp / 256][m][8] bytes e + 127: scales[g][r][i] of row r's columns
  *                256 g + 32 i .. + 31; 255: the block is NaN.  8-byte aligned.
- * Quantizing takes e = max(floor(log2 amax) - 2, -127) of a block's largest magnitude amax and
+ * Quantizing takes e = floor(log2 amax) - 2, from -127 to 127, of a block's largest magnitude amax and
  * the nearest code of x / 2^e, ties to the even code, past 6 the code of 6; a block that holds NaN
  * or an infinity becomes NaN.  Exact in every step but the rounding.
  * m at least 1 and below 2^24, k at least 1 and below 2^22. */
@@ -535,8 +535,8 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
 int sage_mxfp4_quantize(const void* x, int64_t x_rs, int64_t m, int64_t k, int dtype, void* codes, void* scales,
                         hipStream_t stream);
 
-/* out: [m][k] contiguous; what the codes stand for, in fp16 rounded where it is subnormal there
- * and infinite past 65504. */
+/* out: [m][k] contiguous; what the codes stand for, in bf16 infinite from 2^128 on (no 16-bit value's
+ * code, but a norm's), in fp16 rounded where it is subnormal there and infinite past 65504. */
 int sage_mxfp4_dequantize(const void* codes, const void* scales, int64_t m, int64_t k, int dtype, void* out,
                           hipStream_t stream);
 

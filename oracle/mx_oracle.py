@@ -33,8 +33,8 @@ def quantize(x: Tensor) -> tuple[Tensor, Tensor]:
     amax = b.abs().amax(-1)
     finite = torch.isfinite(b).all(-1)
     e = torch.frexp(torch.where(finite, amax, 1.0))[1].double() - 1  # amax = m 2^e, 1 <= m < 2
-    e = torch.where(amax == 0, -127.0, (e - 2).clamp(min=-127.0))
-    r = torch.where(finite[..., None], b, 0.0) / torch.exp2(e)[..., None]
+    e = torch.where(amax == 0, -127.0, (e - 2).clamp(-127.0, 127.0))
+    r = (torch.where(finite[..., None], b, 0.0) / torch.exp2(e)[..., None]).clamp(-8.0, 8.0)
     # the nearest of the values; of two equally near the even code
     table = torch.tensor(VALUES, dtype=torch.float64, device=x.device)
     code = torch.zeros(r.shape, dtype=torch.uint8, device=x.device)

@@ -682,6 +682,34 @@ def test_norms_of_extreme_sizes(cuda):
                 _same(q, O.quantize(want), f"{bad} {key}")
 
 
+def test_norms_past_the_range_of_fp32(cuda):
+    """Values of 2^128 and more, which a block's scale can hold up to 6 x 2^127 and which are the code of 6
+    past that; beside blocks that fp32 holds, and beside an infinity."""
+    import futudiffu_amd as F
+    for C in (520, 1001, 3840):
+        v = {k: None if t is None else t.to(cuda) for k, t in _norm_inputs(2, 9, C, BF, F32, seed=5).items()}
+        few = torch.arange(C, device=cuda) // 32 % 3 == 0
+        top = 0
+        for zoom in (-4, -2, -1, 0, 1, 2, 3, 9, 30, 100):
+            for part in (torch.ones_like(few), few):
+                print(C, zoom, bool(part.all()), flush=True)
+                w = torch.where(part, v["weight"] * 2.0 ** 126, v["weight"])
+                w2 = torch.where(part, v["next_weight"] * 2.0 ** 126, v["next_weight"])
+                u = dict(v, weight=w, next_weight=w2, cond=v["cond"] * 2.0 ** zoom, next_scale=v["next_scale"] * 2.0 ** zoom)
+                got = F.rms_norm_modulate_mxfp4(u["x"], w, u["cond"], eps=EPS)
+                _same(got, O.quantize(O.norm_values(u["x"], w, u["cond"], None, EPS)), zoom)
+                h, y = O.norm_values(u["x"], v["weight"], v["cond"], None, EPS, u["residual"], w2, u["next_scale"])
+                got2 = F.rms_norm_gate_residual_modulate_mxfp4(u["residual"], u["x"], v["weight"], v["cond"], w2,
+                                                               u["next_scale"], eps=EPS)[1]
+                _same(got2, O.quantize(y), zoom)
+                top = max(top, int(got.scales[got.scales < 255].max()))
+        assert top == 254
+        bad = w.clone()
+        bad[3] = float("inf")
+        _same(F.rms_norm_modulate_mxfp4(v["x"], bad, v["cond"], eps=EPS),
+              O.quantize(O.norm_values(v["x"], bad, v["cond"], None, EPS)), "inf")
+
+
 def _norm_codes(v):
     import futudiffu_amd as F
     x, k = v["x"], v["doc_ids"]

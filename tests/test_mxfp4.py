@@ -55,6 +55,15 @@ def test_oracle_scales():
     assert back[0, :32].isnan().all() and back[1, 32:].isnan().all() and not back[0, 32:].isnan().any()
 
 
+def test_oracle_past_the_largest_scale():
+    """The scale stops at 2^127 and the codes at 6."""
+    x = torch.zeros(5, 32, dtype=torch.float64)
+    x[:, 0] = torch.tensor([1.9 * 2.0 ** 128, 2.0 ** 129, 7.9 * 2.0 ** 127, 2.0 ** 130, 2.0 ** 200], dtype=torch.float64)
+    codes, scales = O.quantize(x)
+    assert scales[0, :, 0].tolist() == [253, 254, 254, 254, 254]
+    assert O.dequantize(codes, scales, 32)[:, 0].tolist() == [1.5 * 2.0 ** 128, 2.0 ** 129] + [6 * 2.0 ** 127] * 3
+
+
 def test_oracle_keeps_what_it_can_hold():
     """Values of a block's grid come back exactly; everything else within half a step of its place."""
     g = torch.Generator().manual_seed(1)
