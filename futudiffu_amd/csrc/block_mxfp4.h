@@ -226,10 +226,17 @@ std::tuple<Tensor, Tensor, Tensor> mx_gate_modulate(const Tensor& residual, cons
 
 // ---------------------------------------------------------------- autograd
 
+// What x's gradient takes: refused before the forward, not in the backward.
+void check_for_dx(int64_t rows, int64_t columns) {
+  TORCH_CHECK_VALUE(rows * ((columns + 7) / 8 * 8) * 2 < (int64_t)1 << 31, "x wants a gradient: a weight of ", rows, " x ",
+                    columns, " has 2^31 bytes or more in 16 bits (detach x, or split the weight)");
+}
+
 struct MxLinearFn : torch::autograd::Function<MxLinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& codes, const Tensor& scales,
                         int64_t columns, const OptTensor& bias, const OptTensor& residual,
                         const std::string& activation) {
+    if (x.requires_grad() && codes.dim() == 2) check_for_dx(codes.size(0), columns);
     // a residual's gradient alone needs no z
     const auto [out, z] = mx_linear_forward(x, codes, scales, columns, bias, residual, activation,
                                             any_requires({&x, &some(bias)}));

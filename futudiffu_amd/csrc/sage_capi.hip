@@ -1307,6 +1307,7 @@ int sage_mxfp4_linear(const void* x, int64_t x_rs, const void* x_codes, const vo
 size_t sage_mxfp4_linear_bwd_workspace_bytes(const void* dout, int64_t d_rs, int64_t m, int64_t n, int64_t k,
                                              int activation, int want) {
   if (check_mx_linear(m, n, k, SAGE_DTYPE_BF16, activation)) return 0;
+  if (want & 1 && check_linear(m, n, k, 0, SAGE_DTYPE_BF16, activation)) return 0;
   return LinearBwd(dout, d_rs, nullptr, 0, nullptr, 0, m, n, k, activation, want & 5, true).bytes;
 }
 
@@ -1314,7 +1315,8 @@ int sage_mxfp4_linear_bwd(const void* dout, int64_t d_rs, const void* w_codes, c
                           int64_t m, int64_t n, int64_t k, int dtype, int activation, int bias_fp32, void* workspace,
                           size_t workspace_bytes, void* dx, void* dbias, hipStream_t stream) {
   if (const int e = check_mx_linear(m, n, k, dtype, activation)) return e;
-  if (const int e = check_linear(m, n, k, 0, dtype, activation)) return e;  // the weight's 16-bit rows
+  if (dx)
+    if (const int e = check_linear(m, n, k, 0, dtype, activation)) return e;  // the weight's 16-bit rows
   const int want = (dx ? 1 : 0) | (dbias ? 4 : 0);
   if (!dout || (dx && (!w_codes || !w_scales)) || (activation != SAGE_ACT_NONE && !z))
     return fail(SAGE_ERR_ARG, "null tensor pointer");

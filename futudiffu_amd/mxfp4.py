@@ -122,6 +122,9 @@ _b._define("mxfp4_linear_codes(Tensor x_codes, Tensor x_scales, int x_columns, T
 
 def _linear_setup(ctx, inputs, output):
     x, codes, scales, columns, bias, residual, activation, keep_z = inputs
+    if x.requires_grad and codes.shape[0] * ((columns + 7) // 8 * 8) * 2 >= 1 << 31:
+        raise ValueError(f"x wants a gradient: a weight of {codes.shape[0]} x {columns} has 2^31 bytes or more in 16 bits "
+                         "(detach x, or split the weight)")
     ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(codes, scales, bias, output[1])
     ctx.columns, ctx.activation = columns, activation
@@ -179,7 +182,8 @@ def mxfp4_linear(x: Tensor | MXFP4, weight: MXFP4, bias: Tensor | None = None, r
 
     The gradient of a tensor ``x`` is ``dz weight``, rounded once: for an activation the forward keeps
     ``z`` in fp32, and ``dz = dout * act'(z)`` enters the product as two bfloat16 parts.  Without
-    one ``dz`` is ``dout``, and the weight's values are taken in ``x``'s type.
+    one ``dz`` is ``dout``, and the weight's values are taken in ``x``'s type.  An ``x`` that wants a
+    gradient needs a weight of under 2^31 bytes in 16 bits.
     """
     if isinstance(x, MXFP4):
         if _traced_without_grad(bias, residual):

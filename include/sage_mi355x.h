@@ -561,8 +561,8 @@ int sage_mxfp4_linear(const void* x, int64_t x_rs, const void* x_codes, const vo
 /* Gradients, the rounding of x taken as the identity: dz = dout * act'(z), dx = dz weight, dbias =
  * dz's column sums; each null if not wanted.  Of an activation dz enters the product as two bf16
  * matrices (2^-17 of a value is lost) and the weight in bf16; without one it is dout itself and the
- * weight's values are in dtype.  Arguments as in sage_linear_bwd; the weight's 16-bit
- * rows (formed in the workspace) have under 2^31 bytes. */
+ * weight's values are in dtype.  Arguments as in sage_linear_bwd; for dx the weight's
+ * 16-bit rows (formed in the workspace) have under 2^31 bytes. */
 size_t sage_mxfp4_linear_bwd_workspace_bytes(const void* dout, int64_t d_rs, int64_t m, int64_t n, int64_t k,
                                              int activation, int want);
 int sage_mxfp4_linear_bwd(const void* dout, int64_t d_rs, const void* w_codes, const void* w_scales, const float* z,

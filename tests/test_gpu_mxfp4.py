@@ -871,6 +871,27 @@ def test_second_derivatives_raise(cuda, act):
         assert torch.equal(torch.autograd.grad(call(v["x"], v["bias"], r), r, d, create_graph=True)[0], d)
 
 
+def test_training_over_a_weight_too_large_for_dx(cuda):
+    """2^31 elements: the bias and the residual train; an x that wants a gradient is refused by the forward."""
+    import futudiffu_amd as F
+    n, k = 1 << 19, 4096
+    w = F.MXFP4(torch.zeros(n, k // 2, dtype=torch.uint8, device=cuda),
+                torch.full((k // 256, n, 8), 127, dtype=torch.uint8, device=cuda), k)
+    w.codes[n - 1, k // 2 - 1] = 0x20  # 1 in the last column
+    g = torch.Generator().manual_seed(1)
+    x, d = torch.randn(3, k, generator=g).to(BF).to(cuda), torch.randn(3, n, generator=g).to(BF).to(cuda)
+    b, r = torch.zeros(n, device=cuda, requires_grad=True), torch.randn(3, n, generator=g).to(BF).to(cuda).requires_grad_()
+    out = F.mxfp4_linear(x, w, b, r)
+    db, dr = torch.autograd.grad(out, (b, r), d)
+    assert torch.equal(out[:, :-1], r[:, :-1]) and torch.equal(dr, d)
+    q = O.rounded(x)[:, -1]
+    assert torch.equal(out[:, -1], (q + r[:, -1].double()).to(BF))
+    assert B.worst(db, d.double().sum(0), 4 * 2.0 ** -24 * d.double().abs().sum(0)) <= 1.0
+    for call in (lambda t: F.mxfp4_linear(t, w, b, r), lambda t: torch.ops.futudiffu_ii.mxfp4_linear(t, *w, b, r, "none", True)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call(x.detach().requires_grad_())
+
+
 # ---------------------------------------------------------------- together
 
 H, D, C, F_ = 4, 64, 256, 640

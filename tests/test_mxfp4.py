@@ -210,6 +210,22 @@ def test_gradients_of_the_op_are_not_differentiated(act):
                         grad(create_graph=True)
 
 
+def test_a_weight_too_large_for_dx():
+    """Refused by the forward where x wants a gradient; a bias's gradient needs no rows of the weight."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        n, k = 1 << 19, 4096
+        x, b = torch.empty(3, k, dtype=BF), torch.empty(n, requires_grad=True)
+        w = torch.empty(n, k // 2, dtype=torch.uint8), torch.empty(k // 256, n, 8, dtype=torch.uint8), k
+
+        def out(x):
+            return torch.ops.futudiffu_ii.mxfp4_linear(x, *w, b, None, "none", True)[0]
+
+        assert torch.autograd.grad(out(x), b, torch.empty(3, n, dtype=BF))[0].shape == (n,)
+        with pytest.raises(ValueError, match="2\\^31"):
+            out(x.requires_grad_())
+
+
 # ---- the C entries
 
 @fake_addresses
@@ -262,6 +278,18 @@ def test_linear_backward_entry_refuses(over, status, msg):
     a.update(over)
     assert lib.sage_mxfp4_linear_bwd(*a.values()) == status
     assert msg in lib.sage_last_error().decode()
+
+
+@fake_addresses
+def test_bias_gradient_over_a_large_weight():
+    """The limit on the weight's 16-bit rows is dx's."""
+    lib = _lib.load()
+    n, k = 1 << 19, 4096
+    size = lib.sage_mxfp4_linear_bwd_workspace_bytes
+    assert size(64, n, 4, n, k, 0, 1) == size(64, n, 4, n, k, 0, 5) == 0 < size(64, n, 4, n, k, 0, 4)
+    args = (64, n, 64, 64, None, 4, n, k, 0, 0, 0, None, 0)
+    assert lib.sage_mxfp4_linear_bwd(*args, None, 64, None) == 3 and "workspace of" in lib.sage_last_error().decode()
+    assert lib.sage_mxfp4_linear_bwd(*args, 64, 64, None) == 1 and "2^31" in lib.sage_last_error().decode()
 
 
 @fake_addresses
