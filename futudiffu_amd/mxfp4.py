@@ -182,7 +182,8 @@ def mxfp4_linear(x: Tensor | MXFP4, weight: MXFP4, bias: Tensor | None = None, r
 
     The gradient of a tensor ``x`` is ``dz weight``, rounded once: for an activation the forward keeps
     ``z`` in fp32, and ``dz = dout * act'(z)`` enters the product as two bfloat16 parts.  Without
-    one ``dz`` is ``dout``, and the weight's values are taken in ``x``'s type.  An ``x`` that wants a
+    one ``dz`` is ``dout``, and the weight's values are taken in ``x``'s type (exact in bfloat16; in
+    float16 infinite past 65504, and rounded under 2^-23).  An ``x`` that wants a
     gradient needs a weight of under 2^31 bytes in 16 bits.
     """
     if isinstance(x, MXFP4):

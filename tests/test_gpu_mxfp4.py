@@ -381,6 +381,37 @@ def test_dz_past_the_types_range(cuda, dtype):
         _check(_run(v, "swiglu"), _want(v, "swiglu"), f"{dtype} {zoom}")
 
 
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_fp16_over_weights_past_its_range(cuda, act):
+    """Blocks of a weight with scales from 2^-60 to 2^30 under an fp16 x, its columns sized so that the outputs
+    fit: the forward takes every code as it is.  So does the gradient of an activation; without one
+    dx takes the weight's values in fp16, infinite past 65504, in steps of 2^-24 under 2^-14, 0 where
+    they are smaller."""
+    M, K, N = 70, 352, 40
+    v = _inputs(M, K, N, act, FP, F32, False, seed=8, device=cuda)
+    w = v["weight"]
+    zoom = torch.tensor([0, -60, 14, -14, -18, -22, -25, 20, 30, 2, 0], device=cuda)  # of each block of 32 columns
+    scales = w.scales.transpose(0, 1).reshape(N, -1).int()
+    scales[:, :11] = (scales[:, :11] + zoom).clamp(0, 254)
+    scales = scales.to(torch.uint8).reshape(N, 2, 8).transpose(0, 1).contiguous()
+    v.update(weight=w._replace(scales=scales), values=O.dequantize(w.codes, scales, K),
+             x=(v["x"].float() * torch.exp2(-zoom.clamp_min(0).float()).repeat_interleave(32)).to(FP))
+    if act != "none":
+        v["dout"] = v["dout"] * 2.0 ** -20  # the largest block's dx fits
+    got, want = _run(v, act), _want(v, act)
+    in_fp16 = v["values"].to(FP).double()
+    past = in_fp16.isinf().any(0)
+    assert past.any() and ((in_fp16 != v["values"]) & ~in_fp16.isinf()).any() and torch.isfinite(got["out"]).all()
+    if act == "none":
+        assert not torch.isfinite(got["dx"][:, past]).any()
+        d, used = v["dout"].double(), in_fp16[:, ~past]
+        exact = d @ used
+        exact = torch.where(exact.abs() >= 65520, exact.sign() * torch.inf, exact)  # what fp16 rounds to infinity
+        want["dx"] = (exact, (N + 2) * 2.0 ** -24 * (d.abs() @ used.abs()))
+        got["dx"] = got["dx"][:, ~past]
+    _check(got, want, act)
+
+
 def test_other_stream_overlap_and_graph(cuda):
     a = _inputs(700, 1032, 640, "swiglu", BF, BF, True, seed=1, device=cuda)
     b = _inputs(40, 2048, 1000, "silu", FP, None, False, seed=2, device=cuda)
