@@ -381,6 +381,65 @@ def test_dz_past_the_types_range(cuda, dtype):
         _check(_run(v, "swiglu"), _want(v, "swiglu"), f"{dtype} {zoom}")
 
 
+def _differences(act, call, grads, v, steps):
+    """For the leaves of `steps`: the directional derivative from call's outputs by central differences of a
+    whole and a half step, extrapolated ((4 d(1/2) - d(1)) / 3), that from grads, and how far they may
+    be apart: the outputs' roundings (half a step of fp16, and MFMA of the product's size through the
+    slopes) and the gradients' in quadrature, six times, and what the extrapolation leaves in 64 bits."""
+    d, w, want = v["dout"].double(), v["values"], _want(v, act)
+
+    def slope(value):
+        one, half = (value(t) - value(-t) for t in (1, 0.5))
+        return float((4 * half - one / 2) / 3)
+
+    q = O.rounded(v["x"])
+    more = 1.13 * O.MFMA * (q.abs() @ w.abs().T)
+    if act == "swiglu":
+        z1, z2 = (q @ w.T + v["bias"].double()).abs().chunk(2, -1)
+        more = more.chunk(2, -1)[0] * z2 + more.chunk(2, -1)[1] * z1
+    # a half step's pair of outputs enters 4 / 3 times each, a whole step's 1 / 6
+    out = (((want["out"][0].abs() + 1) * 2.0 ** -11 + more) * d).norm() * (2 * (16 + 1 / 4) / 9) ** 0.5
+    found = []
+    for leaf, s in steps.items():
+        moved = lambda t: {**v, leaf: v[leaf] + t * s}  # noqa: E731
+        num = slope(lambda t: (call(moved(t)).double() * d).sum())
+        ana = float((grads[leaf].double() * s.double()).sum())
+        left = slope(lambda t: (_want(moved(t), act, False)["out"][0] * d).sum()) - float((want["d" + leaf][0] * s.double()).sum())
+        own = (grads[leaf].double() * torch.finfo(grads[leaf].dtype).eps / 2 * s.double()).norm()
+        found.append((leaf, num, ana, abs(left) + 6 * float(out + own)))
+    return found
+
+
+def _difference_inputs(act, device):
+    """x and its steps, whole and halved, are multiples that the codes hold exactly; the steps go up the
+    gradient in a few columns of each row, so that the derivative stands far above the roundings."""
+    v = _inputs(40, 64, 24, act, FP, F32, False, seed=2, device=device)
+    g = torch.Generator().manual_seed(6)
+    x = torch.randint(-1, 2, (40, 64), generator=g).double()
+    x[:, ::32] = 4.0  # the scale stays 1
+    v["x"] = (x / 4).to(FP).to(device)
+    want = _want(v, act)
+    pick = torch.rand(40, 64, generator=g) < 0.15
+    pick[:, ::32] = False
+    steps = {"x": (want["dx"][0].sign() * pick.to(device) / 4).to(FP), "bias": (want["dbias"][0].sign() / 4).float()}
+    for t in (1, -1, 0.5, -0.5):
+        moved = v["x"] + t * steps["x"]
+        assert torch.equal(O.rounded(moved), moved.double())
+    return v, steps
+
+
+@pytest.mark.parametrize("act", ["none", "silu", "gelu", "swiglu"])
+def test_gradient_against_extrapolated_differences(cuda, act):
+    """The gradients of x and the bias against differences of the outputs; what is allowed is a small
+    part of the derivative, so a gradient that lacks a factor, a term or half of a swiglu fails."""
+    v, steps = _difference_inputs(act, cuda)
+    got = _run(v, act)
+    call = lambda v: _run(v, act, grads=False)["out"]  # noqa: E731
+    for leaf, num, ana, allowed in _differences(act, call, {"x": got["dx"], "bias": got["dbias"]}, v, steps):
+        print(act, leaf, num, ana, allowed, flush=True)
+        assert allowed < 0.02 * abs(ana) and abs(num - ana) <= allowed, (act, leaf, num, ana, allowed)
+
+
 @pytest.mark.parametrize("act", ["none", "silu"])
 def test_fp16_over_weights_past_its_range(cuda, act):
     """Blocks of a weight with scales from 2^-60 to 2^30 under an fp16 x, its columns sized so that the outputs
