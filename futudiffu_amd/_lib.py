@@ -94,10 +94,10 @@ SIGNATURES = {
     "sage_mxfp4_linear_bwd": (_c.c_int, [
         _P, _I64, _P, _P, _P, _I64, _I64, _I64, _c.c_int, _c.c_int, _c.c_int, _P, _c.c_size_t, _P, _P, _P]),
     "sage_rms_norm_modulate_mxfp4": (_c.c_int, [
-        _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _c.c_int, _c.c_int, _c.c_float, _P, _P, _P]),
+        _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _c.c_int, _c.c_int, _c.c_double, _P, _P, _P]),
     "sage_rms_norm_gate_residual_modulate_mxfp4": (_c.c_int, [
         _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
-        _c.c_int, _c.c_int, _c.c_float, _P, _P, _P, _P]),
+        _c.c_int, _c.c_int, _c.c_double, _P, _P, _P, _P]),
 }
 
 _lock = threading.Lock()

@@ -200,7 +200,7 @@ std::tuple<Tensor, Tensor> mx_modulate(const Tensor& x, const OptTensor& weight,
   if (!a.empty()) {
     const Tokens xt(x);
     const Launch on(x);
-    check_status(lib.sage_rms_norm_modulate_mxfp4(xt.p(), xt.bs, xt.rs, ptr(a.weight), COND(a.cond), TAIL(a),
+    check_status(lib.sage_rms_norm_modulate_mxfp4(xt.p(), xt.bs, xt.rs, ptr(a.weight), COND(a.cond), SIZES(a), (a).eps64,
                                                   codes.data_ptr(), scales.data_ptr(), on.stream));
   }
   return {codes, scales};
@@ -219,7 +219,7 @@ std::tuple<Tensor, Tensor, Tensor> mx_gate_modulate(const Tensor& residual, cons
     const Launch on(x);
     check_status(lib.sage_rms_norm_gate_residual_modulate_mxfp4(
         rt.p(), rt.bs, rt.rs, xt.p(), xt.bs, xt.rs, ptr(a.weight), COND(a.cond), ptr(a.next_weight),
-        COND(a.next_scale), TAIL(a), hidden.data_ptr(), codes.data_ptr(), scales.data_ptr(), on.stream));
+        COND(a.next_scale), SIZES(a), (a).eps64, hidden.data_ptr(), codes.data_ptr(), scales.data_ptr(), on.stream));
   }
   return {hidden, codes, scales};
 }

@@ -132,12 +132,13 @@ struct Norm {
   int64_t B, N, C, groups = 1;
   int dtype, f32 = 0;
   float eps;
+  double eps64;
   Tensor weight, next_weight, doc;
   Cond cond, next_scale;
 
   Norm(const Tensor& x, const OptTensor& w, const char* cond_name, const OptTensor& k, const OptTensor& ids, double e,
        const OptTensor& w2 = std::nullopt, const OptTensor& s2 = std::nullopt)
-      : eps((float)e) {
+      : eps((float)e), eps64(e) {
     TORCH_CHECK_VALUE(x.dim() == 2 || x.dim() == 3, "x must be [B, N, C] or [N, C], got ", x.sizes());
     B = x.dim() == 3 ? x.size(0) : 1;
     N = x.size(-2);
@@ -203,7 +204,8 @@ struct Norm {
 };
 
 #define COND(k) ptr((k).t), (k).bs, (k).gs
-#define TAIL(a) (a).groups, (a).ids(), (a).B, (a).N, (a).C, (a).dtype, (a).f32, (a).eps
+#define SIZES(a) (a).groups, (a).ids(), (a).B, (a).N, (a).C, (a).dtype, (a).f32
+#define TAIL(a) SIZES(a), (a).eps
 
 Tensor modulate_forward(const Tensor& x, const OptTensor& weight, const OptTensor& scale, const OptTensor& doc_ids,
                         double eps) {

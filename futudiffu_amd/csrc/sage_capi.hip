@@ -1335,10 +1335,12 @@ int sage_mxfp4_linear_bwd(const void* dout, int64_t d_rs, const void* w_codes, c
 
 int sage_rms_norm_modulate_mxfp4(const void* x, int64_t x_bs, int64_t x_rs, const void* weight, const void* scale,
                                  int64_t scale_bs, int64_t scale_gs, int64_t groups, const int32_t* doc_ids, int64_t b,
-                                 int64_t n, int64_t c, int dtype, int fp32_params, float eps, void* codes,
+                                 int64_t n, int64_t c, int dtype, int fp32_params, double eps, void* codes,
                                  void* scales, hipStream_t stream) {
   sage::NormArgs a = norm_args(x, x_bs, x_rs, weight, scale, scale_bs, scale_gs, groups, doc_ids, b, n, c,
-                               fp32_params, eps);
+                               fp32_params, (float)eps);
+  a.eps64 = eps;
+  if (!(eps >= 0.0)) return fail(SAGE_ERR_ARG, "eps must be >= 0");
   if (const int e = check_norm(a, b, n, c, groups, dtype, fp32_params)) return e;
   if (!x) return fail(SAGE_ERR_ARG, "null tensor pointer");
   if (const int e = check_norm_align(a)) return e;
@@ -1352,9 +1354,11 @@ int sage_rms_norm_gate_residual_modulate_mxfp4(
     const void* residual, int64_t r_bs, int64_t r_rs, const void* x, int64_t x_bs, int64_t x_rs, const void* weight,
     const void* gate, int64_t gate_bs, int64_t gate_gs, const void* next_weight, const void* next_scale,
     int64_t scale_bs, int64_t scale_gs, int64_t groups, const int32_t* doc_ids, int64_t b, int64_t n, int64_t c,
-    int dtype, int fp32_params, float eps, void* hidden, void* codes, void* scales, hipStream_t stream) {
+    int dtype, int fp32_params, double eps, void* hidden, void* codes, void* scales, hipStream_t stream) {
   sage::NormArgs a = norm_args(x, x_bs, x_rs, weight, gate, gate_bs, gate_gs, groups, doc_ids, b, n, c, fp32_params,
-                               eps);
+                               (float)eps);
+  a.eps64 = eps;
+  if (!(eps >= 0.0)) return fail(SAGE_ERR_ARG, "eps must be >= 0");
   if (const int e = check_norm(a, b, n, c, groups, dtype, fp32_params)) return e;
   if (!residual || !x || !hidden) return fail(SAGE_ERR_ARG, "null tensor pointer");
   a.res = {residual, r_bs, r_rs};

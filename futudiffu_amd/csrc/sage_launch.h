@@ -346,7 +346,7 @@ struct NormArgs {
   int b, c;
   int64_t n;
   float eps;
-  double inv_c;  // 1 / c, of the norms into MXFP4
+  double inv_c, eps64;  // of the norms into MXFP4: 1 / c, and eps in 64 bits
   // contiguous outputs [B, N, C]; dx may be null in the backward
   void *out, *hidden, *dx, *dres;
   // parameter gradients (each may be null), in the parameters' types

@@ -347,8 +347,8 @@ __device__ __forceinline__ double token_sum64(double v, double* red, int wave) {
 
 // 1 / sqrt(sum_sq / c + eps) by v_rsq_f64 (2^-23 off or less) and one step of third order: a sixth of the
 // instructions of the library's root and quotient.
-__device__ __forceinline__ double rrms64(double sum_sq, double inv_c, float eps) {
-  const double v = fma(sum_sq, inv_c, (double)eps), r = __builtin_amdgcn_rsq(v);
+__device__ __forceinline__ double rrms64(double sum_sq, double inv_c, double eps) {
+  const double v = fma(sum_sq, inv_c, eps), r = __builtin_amdgcn_rsq(v);
   const double e = fma(-v * r, r, 1.0);
   return e == e ? fma(r * e, fma(e, 0.375, 0.5), r) : r;  // of 0 and infinity
 }
@@ -457,7 +457,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_mx_kernel(NormArgs
 #pragma unroll
   for (int j = 0; j < kPer; ++j) s = fma((double)x[j], (double)x[j], s);
   s = token_sum64<TPR>(s, red, wave);
-  double rr = gated ? rrms64(s, a.inv_c, a.eps) : 0.0;
+  double rr = gated ? rrms64(s, a.inv_c, a.eps64) : 0.0;
   double h[kPer];  // what the last norm takes
   if constexpr (kGate) {
     const __amdgpu_buffer_rsrc_t rs = raw_rsrc(static_cast<T*>(a.hidden) + row * a.c, (uint32_t)c * 2);
@@ -495,7 +495,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_mx_kernel(NormArgs
       }
     }
     s = token_sum64<TPR>(s, red2, wave);
-    rr = rrms64(s, a.inv_c, a.eps);
+    rr = rrms64(s, a.inv_c, a.eps64);
   }
   // rf * wm can leave fp32's range at the bottom only where |wm| is under 2^-66, so that the value is 0 beside
   // any block that counts

@@ -569,13 +569,13 @@ int sage_mxfp4_linear_bwd(const void* dout, int64_t d_rs, const void* w_codes, c
                           int64_t m, int64_t n, int64_t k, int dtype, int activation, int bias_fp32, void* workspace,
                           size_t workspace_bytes, void* dx, void* dbias, hipStream_t stream);
 
-/* sage_rms_norm_modulate with its output in MXFP4, quantized from the unrounded values (sums
- * in fp64; a value next to a border between two codes is decided there and falls on its own
+/* sage_rms_norm_modulate with its output in MXFP4, quantized from the unrounded values (eps and
+ * sums in fp64; a value next to a border between two codes is decided there and falls on its own
  * side).  codes, scales: b * n rows of c columns. */
 int sage_rms_norm_modulate_mxfp4(const void* x, int64_t x_bs, int64_t x_rs, const void* weight,
                                  const void* scale, int64_t scale_bs, int64_t scale_gs, int64_t groups,
                                  const int32_t* doc_ids, int64_t b, int64_t n, int64_t c, int dtype,
-                                 int fp32_params, float eps, void* codes, void* scales, hipStream_t stream);
+                                 int fp32_params, double eps, void* codes, void* scales, hipStream_t stream);
 
 /* sage_rms_norm_gate_residual_modulate with the second norm's output in MXFP4; hidden is
  * rounded once from fp64. */
@@ -583,7 +583,7 @@ int sage_rms_norm_gate_residual_modulate_mxfp4(
     const void* residual, int64_t r_bs, int64_t r_rs, const void* x, int64_t x_bs, int64_t x_rs,
     const void* weight, const void* gate, int64_t gate_bs, int64_t gate_gs, const void* next_weight,
     const void* next_scale, int64_t scale_bs, int64_t scale_gs, int64_t groups, const int32_t* doc_ids,
-    int64_t b, int64_t n, int64_t c, int dtype, int fp32_params, float eps, void* hidden, void* codes,
+    int64_t b, int64_t n, int64_t c, int dtype, int fp32_params, double eps, void* hidden, void* codes,
     void* scales, hipStream_t stream);
 
 #ifdef __cplusplus

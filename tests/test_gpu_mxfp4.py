@@ -824,6 +824,32 @@ def test_norms_decide_next_to_borders(cuda):
             assert near > 0
 
 
+def test_norms_take_eps_in_64_bits(cuda):
+    """An eps whose nearest fp32 value would put channels on the other side of a border between two codes:
+    rows of ones, so that a channel is its weight over sqrt(1 + eps)."""
+    import futudiffu_amd as F
+    x = torch.ones(1, 3, 64, dtype=BF, device=cuda)
+    told = 0
+    for i in range(1, 3000):
+        eps = 0.1 + i / 10007
+        single = float(torch.tensor(eps, dtype=F32))
+        borders = torch.tensor([5.0, 3.5, 2.5, 1.75, 1.25, 0.75, 0.25], dtype=torch.float64)
+        w = (borders * (1 + eps) ** 0.5).float().double()
+        apart = ((w / (1 + eps) ** 0.5 > borders) != (w / (1 + single) ** 0.5 > borders)).nonzero().flatten()
+        if len(apart) == 0:
+            continue
+        told += 1
+        weight = torch.ones(64)
+        weight[0], weight[32] = 5.5, 5.5  # the scales are 1
+        weight[40:40 + len(apart)] = w[apart].float()
+        weight = weight.to(cuda)
+        q = F.rms_norm_modulate_mxfp4(x, weight, eps=eps)
+        _same(q, O.quantize(O.norm_values(x, weight, None, None, eps)), eps)
+        q = F.rms_norm_gate_residual_modulate_mxfp4(x, torch.zeros_like(x), None, None, weight, eps=eps)[1]
+        _same(q, O.quantize(O.norm_values(x, weight, None, None, eps)), eps)
+    assert told >= 10, told
+
+
 # ---------------------------------------------------------------- traced, refused
 
 def _calls(device, seed=0):

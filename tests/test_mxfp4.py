@@ -315,6 +315,15 @@ def test_norm_entries_refuse():
     assert two(*rest, *tail, 129, 64, 64, None) == 2 and "aligned" in err()
 
 
+@fake_addresses
+def test_norm_entries_take_eps_in_64_bits():
+    """No eps under 0, however small, and NaN neither."""
+    lib = _lib.load()
+    for eps in (-1e-300, -1.0, float("nan")):
+        assert lib.sage_rms_norm_modulate_mxfp4(16, 64, 8, 32, 48, 8, 0, 1, None, 2, 8, 8, 0, 0, eps, 64, 64, None) == 1
+        assert "eps" in lib.sage_last_error().decode()
+
+
 def test_workspace_sizes():
     """x's codes and scales and the cut tiles' sums: none for sizes that the calls refuse, and with
     codes given never more than without."""
