@@ -1200,7 +1200,8 @@ int check_mx_linear(int64_t m, int64_t n, int64_t k, int dtype, int activation) 
 // offsets, which it quantizes itself where they are few and short.
 enum { kMxCodes = 0, kMxRows = 1, kMxNearRows = 2 };
 int mx_rows(const void* x, int64_t rs, int64_t m, int64_t k) {
-  return !x ? kMxCodes : in_place(x, rs, m, k) && (m == 1 || rs < (int64_t)1 << 22) ? kMxNearRows : kMxRows;
+  return !x ? kMxCodes
+         : in_place(x, rs, m, k) && (m == 1 || (rs >= 0 && rs < (int64_t)1 << 22)) ? kMxNearRows : kMxRows;
 }
 
 // Codes and scales of x in the workspace, and what follows them.

@@ -549,8 +549,8 @@ int sage_mxfp4_dequantize(const void* codes, const void* scales, int64_t m, int6
  *   others       as in sage_linear (dtype: of x, residual, out and a bias that is not fp32).
  *   workspace    sage_mxfp4_linear_workspace_bytes(...) bytes, 16-byte aligned; needs no
  *                clearing.  quantize_x: 0 where x_codes are given, 1 for an x, 2 for an x whose rows
- *                are on 16-byte boundaries, k a multiple of 8 and x_rs under 2^22 (never more than
- *                for 1); other_rows as in sage_linear. */
+ *                are on 16-byte boundaries, k a multiple of 8 and x_rs from 0 to under 2^22 (never
+ *                more than for 1); other_rows as in sage_linear. */
 size_t sage_mxfp4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int activation, int quantize_x,
                                          int other_rows);
 int sage_mxfp4_linear(const void* x, int64_t x_rs, const void* x_codes, const void* x_scales, const void* w_codes,

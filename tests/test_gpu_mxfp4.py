@@ -615,6 +615,25 @@ def test_few_rows_quantize_in_place(cuda, K, N):
             _check({"out": F.mxfp4_linear(x, *args, activation=act)}, {"out": _want(v, act, False)["out"]}, act)
 
 
+def test_rows_that_lie_backwards(cuda):
+    """By the C entry: x's rows at a negative stride, the last one first in memory."""
+    from futudiffu_amd import _lib
+    import futudiffu_amd as F
+    lib = _lib.load()
+    M, K, N = 4, 264, 48
+    v = _inputs(M, K, N, "none", BF, None, False, seed=4, device=cuda)
+    back = v["x"].flip(0).contiguous()
+    want = F.mxfp4_linear(v["x"], v["weight"])
+    out = torch.empty(M, N, dtype=BF, device=cuda)
+    size = lib.sage_mxfp4_linear_workspace_bytes(M, N, K, 0, 1, 0)
+    ws = torch.empty(size, dtype=torch.uint8, device=cuda)
+    status = lib.sage_mxfp4_linear(back[M - 1:].data_ptr(), -K, None, None, v["weight"].codes.data_ptr(),
+                                   v["weight"].scales.data_ptr(), None, 0, None, 0, M, N, K, 0, 0, ws.data_ptr(), size, None,
+                                   out.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert status == 0 and torch.equal(out, want)
+
+
 @pytest.mark.parametrize("M,K,N", [(667, 1001, 779), (2000, 3840, 16), (7000, 264, 24), (192, 1536, 3840), (1025, 72, 8),
                                    (97, 776, 8300)])
 def test_few_columns(cuda, M, K, N):

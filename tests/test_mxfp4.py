@@ -266,6 +266,16 @@ def test_linear_entry_refuses(over, status, msg):
 
 
 @fake_addresses
+def test_linear_entry_reads_rows_in_any_order():
+    """Rows that lie backwards are quantized by the kernel that takes any stride: the few-row product's own
+    offsets are 32-bit and not negative."""
+    lib = _lib.load()
+    args = (64, 64, None, 0, None, 0, 4, 16, 40, 0, 0, None, 0, None, 64, None)
+    assert lib.sage_mxfp4_linear(1 << 20, -40, None, None, *args) == 3
+    assert "workspace of" in lib.sage_last_error().decode()
+
+
+@fake_addresses
 @pytest.mark.parametrize("over,status,msg", [
     (dict(m=0), 1, "positive"), (dict(k=1 << 22), 1, "exceeds"), (dict(act=7), 1, "activation"),
     (dict(d=None), 1, "null"), (dict(w=None), 1, "null"), (dict(act=1), 1, "null"), (dict(drs=15), 1, "apart"),
