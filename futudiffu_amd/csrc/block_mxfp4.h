@@ -162,6 +162,8 @@ std::tuple<Tensor, Tensor> mx_linear_backward(const Tensor& dout, const Tensor& 
                                               int64_t columns, const OptTensor& bias, const OptTensor& z,
                                               const std::string& activation, const Wanted& wanted) {
   refuse_tangents({&dout, &some(bias)});
+  TORCH_CHECK_VALUE(wanted.size() == 2, "wanted must say whether x and the bias want a gradient, got ", wanted.size(),
+                    " values");
   TORCH_CHECK_VALUE(dout.dim() >= 1, "dout must be [..., N], got a scalar");
   const MxLinear a(dout.sizes(), columns, dout.scalar_type(), codes, scales, columns, bias, activation);
   a.check_out("dout", dout);

@@ -210,6 +210,13 @@ def test_gradients_of_the_op_are_not_differentiated(act):
                         grad(create_graph=True)
 
 
+@pytest.mark.parametrize("wanted", [[], [True], [True, True, True]])
+def test_gradient_op_takes_two_wanted(wanted):
+    w = _weight(6, 40)
+    with pytest.raises(ValueError, match="wanted must"):
+        torch.ops.futudiffu_ii.mxfp4_linear_backward(torch.zeros(2, 6, dtype=BF), *w, None, None, "none", wanted)
+
+
 def test_a_weight_too_large_for_dx():
     """Refused by the forward where x wants a gradient; a bias's gradient needs no rows of the weight."""
     from torch._subclasses.fake_tensor import FakeTensorMode
