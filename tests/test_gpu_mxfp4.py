@@ -352,7 +352,10 @@ def test_gradient_against_differences(cuda):
 
 @pytest.mark.parametrize("M,K,N,act,dtype", [(667, 1001, 779, "silu", FP), (331, 520, 777, "gelu", BF),
                                              (700, 264, 300, "swiglu", BF), (40, 72, 65, "swiglu", FP),
-                                             (1300, 700, 5000, "silu", BF), (64, 1032, 4100, "swiglu", FP)])
+                                             (1300, 700, 5000, "silu", BF), (64, 1032, 4100, "swiglu", FP),
+                                             # large tiles, whole and in pieces, with rows of any alignment too
+                                             (4200, 4100, 320, "silu", FP), (2304, 4096, 600, "gelu", FP),
+                                             (2304, 4095, 2000, "gelu", FP), (1, 520, 72, "swiglu", FP)])
 def test_dx_has_its_own_rounding_alone(cuda, M, K, N, act, dtype):
     """How far dx is from the exact gradient, over all elements, against the exact values rounded
     to its type: what enters the product loses 2^-17 of a value or less, beside the 2^-12 (rms, of fp16)
@@ -573,6 +576,21 @@ def test_offsets_past_32_bits(cuda):
         want[at] = (rows.double() @ w.double().T).to(BF)
         assert torch.equal(out.cpu(), want)
         assert torch.equal(F.mxfp4_linear(q, F.mxfp4_quantize(w.to(cuda))), out)
+
+
+def test_gradients_past_32_bits(cuda):
+    """An activation's dz of more than 2^32 bytes in each of its parts: few rows of dout are not zero."""
+    import futudiffu_amd as F
+    M, K, N = (1 << 20) + 37, 24, 2056
+    v = _inputs(9, K, N, "silu", BF, None, False, seed=6, device=cuda)
+    at = torch.tensor([0, 1, (1 << 19) - 1, 1 << 19, (1 << 20) - 1, 1 << 20, (1 << 20) + 5, M - 2, M - 1], device=cuda)
+    x, d = torch.zeros(M, K, dtype=BF, device=cuda), torch.zeros(M, N, dtype=BF, device=cuda)
+    x[at], d[at] = v["x"], v["dout"]
+    x.requires_grad_()
+    dx, = torch.autograd.grad(F.mxfp4_linear(x, v["weight"], activation="silu"), x, d)
+    _check({"dx": dx[at]}, _want(v, "silu"))
+    dx[at] = 0
+    assert not dx.any()
 
 
 @pytest.mark.parametrize("M,K,N", [(49, 264, 8200), (64, 520, 8184), (48, 1000, 9000), (33, 264, 40), (1, 5000, 15360),
