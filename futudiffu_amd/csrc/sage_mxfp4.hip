@@ -347,8 +347,9 @@ constexpr int kPlain = 8, kAny = 9;
 
 // One tile.  LDS holds D stages; a stage is two steps of 64 columns, the next step's fragments read under
 // this one's products.  Before a stage's last step the next stage has arrived and every wave has read
-// this one's last fragments: behind that barrier the loads of the stage D further on go into its place.
-// Scales go straight to registers, 256 columns ahead.  FIN: the activation (kPlain: no bias and no
+// this one's last fragments: behind that barrier A's loads of the stage D further on go into its place,
+// and B's under the next stage's first step.  The scales of two stages go to one of D / 2 places behind
+// the ring, with A's loads, D stages ahead.  FIN: the activation (kPlain: no bias and no
 // residual either), a kernel each, so that none carries the others' registers; or kAny for rows that
 // take no 16-byte accesses.
 template <typename T, typename TL, int FIN>
@@ -532,11 +533,11 @@ __device__ __forceinline__ MxPlace whole_at(const GemmArgs& a, int t) {
 // The product by large tiles, one workgroup a CU, and behind them by small ones that cover what is left: the
 // rows past the last whole tile row, and the whole tiles of a last round that would leave most of the card
 // idle.
-// A stage of 256 columns takes a CU 1.24 us when few work, 85 % of the matrix instructions' rate, and 1.85 when
-// all do: the power then allows the matrix instructions alone 5600 to 6300 TFLOP/s on random codes (8500 on zeros).
-// 8192 x 8192 x 8192 258 us, 4250 TFLOP/s (the library's product of the same codes 3185); 4416 x 3840 onto 11520 112
-// us, 3470, with a bias 118; with a swiglu onto 2 x 10240 194 us, 3580: a contraction of 15 stages leaves a
-// fifth of the time to starts and epilogues.
+// A stage of 256 columns takes a CU 1.24 us when few work (2980 cycles, of which the matrix instructions need
+// 2048), and 1.85 when all do: the power then allows the matrix instructions alone 5600 to 6300 TFLOP/s on
+// random codes (8500 on zeros).  8192 x 8192 x 8192 258 to 267 us, 4130 to 4250 TFLOP/s (the library's product of
+// the same codes 3180 to 3630); 4416 x 3840 onto 11520 112 us, 3470, with a bias 118; with a swiglu onto 2 x 10240
+// 194 us, 3580: of a round's 63000 cycles, 15 stages of the contraction, 18000 are its start and epilogue.
 // Kept out: a persistent workgroup that asks for the next tile during the epilogue (3 % for a product alone, and
 // with a bias or an activation its registers spilled); 128 x 256 tiles by two workgroups a CU (their operands' way
 // to LDS bounds them); rings of five and more stages and other orders of the tiles (no difference); each half
@@ -612,7 +613,9 @@ __global__ __launch_bounds__(MxSmall::NT, 2) void mx_small_kernel(MxGemmArgs x) 
 // 11520 it is 8.5 and 8.7, and with more the kernel before is faster.
 // What bounds it are the operands' way into LDS (15 TB/s over the chip) and the start: 22 MB of W onto 11520 take
 // 6.2 us with up to 16 rows, 4.4 at the rate of a copy.  Operands read to registers as the matrix
-// instructions take them, without LDS, were slower from 8 rows on (32 rows 12 us, now 7.6).
+// instructions take them, without LDS, were slower from 8 rows on (32 rows 12 us, now 7.6).  Every workgroup
+// reads all of x: of the 66 MB that 32 rows onto 11520 take to LDS 44 are x's.  (In QX x's codes lie 128 bytes
+// apart without W's permutation: rows 0 and 2, and 1 and 3, share banks.)
 template <typename T, int MT, bool GLU, int W, int D, bool QX>
 __global__ __launch_bounds__(64 * W) void mx_skinny_kernel(MxGemmArgs args) {
   const GemmArgs& a = args.g;
@@ -848,7 +851,7 @@ hipError_t run_mx_tiles(const MxGemmArgs& x, hipStream_t st) {
 
 // Waves and LDS slots of a wave.  Up to as many workgroups as the chip holds of them: four waves with deep rings,
 // more bytes in flight on a CU (3840 columns of 3840, one row: 3.7 us against 4.9 for the other).  Past that: two
-// waves, four and more workgroups a CU, so that all run at once (11520 columns: 6.2 us against 7.7; with 64
+// waves, four and more workgroups a CU (with 64 rows three), so that all run at once (11520 columns: 6.2 us against 7.7; with 64
 // rows 10.7 against 14.5; 15360 of 256: 2.9 against 4.2).
 template <int MT, bool GLU, bool QX>
 struct SkinnyShape {
@@ -856,7 +859,7 @@ struct SkinnyShape {
   static constexpr int XLDS = QX ? kMxQuantCols / 256 * kMxQuantRows * 136 : 0;
   static constexpr int fit(int bytes) { return (bytes - XLDS) / STAGE; }
   static constexpr int bound(int d, int lo, int hi) { return d < lo ? lo : d > hi ? hi : d; }
-  // LDS: 80 KB (64 rows: all of it), or 40 KB
+  // LDS: 80 KB (64 rows: all of it), or 40 KB (64 rows: 42.5, the two slots that it needs)
   static constexpr int FEW = bound(fit(80 * 1024) / 4, MT == 4 ? 3 : 2, 4), MANY = bound(fit(40 * 1024) / 2, 2, 3);
   // the same with QX: its sums are those of the codes, bit for bit
   static constexpr int FEW_SLOTS = MT == 4 ? 256 : 512;
