@@ -292,6 +292,23 @@ def test_not_finite_values_stay_in_their_row(cuda, M, K, N):
     assert torch.isnan(got["dx"][0]).all() and torch.equal(got["dx"][1:], clean["dx"][1:])
 
 
+@pytest.mark.parametrize("act", ["silu", "swiglu"])
+def test_gradients_that_are_not_finite_stay_in_their_row(cuda, act):
+    """NaN and infinities of dout through both parts of dz: an infinity is no NaN before it meets the weight."""
+    v = _inputs(150, 264, 72, act, BF, F32, False, seed=1, device=cuda)
+    v["weight"] = v["weight"]._replace(codes=v["weight"].codes & 0x77)  # no value is negative
+    v["weight"].codes[0, 0] = 0x22
+    u = dict(v, dout=v["dout"].abs())
+    u["dout"][3, 7], u["dout"][5, 0] = float("nan"), float("inf")
+    u["bias"] = v["bias"].abs() + 30.0  # act' and the gates are positive
+    clean = _run(dict(u, dout=v["dout"].abs()), act)
+    got = _run(u, act)
+    assert torch.isnan(got["dx"][3]).all() and got["dx"][5, 0] == float("inf")
+    keep = [i for i in range(150) if i not in (3, 5)]
+    assert torch.equal(got["dx"][keep], clean["dx"][keep]) and torch.isfinite(clean["dx"]).all()
+    assert torch.isnan(got["dbias"][7]) and got["dbias"][0] == float("inf")
+
+
 def test_scales_of_the_whole_range(cuda):
     """The smallest and largest scales on both sides: their product, not the scales, has to fit."""
     import futudiffu_amd as F
