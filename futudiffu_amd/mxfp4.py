@@ -40,7 +40,7 @@ class MXFP4(NamedTuple):
     low half of its byte (sign, two bits of exponent, one of mantissa), zeros behind the last.
     ``scales``: uint8 ``[P / 256, rows, 8]``, ``rows`` the product of the leading sizes:
     ``scales[g, r, i]`` is ``e + 127`` of row ``r``'s columns ``256 g + 32 i`` to ``.. + 31``, 255 for
-    NaN.
+    NaN (of a block behind the last column any but 255: the products read it).
     """
 
     codes: Tensor

@@ -525,7 +525,8 @@ int sage_linear_bwd(const void* dout, int64_t d_rs, const void* x, int64_t x_rs,
  *   codes        [m][kp / 2] bytes, kp = k rounded up to 256: the even column in the low half
  *                of its byte, zeros behind column k.  16-byte aligned.
  *   scales       [kp / 256][m][8] bytes e + 127: scales[g][r][i] of row r's columns
- *                256 g + 32 i .. + 31; 255: the block is NaN.  8-byte aligned.
+ *                256 g + 32 i .. + 31; 255: the block is NaN (behind column k any but 255: the products
+ *                read it).  8-byte aligned.
  * Quantizing takes e = floor(log2 amax) - 2, from -127 to 127, of a block's largest magnitude amax and
  * the nearest code of x / 2^e, ties to the even code, past 6 the code of 6; a block that holds NaN
  * or an infinity becomes NaN.  Exact in every step but the rounding.
