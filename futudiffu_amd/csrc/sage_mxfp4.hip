@@ -851,8 +851,8 @@ hipError_t run_mx_tiles(const MxGemmArgs& x, hipStream_t st) {
 
 // Waves and LDS slots of a wave.  Up to as many workgroups as the chip holds of them: four waves with deep rings,
 // more bytes in flight on a CU (3840 columns of 3840, one row: 3.7 us against 4.9 for the other).  Past that: two
-// waves, four and more workgroups a CU (with 64 rows three), so that all run at once (11520 columns: 6.2 us against 7.7; with 64
-// rows 10.7 against 14.5; 15360 of 256: 2.9 against 4.2).
+// waves, four and more workgroups a CU (with 64 rows three), so that all run at once (11520 columns: 6.2 us
+// against 7.7; with 64 rows 10.7 against 14.5; 15360 of 256: 2.9 against 4.2).
 template <int MT, bool GLU, bool QX>
 struct SkinnyShape {
   static constexpr int STAGE = ((GLU ? 2 : 1) + (QX ? 0 : MT)) * 2176;

@@ -425,10 +425,11 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&y)[kVec], bool odd, i
 // Forward of the modulated norms with y in MXFP4: norm_fwd_kernel's shares.  fp32 would put one value in
 // 10^6 on the other side of a border between two codes, a whole step away: sums, and the hidden stream, are
 // fp64, and the codes those of the exact values (mx_codes).  The instructions bound it (401 a wave for its 16
-// channels a lane, of them 39 fp64 sums and products and 44 conversions; gated 730, 118 and 118): 24 us for 6912 tokens of 3840 channels modulated, 35 us for 4416 gated and modulated, where
-// the bytes take 13.5 and 22.6.  All of it in fp64 took 30.5 and 39.2; a wave a token with 64 channels a lane,
-// which does the sums over lanes once for four times the channels, 25.7 and, for its registers, 69; several
-// tokens a workgroup with their parameters kept and the next token's rows on their way, 24.6 and 33.9 at best.
+// channels a lane, of them 39 fp64 sums and products and 44 conversions; gated 730, 118 and 118): 25 us for 6912
+// tokens of 3840 channels modulated, 35 us for 4416 gated and modulated, where the bytes take 13.5 and 22.6.  All
+// of it in fp64 took 30.5 and 39.2; a wave a token with 64 channels a lane, which does the sums over lanes once
+// for four times the channels, 25.7 and, for its registers, 69; several tokens a workgroup with their
+// parameters kept and the next token's rows on their way, 24.6 and 33.9 at best.
 template <typename T, int OP, int TPR, bool VEC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_mx_kernel(NormArgs a, uint8_t* codes, uint8_t* scales) {
   constexpr int NT = TPR > 256 ? TPR : 256;
